@@ -10,7 +10,8 @@ Public surface (same names as the reference project):
 
 Additions next to that surface: ``quantize_tensors`` (batched), ``fuse_linears`` /
 ``fuse_sibling_linears`` (q/k/v and gate/up as one launch), ``save_quantized*`` /
-``load_quantized*`` (on-disk format).
+``load_quantized*`` (on-disk format); ``QuantizedKVCache``, ``norm_rotate``, ``norm_rotate_store``, ``rotary_table`` and
+``cache_attention`` (queries, keys, a 4-bit key/value cache and the attention over it).
 
 All arithmetic runs in ``lib/libatlas_b200.so`` (build: ``python -m atlasinfer_b200.build``).
 """
@@ -20,6 +21,7 @@ from .quant.serialization import (load_quantized, load_quantized_model, load_qua
                                   save_quantized_model, save_quantized_state)
 from .integration.atlas_wrappers import FusedLinearGroup, QuantizedLinear, fuse_linears
 from .integration.model_modifier import apply_atlas_quantization_to_model, fuse_sibling_linears
+from .kv_cache import QuantizedKVCache, cache_attention, norm_rotate, norm_rotate_store, rotary_table
 
 __all__ = [
     "QuantizedTensor", "quantize_tensor", "dequantize_tensor", "clear_dequantized_cache",
@@ -28,5 +30,6 @@ __all__ = [
     "quantize_tensors", "fuse_linears", "fuse_sibling_linears", "FusedLinearGroup",
     "save_quantized", "load_quantized", "save_quantized_state", "load_quantized_state",
     "save_quantized_model", "load_quantized_model",
+    "QuantizedKVCache", "norm_rotate", "norm_rotate_store", "rotary_table", "cache_attention",
 ]
 __version__ = "0.1.0"

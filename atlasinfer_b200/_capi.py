@@ -28,6 +28,7 @@ EXPORTS = (
     "atlas_qlinear_plain_launch", "atlas_qlinear_gemm_plan", "atlas_peer_wait", "atlas_peer_push", "atlas_peer_alloc", "atlas_peer_free", "atlas_peer_export", "atlas_peer_import",
     "atlas_peer_release",
     "atlas_qlinear_gemm_workspace_bytes", "atlas_qlinear_gemm", "atlas_qlinear_gemm_gather",
+    "atlas_kv_page_bytes", "atlas_norm_rotate", "atlas_kv_load", "atlas_kv_attention_workspace_bytes", "atlas_kv_attention",
 )
 
 MAX_PEERS = 8
@@ -65,6 +66,33 @@ class RepackItem(ctypes.Structure):
                 ("tiles", ctypes.c_void_p), ("scales_tiled", ctypes.c_void_p), ("outlier_row_ptr", ctypes.c_void_p),
                 ("outlier_chunk_ptr", ctypes.c_void_p), ("outlier_entries", ctypes.c_void_p),
                 ("outlier_vals_sorted", ctypes.c_void_p), ("entry_base", ctypes.c_int64)]
+
+
+class Tokens(ctypes.Structure):
+    """``AtlasTokens`` of include/atlas_b200.h."""
+
+    _fields_ = [("dtype", ctypes.c_int32), ("q_heads", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+                ("tokens", ctypes.c_int64), ("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+                ("q_token_stride", ctypes.c_int64), ("q_head_stride", ctypes.c_int64), ("k_token_stride", ctypes.c_int64),
+                ("k_head_stride", ctypes.c_int64), ("v_token_stride", ctypes.c_int64), ("v_head_stride", ctypes.c_int64),
+                ("q_out", ctypes.c_void_p), ("k_out", ctypes.c_void_p), ("table", ctypes.c_void_p), ("table_rows", ctypes.c_int64),
+                ("positions", ctypes.c_void_p), ("q_weight", ctypes.c_void_p), ("k_weight", ctypes.c_void_p),
+                ("eps", ctypes.c_float), ("weight_offset", ctypes.c_float), ("rotary_dim", ctypes.c_int32),
+                ("interleaved", ctypes.c_int32), ("weights_f32", ctypes.c_int32), ("position_bytes", ctypes.c_int32),
+                ("cache", ctypes.c_void_p), ("num_pages", ctypes.c_int64), ("slots", ctypes.c_void_p),
+                ("page_size", ctypes.c_int32), ("slot_bytes", ctypes.c_int32)]
+
+
+class KvAttention(ctypes.Structure):
+    """``AtlasKvAttention`` of include/atlas_b200.h."""
+
+    _fields_ = [("dtype", ctypes.c_int32), ("q_heads", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+                ("q", ctypes.c_void_p), ("q_token_stride", ctypes.c_int64), ("q_head_stride", ctypes.c_int64), ("out", ctypes.c_void_p),
+                ("total_queries", ctypes.c_int64), ("batch", ctypes.c_int64), ("max_queries", ctypes.c_int64),
+                ("cache", ctypes.c_void_p), ("num_pages", ctypes.c_int64), ("page_size", ctypes.c_int32), ("window", ctypes.c_int32),
+                ("sinks", ctypes.c_int32), ("scale", ctypes.c_float), ("page_table", ctypes.c_void_p), ("table_stride", ctypes.c_int64),
+                ("max_pages", ctypes.c_int64), ("lengths", ctypes.c_void_p), ("query_starts", ctypes.c_void_p),
+                ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t), ("status", ctypes.c_void_p)]
 
 
 _lib: Optional[ctypes.CDLL] = None
@@ -146,6 +174,16 @@ def load() -> ctypes.CDLL:
     L.atlas_qlinear_gemm_workspace_bytes.argtypes = [i64, i64, i64]
     L.atlas_qlinear_gemm.restype = i32
     L.atlas_qlinear_gemm.argtypes = lin + [vp, sz, vp, vp]
+    L.atlas_kv_page_bytes.restype = sz
+    L.atlas_kv_page_bytes.argtypes = [i32, i32]
+    L.atlas_norm_rotate.restype = i32
+    L.atlas_norm_rotate.argtypes = [ctypes.POINTER(Tokens), vp]
+    L.atlas_kv_load.restype = i32
+    L.atlas_kv_load.argtypes = [vp, i64, i32, i32, i32, vp, i32, i64, i32, vp, vp, vp]
+    L.atlas_kv_attention_workspace_bytes.restype = sz
+    L.atlas_kv_attention_workspace_bytes.argtypes = [ctypes.POINTER(KvAttention)]
+    L.atlas_kv_attention.restype = i32
+    L.atlas_kv_attention.argtypes = [ctypes.POINTER(KvAttention), vp]
     _lib = L
     return L
 

@@ -3,7 +3,7 @@
     python -m atlasinfer_b200.build [--force] [--verbose]
 
 The library is compiled from ``csrc/*.cu`` against ``include/atlas_b200.h`` and
-written to ``atlasinfer_b200/lib/``, and beside it the module ``csrc/native.cpp``
+written to ``atlasinfer_b200/lib/``, and beside it the module ``csrc/native*.cpp``
 (the host path of the Python surface, which calls the library).  nvcc
 cross-compiles without a GPU.
 """
@@ -21,7 +21,8 @@ CSRC = os.path.join(PKG, "csrc")
 LIB_DIR = os.path.join(PKG, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libatlas_b200.so")
 
-SOURCES = ["capi.cu", "quantize.cu", "dequant_repack.cu", "gemv.cu", "stream.cu", "peer.cu", "gemm.cu", "gemm_tile.cu"]
+SOURCES = ["capi.cu", "quantize.cu", "dequant_repack.cu", "gemv.cu", "stream.cu", "peer.cu", "gemm.cu", "gemm_tile.cu",
+           "kv_tokens.cu", "kv_attention.cu"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
@@ -45,7 +46,7 @@ def _inputs():
 
 
 NATIVE_NAME = "_atlas_native"
-NATIVE_SRC = os.path.join(CSRC, "native.cpp")
+NATIVE_SOURCES = [os.path.join(CSRC, "native.cpp"), os.path.join(CSRC, "native_kv.cpp")]
 
 
 def native_path() -> str:
@@ -65,10 +66,10 @@ def _stale(target: str, sources) -> bool:
 
 
 def build_native(force: bool = False, verbose: bool = False) -> str:
-    """Compile the host path (``csrc/native.cpp``, against torch's headers) if it is missing or old; return its path."""
+    """Compile the host path (``csrc/native*.cpp``, against torch's headers) if it is missing or old; return its path."""
     header = os.path.join(ROOT, "include", "atlas_b200.h")
     target = native_path()
-    if not force and not _stale(target, [NATIVE_SRC, header]):
+    if not force and not _stale(target, [*NATIVE_SOURCES, header]):
         return target
     import torch
     from torch.utils import cpp_extension
@@ -79,7 +80,7 @@ def build_native(force: bool = False, verbose: bool = False) -> str:
     torch_lib = os.path.join(os.path.dirname(torch.__file__), "lib")
     cxx = "/usr/bin/g++" if os.path.exists("/usr/bin/g++") else (shutil.which("g++") or "c++")
     cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", f"-DTORCH_EXTENSION_NAME={NATIVE_NAME}",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", *(f"-I{d}" for d in dirs), NATIVE_SRC,
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", *(f"-I{d}" for d in dirs), *NATIVE_SOURCES,
            "-o", target, f"-L{LIB_DIR}", "-l:libatlas_b200.so", "-Wl,-rpath,$ORIGIN", f"-L{torch_lib}",
            "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python"]
     res = subprocess.run(cmd, capture_output=True, text=True)

@@ -1,0 +1,720 @@
+// Attention of few queries over the 4-bit cache (decode, drafts), and of many a few rows at a time.
+//
+// For the rows of one kv head (queries x query heads that share it) the cache is the 16-row operand of mma.m16n8k16 and the
+// rows its 8 columns:
+//   S[token][row] = sum over groups of 64 channels of s_token * sum (c - z) q       (c - z: exact small integers in fp16)
+//   p = 2^(S' - m), O[channel][row] += sum over tokens of (s (c - z)) p             (s (c - z): exact in fp16)
+// so that the only roundings are those of p to fp16 and of the output.  A warp walks 16-token slabs, which it brings in by
+// bulk copies of its own, with a softmax state of its own; nothing is shared until its range is done.
+//
+// Every (sequence, kv head) is a run of units (slabs that some row sees), and all runs together are cut evenly among the
+// warps of one CTA per SM from the lengths on the device: ragged batches balance, and a captured graph serves any lengths.
+// A run that lies within a warp goes straight to the output; pieces of the others are joined in shared memory, in order, and
+// what goes beyond a CTA is left in the workspace for kv_join_kernel.
+#include <algorithm>
+
+#include "kv_cache.cuh"
+#include "tensor_core.cuh"
+
+namespace atlas {
+
+namespace {
+
+constexpr float KV_HEADROOM = 8.0f;   // log2: how far a score may pass the running maximum before sums are rescaled
+constexpr float KV_SHIFT = 6.0f;      // log2: p is kept as 2^6 p, up to 2^14 in fp16; what is below 2^-31 of the maximum vanishes
+
+struct Attention {
+    const char *q;               // bytes
+    int64_t q_token_stride, q_head_stride;
+    char *out;
+    const uint8_t *cache;
+    const int32_t *page_table, *lengths, *query_starts;
+    float *partial;
+    int32_t *status;
+    int64_t num_pages, table_stride, max_tokens, total_queries, uniform;
+    int batch, q_heads, kv_heads, group, page_size, window, sinks;   // group: query heads of a kv head
+    float scale_log2;
+    int min_units;               // per warp
+};
+
+// A row tile of a sequence: its queries and the units that they see.
+struct Run {
+    int64_t first_query;         // of the sequence, in q
+    int length, queries;
+    int sink_units, window_unit, units;   // units 0 .. sink_units - 1, then window_unit ...
+    __device__ __forceinline__ int slab(int u) const { return u < sink_units ? u : u - sink_units + window_unit; }
+};
+
+__device__ __forceinline__ Run make_run(const Attention &a, int b, int row0, int rows) {
+    Run r;
+    int64_t q0, q1;
+    if (a.query_starts) {
+        q0 = min(max((int64_t)a.query_starts[b], (int64_t)0), a.total_queries);
+        q1 = min(max((int64_t)a.query_starts[b + 1], q0), a.total_queries);
+    } else {
+        q0 = b * a.uniform, q1 = q0 + a.uniform;
+    }
+    r.first_query = q0;
+    r.queries = (int)(q1 - q0);
+    r.length = (int)min(max((int64_t)a.lengths[b], (int64_t)0), a.max_tokens);
+    r.sink_units = r.window_unit = r.units = 0;
+    const int64_t all = (int64_t)r.queries * a.group;
+    if (row0 >= all) return r;
+    const int p0 = r.length - r.queries + row0 / a.group, p1 = r.length - r.queries + (int)((min(all, (int64_t)row0 + rows) - 1) / a.group);
+    if (p1 < 0) return r;
+    const int end = p1 / KV_SLAB + 1;
+    if (a.window) {
+        r.window_unit = max(0, p0 - a.window + 1) / KV_SLAB;
+        r.sink_units = min((min(a.sinks, p1 + 1) + KV_SLAB - 1) / KV_SLAB, r.window_unit);
+    }
+    r.units = r.sink_units + end - r.window_unit;
+    return r;
+}
+
+// Units of all sequences (times the kv heads), the same in every warp that asks.
+__device__ __forceinline__ int64_t all_units(const Attention &a, int row0, int rows) {
+    int64_t sum = 0;
+    for (int b = threadIdx.x & 31; b < a.batch; b += 32) sum += make_run(a, b, row0, rows).units;
+#pragma unroll
+    for (int k = 16; k; k /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+    return sum * a.kv_heads;
+}
+__device__ __forceinline__ int64_t units_per_warp(const Attention &a, int64_t total, int64_t warps) {
+    return max((total + warps - 1) / warps, (int64_t)a.min_units);
+}
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ uint32_t h2(__half2 v) { return *reinterpret_cast<uint32_t *>(&v); }
+__device__ __forceinline__ __half2 h2(uint32_t v) { return *reinterpret_cast<__half2 *>(&v); }
+
+// The four pairs of a word of codes, minus the zero point: `bias` is 1024 + z, `bias16` 64 + z.
+__device__ __forceinline__ void open_word(uint32_t w, __half2 bias, __half2 bias16, __half2 (&v)[4]) {
+    const __half2 sixteenth = __float2half2_rn(0.0625f);
+    const uint32_t u = w >> 8;
+    v[0] = __hsub2(h2((w & 0x000f000fu) | 0x64006400u), bias);
+    v[1] = __hfma2(h2((w & 0x00f000f0u) | 0x64006400u), sixteenth, __hneg2(bias16));   // (1024 + 16 c) / 16 - (64 + z)
+    v[2] = __hsub2(h2((u & 0x000f000fu) | 0x64006400u), bias);
+    v[3] = __hfma2(h2((u & 0x00f000f0u) | 0x64006400u), sixteenth, __hneg2(bias16));
+}
+
+template <int D, int NT, int WARPS, int STAGES>
+struct Shape {
+    static constexpr int ROWS = 8 * NT, GROUPS = D / 64, WORDS = D / 32;   // words: a lane's, of a token's key
+    static constexpr int SLAB = kv_slab_bytes(D);
+    static constexpr int PIECE = ROWS * (D + 2) * 4;       // maximum, sum and output of the rows
+    static constexpr int RING = STAGES * SLAB;             // a warp's; holds its last piece in the end
+    static constexpr int SMEM = WARPS * (RING + PIECE) + WARPS * STAGES * 8 + 2 * WARPS * 16 + 16;
+    static_assert(PIECE <= RING, "a piece has to fit the ring");
+};
+
+// The state of a warp: maxima, sums and outputs of the rows in the layout of the accumulators.
+template <int D, int NT>
+struct State {
+    float o[NT][D / 16][4];
+    float l[NT][4];
+    float m[NT][2];              // of rows 2 t and 2 t + 1, log2; -inf before the first visible score
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) o[n][i][k] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) l[n][k] = 0.0f;
+            m[n][0] = m[n][1] = -INFINITY;
+        }
+    }
+};
+
+template <bool BF16>
+__device__ __forceinline__ uint2 pack4(float a, float b, float c, float d) {
+    if (BF16) {
+        const __nv_bfloat162 x = __floats2bfloat162_rn(a, b), y = __floats2bfloat162_rn(c, d);
+        return make_uint2(*reinterpret_cast<const uint32_t *>(&x), *reinterpret_cast<const uint32_t *>(&y));
+    }
+    const __half2 x = __floats2half2_rn(a, b), y = __floats2half2_rn(c, d);
+    return make_uint2(*reinterpret_cast<const uint32_t *>(&x), *reinterpret_cast<const uint32_t *>(&y));
+}
+
+// Where a row's output is, or null.
+__device__ __forceinline__ char *out_row(const Attention &a, const Run &r, int h, int row, int d) {
+    const int query = row / a.group;
+    if (query >= r.queries) return nullptr;
+    return a.out + ((r.first_query + query) * a.q_heads + h * a.group + row % a.group) * (int64_t)d * 2;
+}
+
+template <int D, int NT, int WARPS, int STAGES, bool BF16>
+__global__ void __launch_bounds__(WARPS * 32, 1) kv_attention_kernel(const Attention a) {
+    using S = Shape<D, NT, WARPS, STAGES>;
+    extern __shared__ __align__(128) uint8_t smem[];
+    uint8_t *const ring_all = smem, *const heads_all = smem + WARPS * S::RING;
+    uint64_t *const bars = reinterpret_cast<uint64_t *>(heads_all + WARPS * S::PIECE);
+    // run (sequence * kv_heads + head) of every warp's first and last piece, or -1, and whether the run begins or ends there
+    int4 *const notes = reinterpret_cast<int4 *>(bars + WARPS * STAGES);
+
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, g = lane / 4, t = lane % 4;
+    const int row0 = blockIdx.y * S::ROWS;
+    const uint32_t ring = smem_u32(ring_all + warp * S::RING);
+    const uint8_t *const ring_ptr = ring_all + warp * S::RING;
+    const uint32_t bar = smem_u32(bars + warp * STAGES);
+    if (lane == 0) {
+        for (int i = 0; i < STAGES; ++i) mbar_init(bar + 8 * i, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        notes[2 * warp] = notes[2 * warp + 1] = make_int4(-1, 0, 0, 0);
+    }
+    __syncwarp();
+
+    const int64_t total = all_units(a, row0, S::ROWS);
+    const int64_t quota = units_per_warp(a, total, (int64_t)gridDim.x * WARPS);
+    const int64_t begin = ((int64_t)blockIdx.x * WARPS + warp) * quota, end = min(total, begin + quota);
+
+    if (begin < end) {
+        // the sequence, head and unit that the range begins with
+        int b = 0;
+        int64_t before = 0;      // units of the sequences in front
+        for (int base = 0; base < a.batch; base += 32) {
+            const int mine = base + lane < a.batch ? make_run(a, base + lane, row0, S::ROWS).units : 0;
+            int64_t sum = (int64_t)mine * a.kv_heads;
+#pragma unroll
+            for (int k = 1; k < 32; k *= 2) {
+                const int64_t other = __shfl_up_sync(0xffffffffu, sum, k);
+                if (lane >= k) sum += other;
+            }
+            const uint32_t past = __ballot_sync(0xffffffffu, before + sum > begin);
+            if (past) {
+                const int at = __ffs(past) - 1;
+                b = base + at;
+                before += __shfl_sync(0xffffffffu, sum - (int64_t)mine * a.kv_heads, at);
+                break;
+            }
+            before += __shfl_sync(0xffffffffu, sum, 31);
+        }
+        Run run = make_run(a, b, row0, S::ROWS);
+        int head = (int)((begin - before) / run.units);
+        int unit = (int)((begin - before) % run.units);
+
+        // the producer's own place, up to STAGES units ahead; pages of the next 32 units of its run, one a lane
+        Run p_run = run;
+        int p_b = b, p_head = head, p_unit = unit, p_first = 0, p_count = 0, issued = 0, page_ahead = -1;
+        const int todo = (int)(end - begin);
+        auto produce = [&]() {
+            if (issued >= todo) return;
+            if (p_unit >= p_run.units) {
+                p_unit = 0;
+                if (++p_head == a.kv_heads) {
+                    p_head = 0;
+                    do p_run = make_run(a, ++p_b, row0, S::ROWS); while (p_run.units == 0);
+                }
+                p_count = 0;
+            }
+            if (p_count == 0 || p_unit >= p_first + p_count) {
+                p_first = p_unit;
+                p_count = min(32, p_run.units - p_unit);
+                page_ahead = -1;
+                if (lane < p_count) page_ahead = a.page_table[p_b * a.table_stride + p_run.slab(p_unit + lane) * KV_SLAB / a.page_size];
+            }
+            const int page = __shfl_sync(0xffffffffu, page_ahead, p_unit - p_first);
+            if (lane == 0) {
+                const int stage = issued % STAGES, token = p_run.slab(p_unit) * KV_SLAB;
+                const bool known = page >= 0 && page < a.num_pages;
+                const uint32_t at = bar + 8 * stage;
+                if (known) {
+                    const uint8_t *src = a.cache + (((int64_t)page * a.kv_heads + p_head) * (a.page_size / KV_SLAB) + token % a.page_size / KV_SLAB) * S::SLAB;
+                    mbar_arrive_expect_tx(at, S::SLAB);
+                    bulk_load_1d(ring + stage * S::SLAB, src, S::SLAB, at);
+                } else {   // a page that is not there: a NaN in the first scale of the keys says so, the slab is passed over
+                    *reinterpret_cast<volatile uint16_t *>(ring_all + warp * S::RING + stage * S::SLAB + kv_key_params(D)) = 0x7fff;
+                    fence_async_smem();   // (the stage's next slab comes by the other proxy)
+                    mbar_arrive(at);
+                }
+            }
+            ++issued;
+            ++p_unit;
+        };
+        for (int i = 0; i < STAGES; ++i) produce();
+
+        State<D, NT> st;
+        uint32_t qf[NT][S::WORDS][4];
+        float factor[NT][2];       // log2 units of a row's scores
+        int place[NT][2];          // positions of rows 2 t and 2 t + 1, -1: no such row
+        int p_lo = 0, p_hi = 0;    // positions of the tile's first and last query
+        bool fresh = true, first_piece = true, failed = false;
+        const bool begins_inside = unit != 0;
+        int done = 0;
+
+        auto leave = [&](bool whole_run, bool ends) {
+            // to the output (a run that began and ended here), or to shared memory
+            if (whole_run) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        char *dst = out_row(a, run, head, row0 + 8 * n + 2 * t + e, D);
+                        const float inv = st.l[n][e] > 0.0f || st.l[n][e] != st.l[n][e] ? 1.0f / st.l[n][e] : 0.0f;
+#pragma unroll
+                        for (int j = 0; j < S::WORDS; ++j)
+                            if (dst)
+                                *reinterpret_cast<uint2 *>(dst + (32 * j + 4 * g) * 2) =
+                                    pack4<BF16>(st.o[n][2 * j][e] * inv, st.o[n][2 * j][2 + e] * inv, st.o[n][2 * j + 1][e] * inv, st.o[n][2 * j + 1][2 + e] * inv);
+                    }
+                return;
+            }
+            float *piece = reinterpret_cast<float *>(first_piece ? heads_all + warp * S::PIECE : ring_all + warp * S::RING);
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int row = 8 * n + 2 * t + e;
+                    if (g == 0) {
+                        piece[row] = st.m[n][e];
+                        piece[S::ROWS + row] = st.l[n][e];
+                    }
+#pragma unroll
+                    for (int j = 0; j < S::WORDS; ++j)
+                        *reinterpret_cast<float4 *>(piece + 2 * S::ROWS + row * D + 32 * j + 4 * g) =
+                            make_float4(st.o[n][2 * j][e], st.o[n][2 * j][2 + e], st.o[n][2 * j + 1][e], st.o[n][2 * j + 1][2 + e]);
+                }
+            if (lane == 0) notes[2 * warp + (first_piece ? 0 : 1)] = make_int4(b * a.kv_heads + head, 1, ends, 0);
+        };
+
+        for (; done < todo; ++done) {
+            if (fresh) {           // another run: its queries into registers
+                st.clear();
+                fresh = false;
+                p_lo = run.length - run.queries + row0 / a.group;
+                p_hi = run.length - 1;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const int row = row0 + 8 * n + g, query = row / a.group;
+                    const bool there = query < run.queries;
+                    const char *src = a.q + (run.first_query + query) * a.q_token_stride + (head * a.group + row % a.group) * a.q_head_stride;
+                    float top = 0.0f;
+                    uint4 raw[S::WORDS];
+#pragma unroll
+                    for (int j = 0; j < S::WORDS; ++j) {
+                        raw[j] = there ? *reinterpret_cast<const uint4 *>(src + (32 * j + 8 * t) * 2) : make_uint4(0, 0, 0, 0);
+                        if (BF16) {
+                            const uint32_t w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                top = fmaxf(top, fmaxf(fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xffff0000u))));
+                        }
+                    }
+                    float unscale = 1.0f;
+                    if (BF16) {
+                        // bf16 rows become fp16 times a power of two, chosen so that the largest is in [1, 2): exact, but for
+                        // numbers below 2^-14 of it, which are off by 2^-25 of it at most
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                        const int ex = min(max((__float_as_int(top) >> 23) & 0xff, 8), 246);
+                        const float down = __int_as_float((254 - ex) << 23);
+                        unscale = __int_as_float(ex << 23);
+#pragma unroll
+                        for (int j = 0; j < S::WORDS; ++j) {
+                            const uint32_t w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                qf[n][j][i] = h2(__floats2half2_rn(__uint_as_float(w[i] << 16) * down, __uint_as_float(w[i] & 0xffff0000u) * down));
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < S::WORDS; ++j) qf[n][j][0] = raw[j].x, qf[n][j][1] = raw[j].y, qf[n][j][2] = raw[j].z, qf[n][j][3] = raw[j].w;
+                    }
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        factor[n][e] = a.scale_log2 * __shfl_sync(0xffffffffu, unscale, (2 * t + e) * 4);
+                        const int r = row0 + 8 * n + 2 * t + e;
+                        place[n][e] = r / a.group < run.queries ? run.length - run.queries + r / a.group : -1;
+                    }
+                }
+            }
+
+            const int stage = done % STAGES;
+            if (!__all_sync(0xffffffffu, mbar_wait(bar + 8 * stage, (done / STAGES) & 1))) {
+                failed = true;
+                break;
+            }
+            const uint8_t *slab = ring_ptr + stage * S::SLAB;
+            const int token0 = run.slab(unit) * KV_SLAB;
+            const bool there = *reinterpret_cast<const uint16_t *>(slab + kv_key_params(D)) != 0x7fffu;
+            if (there) {
+                // scores
+                float s[NT][4];
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) s[n][k] = 0.0f;
+#pragma unroll
+                for (int gr = 0; gr < S::GROUPS; ++gr) {
+                    const __half2 lo = *reinterpret_cast<const __half2 *>(slab + kv_key_params(D) + (g * S::GROUPS + gr) * 4);
+                    const __half2 hi = *reinterpret_cast<const __half2 *>(slab + kv_key_params(D) + ((g + 8) * S::GROUPS + gr) * 4);
+                    const __half2 bl = __high2half2(lo), bh = __high2half2(hi), off = __float2half2_rn(960.0f);
+                    const __half2 bl16 = __hsub2(bl, off), bh16 = __hsub2(bh, off);
+                    float acc[NT][4];
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) acc[n][k] = 0.0f;
+                    const uint2 w0 = *reinterpret_cast<const uint2 *>(slab + kv_key_word(D, g, t + 8 * gr)), w1 = *reinterpret_cast<const uint2 *>(slab + kv_key_word(D, g + 8, t + 8 * gr));
+                    const uint32_t low[2] = {w0.x, w0.y}, high[2] = {w1.x, w1.y};
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        __half2 x[4], y[4];
+                        open_word(low[j], bl, bl16, x);
+                        open_word(high[j], bh, bh16, y);
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+#pragma unroll
+                            for (int n = 0; n < NT; ++n)
+                                mma_f16(acc[n], h2(x[2 * i]), h2(y[2 * i]), h2(x[2 * i + 1]), h2(y[2 * i + 1]), qf[n][2 * gr + j][2 * i], qf[n][2 * gr + j][2 * i + 1]);
+                    }
+                    const float sl = __low2float(lo), sh = __low2float(hi);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        s[n][0] += acc[n][0] * sl, s[n][1] += acc[n][1] * sl;
+                        s[n][2] += acc[n][2] * sh, s[n][3] += acc[n][3] * sh;
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) s[n][k] *= factor[n][k & 1];
+                const bool all_seen = token0 + KV_SLAB - 1 <= p_lo && (!a.window || token0 > p_hi - a.window || token0 + KV_SLAB <= a.sinks);
+                if (!all_seen) {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const int token = token0 + g + (k / 2) * 8, p = place[n][k & 1];
+                            if (token > p || (a.window && token <= p - a.window && token >= a.sinks)) s[n][k] = -INFINITY;
+                        }
+                }
+                // the maximum moves only where a score passes it by more than 2^8
+                bool passes = false;
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) passes |= s[n][k] > st.m[n][k & 1] + KV_HEADROOM;
+                if (__any_sync(0xffffffffu, passes)) {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            float top = fmaxf(fmaxf(s[n][e], s[n][2 + e]), st.m[n][e]);
+                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                            const float shrink = st.m[n][e] == -INFINITY ? 0.0f : exp2_fast(st.m[n][e] - top);
+                            st.m[n][e] = top;
+                            st.l[n][e] *= shrink, st.l[n][2 + e] *= shrink;
+#pragma unroll
+                            for (int i = 0; i < D / 16; ++i) st.o[n][i][e] *= shrink, st.o[n][i][2 + e] *= shrink;
+                        }
+                }
+                uint32_t pb[NT][2];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    float p[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const float ref = st.m[n][k & 1] == -INFINITY ? 0.0f : st.m[n][k & 1] - KV_SHIFT;
+                        p[k] = exp2_fast(s[n][k] - ref);
+                    }
+                    pb[n][0] = transpose8x8(h2(__floats2half2_rn(p[0], p[1])));
+                    pb[n][1] = transpose8x8(h2(__floats2half2_rn(p[2], p[3])));
+                    mma_f16(st.l[n], 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, pb[n][0], pb[n][1]);   // sums of what is used
+                }
+                // outputs
+#pragma unroll
+                for (int gr = 0; gr < S::GROUPS; ++gr) {
+                    uint2 p0 = *reinterpret_cast<const uint2 *>(slab + kv_value_params(D) + (t * S::GROUPS + gr) * 8);
+                    uint2 p1 = *reinterpret_cast<const uint2 *>(slab + kv_value_params(D) + ((t + 4) * S::GROUPS + gr) * 8);
+                    if (token0 + KV_SLAB > run.length) {   // tokens that are not there may hold anything
+                        uint32_t keep0 = 0, keep1 = 0;
+                        if (token0 + 2 * t < run.length) keep0 |= 0xffffu;
+                        if (token0 + 2 * t + 1 < run.length) keep0 |= 0xffff0000u;
+                        if (token0 + 2 * t + 8 < run.length) keep1 |= 0xffffu;
+                        if (token0 + 2 * t + 9 < run.length) keep1 |= 0xffff0000u;
+                        p0.x &= keep0, p0.y = (p0.y & keep0) | (0x64006400u & ~keep0);
+                        p1.x &= keep1, p1.y = (p1.y & keep1) | (0x64006400u & ~keep1);
+                    }
+                    const __half2 off = __float2half2_rn(960.0f), s0 = h2(p0.x), s1 = h2(p1.x), b0 = h2(p0.y), b1 = h2(p1.y);
+                    const __half2 b016 = __hsub2(b0, off), b116 = __hsub2(b1, off);
+                    const uint8_t *codes = slab + kv_value_codes(D);
+                    const uint2 w0 = *reinterpret_cast<const uint2 *>(codes + kv_value_unit(D, 2 * t, g + 16 * gr)), w1 = *reinterpret_cast<const uint2 *>(codes + kv_value_unit(D, 2 * t + 8, g + 16 * gr));
+                    const uint32_t low[2] = {w0.x, w0.y}, high[2] = {w1.x, w1.y};
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        __half2 x[4], y[4];
+                        open_word(low[j], b0, b016, x);
+                        open_word(high[j], b1, b116, y);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) x[i] = __hmul2(x[i], s0), y[i] = __hmul2(y[i], s1);
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+#pragma unroll
+                            for (int n = 0; n < NT; ++n)
+                                mma_f16(st.o[n][4 * gr + 2 * j + i], h2(x[2 * i]), h2(x[2 * i + 1]), h2(y[2 * i]), h2(y[2 * i + 1]), pb[n][0], pb[n][1]);
+                    }
+                }
+            }
+            __syncwarp();          // everyone has read the stage
+            produce();
+
+            if (++unit == run.units) {
+                const bool whole = !(first_piece && begins_inside);
+                leave(whole, true);
+                first_piece = false;
+                fresh = true;
+                unit = 0;
+                if (done + 1 < todo && ++head == a.kv_heads) {
+                    head = 0;
+                    do run = make_run(a, ++b, row0, S::ROWS); while (run.units == 0);
+                }
+            }
+        }
+        if (failed) {              // a copy that never came: those in flight land (or not, within the limit) before the CTA goes
+            for (int i = done + 1; i < issued; ++i) mbar_wait(bar + 8 * (i % STAGES), (i / STAGES) & 1);
+            if (lane == 0 && a.status) *a.status = 1;
+        } else if (unit) {
+            __syncwarp();
+            leave(false, false);
+        }
+    }
+    __syncthreads();
+
+    // pieces in order: runs that are whole within the CTA go to the output, the others to the workspace
+    for (int i = 0; i < 2 * WARPS;) {
+        const int4 note = notes[i];
+        if (note.x < 0) {
+            ++i;
+            continue;
+        }
+        int last = i;
+        bool ends = note.z != 0;
+        for (int k = i + 1; k < 2 * WARPS && !ends; ++k)
+            if (notes[k].x == note.x) last = k, ends = notes[k].z != 0;
+        const int b = note.x / a.kv_heads, head = note.x % a.kv_heads;
+        const Run run = make_run(a, b, row0, S::ROWS);
+        // whether its first unit lies in front of this CTA
+        bool begins = true;
+        {
+            const int64_t cta_begin = (int64_t)blockIdx.x * WARPS * quota;
+            // (only the CTA's first piece can have begun before it)
+            if (i == 0 || notes[0].x == note.x) {
+                int64_t before = 0;
+                for (int k = lane; k < b; k += 32) before += make_run(a, k, row0, S::ROWS).units;
+#pragma unroll
+                for (int k = 16; k; k /= 2) before += __shfl_xor_sync(0xffffffffu, before, k);
+                begins = before * a.kv_heads + (int64_t)head * run.units >= cta_begin;
+            }
+        }
+        for (int x = threadIdx.x; x < S::ROWS * (D / 4); x += WARPS * 32) {
+            const int row = x / (D / 4), c = x % (D / 4) * 4;
+            float m = -INFINITY, l = 0.0f;
+            float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (int k = i; k <= last; ++k) {
+                if (notes[k].x != note.x) continue;
+                const float *piece = reinterpret_cast<const float *>(k & 1 ? ring_all + (k / 2) * S::RING : heads_all + (k / 2) * S::PIECE);
+                const float pm = piece[row], top = fmaxf(m, pm);
+                const float wa = m == -INFINITY ? 0.0f : exp2_fast(m - top), wb = pm == -INFINITY ? 0.0f : exp2_fast(pm - top);
+                const float4 po = *reinterpret_cast<const float4 *>(piece + 2 * S::ROWS + row * D + c);
+                l = l * wa + piece[S::ROWS + row] * wb;
+                o.x = o.x * wa + po.x * wb, o.y = o.y * wa + po.y * wb, o.z = o.z * wa + po.z * wb, o.w = o.w * wa + po.w * wb;
+                m = top;
+            }
+            if (begins && ends) {
+                char *dst = out_row(a, run, head, row0 + row, D);
+                const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+                if (dst) *reinterpret_cast<uint2 *>(dst + c * 2) = pack4<BF16>(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+            } else {
+                float *piece = a.partial + (((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 2 + (begins ? 1 : 0)) * (S::PIECE / 4);
+                if (c == 0) piece[row] = m, piece[S::ROWS + row] = l;
+                *reinterpret_cast<float4 *>(piece + 2 * S::ROWS + row * D + c) = o;
+            }
+        }
+        i = last + 1;
+    }
+}
+
+// One CTA a run: joins what several CTAs of kv_attention_kernel have left of it, in their order, and zeroes rows of runs
+// without units.  It finds the CTAs from the lengths, before the kernel in front has ended.
+template <int D, int NT, int WARPS, bool BF16>
+__global__ void __launch_bounds__(128) kv_join_kernel(const Attention a, int ctas) {
+    constexpr int ROWS = 8 * NT, PIECE = ROWS * (D + 2);
+    const int b = blockIdx.x / a.kv_heads, head = blockIdx.x % a.kv_heads, lane = threadIdx.x & 31, row0 = blockIdx.y * ROWS;
+    const Run run = make_run(a, b, row0, ROWS);
+    int64_t before = 0;
+    for (int k = lane; k < b; k += 32) before += make_run(a, k, row0, ROWS).units;
+#pragma unroll
+    for (int k = 16; k; k /= 2) before += __shfl_xor_sync(0xffffffffu, before, k);
+    const int64_t quota = units_per_warp(a, all_units(a, row0, ROWS), (int64_t)ctas * WARPS) * WARPS;
+    const int64_t first = before * a.kv_heads + (int64_t)head * run.units;
+    const int64_t c0 = first / quota, c1 = run.units ? (first + run.units - 1) / quota : c0;
+    if (run.units && c0 == c1) return;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    for (int x = threadIdx.x; x < ROWS * (D / 4); x += 128) {
+        const int row = x / (D / 4), c = x % (D / 4) * 4;
+        char *dst = out_row(a, run, head, row0 + row, D);
+        if (!dst) continue;
+        float m = -INFINITY, l = 0.0f;
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (run.units)
+            for (int64_t k = c0; k <= c1; ++k) {
+                const float *piece = a.partial + (((int64_t)blockIdx.y * ctas + k) * 2 + (k == c0 ? 1 : 0)) * PIECE;
+                const float pm = piece[row], top = fmaxf(m, pm);
+                const float wa = m == -INFINITY ? 0.0f : exp2_fast(m - top), wb = pm == -INFINITY ? 0.0f : exp2_fast(pm - top);
+                const float4 po = *reinterpret_cast<const float4 *>(piece + 2 * ROWS + row * D + c);
+                l = l * wa + piece[ROWS + row] * wb;
+                o.x = o.x * wa + po.x * wb, o.y = o.y * wa + po.y * wb, o.z = o.z * wa + po.z * wb, o.w = o.w * wa + po.w * wb;
+                m = top;
+            }
+        const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+        *reinterpret_cast<uint2 *>(dst + c * 2) = pack4<BF16>(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+    }
+}
+
+int sm_count() {
+    int dev = 0, sms = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return 148;
+    static thread_local int known_dev = -1, known = 0;
+    if (known_dev != dev) {
+        if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+        known_dev = dev, known = sms;
+    }
+    return known;
+}
+
+struct Plan {
+    int nt, warps, stages;
+    int64_t tiles;
+    size_t piece_bytes;
+};
+Plan plan_of(const AtlasKvAttention &p) {
+    Plan plan;
+    const int64_t rows = p.max_queries * (p.q_heads / p.kv_heads);
+    plan.nt = rows > 8 ? 2 : 1;
+    plan.tiles = ceil_div_i64(std::max<int64_t>(rows, 1), 8 * plan.nt);
+    plan.piece_bytes = (size_t)8 * plan.nt * (p.head_dim + 2) * 4;
+    return plan;
+}
+
+template <int D, int NT, int WARPS, int STAGES, bool BF16>
+int launch(const Attention &a, int64_t tiles, int ctas, cudaStream_t stream) {
+    using S = Shape<D, NT, WARPS, STAGES>;
+    auto *kernel = kv_attention_kernel<D, NT, WARPS, STAGES, BF16>;
+    int e = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM), "atlas_kv_attention");
+    if (e != ATLAS_OK) return e;
+    kernel<<<dim3((unsigned)ctas, (unsigned)tiles), WARPS * 32, S::SMEM, stream>>>(a);
+    e = check_cuda(cudaGetLastError(), "atlas_kv_attention");
+    if (e != ATLAS_OK) return e;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3((unsigned)(a.batch * a.kv_heads), (unsigned)tiles);
+    config.blockDim = dim3(128);
+    config.stream = stream;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &attr;
+    config.numAttrs = 1;
+    return check_cuda(cudaLaunchKernelEx(&config, kv_join_kernel<D, NT, WARPS, BF16>, a, ctas), "atlas_kv_attention");
+}
+
+template <int D, bool BF16>
+int launch_nt(const Attention &a, const Plan &plan, int ctas, cudaStream_t stream) {
+    if constexpr (D == 64) return plan.nt == 1 ? launch<64, 1, 16, 8, BF16>(a, plan.tiles, ctas, stream) : launch<64, 2, 16, 8, BF16>(a, plan.tiles, ctas, stream);
+    if constexpr (D == 128) return plan.nt == 1 ? launch<128, 1, 16, 4, BF16>(a, plan.tiles, ctas, stream) : launch<128, 2, 12, 4, BF16>(a, plan.tiles, ctas, stream);
+    if constexpr (D == 256) return plan.nt == 1 ? launch<256, 1, 8, 4, BF16>(a, plan.tiles, ctas, stream) : launch<256, 2, 6, 4, BF16>(a, plan.tiles, ctas, stream);
+    return ATLAS_ERR_UNSUPPORTED;
+}
+
+bool aligned16(const void *p, int64_t a, int64_t b) { return !((reinterpret_cast<uintptr_t>(p) | (uintptr_t)a | (uintptr_t)b) & 15); }
+
+int check_arguments(const AtlasKvAttention *p, const char *what) {
+    ATLAS_RETURN_IF(!p, ATLAS_ERR_BAD_ARGUMENT, "%s: no arguments", what);
+    const int shape = check_kv_shape(p->num_pages, p->kv_heads, p->head_dim, p->page_size, what);
+    if (shape != ATLAS_OK) return shape;
+    ATLAS_RETURN_IF(p->dtype != ATLAS_DTYPE_F16 && p->dtype != ATLAS_DTYPE_BF16, ATLAS_ERR_BAD_ARGUMENT, "%s: dtype %d", what, p->dtype);
+    ATLAS_RETURN_IF(p->q_heads < 1 || p->q_heads % p->kv_heads || p->q_heads / p->kv_heads > 1024, ATLAS_ERR_BAD_ARGUMENT,
+                    "%s: %d query heads on %d kv heads", what, p->q_heads, p->kv_heads);
+    ATLAS_RETURN_IF(p->total_queries < 0 || p->batch < 0 || p->max_queries < 0 || p->window < 0 || p->sinks < 0 || p->max_pages < 0,
+                    ATLAS_ERR_BAD_ARGUMENT, "%s: negative size", what);
+    ATLAS_RETURN_IF(p->total_queries > (1 << 24) || p->batch * (int64_t)p->kv_heads > 0x7fffffff || p->max_queries > (1 << 24) ||
+                        p->max_pages * (int64_t)p->page_size > (1 << 30),
+                    ATLAS_ERR_UNSUPPORTED, "%s: %lld queries of %lld sequences over up to %lld tokens", what, (long long)p->total_queries,
+                    (long long)p->batch, (long long)p->max_pages * p->page_size);
+    return ATLAS_OK;
+}
+
+}  // namespace
+}  // namespace atlas
+
+extern "C" {
+
+size_t atlas_kv_attention_workspace_bytes(const AtlasKvAttention *p) {
+    using namespace atlas;
+    if (check_arguments(p, "atlas_kv_attention_workspace_bytes") != ATLAS_OK) return 0;
+    const Plan plan = plan_of(*p);
+    return (size_t)plan.tiles * sm_count() * 2 * plan.piece_bytes;
+}
+
+int atlas_kv_attention(const AtlasKvAttention *p, void *stream) {
+    using namespace atlas;
+    clear_error();
+    const char *what = "atlas_kv_attention";
+    const int args = check_arguments(p, what);
+    if (args != ATLAS_OK) return args;
+    if (p->total_queries == 0 || p->batch == 0) return ATLAS_OK;
+    ATLAS_RETURN_IF(!p->query_starts && p->total_queries % p->batch, ATLAS_ERR_BAD_ARGUMENT, "%s: %lld queries of %lld sequences without query_starts", what,
+                    (long long)p->total_queries, (long long)p->batch);
+    ATLAS_RETURN_IF(p->max_queries < (p->query_starts ? 1 : p->total_queries / p->batch), ATLAS_ERR_BAD_ARGUMENT, "%s: max_queries %lld", what,
+                    (long long)p->max_queries);
+    ATLAS_RETURN_IF(!p->q || !p->out || !p->lengths || (p->num_pages && !p->cache) || (p->max_pages && !p->page_table), ATLAS_ERR_BAD_ARGUMENT,
+                    "%s: null pointer", what);
+    ATLAS_RETURN_IF(!aligned16(p->q, 2 * p->q_token_stride, 2 * p->q_head_stride) || !aligned16(p->out, 0, 0) || !aligned16(p->cache, 0, 0) ||
+                        (reinterpret_cast<uintptr_t>(p->workspace) & 255),
+                    ATLAS_ERR_BAD_ARGUMENT, "%s: pointers and strides must be multiples of 16 bytes, the workspace of 256", what);
+    const int dev = check_device();
+    if (dev != ATLAS_OK) return dev;
+    const Plan plan = plan_of(*p);
+    const int ctas = sm_count();
+    ATLAS_RETURN_IF(plan.tiles > 65535, ATLAS_ERR_UNSUPPORTED, "%s: %lld queries in a sequence", what, (long long)p->max_queries);
+    ATLAS_RETURN_IF(!p->workspace || p->workspace_bytes < (size_t)plan.tiles * ctas * 2 * plan.piece_bytes, ATLAS_ERR_CAPACITY, "%s: workspace of %zu bytes",
+                    what, p->workspace_bytes);
+
+    Attention a = {};
+    a.q = (const char *)p->q, a.q_token_stride = 2 * p->q_token_stride, a.q_head_stride = 2 * p->q_head_stride;
+    a.out = (char *)p->out, a.cache = (const uint8_t *)p->cache;
+    a.page_table = p->page_table, a.lengths = p->lengths, a.query_starts = p->query_starts;
+    a.partial = (float *)p->workspace, a.status = p->status;
+    a.num_pages = p->num_pages, a.table_stride = p->table_stride, a.max_tokens = p->max_pages * p->page_size;
+    a.total_queries = p->total_queries, a.uniform = p->query_starts ? 0 : p->total_queries / p->batch;
+    a.batch = (int)p->batch, a.q_heads = p->q_heads, a.kv_heads = p->kv_heads, a.group = p->q_heads / p->kv_heads;
+    a.page_size = p->page_size, a.window = p->window, a.sinks = p->sinks;
+    a.scale_log2 = p->scale * 1.4426950408889634f;
+    a.min_units = 1;
+    const bool bf16 = p->dtype == ATLAS_DTYPE_BF16;
+    cudaStream_t s = (cudaStream_t)stream;
+    switch (p->head_dim) {
+        case 64: return bf16 ? launch_nt<64, true>(a, plan, ctas, s) : launch_nt<64, false>(a, plan, ctas, s);
+        case 128: return bf16 ? launch_nt<128, true>(a, plan, ctas, s) : launch_nt<128, false>(a, plan, ctas, s);
+        default: return bf16 ? launch_nt<256, true>(a, plan, ctas, s) : launch_nt<256, false>(a, plan, ctas, s);
+    }
+}
+
+}  // extern "C"

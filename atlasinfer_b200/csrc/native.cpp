@@ -19,14 +19,18 @@
 
 namespace py = pybind11;
 
-namespace {
-
 // raises what the Python package raises for a status of the C ABI
-void check(int status, const char *what) {
+void check_status_code(int status, const char *what) {
     if (status == ATLAS_OK) return;
     py::gil_scoped_acquire gil;
     py::module_::import("atlasinfer_b200._capi").attr("check")(status, what);
 }
+
+void bind_kv(py::module_ &m);   // native_kv.cpp
+
+namespace {
+
+void check(int status, const char *what) { check_status_code(status, what); }
 
 const void *ptr_or_null(const at::Tensor &t) { return t.numel() ? t.data_ptr() : nullptr; }
 
@@ -356,4 +360,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("build_layout", &build_layout, py::call_guard<py::gil_scoped_release>());
     m.def("quantize_many", &quantize_many, py::call_guard<py::gil_scoped_release>());
     m.def("linear", &linear, py::call_guard<py::gil_scoped_release>());
+    bind_kv(m);
 }

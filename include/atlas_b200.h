@@ -380,6 +380,106 @@ ATLAS_API int atlas_qlinear_gemm(const void *x, int dtype, int64_t m, int64_t ld
                                  int64_t ldy, void *workspace, size_t workspace_bytes, int32_t *status,
                                  void *stream);
 
+/* ---- queries, keys and the 4-bit cache ---------------------------------------------
+ * No counterpart in the reference (its attention is the model's own; its cache
+ * is tiered, not quantized).  What a decoder layer does between its q/k/v
+ * projection and its output projection.
+ *
+ * The cache is paged: num_pages pages of page_size tokens (a multiple of 16) of
+ * kv_heads heads, [page][head][atlas_kv_page_bytes].  Every 64 channels of a
+ * token and head have a 4-bit code each, an fp16 scale s and a zero point z:
+ * value = s (c - z), c and z in 0..15, s of 7 significant bits, which is exact
+ * in fp16.  For a group with lo = min(x, 0), hi = max(x, 0): s = (hi - lo) / 15
+ * rounded up to 7 bits, in [2^-18, 4352]; z = rint(-lo / s);
+ * c = clamp(rint(x / s) + z, 0, 15).  NaN is stored as 0, values saturate at
+ * +-65280, so the cache holds finite numbers only.  A token's place is its
+ * slot, page * page_size + offset.  head_dim is 64, 128 or 256.
+ */
+ATLAS_API size_t atlas_kv_page_bytes(int head_dim, int page_size);
+
+/* Norms of queries and keys, their rotation, and keys and values stored, in one pass.
+ *   dtype            of q, k, v, q_out, k_out (ATLAS_DTYPE_*)
+ *   q, k, v          [tokens][heads][head_dim], strides in elements; the last
+ *                    dimension is contiguous; pointers and strides are
+ *                    multiples of 16 bytes.  q may be absent (q_heads 0); v is
+ *                    only read if there is a cache
+ *   q_out, k_out     contiguous; k_out may be NULL if there is a cache
+ *   table            fp32 [table_rows][rotary_dim], cosines then sines of a
+ *                    position's rotary_dim / 2 angles, or NULL (no rotation);
+ *                    rotary_dim is a multiple of 16.  Pairs are channels i and
+ *                    i + rotary_dim / 2, or 2 i and 2 i + 1 (`interleaved`)
+ *   positions        [tokens] int32 or int64 (position_bytes); a token whose
+ *                    position is not a row of the table becomes NaN
+ *   q_weight, k_weight   [head_dim] of `dtype`, or fp32 (weights_f32), or NULL:
+ *                    x * rsqrt(mean(x^2) + eps) * (weight + weight_offset)
+ *   cache, slots     [tokens] int32 or int64 (slot_bytes); tokens whose slot is
+ *                    not in the cache are not stored.  No slot twice in a call
+ */
+typedef struct AtlasTokens {
+    int32_t dtype;
+    int32_t q_heads, kv_heads, head_dim;
+    int64_t tokens;
+    const void *q, *k, *v;
+    int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+    void *q_out, *k_out;
+    const float *table;
+    int64_t table_rows;
+    const void *positions;
+    const void *q_weight, *k_weight;
+    float eps, weight_offset;
+    int32_t rotary_dim, interleaved, weights_f32, position_bytes;
+    void *cache;
+    int64_t num_pages;
+    const void *slots;
+    int32_t page_size, slot_bytes;
+} AtlasTokens;
+ATLAS_API int atlas_norm_rotate(const AtlasTokens *tokens, void *stream);
+
+/* Stored keys and values back, contiguous [tokens][kv_heads][head_dim] of `dtype`
+ * (fp16: exactly what is stored).  Slots outside the cache give zeros. */
+ATLAS_API int atlas_kv_load(const void *cache, int64_t num_pages, int kv_heads, int head_dim, int page_size, const void *slots,
+                            int slot_bytes, int64_t tokens, int dtype, void *k_out, void *v_out, void *stream);
+
+/* Attention of queries over the cache.  Sequence b has lengths[b] tokens in the
+ * cache, the last of which are its queries' own: query i of n is at position
+ * p = lengths[b] - n + i and sees key j if j <= p and (window == 0, j > p -
+ * window, or j < sinks).  out = softmax(scale q k^T) v over what it sees; a row
+ * that sees nothing is 0.  Query head h reads head h / (q_heads / kv_heads).
+ *   q, out           [total_queries][q_heads][head_dim]; q with strides in
+ *                    elements (multiples of 16 bytes), out contiguous
+ *   page_table       int32 [batch][table_stride]: page of a sequence's tokens
+ *                    i page_size ..., max_pages of them at most.  Only pages
+ *                    with tokens that some query sees are read; a page outside
+ *                    the cache counts as hidden
+ *   query_starts     int32 [batch + 1] first query of every sequence, or NULL:
+ *                    total_queries / batch each
+ *   max_queries      at least the queries of any sequence
+ *   workspace        atlas_kv_attention_workspace_bytes(...) bytes, 256-byte
+ *                    aligned; contents irrelevant before and after
+ *   status           device int32 or NULL, set non-zero if a bounded wait ran out
+ * lengths, query_starts and page_table are read on the device only.
+ */
+typedef struct AtlasKvAttention {
+    int32_t dtype;
+    int32_t q_heads, kv_heads, head_dim;
+    const void *q;
+    int64_t q_token_stride, q_head_stride;
+    void *out;
+    int64_t total_queries, batch, max_queries;
+    const void *cache;
+    int64_t num_pages;
+    int32_t page_size, window, sinks;
+    float scale;
+    const int32_t *page_table;
+    int64_t table_stride, max_pages;
+    const int32_t *lengths, *query_starts;
+    void *workspace;
+    size_t workspace_bytes;
+    int32_t *status;
+} AtlasKvAttention;
+ATLAS_API size_t atlas_kv_attention_workspace_bytes(const AtlasKvAttention *attention);
+ATLAS_API int atlas_kv_attention(const AtlasKvAttention *attention, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
