@@ -13,50 +13,21 @@
 // what goes beyond a CTA is left in the workspace for kv_join_kernel.
 #include <algorithm>
 
-#include "kv_cache.cuh"
-#include "tensor_core.cuh"
+#include "kv_attention.cuh"
 
 namespace atlas {
 
 namespace {
 
-constexpr float KV_HEADROOM = 8.0f;   // log2: how far a score may pass the running maximum before sums are rescaled
-constexpr float KV_SHIFT = 6.0f;      // log2: p is kept as 2^6 p, up to 2^14 in fp16; what is below 2^-31 of the maximum vanishes
-
-struct Attention {
-    const char *q;               // bytes
-    int64_t q_token_stride, q_head_stride;
-    char *out;
-    const uint8_t *cache;
-    const int32_t *page_table, *lengths, *query_starts;
-    float *partial;
-    int32_t *status;
-    int64_t num_pages, table_stride, max_tokens, total_queries, uniform;
-    int batch, q_heads, kv_heads, group, page_size, window, sinks;   // group: query heads of a kv head
-    float scale_log2;
-    int min_units;               // per warp
-};
-
 // A row tile of a sequence: its queries and the units that they see.
-struct Run {
-    int64_t first_query;         // of the sequence, in q
-    int length, queries;
+struct Run : Sequence {
     int sink_units, window_unit, units;   // units 0 .. sink_units - 1, then window_unit ...
     __device__ __forceinline__ int slab(int u) const { return u < sink_units ? u : u - sink_units + window_unit; }
 };
 
 __device__ __forceinline__ Run make_run(const Attention &a, int b, int row0, int rows) {
     Run r;
-    int64_t q0, q1;
-    if (a.query_starts) {
-        q0 = min(max((int64_t)a.query_starts[b], (int64_t)0), a.total_queries);
-        q1 = min(max((int64_t)a.query_starts[b + 1], q0), a.total_queries);
-    } else {
-        q0 = b * a.uniform, q1 = q0 + a.uniform;
-    }
-    r.first_query = q0;
-    r.queries = (int)(q1 - q0);
-    r.length = (int)min(max((int64_t)a.lengths[b], (int64_t)0), a.max_tokens);
+    static_cast<Sequence &>(r) = sequence(a, b);
     r.sink_units = r.window_unit = r.units = 0;
     const int64_t all = (int64_t)r.queries * a.group;
     if (row0 >= all) return r;
@@ -92,24 +63,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
     return r;
 }
-__device__ __forceinline__ float exp2_fast(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-__device__ __forceinline__ uint32_t h2(__half2 v) { return *reinterpret_cast<uint32_t *>(&v); }
-__device__ __forceinline__ __half2 h2(uint32_t v) { return *reinterpret_cast<__half2 *>(&v); }
-
-// The four pairs of a word of codes, minus the zero point: `bias` is 1024 + z, `bias16` 64 + z.
-__device__ __forceinline__ void open_word(uint32_t w, __half2 bias, __half2 bias16, __half2 (&v)[4]) {
-    const __half2 sixteenth = __float2half2_rn(0.0625f);
-    const uint32_t u = w >> 8;
-    v[0] = __hsub2(h2((w & 0x000f000fu) | 0x64006400u), bias);
-    v[1] = __hfma2(h2((w & 0x00f000f0u) | 0x64006400u), sixteenth, __hneg2(bias16));   // (1024 + 16 c) / 16 - (64 + z)
-    v[2] = __hsub2(h2((u & 0x000f000fu) | 0x64006400u), bias);
-    v[3] = __hfma2(h2((u & 0x00f000f0u) | 0x64006400u), sixteenth, __hneg2(bias16));
-}
-
 template <int D, int NT, int WARPS, int STAGES>
 struct Shape {
     static constexpr int ROWS = 8 * NT, GROUPS = D / 64, WORDS = D / 32;   // words: a lane's, of a token's key
@@ -139,23 +92,6 @@ struct State {
         }
     }
 };
-
-template <bool BF16>
-__device__ __forceinline__ uint2 pack4(float a, float b, float c, float d) {
-    if (BF16) {
-        const __nv_bfloat162 x = __floats2bfloat162_rn(a, b), y = __floats2bfloat162_rn(c, d);
-        return make_uint2(*reinterpret_cast<const uint32_t *>(&x), *reinterpret_cast<const uint32_t *>(&y));
-    }
-    const __half2 x = __floats2half2_rn(a, b), y = __floats2half2_rn(c, d);
-    return make_uint2(*reinterpret_cast<const uint32_t *>(&x), *reinterpret_cast<const uint32_t *>(&y));
-}
-
-// Where a row's output is, or null.
-__device__ __forceinline__ char *out_row(const Attention &a, const Run &r, int h, int row, int d) {
-    const int query = row / a.group;
-    if (query >= r.queries) return nullptr;
-    return a.out + ((r.first_query + query) * a.q_heads + h * a.group + row % a.group) * (int64_t)d * 2;
-}
 
 template <int D, int NT, int WARPS, int STAGES, bool BF16>
 __global__ void __launch_bounds__(WARPS * 32, 1) kv_attention_kernel(const Attention a) {
@@ -669,6 +605,7 @@ extern "C" {
 size_t atlas_kv_attention_workspace_bytes(const AtlasKvAttention *p) {
     using namespace atlas;
     if (check_arguments(p, "atlas_kv_attention_workspace_bytes") != ATLAS_OK) return 0;
+    if (kv_prompt_serves(*p)) return kv_prompt_workspace_bytes(*p);
     const Plan plan = plan_of(*p);
     return (size_t)plan.tiles * sm_count() * 2 * plan.piece_bytes;
 }
@@ -693,9 +630,10 @@ int atlas_kv_attention(const AtlasKvAttention *p, void *stream) {
     if (dev != ATLAS_OK) return dev;
     const Plan plan = plan_of(*p);
     const int ctas = sm_count();
-    ATLAS_RETURN_IF(plan.tiles > 65535, ATLAS_ERR_UNSUPPORTED, "%s: %lld queries in a sequence", what, (long long)p->max_queries);
-    ATLAS_RETURN_IF(!p->workspace || p->workspace_bytes < (size_t)plan.tiles * ctas * 2 * plan.piece_bytes, ATLAS_ERR_CAPACITY, "%s: workspace of %zu bytes",
-                    what, p->workspace_bytes);
+    ATLAS_RETURN_IF(!kv_prompt_serves(*p) && plan.tiles > 65535, ATLAS_ERR_UNSUPPORTED, "%s: %lld queries in a sequence", what, (long long)p->max_queries);
+    const size_t bytes = atlas_kv_attention_workspace_bytes(p);
+    ATLAS_RETURN_IF(bytes && (!p->workspace || p->workspace_bytes < bytes), ATLAS_ERR_CAPACITY, "%s: workspace of %zu bytes, %zu needed", what,
+                    p->workspace_bytes, bytes);
 
     Attention a = {};
     a.q = (const char *)p->q, a.q_token_stride = 2 * p->q_token_stride, a.q_head_stride = 2 * p->q_head_stride;
@@ -710,6 +648,7 @@ int atlas_kv_attention(const AtlasKvAttention *p, void *stream) {
     a.min_units = 1;
     const bool bf16 = p->dtype == ATLAS_DTYPE_BF16;
     cudaStream_t s = (cudaStream_t)stream;
+    if (kv_prompt_serves(*p)) return kv_prompt(a, *p, s);
     switch (p->head_dim) {
         case 64: return bf16 ? launch_nt<64, true>(a, plan, ctas, s) : launch_nt<64, false>(a, plan, ctas, s);
         case 128: return bf16 ? launch_nt<128, true>(a, plan, ctas, s) : launch_nt<128, false>(a, plan, ctas, s);

@@ -1,0 +1,86 @@
+// What the kernels of attention over the 4-bit cache share.
+#pragma once
+#include "kv_cache.cuh"
+#include "tensor_core.cuh"
+
+namespace atlas {
+
+struct Attention {
+    const char *q;               // bytes
+    int64_t q_token_stride, q_head_stride;
+    char *out;
+    const uint8_t *cache;
+    const int32_t *page_table, *lengths, *query_starts;
+    float *partial;
+    int32_t *status;
+    int64_t num_pages, table_stride, max_tokens, total_queries, uniform;
+    int batch, q_heads, kv_heads, group, page_size, window, sinks;   // group: query heads of a kv head
+    float scale_log2;
+    int min_units;               // per warp
+};
+
+// Prompts: kv_prompt.cu.  Bytes of workspace, and the launch.
+bool kv_prompt_serves(const AtlasKvAttention &p);
+size_t kv_prompt_workspace_bytes(const AtlasKvAttention &p);
+int kv_prompt(const Attention &a, const AtlasKvAttention &p, cudaStream_t stream);
+
+namespace {
+
+struct Sequence {
+    int64_t first_query;         // in q
+    int length, queries;
+};
+__device__ __forceinline__ Sequence sequence(const Attention &a, int b) {
+    Sequence r;
+    int64_t q0, q1;
+    if (a.query_starts) {
+        q0 = min(max((int64_t)a.query_starts[b], (int64_t)0), a.total_queries);
+        q1 = min(max((int64_t)a.query_starts[b + 1], q0), a.total_queries);
+    } else {
+        q0 = b * a.uniform, q1 = q0 + a.uniform;
+    }
+    r.first_query = q0;
+    r.queries = (int)(q1 - q0);
+    r.length = (int)min(max((int64_t)a.lengths[b], (int64_t)0), a.max_tokens);
+    return r;
+}
+// Where a row's output is, or null.
+__device__ __forceinline__ char *out_row(const Attention &a, const Sequence &r, int h, int row, int d) {
+    const int query = row / a.group;
+    if (query >= r.queries) return nullptr;
+    return a.out + ((r.first_query + query) * a.q_heads + h * a.group + row % a.group) * (int64_t)d * 2;
+}
+
+constexpr float KV_HEADROOM = 8.0f;   // log2: how far a score may pass the running maximum before sums are rescaled
+constexpr float KV_SHIFT = 6.0f;      // log2: p is kept as 2^6 p, up to 2^14 in fp16; what is below 2^-31 of the maximum vanishes
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ uint32_t h2(__half2 v) { return *reinterpret_cast<uint32_t *>(&v); }
+__device__ __forceinline__ __half2 h2(uint32_t v) { return *reinterpret_cast<__half2 *>(&v); }
+
+// The four pairs of a word of codes, minus the zero point: `bias` is 1024 + z, `bias16` 64 + z.
+__device__ __forceinline__ void open_word(uint32_t w, __half2 bias, __half2 bias16, __half2 (&v)[4]) {
+    const __half2 sixteenth = __float2half2_rn(0.0625f);
+    const uint32_t u = w >> 8;
+    v[0] = __hsub2(h2((w & 0x000f000fu) | 0x64006400u), bias);
+    v[1] = __hfma2(h2((w & 0x00f000f0u) | 0x64006400u), sixteenth, __hneg2(bias16));   // (1024 + 16 c) / 16 - (64 + z)
+    v[2] = __hsub2(h2((u & 0x000f000fu) | 0x64006400u), bias);
+    v[3] = __hfma2(h2((u & 0x00f000f0u) | 0x64006400u), sixteenth, __hneg2(bias16));
+}
+
+template <bool BF16>
+__device__ __forceinline__ uint2 pack4(float a, float b, float c, float d) {
+    if (BF16) {
+        const __nv_bfloat162 x = __floats2bfloat162_rn(a, b), y = __floats2bfloat162_rn(c, d);
+        return make_uint2(*reinterpret_cast<const uint32_t *>(&x), *reinterpret_cast<const uint32_t *>(&y));
+    }
+    const __half2 x = __floats2half2_rn(a, b), y = __floats2half2_rn(c, d);
+    return make_uint2(*reinterpret_cast<const uint32_t *>(&x), *reinterpret_cast<const uint32_t *>(&y));
+}
+
+}  // namespace
+}  // namespace atlas
