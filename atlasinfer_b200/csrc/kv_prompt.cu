@@ -46,6 +46,11 @@ struct Prompt {
 
 constexpr uint32_t pr_idesc(int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24); }
 
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
 __device__ __forceinline__ void store_transposable(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
@@ -211,12 +216,11 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_prompt_kernel(const Attentio
         }
     } else if (warp == PR_MMA) {
         // ------------------------------ MMAs ------------------------------
-        const bool leader = lane == 0;
         const uint64_t dk0 = make_smem_desc(base + P::OFF_K), dv0 = make_smem_desc(base + P::OFF_V);
         bool ok = tiles == 0 || mbar_wait_warp(bar(P::Q_FULL), 0, s_abort);
         auto qk = [&](int j, int tile, int buffer) {   // the address field counts 16-byte units
             const uint64_t dk = dk0 + (uint64_t)((j % KS) * (P::KV_BYTES >> 4));
-            if (leader) {
+            if (elect_one()) {
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k)
                     umma_f16_ts(tmem + P::T_S + buffer * PR_KEYS, tmem + P::T_Q + tile * (D / 2) + k * 8, dk + (uint64_t)((k / 4) * 512 + (k % 4) * 2), pr_idesc(PR_KEYS), k != 0);
@@ -225,13 +229,13 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_prompt_kernel(const Attentio
         };
         auto pv = [&](int j, int tile, int buffer) {
             const uint64_t dv = dv0 + (uint64_t)((j % KS) * (P::KV_BYTES >> 4));
-            if (leader) {
+            if (elect_one()) {
 #pragma unroll
                 for (int k = 0; k < PR_KEYS / 16; ++k)
                     umma_f16_ts(tmem + tile * D, tmem + P::T_S + buffer * PR_KEYS + k * 8, dv + (uint64_t)(k * 2), pr_idesc(D), (j | k) != 0);
             }
         };
-        auto commit = [&](int i) { if (leader) umma_commit(bar(i)); };
+        auto commit = [&](int i) { if (elect_one()) umma_commit(bar(i)); };
         if constexpr (TILES == 2) {
             // S of a row tile is written behind the product that has read P from the same columns: the tensor core works in order
             for (int j = 0; j <= tiles && ok && tiles; ++j) {
