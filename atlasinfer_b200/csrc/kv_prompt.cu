@@ -20,27 +20,27 @@ namespace atlas {
 
 namespace {
 
-constexpr int PR_KEYS = 64, PR_THREADS = 14 * 32;
-constexpr int PR_REBUILD = 8, PR_MMA = 12, PR_LOAD = 13;   // first warps of the roles
+constexpr int PR_THREADS = 16 * 32;
+constexpr int PR_REBUILD = 8, PR_REBUILDERS = 6, PR_MMA = 14, PR_LOAD = 15;   // first warps of the roles
 
 template <int D>
 struct Prompt {
-    static constexpr int TILES = D == 256 ? 1 : 2;
-    static constexpr int ROWS = 128 * TILES;
+    static constexpr int TILES = D == 256 ? 1 : 2, KEYS = D == 256 ? 64 : 128;
+    static constexpr int ROWS = 128 * TILES, SLABS = KEYS / KV_SLAB;
     static constexpr int GROUPS = D / 64, SLAB = kv_slab_bytes(D);
-    static constexpr int KV_BYTES = PR_KEYS * D * 2;        // a K tile: D / 64 subtiles of 64 rows (tokens); a V tile: D rows (channels)
-    static constexpr int KS = D == 256 ? 2 : 3, RS = D == 256 ? 2 : 4;   // stages: rebuilt tiles, raw tiles
-    static constexpr int RAW_BYTES = 4 * SLAB;
-    static constexpr uint32_t OFF_K = 0, OFF_V = OFF_K + KS * KV_BYTES, OFF_RAW = OFF_V + KS * KV_BYTES, OFF_INFO = OFF_RAW + RS * RAW_BYTES;
-    static constexpr uint32_t OFF_BAR = OFF_INFO + 16 * 4;
-    // barriers
-    static constexpr int RAW_FULL = 0, RAW_EMPTY = RAW_FULL + RS, K_FULL = RAW_EMPTY + RS, K_EMPTY = K_FULL + KS, V_FULL = K_EMPTY + KS, V_EMPTY = V_FULL + KS,
-                         S_FULL = V_EMPTY + KS, P_FULL = S_FULL + 2, O_DONE = P_FULL + 2, Q_FULL = O_DONE + 1, DRAIN = Q_FULL + 1,
-                         BARS = DRAIN + 1;
+    static constexpr int Q_BYTES = 128 * D * 2;             // a Q tile: D / 64 subtiles of 128 rows of 128 bytes
+    static constexpr int KV_BYTES = KEYS * D * 2;           // a K tile: D / 64 subtiles of KEYS rows (tokens); a V tile: KEYS / 64 subtiles of D rows (channels)
+    static constexpr int STAGES = 2, RING = D == 64 ? 24 : D == 128 ? 12 : 6;   // rebuilt tiles; halves of slabs, of keys and of values
+    static constexpr int HALF = SLAB / 2;                   // codes, then scales and zero points
+    static constexpr uint32_t OFF_Q = 0, OFF_K = OFF_Q + TILES * Q_BYTES, OFF_V = OFF_K + STAGES * KV_BYTES, OFF_RAW = OFF_V + STAGES * KV_BYTES;
+    static constexpr uint32_t OFF_INFO = OFF_RAW + 2 * RING * HALF, OFF_BAR = OFF_INFO + 16 * 8;
+    // barriers; those of S and of O have a place for each of four tiles in a row, so that who comes late can tell them apart
+    static constexpr int RAW_FULL = 0, RAW_EMPTY = RAW_FULL + 2 * RING, K_FULL = RAW_EMPTY + 2 * RING, V_FULL = K_FULL + STAGES, S_FULL = V_FULL + STAGES,
+                         P_FULL = S_FULL + 8, O_DONE = P_FULL + 2, Q_FULL = O_DONE + 4, DRAIN = Q_FULL + 1, BARS = DRAIN + 1;
     static constexpr uint32_t OFF_TMEM = OFF_BAR + BARS * 8, TOTAL = OFF_TMEM + 16 + 1024 /* alignment */;
-    // columns of tensor memory: O, then S (P over it), then Q
-    static constexpr uint32_t T_S = TILES * D, T_Q = T_S + 2 * PR_KEYS, T_COLS = 512;
-    static_assert(T_Q + TILES * D / 2 <= T_COLS, "tensor memory");
+    // columns of tensor memory: O, then S (P over it)
+    static constexpr uint32_t T_S = TILES * D, T_COLS = 512;
+    static_assert(T_S + 256 <= T_COLS, "tensor memory");
     static_assert(TOTAL <= 227 * 1024, "shared memory");
 };
 
@@ -54,42 +54,75 @@ __device__ __forceinline__ bool elect_one() {
 __device__ __forceinline__ void store_transposable(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
+__device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+        ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+          "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        : "memory");
+}
+// Pairs of fp32 numbers, one instruction for both.
+using f32x2 = uint64_t;
+__device__ __forceinline__ f32x2 pair(float lo, float hi) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void unpair(f32x2 v, float &lo, float &hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// The lowest n bits.
+__device__ __forceinline__ uint32_t first_bits(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
+// A wait of a whole (converged) warp: one poll where the phase is over already.
+template <int NS = 0>
+__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, const volatile int *abort_flag) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    return mbar_wait_warp<NS>(bar, parity, abort_flag);
+}
 
-// The tiles of 64 tokens that rows p0 .. p1 (positions) see.
+// The tiles of tokens that rows at positions up to p1 see, the first of them at p0.
+template <int KEYS>
 struct Walk {
     int p1, window_start, sinks, window_tile, sink_tiles, tiles;
+    __device__ __forceinline__ Walk(const Attention &a, int p0, int p1) : p1(p1), window_start(0), sinks(0), window_tile(0), sink_tiles(0), tiles(0) {
+        if (p1 < 0) return;
+        if (a.window) {
+            window_start = max(0, p0 - a.window + 1);
+            sinks = min(a.sinks, p1 + 1);
+            window_tile = window_start / KEYS;
+            sink_tiles = min((sinks + KEYS - 1) / KEYS, window_tile);
+        }
+        tiles = sink_tiles + p1 / KEYS + 1 - window_tile;
+    }
     __device__ __forceinline__ int tile(int j) const { return j < sink_tiles ? j : j - sink_tiles + window_tile; }
     // whether a slab has a token that some row sees
     __device__ __forceinline__ bool slab_seen(int s) const { return s * KV_SLAB <= p1 && (s * KV_SLAB + KV_SLAB > window_start || s * KV_SLAB < sinks); }
 };
-__device__ __forceinline__ Walk make_walk(const Attention &a, int p0, int p1) {
-    Walk w = {p1, 0, 0, 0, 0, 0};
-    if (p1 < 0) return w;
-    if (a.window) {
-        w.window_start = max(0, p0 - a.window + 1);
-        w.sinks = min(a.sinks, p1 + 1);
-        w.window_tile = w.window_start / PR_KEYS;
-        w.sink_tiles = min((w.sinks + PR_KEYS - 1) / PR_KEYS, w.window_tile);
-    }
-    w.tiles = w.sink_tiles + p1 / PR_KEYS + 1 - w.window_tile;
-    return w;
-}
 
 template <int D, bool BF16>
 __global__ void __launch_bounds__(PR_THREADS, 1) kv_prompt_kernel(const Attention a, int splits) {
     using P = Prompt<D>;
-    constexpr int KS = P::KS, RS = P::RS, TILES = P::TILES;
+    constexpr int TILES = P::TILES, KEYS = P::KEYS, SLABS = P::SLABS, STAGES = P::STAGES, RING = P::RING;
     extern __shared__ uint8_t smem_raw[];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
-    const int b = blockIdx.z / splits, split = blockIdx.z % splits, head = blockIdx.y;
-    // later rows see more: they go first
-    const int row0 = (int)(gridDim.x - 1 - blockIdx.x) * P::ROWS;
+    const int head = blockIdx.x % a.kv_heads, b = blockIdx.x / a.kv_heads / splits, split = blockIdx.x / a.kv_heads % splits;
+    // later rows see more: those of all heads and sequences go first
+    const int row0 = (int)(gridDim.y - 1 - blockIdx.y) * P::ROWS;
     const Sequence seq = sequence(a, b);
     const int rows = (int)min((int64_t)P::ROWS, (int64_t)seq.queries * a.group - row0);
     if (rows <= 0) return;
+    const int used = TILES == 2 && rows > 128 ? 2 : 1;   // row tiles with rows
     const int p_first = seq.length - seq.queries + row0 / a.group, p_last = seq.length - seq.queries + (row0 + rows - 1) / a.group;
-    const Walk walk = make_walk(a, p_first, p_last);
+    const Walk<KEYS> walk(a, p_first, p_last);
     const int j0 = (int)((int64_t)walk.tiles * split / splits), tiles = (int)((int64_t)walk.tiles * (split + 1) / splits) - j0;
 
     const uint32_t raw_base = smem_u32(smem_raw), base = (raw_base + 1023u) & ~1023u;
@@ -97,18 +130,17 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_prompt_kernel(const Attentio
     auto bar = [&](int i) { return base + P::OFF_BAR + 8u * (uint32_t)i; };
     volatile uint32_t *const tmem_slot = reinterpret_cast<volatile uint32_t *>(sm + P::OFF_TMEM);
     volatile int *const s_abort = reinterpret_cast<volatile int *>(sm + P::OFF_TMEM + 8);
-    volatile uint32_t *const info = reinterpret_cast<volatile uint32_t *>(sm + P::OFF_INFO);   // slabs of a tile that are not there
+    volatile uint8_t *const gone = sm + P::OFF_INFO;   // [tile % 16][slab]: whether the slab is not there
 
     if (tid == 0) {
-        for (int i = 0; i < RS; ++i) mbar_init(bar(P::RAW_FULL + i), 1), mbar_init(bar(P::RAW_EMPTY + i), 4);
-        for (int i = 0; i < KS; ++i) {
-            mbar_init(bar(P::K_FULL + i), 4), mbar_init(bar(P::K_EMPTY + i), 1);
-            mbar_init(bar(P::V_FULL + i), 4), mbar_init(bar(P::V_EMPTY + i), 1);
-        }
-        for (int i = 0; i < 2; ++i) mbar_init(bar(P::S_FULL + i), 1), mbar_init(bar(P::P_FULL + i), 4);
-        mbar_init(bar(P::O_DONE), 1);
+        for (int i = 0; i < 2 * RING; ++i) mbar_init(bar(P::RAW_FULL + i), 1), mbar_init(bar(P::RAW_EMPTY + i), 1);
+        for (int i = 0; i < STAGES; ++i) mbar_init(bar(P::K_FULL + i), SLABS), mbar_init(bar(P::V_FULL + i), SLABS);
+        for (int i = 0; i < 8; ++i) mbar_init(bar(P::S_FULL + i), 1);
+        for (int i = 0; i < 2; ++i) mbar_init(bar(P::P_FULL + i), 4);
+        for (int i = 0; i < 4; ++i) mbar_init(bar(P::O_DONE + i), 1);
         mbar_init(bar(P::Q_FULL), 4 * TILES);
         mbar_init(bar(P::DRAIN), 1);
+        for (int i = 0; i < 16; ++i) reinterpret_cast<volatile uint64_t *>(gone)[i] = 0;
         *s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -120,250 +152,294 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_prompt_kernel(const Attentio
     __syncthreads();
     tcgen05_fence_after();
     const uint32_t tmem = *tmem_slot;
-    int issued = 0;              // raw tiles asked for (loader), MMA groups committed (MMA warp)
+    int issued = 0;              // tiles whose half slab this lane has asked for (loader)
+    // S of row tile i (two row tiles), or into buffer j % 2 (one)
+    auto s_full = [&](int i, int j) { return bar(P::S_FULL + (TILES == 2 ? 4 * i : 0) + j % 4); };
+    auto s_parity = [&](int j) { return (uint32_t)((j / 4) & 1); };
 
     if (warp == PR_LOAD) {
         // ------------------------------ slabs ------------------------------
-        int pages = -1;          // lane i: page of slab i % 4 of tile i / 4 of this batch of 8 tiles
-        bool pages_seen = false;
-        for (int j = 0; j < tiles; ++j) {
-            if (j % 8 == 0) {
-                const int jj = j + lane / 4, s = walk.tile(j0 + jj) * 4 + lane % 4;
-                pages_seen = jj < tiles && walk.slab_seen(s);
-                pages = pages_seen ? a.page_table[b * a.table_stride + s * KV_SLAB / a.page_size] : -1;
+        // Lane i brings the keys of slab i of every tile, lane 16 + i the values, each as far ahead as its ring has room.
+        const int slab = lane % 16, part = lane / 16;
+        const bool mine = slab < SLABS;
+        auto page_of = [&](int j) {
+            const int s = walk.tile(j0 + j) * SLABS + slab;
+            return j < tiles && walk.slab_seen(s) ? a.page_table[b * a.table_stride + s * KV_SLAB / a.page_size] : -1;
+        };
+        int page = mine ? page_of(0) : -1, idle = 0;
+        int slot = part * RING + slab, round = 0;   // the half slab's place, and how often the ring has gone round
+        while (true) {
+            const bool go = mine && issued < tiles && (round == 0 || mbar_try_wait(bar(P::RAW_EMPTY + slot), (uint32_t)((round - 1) & 1)));
+            if (go) {
+                const bool there = page >= 0 && page < a.num_pages;
+                gone[issued % 16 * 8 + slab] = !there;
+                mbar_arrive_expect_tx(bar(P::RAW_FULL + slot), there ? P::HALF : 0);
+                if (there) {
+                    const int token = (walk.tile(j0 + issued) * SLABS + slab) * KV_SLAB;
+                    const uint8_t *src = a.cache + (((int64_t)page * a.kv_heads + head) * (a.page_size / KV_SLAB) + token % a.page_size / KV_SLAB) * P::SLAB;
+                    const uint32_t dst = base + P::OFF_RAW + slot * P::HALF;
+                    bulk_load_1d(dst, src + part * kv_value_codes(D), 8 * D, bar(P::RAW_FULL + slot));
+                    bulk_load_1d(dst + 8 * D, src + (part ? kv_value_params(D) : kv_key_params(D)), D, bar(P::RAW_FULL + slot));
+                }
+                page = page_of(++issued);
+                slot += SLABS;
+                if (slot >= (part + 1) * RING) slot -= RING, ++round;
             }
-            const int stage = j % RS;
-            if (j >= RS && !mbar_wait_warp<20>(bar(P::RAW_EMPTY + stage), (uint32_t)((j / RS - 1) & 1), s_abort)) { *s_abort = 1; break; }
-            const int from = (j % 8) * 4 + lane % 4, page = __shfl_sync(0xffffffffu, pages, from);
-            const bool there = page >= 0 && page < a.num_pages;
-            const uint32_t present = __ballot_sync(0xffffffffu, there && lane < 4);
-            if (lane == 0) {
-                info[j % 16] = ~present & 15u;
-                mbar_arrive_expect_tx(bar(P::RAW_FULL + stage), (uint32_t)__popc(present) * P::SLAB);
+            if (!__any_sync(0xffffffffu, mine && issued < tiles)) break;
+            if (__any_sync(0xffffffffu, go)) {
+                idle = 0;
+            } else {
+                if (++idle > SPIN_LIMIT) *s_abort = 1;
+                if (__any_sync(0xffffffffu, *s_abort != 0)) break;
+                __nanosleep(100);
             }
-            __syncwarp();
-            if (lane < 4 && there) {
-                const int token = (walk.tile(j0 + j) * 4 + lane) * KV_SLAB;
-                const uint8_t *src = a.cache + (((int64_t)page * a.kv_heads + head) * (a.page_size / KV_SLAB) + token % a.page_size / KV_SLAB) * P::SLAB;
-                bulk_load_1d(base + P::OFF_RAW + stage * P::RAW_BYTES + lane * P::SLAB, src, P::SLAB, bar(P::RAW_FULL + stage));
-            }
-            issued = j + 1;
         }
     } else if (warp >= PR_REBUILD && warp < PR_MMA) {
-        // ------------------------------ codes to fp16 ------------------------------
-        const int slab = warp - PR_REBUILD, g = lane / 4, t = lane % 4;
-        const int spread = (g & 1) * 4 + g / 2;   // eight lanes that store at a time: rows 4 apart, so that the swizzle keeps them apart
-        for (int j = 0; j < tiles; ++j) {
-            const int rs = j % RS, ks = j % KS;
-            if (!mbar_wait_warp<20>(bar(P::RAW_FULL + rs), (uint32_t)((j / RS) & 1), s_abort)) { *s_abort = 1; break; }
-            const uint8_t *src = sm + P::OFF_RAW + rs * P::RAW_BYTES + slab * P::SLAB;
-            const bool absent = (info[j % 16] >> slab) & 1;
-            const int token0 = walk.tile(j0 + j) * PR_KEYS + slab * KV_SLAB;
-            if (j >= KS && !mbar_wait_warp<20>(bar(P::K_EMPTY + ks), (uint32_t)((j / KS - 1) & 1), s_abort)) { *s_abort = 1; break; }
-            uint8_t *const kt = sm + P::OFF_K + ks * P::KV_BYTES;
+        // ------------------------------ codes to fp16: a warp a slab, half of the warps keys, half values ------------------------------
+        const int g = lane / 4, t = lane % 4;
+        const bool keys = warp < PR_REBUILD + PR_REBUILDERS / 2;
+        const __half2 off = __float2half2_rn(960.0f);
+        uint2 w[2][P::GROUPS];   // of both halves of the slab: codes, then scales and zero points
+        for (int n = (warp - PR_REBUILD) % (PR_REBUILDERS / 2); n < tiles * SLABS; n += PR_REBUILDERS / 2) {
+            const int j = n / SLABS, slab = n % SLABS, slot = (keys ? 0 : RING) + n % RING, st = j % STAGES;
+            if (!wait_warp<20>(bar(P::RAW_FULL + slot), (uint32_t)((n / RING) & 1), s_abort)) { *s_abort = 1; break; }
+            const uint8_t *src = sm + P::OFF_RAW + slot * P::HALF;
+            if (keys) {
+                const int spread = (g & 1) * 4 + g / 2;   // eight lanes that store at a time: rows 4 apart, so that the swizzle keeps them apart
+                __half2 sb[2][P::GROUPS];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int token = 8 * h + spread, row = slab * KV_SLAB + token;
+                for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int gr = 0; gr < P::GROUPS; ++gr) {
-                    const __half2 sb = *reinterpret_cast<const __half2 *>(src + kv_key_params(D) + (token * P::GROUPS + gr) * 4);
-                    const __half2 s = __low2half2(sb), bias = __high2half2(sb), bias16 = __hsub2(bias, __float2half2_rn(960.0f));
-                    const uint2 w = *reinterpret_cast<const uint2 *>(src + kv_key_word(D, token, t + 8 * gr));
+                    for (int gr = 0; gr < P::GROUPS; ++gr) {
+                        w[h][gr] = *reinterpret_cast<const uint2 *>(src + kv_key_word(D, 8 * h + spread, t + 8 * gr));
+                        sb[h][gr] = *reinterpret_cast<const __half2 *>(src + 8 * D + ((8 * h + spread) * P::GROUPS + gr) * 4);
+                    }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(P::RAW_EMPTY + slot));
+                // the products with the K of this place are done with the last S made of it
+                if (j >= STAGES && !wait_warp<20>(s_full(used - 1, j - STAGES), s_parity(j - STAGES), s_abort)) { *s_abort = 1; break; }
+                uint8_t *const kt = sm + P::OFF_K + st * P::KV_BYTES;
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        __half2 v[4];
-                        open_word(i ? w.y : w.x, bias, bias16, v);
-                        *reinterpret_cast<uint4 *>(kt + gr * 8192 + row * 128 + (((4 * i + t) ^ (row & 7)) << 4)) =
-                            make_uint4(h2(__hmul2(v[0], s)), h2(__hmul2(v[1], s)), h2(__hmul2(v[2], s)), h2(__hmul2(v[3], s)));
+                for (int h = 0; h < 2; ++h) {
+                    const int row = slab * KV_SLAB + 8 * h + spread;
+#pragma unroll
+                    for (int gr = 0; gr < P::GROUPS; ++gr) {
+                        const __half2 s = __low2half2(sb[h][gr]), bias = __high2half2(sb[h][gr]), bias16 = __hsub2(bias, off);
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            __half2 v[4];
+                            open_word(i ? w[h][gr].y : w[h][gr].x, bias, bias16, v);
+                            *reinterpret_cast<uint4 *>(kt + gr * KEYS * 128 + row * 128 + (((4 * i + t) ^ (row & 7)) << 4)) =
+                                make_uint4(h2(__hmul2(v[0], s)), h2(__hmul2(v[1], s)), h2(__hmul2(v[2], s)), h2(__hmul2(v[3], s)));
+                        }
                     }
                 }
+            } else {
+                uint2 sb[2][P::GROUPS];
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int gr = 0; gr < P::GROUPS; ++gr) {
+                        w[h][gr] = *reinterpret_cast<const uint2 *>(src + kv_value_unit(D, 8 * h + 2 * t, g + 16 * gr));
+                        sb[h][gr] = *reinterpret_cast<const uint2 *>(src + 8 * D + ((4 * h + t) * P::GROUPS + gr) * 8);
+                    }
+                const bool absent = gone[j % 16 * 8 + slab];
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(P::RAW_EMPTY + slot));
+                const int token0 = walk.tile(j0 + j) * KEYS + slab * KV_SLAB;
+                if (absent || token0 + KV_SLAB > seq.length) {
+                    // tokens that are not there may hold anything: zeros (their weights are zero too, but not times NaN)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int token = token0 + 8 * h + 2 * t;
+                        const uint32_t keep = absent ? 0u : (token < seq.length ? 0xffffu : 0u) | (token + 1 < seq.length ? 0xffff0000u : 0u);
+#pragma unroll
+                        for (int gr = 0; gr < P::GROUPS; ++gr) sb[h][gr].x &= keep, sb[h][gr].y = (sb[h][gr].y & keep) | (0x64006400u & ~keep);
+                    }
+                }
+                // the product with the V of this place is done with the S after it (with one row tile: it says so itself)
+                if (j >= STAGES) {
+                    const bool ok = TILES == 2 ? wait_warp<20>(s_full(used - 1, j - STAGES + 1), s_parity(j - STAGES + 1), s_abort)
+                                               : wait_warp<20>(bar(P::O_DONE + (j - STAGES) % 4), s_parity(j - STAGES), s_abort);
+                    if (!ok) { *s_abort = 1; break; }
+                }
+                const uint32_t vt = base + P::OFF_V + st * P::KV_BYTES + (slab / 4) * (D * 128);
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int gr = 0; gr < P::GROUPS; ++gr) {
+                        const __half2 s = h2(sb[h][gr].x), bias = h2(sb[h][gr].y), bias16 = __hsub2(bias, off);
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            __half2 v[4];
+                            open_word(i ? w[h][gr].y : w[h][gr].x, bias, bias16, v);
+                            // row 32 j + 8 p + g of the tile is channel 32 j + 4 g + p: eight neighbouring rows a matrix
+                            store_transposable(vt + (uint32_t)((32 * (2 * gr + i) + lane) * 128 + (((2 * (slab % 4) + h) ^ (lane & 7)) << 4)), h2(__hmul2(v[0], s)),
+                                               h2(__hmul2(v[1], s)), h2(__hmul2(v[2], s)), h2(__hmul2(v[3], s)));
+                        }
+                    }
             }
             fence_async_smem();
             __syncwarp();
-            if (lane == 0) mbar_arrive(bar(P::K_FULL + ks));
-            if (j >= KS && !mbar_wait_warp<20>(bar(P::V_EMPTY + ks), (uint32_t)((j / KS - 1) & 1), s_abort)) { *s_abort = 1; break; }
-            const uint32_t vt = base + P::OFF_V + ks * P::KV_BYTES;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                // tokens that are not there may hold anything: zeros (their weights are zero too, but not times NaN)
-                uint32_t keep = 0xffffffffu;
-                const int token = token0 + 8 * h + 2 * t;
-                if (absent || token0 + KV_SLAB > seq.length)
-                    keep = absent ? 0u : (token < seq.length ? 0xffffu : 0u) | (token + 1 < seq.length ? 0xffff0000u : 0u);
-#pragma unroll
-                for (int gr = 0; gr < P::GROUPS; ++gr) {
-                    uint2 sb = *reinterpret_cast<const uint2 *>(src + kv_value_params(D) + ((4 * h + t) * P::GROUPS + gr) * 8);
-                    sb.x &= keep;
-                    sb.y = (sb.y & keep) | (0x64006400u & ~keep);
-                    const __half2 s = h2(sb.x), bias = h2(sb.y), bias16 = __hsub2(bias, __float2half2_rn(960.0f));
-                    const uint2 w = *reinterpret_cast<const uint2 *>(src + kv_value_codes(D) + kv_value_unit(D, 8 * h + 2 * t, g + 16 * gr));
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        __half2 v[4];
-                        open_word(i ? w.y : w.x, bias, bias16, v);
-                        // row 32 j + 8 p + g of the tile is channel 32 j + 4 g + p: eight neighbouring rows a matrix
-                        store_transposable(vt + (uint32_t)((32 * (2 * gr + i) + lane) * 128 + (((2 * slab + h) ^ (lane & 7)) << 4)), h2(__hmul2(v[0], s)), h2(__hmul2(v[1], s)),
-                                           h2(__hmul2(v[2], s)), h2(__hmul2(v[3], s)));
-                    }
-                }
-            }
-            fence_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(bar(P::V_FULL + ks));
-                mbar_arrive(bar(P::RAW_EMPTY + rs));
-            }
+            if (lane == 0) mbar_arrive(bar((keys ? P::K_FULL : P::V_FULL) + st));
         }
     } else if (warp == PR_MMA) {
         // ------------------------------ MMAs ------------------------------
-        const uint64_t dk0 = make_smem_desc(base + P::OFF_K), dv0 = make_smem_desc(base + P::OFF_V);
-        bool ok = tiles == 0 || mbar_wait_warp(bar(P::Q_FULL), 0, s_abort);
+        const uint64_t dq0 = make_smem_desc(base + P::OFF_Q), dk0 = make_smem_desc(base + P::OFF_K), dv0 = make_smem_desc(base + P::OFF_V);
+        bool ok = tiles == 0 || wait_warp(bar(P::Q_FULL), 0, s_abort);
         auto qk = [&](int j, int tile, int buffer) {   // the address field counts 16-byte units
-            const uint64_t dk = dk0 + (uint64_t)((j % KS) * (P::KV_BYTES >> 4));
+            const uint64_t dk = dk0 + (uint64_t)((j % STAGES) * (P::KV_BYTES >> 4)), dq = dq0 + (uint64_t)(tile * (P::Q_BYTES >> 4));
+            const uint32_t d = tmem + P::T_S + buffer * KEYS, done = s_full(tile, j);
             if (elect_one()) {
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k)
-                    umma_f16_ts(tmem + P::T_S + buffer * PR_KEYS, tmem + P::T_Q + tile * (D / 2) + k * 8, dk + (uint64_t)((k / 4) * 512 + (k % 4) * 2), pr_idesc(PR_KEYS), k != 0);
-                umma_commit(bar(P::S_FULL + buffer));
+                    umma_f16_ss(d, dq + (uint64_t)((k / 4) * 1024 + (k % 4) * 2), dk + (uint64_t)((k / 4) * (KEYS * 8) + (k % 4) * 2), pr_idesc(KEYS), k != 0);
+                umma_commit(done);
             }
         };
         auto pv = [&](int j, int tile, int buffer) {
-            const uint64_t dv = dv0 + (uint64_t)((j % KS) * (P::KV_BYTES >> 4));
+            const uint64_t dv = dv0 + (uint64_t)((j % STAGES) * (P::KV_BYTES >> 4));
+            const uint32_t d = tmem + tile * D, p = tmem + P::T_S + buffer * KEYS;
             if (elect_one()) {
 #pragma unroll
-                for (int k = 0; k < PR_KEYS / 16; ++k)
-                    umma_f16_ts(tmem + tile * D, tmem + P::T_S + buffer * PR_KEYS + k * 8, dv + (uint64_t)(k * 2), pr_idesc(D), (j | k) != 0);
+                for (int k = 0; k < KEYS / 16; ++k)
+                    umma_f16_ts(d, p + k * 8, dv + (uint64_t)((k / 4) * (D * 8) + (k % 4) * 2), pr_idesc(D), k != 0 ? 1u : (uint32_t)(j != 0));
             }
         };
-        auto commit = [&](int i) { if (elect_one()) umma_commit(bar(i)); };
+        auto commit = [&](uint32_t at) { if (elect_one()) umma_commit(at); };
         if constexpr (TILES == 2) {
             // S of a row tile is written behind the product that has read P from the same columns: the tensor core works in order
             for (int j = 0; j <= tiles && ok && tiles; ++j) {
-                if (j < tiles) ok = mbar_wait_warp(bar(P::K_FULL + j % KS), (uint32_t)((j / KS) & 1), s_abort);
-                if (ok && j > 0) ok = mbar_wait_warp(bar(P::V_FULL + (j - 1) % KS), (uint32_t)(((j - 1) / KS) & 1), s_abort);
-                for (int i = 0; i < 2 && ok; ++i) {
-                    if (j > 0) {
-                        ok = mbar_wait_warp(bar(P::P_FULL + i), (uint32_t)((j - 1) & 1), s_abort);
-                        if (!ok) break;
-                        tcgen05_fence_after();
-                        pv(j - 1, i, i);
-                    } else {
-                        tcgen05_fence_after();
-                    }
+                if (j < tiles) ok = wait_warp(bar(P::K_FULL + j % STAGES), (uint32_t)((j / STAGES) & 1), s_abort);
+                if (ok && j > 0) ok = wait_warp(bar(P::V_FULL + (j - 1) % STAGES), (uint32_t)(((j - 1) / STAGES) & 1), s_abort);
+                for (int i = 0; i < used && ok; ++i) {
+                    if (j > 0) ok = wait_warp(bar(P::P_FULL + i), (uint32_t)((j - 1) & 1), s_abort);
+                    if (!ok) break;
+                    tcgen05_fence_after();
+                    if (j > 0) pv(j - 1, i, i);
                     if (j < tiles) qk(j, i, i);
                 }
-                if (ok && j > 0) commit(P::V_EMPTY + (j - 1) % KS);
-                if (ok && j < tiles) commit(P::K_EMPTY + j % KS);
-                __syncwarp();
             }
-            if (ok && tiles) commit(P::O_DONE);
+            if (ok && tiles) commit(bar(P::O_DONE));
         } else {
             for (int j = -1; j < tiles && ok && tiles; ++j) {
                 if (j + 1 < tiles) {
-                    ok = mbar_wait_warp(bar(P::K_FULL + (j + 1) % KS), (uint32_t)(((j + 1) / KS) & 1), s_abort);
+                    ok = wait_warp(bar(P::K_FULL + (j + 1) % STAGES), (uint32_t)(((j + 1) / STAGES) & 1), s_abort);
                     if (!ok) break;
                     tcgen05_fence_after();
                     qk(j + 1, 0, (j + 1) & 1);
-                    commit(P::K_EMPTY + (j + 1) % KS);
                 }
                 if (j >= 0) {
-                    ok = mbar_wait_warp(bar(P::V_FULL + j % KS), (uint32_t)((j / KS) & 1), s_abort) &&
-                         mbar_wait_warp(bar(P::P_FULL + (j & 1)), (uint32_t)((j / 2) & 1), s_abort);
+                    ok = wait_warp(bar(P::V_FULL + j % STAGES), (uint32_t)((j / STAGES) & 1), s_abort) &&
+                         wait_warp(bar(P::P_FULL + (j & 1)), (uint32_t)((j / 2) & 1), s_abort);
                     if (!ok) break;
                     tcgen05_fence_after();
                     pv(j, 0, j & 1);
-                    commit(P::V_EMPTY + j % KS);
-                    commit(P::O_DONE);
+                    commit(bar(P::O_DONE + j % 4));
                 }
-                __syncwarp();
             }
         }
         if (!ok) *s_abort = 1;
     } else if (warp < 4 * TILES) {
+        // ------------------------------ Q: each warp its own rows ------------------------------
+        constexpr int LANES = D / 8, PER = 32 / LANES;   // lanes of a row, rows at a time
+        const int tile = warp / 4;
+        float factor = fabsf(a.scale_log2);
+        {
+            const int piece = lane % LANES, sub = lane / LANES;
+            const uint32_t flip = a.scale_log2 < 0.0f ? 0x80008000u : 0u;   // a negative scale turns the queries round: maxima of scores are maxima of products
+            uint8_t *const qt = sm + P::OFF_Q + tile * P::Q_BYTES + (piece / 8) * (128 * 128);
+#pragma unroll 1
+            for (int r0 = 0; r0 < 32; r0 += 4 * PER) {
+                uint4 v[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int in_block = warp * 32 + r0 + u * PER + sub, row = row0 + in_block, query = row / a.group;
+                    v[u] = in_block < rows ? *reinterpret_cast<const uint4 *>(a.q + (seq.first_query + query) * a.q_token_stride +
+                                                                             (head * a.group + row % a.group) * a.q_head_stride + piece * 16)
+                                           : make_uint4(0, 0, 0, 0);
+                }
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    uint32_t w[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+                    if (BF16) {
+                        // times a power of two, so that the largest is in [1, 2): exact, but for numbers below 2^-14 of it,
+                        // which are off by 2^-25 of it at most
+                        float top = 0.0f;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) top = fmaxf(top, fmaxf(fabsf(__uint_as_float(w[k] << 16)), fabsf(__uint_as_float(w[k] & 0xffff0000u))));
+#pragma unroll
+                        for (int k = 1; k < LANES; k *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+                        const int ex = min(max((__float_as_int(top) >> 23) & 0xff, 8), 246);
+                        const float down = __int_as_float((254 - ex) << 23), up = __int_as_float(ex << 23);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) w[k] = h2(__floats2half2_rn(__uint_as_float(w[k] << 16) * down, __uint_as_float(w[k] & 0xffff0000u) * down));
+                        // (each lane keeps the factor of the row that it will have)
+                        const int mine = lane - (r0 + u * PER);
+                        const float got = __shfl_sync(0xffffffffu, up, mine >= 0 && mine < PER ? mine * LANES : 0);
+                        if (mine >= 0 && mine < PER) factor *= got;
+                    }
+                    const int r = (warp % 4) * 32 + r0 + u * PER + sub;
+                    *reinterpret_cast<uint4 *>(qt + r * 128 + (((piece % 8) ^ (r & 7)) << 4)) = make_uint4(w[0] ^ flip, w[1] ^ flip, w[2] ^ flip, w[3] ^ flip);
+                }
+            }
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(P::Q_FULL));
+        }
+        factor = fmaxf(factor, 1e-30f);   // (of a scale of zero: masked scores stay -inf)
+
         // ------------------------------ softmax: a thread a row ------------------------------
-        const int tile = warp / 4, in_block = tid, row = row0 + in_block, query = row / a.group;
+        const int in_block = tid, row = row0 + in_block, query = row / a.group;
         const uint32_t lanes = (uint32_t)((warp % 4) * 32) << 16;
         const bool live = in_block < rows;
         const int place = live ? seq.length - seq.queries + query : -1;
         // first and last position of this row tile, for tiles that need no mask
         const int t_first = seq.length - seq.queries + (row0 + tile * 128) / a.group;
         const int t_last = min(p_last, seq.length - seq.queries + (row0 + tile * 128 + 127) / a.group);
-        float factor = a.scale_log2;
-        {
-            const char *src = a.q + (seq.first_query + query) * a.q_token_stride + (head * a.group + row % a.group) * a.q_head_stride;
-            float down = 1.0f;
-            if (BF16) {
-                // times a power of two, so that the largest is in [1, 2): exact, but for numbers below 2^-14 of it, which
-                // are off by 2^-25 of it at most
-                float top = 0.0f;
-                if (live)
-#pragma unroll 4
-                    for (int i = 0; i < D / 8; ++i) {
-                        const uint4 v = *reinterpret_cast<const uint4 *>(src + i * 16);
-                        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) top = fmaxf(top, fmaxf(fabsf(__uint_as_float(w[k] << 16)), fabsf(__uint_as_float(w[k] & 0xffff0000u))));
-                    }
-                const int ex = min(max((__float_as_int(top) >> 23) & 0xff, 8), 246);
-                down = __int_as_float((254 - ex) << 23);
-                factor *= __int_as_float(ex << 23);
-            }
-            // a negative scale turns the queries round, so that maxima of scores are maxima of products
-            const uint32_t flip = factor < 0.0f ? 0x80008000u : 0u;
-            factor = fmaxf(fabsf(factor), 1e-30f);
-#pragma unroll
-            for (int c = 0; c < D / 64; ++c) {
-                uint32_t q[32];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const uint4 v = live ? *reinterpret_cast<const uint4 *>(src + c * 128 + i * 16) : make_uint4(0, 0, 0, 0);
-                    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        q[4 * i + k] = flip ^ (BF16 ? h2(__floats2half2_rn(__uint_as_float(w[k] << 16) * down, __uint_as_float(w[k] & 0xffff0000u) * down)) : w[k]);
-                }
-                tmem_st_32x32b_x32(tmem + lanes + P::T_Q + tile * (D / 2) + c * 32, q);
-            }
-            tmem_st_wait();
-            tcgen05_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar(P::Q_FULL));
-        }
-
         float m = -INFINITY, l = 0.0f;
         bool ok = true;
-        for (int j = 0; j < tiles; ++j) {
-            const int buffer = TILES == 2 ? tile : j & 1, turn = TILES == 2 ? j : j / 2;
-            if (!mbar_wait_warp(bar(P::S_FULL + buffer), (uint32_t)(turn & 1), s_abort)) { ok = false; break; }
+        for (int j = 0; j < tiles && tile < used; ++j) {
+            const int buffer = TILES == 2 ? tile : j & 1;
+            if (!wait_warp(s_full(tile, j), s_parity(j), s_abort)) { ok = false; break; }
             tcgen05_fence_after();
-            const uint32_t ts = tmem + lanes + P::T_S + buffer * PR_KEYS;
-            uint32_t s0[32], s1[32];
-            tmem_ld_32x32b_x32(ts, s0);
-            tmem_ld_32x32b_x32(ts + 32, s1);
-            tmem_ld_wait();
-            const int token0 = walk.tile(j0 + j) * PR_KEYS;
-            const uint32_t absent = info[j % 16];
-            if (absent || token0 + PR_KEYS - 1 > t_first || (a.window && token0 <= t_last - a.window && token0 + PR_KEYS > a.sinks)) {
+            const uint32_t ts = tmem + lanes + P::T_S + buffer * KEYS;
+            const int token0 = walk.tile(j0 + j) * KEYS;
+            const uint64_t absent = reinterpret_cast<volatile uint64_t *>(gone)[j % 16];   // a byte a slab
+            const bool masked = absent || token0 + KEYS - 1 > t_first || (a.window && token0 <= t_last - a.window && token0 + KEYS > a.sinks);
+            // the maximum; where tokens are hidden, -inf goes back
+            float tops[2] = {-INFINITY, -INFINITY};
+            {
+                uint32_t s[2][32];
+                tmem_ld_32x32b_x32(ts, s[0]);
 #pragma unroll
-                for (int i = 0; i < PR_KEYS; ++i) {
-                    const int token = token0 + i;
-                    const bool hidden = token > place || (a.window && token <= place - a.window && token >= a.sinks) || ((absent >> (i / KV_SLAB)) & 1);
-                    if (hidden) (i < 32 ? s0[i % 32] : s1[i % 32]) = 0xff800000u;
+                for (int c = 0; c < KEYS / 32; ++c) {
+                    tmem_ld_wait();
+                    if (c + 1 < KEYS / 32) tmem_ld_32x32b_x32(ts + 32 * (c + 1), s[(c + 1) & 1]);
+                    uint32_t (&v)[32] = s[c & 1];
+                    if (masked) {
+                        const int t0 = token0 + 32 * c;
+                        uint32_t seen = first_bits(place + 1 - t0);
+                        if (a.window) seen &= ~first_bits(place - a.window + 1 - t0) | first_bits(a.sinks - t0);
+                        if ((absent >> (16 * c)) & 0xff) seen &= 0xffff0000u;
+                        if ((absent >> (16 * c + 8)) & 0xff) seen &= 0x0000ffffu;
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] = (seen >> i) & 1 ? v[i] : 0xff800000u;
+                        tmem_st_32x32b_x32(ts + 32 * c, v);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) tops[i & 1] = fmaxf(tops[i & 1], fmaxf(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])));
                 }
+                if (masked) tmem_st_wait();
             }
-            float top = -INFINITY;
-#pragma unroll
-            for (int i = 0; i < 32; ++i) top = fmaxf(top, fmaxf(__uint_as_float(s0[i]), __uint_as_float(s1[i])));
-            top *= factor;
-            bool settled = TILES == 2 || j == 0;   // whether the product in front has been seen to end
-            if (__any_sync(0xffffffffu, top > m + KV_HEADROOM)) {
+            const float top = fmaxf(tops[0], tops[1]) * factor;
+            if (__any_sync(0xffffffffu, top > m + KV_HEADROOM)) {   // rare, but for the first tile: what there is shrinks
                 const float now = fmaxf(m, top), shrink = m == -INFINITY ? 0.0f : exp2_fast(m - now);
                 m = now;
                 l *= shrink;
-                if (j > 0) {     // what there is of O shrinks
+                if (j > 0) {
                     // (two row tiles: S of this tile came behind the product into O)
-                    if (TILES == 1 && !mbar_wait_warp(bar(P::O_DONE), (uint32_t)((j - 1) & 1), s_abort)) { ok = false; break; }
-                    settled = true;
+                    if (TILES == 1 && !wait_warp(bar(P::O_DONE + (j - 1) % 4), s_parity(j - 1), s_abort)) { ok = false; break; }
                     tcgen05_fence_after();
 #pragma unroll 1
                     for (int c = 0; c < D / 32; ++c) {
@@ -376,34 +452,46 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_prompt_kernel(const Attentio
                     }
                 }
             }
+            // the weights, over what has been read of S
             const float ref = m == -INFINITY ? 0.0f : KV_SHIFT - m;
-            float sum = 0.0f;
-            uint32_t p[32];
+            const f32x2 factor2 = pair(factor, factor), ref2 = pair(ref, ref);
+            f32x2 sums = pair(0.0f, 0.0f);
+            {
+                uint32_t s[2][32];
+                tmem_ld_32x32b_x32(ts, s[0]);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                const float x = exp2_fast(fmaf(__uint_as_float(i < 16 ? s0[2 * i] : s1[2 * i - 32]), factor, ref));
-                const float y = exp2_fast(fmaf(__uint_as_float(i < 16 ? s0[2 * i + 1] : s1[2 * i - 31]), factor, ref));
-                sum += x + y;
-                p[i] = h2(__floats2half2_rn(x, y));
+                for (int c = 0; c < KEYS / 32; ++c) {
+                    tmem_ld_wait();
+                    if (c + 1 < KEYS / 32) tmem_ld_32x32b_x32(ts + 32 * (c + 1), s[(c + 1) & 1]);
+                    uint32_t (&v)[32] = s[c & 1], p[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        float x, y;
+                        unpair(fma2(pair(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), factor2, ref2), x, y);
+                        x = exp2_fast(x), y = exp2_fast(y);
+                        sums = add2(sums, pair(x, y));
+                        p[i] = h2(__floats2half2_rn(x, y));
+                    }
+                    tmem_st_32x32b_x16(ts + 16 * c, p);
+                }
             }
-            l += sum;
-            // (every phase is waited for: its parity would not tell the one after the next from it)
-            if (!settled && !mbar_wait_warp(bar(P::O_DONE), (uint32_t)((j - 1) & 1), s_abort)) { ok = false; break; }
-            tmem_st_32x32b_x32(ts, p);
+            float even, odd;
+            unpair(sums, even, odd);
+            l += even + odd;
             tmem_st_wait();
             tcgen05_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(P::P_FULL + buffer));
         }
         // ------------------------------ output ------------------------------
-        if (ok && tiles) ok = mbar_wait_warp(bar(P::O_DONE), TILES == 2 ? 0u : (uint32_t)((tiles - 1) & 1), s_abort);
+        if (ok && tiles && tile < used) ok = wait_warp(bar(P::O_DONE + (TILES == 2 ? 0 : (tiles - 1) % 4)), TILES == 2 ? 0u : s_parity(tiles - 1), s_abort);
         if (!ok) *s_abort = 1;
-        if (__all_sync(0xffffffffu, ok)) {
+        if (__all_sync(0xffffffffu, ok) && tile < used) {
             tcgen05_fence_after();
             const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
             char *dst = live ? out_row(a, seq, head, row, D) : nullptr;
             // (a split leaves maximum, sum and output of each row)
-            float *part = a.partial + ((((int64_t)blockIdx.z * a.kv_heads + head) * gridDim.x + row0 / P::ROWS) * P::ROWS + in_block) * (D + 4);
+            float *part = a.partial + ((((int64_t)b * splits + split) * a.kv_heads + head) * gridDim.y * P::ROWS + row) * (D + 4);
             if (splits > 1 && live) *reinterpret_cast<float2 *>(part) = make_float2(m, l);
 #pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
@@ -436,8 +524,11 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_prompt_kernel(const Attentio
     __syncthreads();
     if (*s_abort) {
         // a wait ran out somewhere: no copy may land, and no MMA run, once this CTA has gone
-        if (warp == PR_LOAD && lane == 0)
-            for (int i = max(0, issued - RS); i < issued; ++i) mbar_wait<100>(bar(P::RAW_FULL + i % RS), (uint32_t)((i / RS) & 1));
+        if (warp == PR_LOAD && lane % 16 < SLABS)
+            for (int j = max(0, issued - RING); j < issued; ++j) {
+                const int n = j * SLABS + lane % 16;
+                mbar_wait<100>(bar(P::RAW_FULL + lane / 16 * RING + n % RING), (uint32_t)((n / RING) & 1));
+            }
         if (warp == PR_MMA && lane == 0) {
             umma_commit(bar(P::DRAIN));
             mbar_wait<100>(bar(P::DRAIN), 0);
@@ -494,7 +585,7 @@ int launch(const Attention &a, const PromptPlan &plan, cudaStream_t stream) {
     auto *kernel = kv_prompt_kernel<D, BF16>;
     int e = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, P::TOTAL), "atlas_kv_attention");
     if (e != ATLAS_OK) return e;
-    kernel<<<dim3((unsigned)plan.blocks, (unsigned)a.kv_heads, (unsigned)(a.batch * plan.splits)), PR_THREADS, P::TOTAL, stream>>>(a, plan.splits);
+    kernel<<<dim3((unsigned)(a.batch * plan.splits * a.kv_heads), (unsigned)plan.blocks), PR_THREADS, P::TOTAL, stream>>>(a, plan.splits);
     e = check_cuda(cudaGetLastError(), "atlas_kv_attention");
     if (e != ATLAS_OK || plan.splits == 1) return e;
     cudaLaunchConfig_t config = {};
@@ -511,7 +602,7 @@ int launch(const Attention &a, const PromptPlan &plan, cudaStream_t stream) {
 
 }  // namespace
 
-bool kv_prompt_serves(const AtlasKvAttention &p) { return p.max_queries * (p.q_heads / p.kv_heads) > 64 && p.batch <= 65535; }
+bool kv_prompt_serves(const AtlasKvAttention &p) { return p.max_queries * (p.q_heads / p.kv_heads) > 64 && p.batch * p.kv_heads <= (1 << 20); }
 
 size_t kv_prompt_workspace_bytes(const AtlasKvAttention &p) { return plan_of(p).bytes; }
 
