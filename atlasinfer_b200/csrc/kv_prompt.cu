@@ -20,27 +20,30 @@ namespace atlas {
 
 namespace {
 
-constexpr int PR_THREADS = 16 * 32;
-constexpr int PR_REBUILD = 8, PR_REBUILDERS = 6, PR_MMA = 14, PR_LOAD = 15;   // first warps of the roles
+constexpr int PR_THREADS = 16 * 32, PR_MMA = 14, PR_LOAD = 15;   // warps of the roles: softmax, rebuilding, MMA, loads
 
 template <int D>
 struct Prompt {
     static constexpr int TILES = D == 256 ? 1 : 2, KEYS = D == 256 ? 64 : 128;
+    static constexpr int REBUILD = 4 * TILES, REBUILDERS = 6;   // first warp, warps (half of them keys, half values)
     static constexpr int ROWS = 128 * TILES, SLABS = KEYS / KV_SLAB;
     static constexpr int GROUPS = D / 64, SLAB = kv_slab_bytes(D);
     static constexpr int Q_BYTES = 128 * D * 2;             // a Q tile: D / 64 subtiles of 128 rows of 128 bytes
     static constexpr int KV_BYTES = KEYS * D * 2;           // a K tile: D / 64 subtiles of KEYS rows (tokens); a V tile: KEYS / 64 subtiles of D rows (channels)
-    static constexpr int STAGES = 2, RING = D == 64 ? 24 : D == 128 ? 12 : 6;   // rebuilt tiles; halves of slabs, of keys and of values
+    static constexpr int STAGES = 2, RING = D == 64 ? 15 : D == 128 ? 12 : 6;   // rebuilt tiles; halves of slabs, of keys and of values
     static constexpr int HALF = SLAB / 2;                   // codes, then scales and zero points
     static constexpr uint32_t OFF_Q = 0, OFF_K = OFF_Q + TILES * Q_BYTES, OFF_V = OFF_K + STAGES * KV_BYTES, OFF_RAW = OFF_V + STAGES * KV_BYTES;
     static constexpr uint32_t OFF_INFO = OFF_RAW + 2 * RING * HALF, OFF_BAR = OFF_INFO + 16 * 8;
     // barriers; those of S and of O have a place for each of four tiles in a row, so that who comes late can tell them apart
     static constexpr int RAW_FULL = 0, RAW_EMPTY = RAW_FULL + 2 * RING, K_FULL = RAW_EMPTY + 2 * RING, V_FULL = K_FULL + STAGES, S_FULL = V_FULL + STAGES,
-                         P_FULL = S_FULL + 8, O_DONE = P_FULL + 2, Q_FULL = O_DONE + 4, DRAIN = Q_FULL + 1, BARS = DRAIN + 1;
+                         P_FULL = S_FULL + 8, O_DONE = P_FULL + 2, Q_FULL = O_DONE + 4, DRAIN = Q_FULL + 1, Q_RAW = DRAIN + 1, BARS = Q_RAW + 4 * TILES;
     static constexpr uint32_t OFF_TMEM = OFF_BAR + BARS * 8, TOTAL = OFF_TMEM + 16 + 1024 /* alignment */;
     // columns of tensor memory: O, then S (P over it)
     static constexpr uint32_t T_S = TILES * D, T_COLS = 512;
     static_assert(T_S + 256 <= T_COLS, "tensor memory");
+    static_assert(REBUILD + REBUILDERS <= PR_MMA, "warps");
+    // A parity tells two rounds of a place apart: who waits for one has to have seen the last, so a place has one lane that fills it and one warp that empties it.
+    static_assert(RING <= 16 && RING % (REBUILDERS / 2) == 0, "rounds of the rings");
     static_assert(TOTAL <= 227 * 1024, "shared memory");
 };
 
@@ -53,6 +56,13 @@ __device__ __forceinline__ bool elect_one() {
 }
 __device__ __forceinline__ void store_transposable(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(taddr) : "memory");
 }
 __device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&v)[16]) {
     asm volatile(
@@ -107,9 +117,20 @@ struct Walk {
     __device__ __forceinline__ bool slab_seen(int s) const { return s * KV_SLAB <= p1 && (s * KV_SLAB + KV_SLAB > window_start || s * KV_SLAB < sinks); }
 };
 
+// Query and member of the group of a row, and of rows further on, without another division.
+struct RowWalk {
+    int query, member;
+    __device__ __forceinline__ RowWalk(const Attention &a, int row) : query(row / a.group), member(row - query * a.group) {}
+    __device__ __forceinline__ void advance(const Attention &a, int rows) {
+        member += rows;
+        while (member >= a.group) member -= a.group, ++query;
+    }
+};
+
 template <int D, bool BF16>
 __global__ void __launch_bounds__(PR_THREADS, 1) kv_prompt_kernel(const Attention a, int splits) {
     using P = Prompt<D>;
+    constexpr int PR_REBUILD = P::REBUILD, PR_REBUILDERS = P::REBUILDERS;
     constexpr int TILES = P::TILES, KEYS = P::KEYS, SLABS = P::SLABS, STAGES = P::STAGES, RING = P::RING;
     extern __shared__ uint8_t smem_raw[];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -140,6 +161,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_prompt_kernel(const Attentio
         for (int i = 0; i < 4; ++i) mbar_init(bar(P::O_DONE + i), 1);
         mbar_init(bar(P::Q_FULL), 4 * TILES);
         mbar_init(bar(P::DRAIN), 1);
+        for (int i = 0; i < 4 * TILES; ++i) mbar_init(bar(P::Q_RAW + i), 1);
         for (int i = 0; i < 16; ++i) reinterpret_cast<volatile uint64_t *>(gone)[i] = 0;
         *s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -152,40 +174,41 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_prompt_kernel(const Attentio
     __syncthreads();
     tcgen05_fence_after();
     const uint32_t tmem = *tmem_slot;
-    int issued = 0;              // tiles whose half slab this lane has asked for (loader)
+    int issued = 0;              // half slabs that this lane has asked for (loader)
     // S of row tile i (two row tiles), or into buffer j % 2 (one)
     auto s_full = [&](int i, int j) { return bar(P::S_FULL + (TILES == 2 ? 4 * i : 0) + j % 4); };
     auto s_parity = [&](int j) { return (uint32_t)((j / 4) & 1); };
 
     if (warp == PR_LOAD) {
         // ------------------------------ slabs ------------------------------
-        // Lane i brings the keys of slab i of every tile, lane 16 + i the values, each as far ahead as its ring has room.
-        const int slab = lane % 16, part = lane / 16;
-        const bool mine = slab < SLABS;
-        auto page_of = [&](int j) {
-            const int s = walk.tile(j0 + j) * SLABS + slab;
-            return j < tiles && walk.slab_seen(s) ? a.page_table[b * a.table_stride + s * KV_SLAB / a.page_size] : -1;
+        // Lane i brings the slabs' keys that belong in place i of the ring, lane 16 + i the values, as far ahead as there is room.
+        const int part = lane / 16, slot = part * RING + lane % 16;
+        const bool mine = lane % 16 < RING;
+        auto page_of = [&](int n) {
+            const int s = walk.tile(j0 + n / SLABS) * SLABS + n % SLABS;
+            return n < tiles * SLABS && walk.slab_seen(s) ? a.page_table[b * a.table_stride + s * KV_SLAB / a.page_size] : -1;
         };
-        int page = mine ? page_of(0) : -1, idle = 0;
-        int slot = part * RING + slab, round = 0;   // the half slab's place, and how often the ring has gone round
+        int n = lane % 16, page = mine ? page_of(n) : -1, idle = 0;
         while (true) {
-            const bool go = mine && issued < tiles && (round == 0 || mbar_try_wait(bar(P::RAW_EMPTY + slot), (uint32_t)((round - 1) & 1)));
+            const bool more = mine && n < tiles * SLABS;
+            const bool go = more && (issued == 0 || mbar_try_wait(bar(P::RAW_EMPTY + slot), (uint32_t)((issued - 1) & 1)));
             if (go) {
                 const bool there = page >= 0 && page < a.num_pages;
-                gone[issued % 16 * 8 + slab] = !there;
+                const int j = n / SLABS, slab = n % SLABS;
+                gone[j % 16 * 8 + slab] = !there;
                 mbar_arrive_expect_tx(bar(P::RAW_FULL + slot), there ? P::HALF : 0);
                 if (there) {
-                    const int token = (walk.tile(j0 + issued) * SLABS + slab) * KV_SLAB;
+                    const int token = (walk.tile(j0 + j) * SLABS + slab) * KV_SLAB;
                     const uint8_t *src = a.cache + (((int64_t)page * a.kv_heads + head) * (a.page_size / KV_SLAB) + token % a.page_size / KV_SLAB) * P::SLAB;
                     const uint32_t dst = base + P::OFF_RAW + slot * P::HALF;
                     bulk_load_1d(dst, src + part * kv_value_codes(D), 8 * D, bar(P::RAW_FULL + slot));
                     bulk_load_1d(dst + 8 * D, src + (part ? kv_value_params(D) : kv_key_params(D)), D, bar(P::RAW_FULL + slot));
                 }
-                page = page_of(++issued);
-                slot += SLABS;
-                if (slot >= (part + 1) * RING) slot -= RING, ++round;
+                ++issued;
+                n += RING;
+                page = page_of(n);
             }
-            if (!__any_sync(0xffffffffu, mine && issued < tiles)) break;
+            if (!__any_sync(0xffffffffu, more)) break;
             if (__any_sync(0xffffffffu, go)) {
                 idle = 0;
             } else {
@@ -194,16 +217,21 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_prompt_kernel(const Attentio
                 __nanosleep(100);
             }
         }
-    } else if (warp >= PR_REBUILD && warp < PR_MMA) {
+    } else if (warp >= PR_REBUILD && warp < PR_REBUILD + PR_REBUILDERS) {
         // ------------------------------ codes to fp16: a warp a slab, half of the warps keys, half values ------------------------------
         const int g = lane / 4, t = lane % 4;
         const bool keys = warp < PR_REBUILD + PR_REBUILDERS / 2;
         const __half2 off = __float2half2_rn(960.0f);
         uint2 w[2][P::GROUPS];   // of both halves of the slab: codes, then scales and zero points
+        bool q_done = false;     // the second place of the tiles has Q's rows first
         for (int n = (warp - PR_REBUILD) % (PR_REBUILDERS / 2); n < tiles * SLABS; n += PR_REBUILDERS / 2) {
             const int j = n / SLABS, slab = n % SLABS, slot = (keys ? 0 : RING) + n % RING, st = j % STAGES;
             if (!wait_warp<20>(bar(P::RAW_FULL + slot), (uint32_t)((n / RING) & 1), s_abort)) { *s_abort = 1; break; }
             const uint8_t *src = sm + P::OFF_RAW + slot * P::HALF;
+            if (st == 1 && !q_done) {
+                if (!wait_warp<20>(bar(P::Q_FULL), 0, s_abort)) { *s_abort = 1; break; }
+                q_done = true;
+            }
             if (keys) {
                 const int spread = (g & 1) * 4 + g / 2;   // eight lanes that store at a time: rows 4 apart, so that the swizzle keeps them apart
                 __half2 sb[2][P::GROUPS];
@@ -340,48 +368,52 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_prompt_kernel(const Attentio
             }
         }
         if (!ok) *s_abort = 1;
-    } else if (warp < 4 * TILES) {
-        // ------------------------------ Q: each warp its own rows ------------------------------
-        constexpr int LANES = D / 8, PER = 32 / LANES;   // lanes of a row, rows at a time
-        const int tile = warp / 4;
+    } else if (warp < PR_REBUILD) {
+        const int tile = warp / 4, in_block = tid, quarter = warp % 4;
+        const int row = row0 + in_block, query = row / a.group;
+        const bool live = in_block < rows;
+        bool ok = true;
+        // ------------------------------ Q: a thread a row ------------------------------
+        // (Rows come by bulk copies, into the second place of the rebuilt tiles, and go to their own swizzled and as fp16.  Loads by
+        // the threads took 10000 cycles of a CTA's first 17000.)
         float factor = fabsf(a.scale_log2);
         {
-            const int piece = lane % LANES, sub = lane / LANES;
+            static_assert(P::ROWS == 2 * KEYS, "the rows of Q in the places of a K and a V tile");
+            constexpr int PIECES = D / 8;
+            uint8_t *const raw = sm + (in_block < KEYS ? P::OFF_K : P::OFF_V) + P::KV_BYTES + (in_block % KEYS) * (D * 2);
+            uint8_t *const qr = sm + P::OFF_Q + tile * P::Q_BYTES + (in_block % 128) * 128;
+            const uint32_t at = bar(P::Q_RAW + warp);
+            if (lane == 0) mbar_arrive_expect_tx(at, (uint32_t)min(max(rows - warp * 32, 0), 32) * (D * 2));
+            __syncwarp();
+            if (live) bulk_load_1d(smem_u32(raw), a.q + (seq.first_query + query) * a.q_token_stride + (head * a.group + row - query * a.group) * a.q_head_stride, D * 2, at);
+            ok = wait_warp<20>(at, 0, s_abort);
             const uint32_t flip = a.scale_log2 < 0.0f ? 0x80008000u : 0u;   // a negative scale turns the queries round: maxima of scores are maxima of products
-            uint8_t *const qt = sm + P::OFF_Q + tile * P::Q_BYTES + (piece / 8) * (128 * 128);
-#pragma unroll 1
-            for (int r0 = 0; r0 < 32; r0 += 4 * PER) {
-                uint4 v[4];
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    const int in_block = warp * 32 + r0 + u * PER + sub, row = row0 + in_block, query = row / a.group;
-                    v[u] = in_block < rows ? *reinterpret_cast<const uint4 *>(a.q + (seq.first_query + query) * a.q_token_stride +
-                                                                             (head * a.group + row % a.group) * a.q_head_stride + piece * 16)
-                                           : make_uint4(0, 0, 0, 0);
-                }
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    uint32_t w[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
-                    if (BF16) {
-                        // times a power of two, so that the largest is in [1, 2): exact, but for numbers below 2^-14 of it,
-                        // which are off by 2^-25 of it at most
-                        float top = 0.0f;
+            float down = 1.0f;
+            if (BF16) {
+                // times a power of two, so that the largest is in [1, 2): exact, but for numbers below 2^-14 of it, which
+                // are off by 2^-25 of it at most
+                float top = 0.0f;
+                if (live)
+#pragma unroll 4
+                    for (int c = 0; c < PIECES; ++c) {   // (from another piece in every lane: their banks differ)
+                        const uint4 v = *reinterpret_cast<const uint4 *>(raw + (c + lane) % PIECES * 16);
+                        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
                         for (int k = 0; k < 4; ++k) top = fmaxf(top, fmaxf(fabsf(__uint_as_float(w[k] << 16)), fabsf(__uint_as_float(w[k] & 0xffff0000u))));
-#pragma unroll
-                        for (int k = 1; k < LANES; k *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
-                        const int ex = min(max((__float_as_int(top) >> 23) & 0xff, 8), 246);
-                        const float down = __int_as_float((254 - ex) << 23), up = __int_as_float(ex << 23);
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) w[k] = h2(__floats2half2_rn(__uint_as_float(w[k] << 16) * down, __uint_as_float(w[k] & 0xffff0000u) * down));
-                        // (each lane keeps the factor of the row that it will have)
-                        const int mine = lane - (r0 + u * PER);
-                        const float got = __shfl_sync(0xffffffffu, up, mine >= 0 && mine < PER ? mine * LANES : 0);
-                        if (mine >= 0 && mine < PER) factor *= got;
                     }
-                    const int r = (warp % 4) * 32 + r0 + u * PER + sub;
-                    *reinterpret_cast<uint4 *>(qt + r * 128 + (((piece % 8) ^ (r & 7)) << 4)) = make_uint4(w[0] ^ flip, w[1] ^ flip, w[2] ^ flip, w[3] ^ flip);
-                }
+                const int ex = min(max((__float_as_int(top) >> 23) & 0xff, 8), 246);
+                down = __int_as_float((254 - ex) << 23);
+                factor *= __int_as_float(ex << 23);
+            }
+#pragma unroll 4
+            for (int i = 0; i < PIECES; ++i) {
+                const int c = (i + lane) % PIECES;
+                const uint4 v = live ? *reinterpret_cast<const uint4 *>(raw + c * 16) : make_uint4(0, 0, 0, 0);
+                uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    w[k] = flip ^ (BF16 ? h2(__floats2half2_rn(__uint_as_float(w[k] << 16) * down, __uint_as_float(w[k] & 0xffff0000u) * down)) : w[k]);
+                *reinterpret_cast<uint4 *>(qr + (c / 8) * (128 * 128) + (((c % 8) ^ (in_block & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
             }
             fence_async_smem();
             __syncwarp();
@@ -390,47 +422,51 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_prompt_kernel(const Attentio
         factor = fmaxf(factor, 1e-30f);   // (of a scale of zero: masked scores stay -inf)
 
         // ------------------------------ softmax: a thread a row ------------------------------
-        const int in_block = tid, row = row0 + in_block, query = row / a.group;
-        const uint32_t lanes = (uint32_t)((warp % 4) * 32) << 16;
-        const bool live = in_block < rows;
+        const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
         const int place = live ? seq.length - seq.queries + query : -1;
         // first and last position of this row tile, for tiles that need no mask
         const int t_first = seq.length - seq.queries + (row0 + tile * 128) / a.group;
         const int t_last = min(p_last, seq.length - seq.queries + (row0 + tile * 128 + 127) / a.group);
+        const uint32_t t_out = tmem + lanes + tile * D;
+        const f32x2 factor2 = pair(factor, factor);
         float m = -INFINITY, l = 0.0f;
-        bool ok = true;
-        for (int j = 0; j < tiles && tile < used; ++j) {
+        for (int j = 0; j < tiles && tile < used && ok; ++j) {
             const int buffer = TILES == 2 ? tile : j & 1;
             if (!wait_warp(s_full(tile, j), s_parity(j), s_abort)) { ok = false; break; }
             tcgen05_fence_after();
             const uint32_t ts = tmem + lanes + P::T_S + buffer * KEYS;
             const int token0 = walk.tile(j0 + j) * KEYS;
             const uint64_t absent = reinterpret_cast<volatile uint64_t *>(gone)[j % 16];   // a byte a slab
-            const bool masked = absent || token0 + KEYS - 1 > t_first || (a.window && token0 <= t_last - a.window && token0 + KEYS > a.sinks);
-            // the maximum; where tokens are hidden, -inf goes back
-            float tops[2] = {-INFINITY, -INFINITY};
-            {
-                uint32_t s[2][32];
-                tmem_ld_32x32b_x32(ts, s[0]);
-#pragma unroll
-                for (int c = 0; c < KEYS / 32; ++c) {
+            if (absent || token0 + KEYS - 1 > t_first || (a.window && token0 <= t_last - a.window && token0 + KEYS > a.sinks)) {
+                // -inf where tokens are hidden
+#pragma unroll 1
+                for (int c = 0; c < SLABS; ++c) {
+                    uint32_t v[16];
+                    tmem_ld_32x32b_x16(ts + 16 * c, v);
+                    const int t0 = token0 + 16 * c;
+                    uint32_t seen = first_bits(place + 1 - t0);
+                    if (a.window) seen &= ~first_bits(place - a.window + 1 - t0) | first_bits(a.sinks - t0);
+                    if ((absent >> (8 * c)) & 0xff) seen = 0;
                     tmem_ld_wait();
-                    if (c + 1 < KEYS / 32) tmem_ld_32x32b_x32(ts + 32 * (c + 1), s[(c + 1) & 1]);
-                    uint32_t (&v)[32] = s[c & 1];
-                    if (masked) {
-                        const int t0 = token0 + 32 * c;
-                        uint32_t seen = first_bits(place + 1 - t0);
-                        if (a.window) seen &= ~first_bits(place - a.window + 1 - t0) | first_bits(a.sinks - t0);
-                        if ((absent >> (16 * c)) & 0xff) seen &= 0xffff0000u;
-                        if ((absent >> (16 * c + 8)) & 0xff) seen &= 0x0000ffffu;
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) v[i] = (seen >> i) & 1 ? v[i] : 0xff800000u;
-                        tmem_st_32x32b_x32(ts + 32 * c, v);
-                    }
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) tops[i & 1] = fmaxf(tops[i & 1], fmaxf(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])));
+                    for (int i = 0; i < 16; ++i) v[i] = (seen >> i) & 1 ? v[i] : 0xff800000u;
+                    tmem_st_32x32b_x16(ts + 16 * c, v);
                 }
-                if (masked) tmem_st_wait();
+                tmem_st_wait();
+            }
+            // the maximum
+            float tops[2] = {-INFINITY, -INFINITY};
+            uint32_t s[2][32];
+            tmem_ld_32x32b_x32(ts, s[0]);
+#pragma unroll 1
+            for (int c = 0; c < KEYS; c += 64) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    tmem_ld_wait();
+                    if (e == 0 || c + 64 < KEYS) tmem_ld_32x32b_x32(ts + c + 32 * (e + 1), s[e ^ 1]);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) tops[i & 1] = fmaxf(tops[i & 1], fmaxf(__uint_as_float(s[e][2 * i]), __uint_as_float(s[e][2 * i + 1])));
+                }
             }
             const float top = fmaxf(tops[0], tops[1]) * factor;
             if (__any_sync(0xffffffffu, top > m + KV_HEADROOM)) {   // rare, but for the first tile: what there is shrinks
@@ -442,37 +478,37 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_prompt_kernel(const Attentio
                     if (TILES == 1 && !wait_warp(bar(P::O_DONE + (j - 1) % 4), s_parity(j - 1), s_abort)) { ok = false; break; }
                     tcgen05_fence_after();
 #pragma unroll 1
-                    for (int c = 0; c < D / 32; ++c) {
-                        uint32_t o[32];
-                        tmem_ld_32x32b_x32(tmem + lanes + tile * D + c * 32, o);
+                    for (int c = 0; c < D / 16; ++c) {
+                        uint32_t o[16];
+                        tmem_ld_32x32b_x16(t_out + c * 16, o);
                         tmem_ld_wait();
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * shrink);
-                        tmem_st_32x32b_x32(tmem + lanes + tile * D + c * 32, o);
+                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * shrink);
+                        tmem_st_32x32b_x16(t_out + c * 16, o);
                     }
                 }
             }
             // the weights, over what has been read of S
             const float ref = m == -INFINITY ? 0.0f : KV_SHIFT - m;
-            const f32x2 factor2 = pair(factor, factor), ref2 = pair(ref, ref);
+            const f32x2 ref2 = pair(ref, ref);
             f32x2 sums = pair(0.0f, 0.0f);
-            {
-                uint32_t s[2][32];
-                tmem_ld_32x32b_x32(ts, s[0]);
+            tmem_ld_32x32b_x32(ts, s[0]);
+#pragma unroll 1
+            for (int c = 0; c < KEYS; c += 64) {
 #pragma unroll
-                for (int c = 0; c < KEYS / 32; ++c) {
+                for (int e = 0; e < 2; ++e) {
                     tmem_ld_wait();
-                    if (c + 1 < KEYS / 32) tmem_ld_32x32b_x32(ts + 32 * (c + 1), s[(c + 1) & 1]);
-                    uint32_t (&v)[32] = s[c & 1], p[16];
+                    if (e == 0 || c + 64 < KEYS) tmem_ld_32x32b_x32(ts + c + 32 * (e + 1), s[e ^ 1]);
+                    uint32_t p[16];
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         float x, y;
-                        unpair(fma2(pair(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), factor2, ref2), x, y);
+                        unpair(fma2(pair(__uint_as_float(s[e][2 * i]), __uint_as_float(s[e][2 * i + 1])), factor2, ref2), x, y);
                         x = exp2_fast(x), y = exp2_fast(y);
                         sums = add2(sums, pair(x, y));
                         p[i] = h2(__floats2half2_rn(x, y));
                     }
-                    tmem_st_32x32b_x16(ts + 16 * c, p);
+                    tmem_st_32x32b_x16(ts + c / 2 + 16 * e, p);
                 }
             }
             float even, odd;
@@ -488,33 +524,46 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_prompt_kernel(const Attentio
         if (!ok) *s_abort = 1;
         if (__all_sync(0xffffffffu, ok) && tile < used) {
             tcgen05_fence_after();
-            const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-            char *dst = live ? out_row(a, seq, head, row, D) : nullptr;
+            const float inv = splits > 1 ? 1.0f : l > 0.0f || l != l ? 1.0f / l : 0.0f;
             // (a split leaves maximum, sum and output of each row)
             float *part = a.partial + ((((int64_t)b * splits + split) * a.kv_heads + head) * gridDim.y * P::ROWS + row) * (D + 4);
             if (splits > 1 && live) *reinterpret_cast<float2 *>(part) = make_float2(m, l);
+            // rows go out whole, by way of Q's place, which nothing reads any more: this warp's rows, their 16-byte pieces shifted by row
+            constexpr int PIECES = D / 8;
+            uint8_t *const stage = sm + P::OFF_Q + warp * (32 * D * 2);
 #pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
                 uint32_t o[32];
                 if (tiles) {
-                    tmem_ld_32x32b_x32(tmem + lanes + tile * D + c * 32, o);
+                    tmem_ld_32x32b_x32(t_out + c * 32, o);
                     tmem_ld_wait();
                 } else {
 #pragma unroll
                     for (int i = 0; i < 32; ++i) o[i] = 0;
                 }
-                auto at = [&](int ch) { return __uint_as_float(o[8 * (ch % 4) + ch / 4]); };   // channel 32 c + ch
-                if (!live) continue;
+                auto at = [&](int ch) { return __uint_as_float(o[8 * (ch % 4) + ch / 4]) * inv; };   // channel 32 c + ch
                 if (splits > 1) {
+                    if (live)
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) *reinterpret_cast<float4 *>(part + 4 + c * 32 + 4 * i) = make_float4(at(4 * i), at(4 * i + 1), at(4 * i + 2), at(4 * i + 3));
-                } else {
+                        for (int i = 0; i < 8; ++i) *reinterpret_cast<float4 *>(part + 4 + c * 32 + 4 * i) = make_float4(at(4 * i), at(4 * i + 1), at(4 * i + 2), at(4 * i + 3));
+                } else if (tiles) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const uint2 x = pack4<BF16>(at(8 * i) * inv, at(8 * i + 1) * inv, at(8 * i + 2) * inv, at(8 * i + 3) * inv);
-                        const uint2 y = pack4<BF16>(at(8 * i + 4) * inv, at(8 * i + 5) * inv, at(8 * i + 6) * inv, at(8 * i + 7) * inv);
-                        *reinterpret_cast<uint4 *>(dst + (c * 32 + 8 * i) * 2) = make_uint4(x.x, x.y, y.x, y.y);
+                        const uint2 x = pack4<BF16>(at(8 * i), at(8 * i + 1), at(8 * i + 2), at(8 * i + 3)), y = pack4<BF16>(at(8 * i + 4), at(8 * i + 5), at(8 * i + 6), at(8 * i + 7));
+                        *reinterpret_cast<uint4 *>(stage + lane * (D * 2) + (((c * 4 + i) ^ (lane % 8)) << 4)) = make_uint4(x.x, x.y, y.x, y.y);
                     }
+                }
+            }
+            if (splits == 1) {
+                __syncwarp();
+                const int piece = lane % PIECES;
+                RowWalk at(a, row0 + warp * 32 + lane / PIECES);
+#pragma unroll 2
+                for (int r = lane / PIECES; r < 32; r += 32 / PIECES) {
+                    if (warp * 32 + r < rows)
+                        *reinterpret_cast<uint4 *>(a.out + (((seq.first_query + at.query) * a.q_heads + head * a.group + at.member) * (int64_t)D + piece * 8) * 2) =
+                            tiles ? *reinterpret_cast<const uint4 *>(stage + r * (D * 2) + ((piece ^ (r % 8)) << 4)) : make_uint4(0, 0, 0, 0);
+                    at.advance(a, 32 / PIECES);
                 }
             }
         }
@@ -524,11 +573,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_prompt_kernel(const Attentio
     __syncthreads();
     if (*s_abort) {
         // a wait ran out somewhere: no copy may land, and no MMA run, once this CTA has gone
-        if (warp == PR_LOAD && lane % 16 < SLABS)
-            for (int j = max(0, issued - RING); j < issued; ++j) {
-                const int n = j * SLABS + lane % 16;
-                mbar_wait<100>(bar(P::RAW_FULL + lane / 16 * RING + n % RING), (uint32_t)((n / RING) & 1));
-            }
+        if (warp == PR_LOAD && issued > 0) mbar_wait<100>(bar(P::RAW_FULL + lane / 16 * RING + lane % 16), (uint32_t)((issued - 1) & 1));
         if (warp == PR_MMA && lane == 0) {
             umma_commit(bar(P::DRAIN));
             mbar_wait<100>(bar(P::DRAIN), 0);
