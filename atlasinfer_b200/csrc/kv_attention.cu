@@ -63,13 +63,45 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
     return r;
 }
+// A lane's words of codes: 8 or 16 bytes, in each of two planes if D is 256.
+template <int D>
+__device__ __forceinline__ void read_words(const uint8_t *p, uint32_t (&w)[D / 32]) {
+    if constexpr (D == 64) {
+        const uint2 v = *reinterpret_cast<const uint2 *>(p);
+        w[0] = v.x, w[1] = v.y;
+    } else {
+#pragma unroll
+        for (int i = 0; i < D / 128; ++i) {
+            const uint4 v = *reinterpret_cast<const uint4 *>(p + i * 1024);
+            w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+        }
+    }
+}
+template <int N>
+__device__ __forceinline__ void read_params(const uint8_t *p, uint32_t (&w)[N]) {
+    if constexpr (N == 1) {
+        w[0] = *reinterpret_cast<const uint32_t *>(p);
+    } else if constexpr (N == 2) {
+        const uint2 v = *reinterpret_cast<const uint2 *>(p);
+        w[0] = v.x, w[1] = v.y;
+    } else {
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i) {
+            const uint4 v = *reinterpret_cast<const uint4 *>(p + i * 16);
+            w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+        }
+    }
+}
+
 template <int D, int NT, int WARPS, int STAGES>
 struct Shape {
     static constexpr int ROWS = 8 * NT, GROUPS = D / 64, WORDS = D / 32;   // words: a lane's, of a token's key
     static constexpr int SLAB = kv_slab_bytes(D);
+    static constexpr int PIECE_BYTES = D == 64 ? 8 : 16, KEY_ROW = 4 * PIECE_BYTES;   // of a lane's codes (in a plane); of a token's
     static constexpr int PIECE = ROWS * (D + 2) * 4;       // maximum, sum and output of the rows
     static constexpr int RING = STAGES * SLAB;             // a warp's; holds its last piece in the end
-    static constexpr int SMEM = WARPS * (RING + PIECE) + WARPS * STAGES * 8 + 2 * WARPS * 16 + 16;
+    static constexpr int SMEM = WARPS * (RING + PIECE + STAGES * 8 + 2 * 16 + 32 * 8);
+    static_assert(STAGES * WARPS % 2 == 0 && SMEM <= 227 * 1024, "shared memory");
     static_assert(PIECE <= RING, "a piece has to fit the ring");
 };
 
@@ -79,6 +111,7 @@ struct State {
     float o[NT][D / 16][4];
     float l[NT][4];
     float m[NT][2];              // of rows 2 t and 2 t + 1, log2; -inf before the first visible score
+    float ref[NT][2];            // what is taken from a score: m - 6, or 0 before the first
     __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -89,6 +122,7 @@ struct State {
 #pragma unroll
             for (int k = 0; k < 4; ++k) l[n][k] = 0.0f;
             m[n][0] = m[n][1] = -INFINITY;
+            ref[n][0] = ref[n][1] = 0.0f;
         }
     }
 };
@@ -101,6 +135,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_attention_kernel(const Atten
     uint64_t *const bars = reinterpret_cast<uint64_t *>(heads_all + WARPS * S::PIECE);
     // run (sequence * kv_heads + head) of every warp's first and last piece, or -1, and whether the run begins or ends there
     int4 *const notes = reinterpret_cast<int4 *>(bars + WARPS * STAGES);
+    uint64_t *const slabs = reinterpret_cast<uint64_t *>(notes + 2 * WARPS) + (threadIdx.x / 32) * 32;
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, g = lane / 4, t = lane % 4;
@@ -144,43 +179,50 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_attention_kernel(const Atten
         int head = (int)((begin - before) / run.units);
         int unit = (int)((begin - before) % run.units);
 
-        // the producer's own place, up to STAGES units ahead; pages of the next 32 units of its run, one a lane
+        // The producer's own place, up to STAGES units ahead.  Every lane finds the slab of one of the next 32 units of its run
+        // (0: not in the cache); lane 0 asks for them one by one.
         Run p_run = run;
-        int p_b = b, p_head = head, p_unit = unit, p_first = 0, p_count = 0, issued = 0, page_ahead = -1;
+        int p_b = b, p_head = head, p_unit = unit, p_left = 0, issued = 0, p_stage = 0;
+        const uint64_t *p_next = slabs;
         const int todo = (int)(end - begin);
         auto produce = [&]() {
             if (issued >= todo) return;
-            if (p_unit >= p_run.units) {
-                p_unit = 0;
-                if (++p_head == a.kv_heads) {
-                    p_head = 0;
-                    do p_run = make_run(a, ++p_b, row0, S::ROWS); while (p_run.units == 0);
+            if (p_left == 0) {
+                if (p_unit >= p_run.units) {
+                    p_unit = 0;
+                    if (++p_head == a.kv_heads) {
+                        p_head = 0;
+                        do p_run = make_run(a, ++p_b, row0, S::ROWS); while (p_run.units == 0);
+                    }
                 }
-                p_count = 0;
+                p_left = min(32, p_run.units - p_unit);
+                __syncwarp();    // (lane 0 has read the last 32)
+                if (lane < p_left) {
+                    const int token = p_run.slab(p_unit + lane) * KV_SLAB, in_table = token / a.page_size;
+                    const int page = a.page_table[p_b * a.table_stride + in_table];
+                    const uint8_t *src = a.cache + (((int64_t)page * a.kv_heads + p_head) * (a.page_size / KV_SLAB) + (token - in_table * a.page_size) / KV_SLAB) * S::SLAB;
+                    slabs[lane] = page >= 0 && page < a.num_pages ? reinterpret_cast<uint64_t>(src) : 0;
+                }
+                __syncwarp();
+                p_unit += p_left;
+                p_next = slabs;
             }
-            if (p_count == 0 || p_unit >= p_first + p_count) {
-                p_first = p_unit;
-                p_count = min(32, p_run.units - p_unit);
-                page_ahead = -1;
-                if (lane < p_count) page_ahead = a.page_table[p_b * a.table_stride + p_run.slab(p_unit + lane) * KV_SLAB / a.page_size];
-            }
-            const int page = __shfl_sync(0xffffffffu, page_ahead, p_unit - p_first);
             if (lane == 0) {
-                const int stage = issued % STAGES, token = p_run.slab(p_unit) * KV_SLAB;
-                const bool known = page >= 0 && page < a.num_pages;
-                const uint32_t at = bar + 8 * stage;
-                if (known) {
-                    const uint8_t *src = a.cache + (((int64_t)page * a.kv_heads + p_head) * (a.page_size / KV_SLAB) + token % a.page_size / KV_SLAB) * S::SLAB;
+                const uint8_t *src = reinterpret_cast<const uint8_t *>(*p_next);
+                const uint32_t at = bar + 8 * p_stage;
+                if (src) {
                     mbar_arrive_expect_tx(at, S::SLAB);
-                    bulk_load_1d(ring + stage * S::SLAB, src, S::SLAB, at);
+                    bulk_load_1d(ring + p_stage * S::SLAB, src, S::SLAB, at);
                 } else {   // a page that is not there: a NaN in the first scale of the keys says so, the slab is passed over
-                    *reinterpret_cast<volatile uint16_t *>(ring_all + warp * S::RING + stage * S::SLAB + kv_key_params(D)) = 0x7fff;
+                    *reinterpret_cast<volatile uint16_t *>(ring_all + warp * S::RING + p_stage * S::SLAB + kv_key_params(D)) = 0x7fff;
                     fence_async_smem();   // (the stage's next slab comes by the other proxy)
                     mbar_arrive(at);
                 }
             }
+            ++p_next;
+            --p_left;
             ++issued;
-            ++p_unit;
+            p_stage = p_stage + 1 == STAGES ? 0 : p_stage + 1;
         };
         for (int i = 0; i < STAGES; ++i) produce();
 
@@ -188,10 +230,11 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_attention_kernel(const Atten
         uint32_t qf[NT][S::WORDS][4];
         float factor[NT][2];       // log2 units of a row's scores
         int place[NT][2];          // positions of rows 2 t and 2 t + 1, -1: no such row
-        int p_lo = 0, p_hi = 0;    // positions of the tile's first and last query
+        int plain_sinks = 0, plain_from = 0, plain_to = 0;   // slabs that all rows see whole: below the first, or from the second to the third
         bool fresh = true, first_piece = true, failed = false;
         const bool begins_inside = unit != 0;
-        int done = 0;
+        int done = 0, stage = 0;
+        uint32_t parity = 0;
 
         auto leave = [&](bool whole_run, bool ends) {
             // to the output (a run that began and ended here), or to shared memory
@@ -232,8 +275,9 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_attention_kernel(const Atten
             if (fresh) {           // another run: its queries into registers
                 st.clear();
                 fresh = false;
-                p_lo = run.length - run.queries + row0 / a.group;
-                p_hi = run.length - 1;
+                plain_to = max(0, run.length - run.queries + row0 / a.group + 1) / KV_SLAB;
+                plain_from = a.window ? max(0, run.length - 1 - a.window + KV_SLAB) / KV_SLAB : 0;
+                plain_sinks = min(a.sinks / KV_SLAB, plain_to);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     const int row = row0 + 8 * n + g, query = row / a.group;
@@ -280,36 +324,37 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_attention_kernel(const Atten
                 }
             }
 
-            const int stage = done % STAGES;
-            if (!__all_sync(0xffffffffu, mbar_wait(bar + 8 * stage, (done / STAGES) & 1))) {
+            if (!__all_sync(0xffffffffu, mbar_wait(bar + 8 * stage, parity))) {
                 failed = true;
                 break;
             }
-            const uint8_t *slab = ring_ptr + stage * S::SLAB;
-            const int token0 = run.slab(unit) * KV_SLAB;
-            const bool there = *reinterpret_cast<const uint16_t *>(slab + kv_key_params(D)) != 0x7fffu;
-            if (there) {
+            const uint8_t *const slab = ring_ptr + stage * S::SLAB;
+            const int at = run.slab(unit);
+            if (++stage == STAGES) stage = 0, parity ^= 1;
+            if (*reinterpret_cast<const uint16_t *>(slab + kv_key_params(D)) != 0x7fffu) {
                 // scores
                 float s[NT][4];
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
                     for (int k = 0; k < 4; ++k) s[n][k] = 0.0f;
+                uint32_t low[S::WORDS], high[S::WORDS], kl[S::GROUPS], kh[S::GROUPS];
+                read_words<D>(slab + g * S::KEY_ROW + t * S::PIECE_BYTES, low);
+                read_words<D>(slab + (g + 8) * S::KEY_ROW + t * S::PIECE_BYTES, high);
+                read_params<S::GROUPS>(slab + kv_key_params(D) + g * S::GROUPS * 4, kl);
+                read_params<S::GROUPS>(slab + kv_key_params(D) + (g + 8) * S::GROUPS * 4, kh);
+                const __half2 off = __float2half2_rn(960.0f);
 #pragma unroll
                 for (int gr = 0; gr < S::GROUPS; ++gr) {
-                    const __half2 lo = *reinterpret_cast<const __half2 *>(slab + kv_key_params(D) + (g * S::GROUPS + gr) * 4);
-                    const __half2 hi = *reinterpret_cast<const __half2 *>(slab + kv_key_params(D) + ((g + 8) * S::GROUPS + gr) * 4);
-                    const __half2 bl = __high2half2(lo), bh = __high2half2(hi), off = __float2half2_rn(960.0f);
-                    const __half2 bl16 = __hsub2(bl, off), bh16 = __hsub2(bh, off);
+                    const __half2 lo = h2(kl[gr]), hi = h2(kh[gr]);
+                    const __half2 bl = __high2half2(lo), bh = __high2half2(hi), bl16 = __hsub2(bl, off), bh16 = __hsub2(bh, off);
                     float acc[NT][4];
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
                         for (int k = 0; k < 4; ++k) acc[n][k] = 0.0f;
-                    const uint2 w0 = *reinterpret_cast<const uint2 *>(slab + kv_key_word(D, g, t + 8 * gr)), w1 = *reinterpret_cast<const uint2 *>(slab + kv_key_word(D, g + 8, t + 8 * gr));
-                    const uint32_t low[2] = {w0.x, w0.y}, high[2] = {w1.x, w1.y};
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
+                    for (int j = 2 * gr; j < 2 * gr + 2; ++j) {
                         __half2 x[4], y[4];
                         open_word(low[j], bl, bl16, x);
                         open_word(high[j], bh, bh16, y);
@@ -317,7 +362,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_attention_kernel(const Atten
                         for (int i = 0; i < 2; ++i)
 #pragma unroll
                             for (int n = 0; n < NT; ++n)
-                                mma_f16(acc[n], h2(x[2 * i]), h2(y[2 * i]), h2(x[2 * i + 1]), h2(y[2 * i + 1]), qf[n][2 * gr + j][2 * i], qf[n][2 * gr + j][2 * i + 1]);
+                                mma_f16(acc[n], h2(x[2 * i]), h2(y[2 * i]), h2(x[2 * i + 1]), h2(y[2 * i + 1]), qf[n][j][2 * i], qf[n][j][2 * i + 1]);
                     }
                     const float sl = __low2float(lo), sh = __low2float(hi);
 #pragma unroll
@@ -330,8 +375,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_attention_kernel(const Atten
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
                     for (int k = 0; k < 4; ++k) s[n][k] *= factor[n][k & 1];
-                const bool all_seen = token0 + KV_SLAB - 1 <= p_lo && (!a.window || token0 > p_hi - a.window || token0 + KV_SLAB <= a.sinks);
-                if (!all_seen) {
+                if (!(at < plain_sinks || (at >= plain_from && at < plain_to))) {
+                    const int token0 = at * KV_SLAB;
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -345,7 +390,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_attention_kernel(const Atten
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) passes |= s[n][k] > st.m[n][k & 1] + KV_HEADROOM;
+                    for (int e = 0; e < 2; ++e) passes |= fmaxf(s[n][e], s[n][2 + e]) > st.m[n][e] + KV_HEADROOM;
                 if (__any_sync(0xffffffffu, passes)) {
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
@@ -357,6 +402,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_attention_kernel(const Atten
                             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
                             const float shrink = st.m[n][e] == -INFINITY ? 0.0f : exp2_fast(st.m[n][e] - top);
                             st.m[n][e] = top;
+                            st.ref[n][e] = top == -INFINITY ? 0.0f : top - KV_SHIFT;
                             st.l[n][e] *= shrink, st.l[n][2 + e] *= shrink;
 #pragma unroll
                             for (int i = 0; i < D / 16; ++i) st.o[n][i][e] *= shrink, st.o[n][i][2 + e] *= shrink;
@@ -367,45 +413,43 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_attention_kernel(const Atten
                 for (int n = 0; n < NT; ++n) {
                     float p[4];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const float ref = st.m[n][k & 1] == -INFINITY ? 0.0f : st.m[n][k & 1] - KV_SHIFT;
-                        p[k] = exp2_fast(s[n][k] - ref);
-                    }
+                    for (int k = 0; k < 4; ++k) p[k] = exp2_fast(s[n][k] - st.ref[n][k & 1]);
                     pb[n][0] = transpose8x8(h2(__floats2half2_rn(p[0], p[1])));
                     pb[n][1] = transpose8x8(h2(__floats2half2_rn(p[2], p[3])));
                     mma_f16(st.l[n], 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, pb[n][0], pb[n][1]);   // sums of what is used
                 }
                 // outputs
+                uint32_t v0[S::WORDS], v1[S::WORDS], q0[2 * S::GROUPS], q1[2 * S::GROUPS];
+                read_words<D>(slab + kv_value_codes(D) + lane * S::PIECE_BYTES, v0);
+                read_words<D>(slab + kv_value_codes(D) + 32 * S::PIECE_BYTES + lane * S::PIECE_BYTES, v1);
+                read_params<2 * S::GROUPS>(slab + kv_value_params(D) + t * S::GROUPS * 8, q0);
+                read_params<2 * S::GROUPS>(slab + kv_value_params(D) + (t + 4) * S::GROUPS * 8, q1);
+                const int left = run.length - at * KV_SLAB;
+                if (left < KV_SLAB) {   // tokens that are not there may hold anything
+                    const uint32_t keep0 = (2 * t < left ? 0xffffu : 0u) | (2 * t + 1 < left ? 0xffff0000u : 0u);
+                    const uint32_t keep1 = (2 * t + 8 < left ? 0xffffu : 0u) | (2 * t + 9 < left ? 0xffff0000u : 0u);
+#pragma unroll
+                    for (int gr = 0; gr < S::GROUPS; ++gr) {
+                        q0[2 * gr] &= keep0, q0[2 * gr + 1] = (q0[2 * gr + 1] & keep0) | (0x64006400u & ~keep0);
+                        q1[2 * gr] &= keep1, q1[2 * gr + 1] = (q1[2 * gr + 1] & keep1) | (0x64006400u & ~keep1);
+                    }
+                }
 #pragma unroll
                 for (int gr = 0; gr < S::GROUPS; ++gr) {
-                    uint2 p0 = *reinterpret_cast<const uint2 *>(slab + kv_value_params(D) + (t * S::GROUPS + gr) * 8);
-                    uint2 p1 = *reinterpret_cast<const uint2 *>(slab + kv_value_params(D) + ((t + 4) * S::GROUPS + gr) * 8);
-                    if (token0 + KV_SLAB > run.length) {   // tokens that are not there may hold anything
-                        uint32_t keep0 = 0, keep1 = 0;
-                        if (token0 + 2 * t < run.length) keep0 |= 0xffffu;
-                        if (token0 + 2 * t + 1 < run.length) keep0 |= 0xffff0000u;
-                        if (token0 + 2 * t + 8 < run.length) keep1 |= 0xffffu;
-                        if (token0 + 2 * t + 9 < run.length) keep1 |= 0xffff0000u;
-                        p0.x &= keep0, p0.y = (p0.y & keep0) | (0x64006400u & ~keep0);
-                        p1.x &= keep1, p1.y = (p1.y & keep1) | (0x64006400u & ~keep1);
-                    }
-                    const __half2 off = __float2half2_rn(960.0f), s0 = h2(p0.x), s1 = h2(p1.x), b0 = h2(p0.y), b1 = h2(p1.y);
+                    const __half2 s0 = h2(q0[2 * gr]), s1 = h2(q1[2 * gr]), b0 = h2(q0[2 * gr + 1]), b1 = h2(q1[2 * gr + 1]);
                     const __half2 b016 = __hsub2(b0, off), b116 = __hsub2(b1, off);
-                    const uint8_t *codes = slab + kv_value_codes(D);
-                    const uint2 w0 = *reinterpret_cast<const uint2 *>(codes + kv_value_unit(D, 2 * t, g + 16 * gr)), w1 = *reinterpret_cast<const uint2 *>(codes + kv_value_unit(D, 2 * t + 8, g + 16 * gr));
-                    const uint32_t low[2] = {w0.x, w0.y}, high[2] = {w1.x, w1.y};
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
+                    for (int j = 2 * gr; j < 2 * gr + 2; ++j) {
                         __half2 x[4], y[4];
-                        open_word(low[j], b0, b016, x);
-                        open_word(high[j], b1, b116, y);
+                        open_word(v0[j], b0, b016, x);
+                        open_word(v1[j], b1, b116, y);
 #pragma unroll
                         for (int i = 0; i < 4; ++i) x[i] = __hmul2(x[i], s0), y[i] = __hmul2(y[i], s1);
 #pragma unroll
                         for (int i = 0; i < 2; ++i)
 #pragma unroll
                             for (int n = 0; n < NT; ++n)
-                                mma_f16(st.o[n][4 * gr + 2 * j + i], h2(x[2 * i]), h2(x[2 * i + 1]), h2(y[2 * i]), h2(y[2 * i + 1]), pb[n][0], pb[n][1]);
+                                mma_f16(st.o[n][2 * j + i], h2(x[2 * i]), h2(x[2 * i + 1]), h2(y[2 * i]), h2(y[2 * i + 1]), pb[n][0], pb[n][1]);
                     }
                 }
             }
