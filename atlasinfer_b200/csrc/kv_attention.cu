@@ -58,6 +58,10 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma_f16_new(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
     uint32_t r;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
@@ -324,7 +328,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_attention_kernel(const Atten
                 }
             }
 
-            if (!__all_sync(0xffffffffu, mbar_wait(bar + 8 * stage, parity))) {
+            if (!__all_sync(0xffffffffu, mbar_try_wait(bar + 8 * stage, parity)) && !__all_sync(0xffffffffu, mbar_wait(bar + 8 * stage, parity))) {
                 failed = true;
                 break;
             }
@@ -334,25 +338,16 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_attention_kernel(const Atten
             if (*reinterpret_cast<const uint16_t *>(slab + kv_key_params(D)) != 0x7fffu) {
                 // scores
                 float s[NT][4];
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) s[n][k] = 0.0f;
                 uint32_t low[S::WORDS], high[S::WORDS], kl[S::GROUPS], kh[S::GROUPS];
                 read_words<D>(slab + g * S::KEY_ROW + t * S::PIECE_BYTES, low);
                 read_words<D>(slab + (g + 8) * S::KEY_ROW + t * S::PIECE_BYTES, high);
                 read_params<S::GROUPS>(slab + kv_key_params(D) + g * S::GROUPS * 4, kl);
                 read_params<S::GROUPS>(slab + kv_key_params(D) + (g + 8) * S::GROUPS * 4, kh);
-                const __half2 off = __float2half2_rn(960.0f);
 #pragma unroll
                 for (int gr = 0; gr < S::GROUPS; ++gr) {
                     const __half2 lo = h2(kl[gr]), hi = h2(kh[gr]);
-                    const __half2 bl = __high2half2(lo), bh = __high2half2(hi), bl16 = __hsub2(bl, off), bh16 = __hsub2(bh, off);
+                    const __half2 bl = __high2half2(lo), bh = __high2half2(hi), bl16 = minus16_of(bl), bh16 = minus16_of(bh);
                     float acc[NT][4];
-#pragma unroll
-                    for (int n = 0; n < NT; ++n)
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) acc[n][k] = 0.0f;
 #pragma unroll
                     for (int j = 2 * gr; j < 2 * gr + 2; ++j) {
                         __half2 x[4], y[4];
@@ -361,15 +356,18 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_attention_kernel(const Atten
 #pragma unroll
                         for (int i = 0; i < 2; ++i)
 #pragma unroll
-                            for (int n = 0; n < NT; ++n)
-                                mma_f16(acc[n], h2(x[2 * i]), h2(y[2 * i]), h2(x[2 * i + 1]), h2(y[2 * i + 1]), qf[n][j][2 * i], qf[n][j][2 * i + 1]);
+                            for (int n = 0; n < NT; ++n) {
+                                if (j == 2 * gr && i == 0)
+                                    mma_f16_new(acc[n], h2(x[2 * i]), h2(y[2 * i]), h2(x[2 * i + 1]), h2(y[2 * i + 1]), qf[n][j][2 * i], qf[n][j][2 * i + 1]);
+                                else
+                                    mma_f16(acc[n], h2(x[2 * i]), h2(y[2 * i]), h2(x[2 * i + 1]), h2(y[2 * i + 1]), qf[n][j][2 * i], qf[n][j][2 * i + 1]);
+                            }
                     }
                     const float sl = __low2float(lo), sh = __low2float(hi);
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        s[n][0] += acc[n][0] * sl, s[n][1] += acc[n][1] * sl;
-                        s[n][2] += acc[n][2] * sh, s[n][3] += acc[n][3] * sh;
-                    }
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) s[n][k] = gr ? fmaf(acc[n][k], k < 2 ? sl : sh, s[n][k]) : acc[n][k] * (k < 2 ? sl : sh);
                 }
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
@@ -437,7 +435,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_attention_kernel(const Atten
 #pragma unroll
                 for (int gr = 0; gr < S::GROUPS; ++gr) {
                     const __half2 s0 = h2(q0[2 * gr]), s1 = h2(q1[2 * gr]), b0 = h2(q0[2 * gr + 1]), b1 = h2(q1[2 * gr + 1]);
-                    const __half2 b016 = __hsub2(b0, off), b116 = __hsub2(b1, off);
+                    const __half2 b016 = minus16_of(b0), b116 = minus16_of(b1);
 #pragma unroll
                     for (int j = 2 * gr; j < 2 * gr + 2; ++j) {
                         __half2 x[4], y[4];

@@ -62,14 +62,20 @@ __device__ __forceinline__ float exp2_fast(float x) {
 __device__ __forceinline__ uint32_t h2(__half2 v) { return *reinterpret_cast<uint32_t *>(&v); }
 __device__ __forceinline__ __half2 h2(uint32_t v) { return *reinterpret_cast<__half2 *>(&v); }
 
-// The four pairs of a word of codes, minus the zero point: `bias` is 1024 + z, `bias16` 64 + z.
-__device__ __forceinline__ void open_word(uint32_t w, __half2 bias, __half2 bias16, __half2 (&v)[4]) {
+// The four pairs of a word of codes, minus the zero point: `bias` is 1024 + z, `minus16` is -(64 + z) = 960 - bias.
+__device__ __forceinline__ uint32_t masked_or(uint32_t w, uint32_t mask, uint32_t bits) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "r"(mask), "r"(bits));
+    return r;
+}
+__device__ __forceinline__ __half2 minus16_of(__half2 bias) { return __hsub2(__float2half2_rn(960.0f), bias); }
+__device__ __forceinline__ void open_word(uint32_t w, __half2 bias, __half2 minus16, __half2 (&v)[4]) {
     const __half2 sixteenth = __float2half2_rn(0.0625f);
     const uint32_t u = w >> 8;
-    v[0] = __hsub2(h2((w & 0x000f000fu) | 0x64006400u), bias);
-    v[1] = __hfma2(h2((w & 0x00f000f0u) | 0x64006400u), sixteenth, __hneg2(bias16));   // (1024 + 16 c) / 16 - (64 + z)
-    v[2] = __hsub2(h2((u & 0x000f000fu) | 0x64006400u), bias);
-    v[3] = __hfma2(h2((u & 0x00f000f0u) | 0x64006400u), sixteenth, __hneg2(bias16));
+    v[0] = __hsub2(h2(masked_or(w, 0x000f000fu, 0x64006400u)), bias);
+    v[1] = __hfma2(h2(masked_or(w, 0x00f000f0u, 0x64006400u)), sixteenth, minus16);   // (1024 + 16 c) / 16 - (64 + z)
+    v[2] = __hsub2(h2(masked_or(u, 0x000f000fu, 0x64006400u)), bias);
+    v[3] = __hfma2(h2(masked_or(u, 0x00f000f0u, 0x64006400u)), sixteenth, minus16);
 }
 
 template <bool BF16>

@@ -221,7 +221,6 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_prompt_kernel(const Attentio
         // ------------------------------ codes to fp16: a warp a slab, half of the warps keys, half values ------------------------------
         const int g = lane / 4, t = lane % 4;
         const bool keys = warp < PR_REBUILD + PR_REBUILDERS / 2;
-        const __half2 off = __float2half2_rn(960.0f);
         uint2 w[2][P::GROUPS];   // of both halves of the slab: codes, then scales and zero points
         bool q_done = false;     // the second place of the tiles has Q's rows first
         for (int n = (warp - PR_REBUILD) % (PR_REBUILDERS / 2); n < tiles * SLABS; n += PR_REBUILDERS / 2) {
@@ -252,7 +251,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_prompt_kernel(const Attentio
                     const int row = slab * KV_SLAB + 8 * h + spread;
 #pragma unroll
                     for (int gr = 0; gr < P::GROUPS; ++gr) {
-                        const __half2 s = __low2half2(sb[h][gr]), bias = __high2half2(sb[h][gr]), bias16 = __hsub2(bias, off);
+                        const __half2 s = __low2half2(sb[h][gr]), bias = __high2half2(sb[h][gr]), bias16 = minus16_of(bias);
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
                             __half2 v[4];
@@ -296,7 +295,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_prompt_kernel(const Attentio
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
                     for (int gr = 0; gr < P::GROUPS; ++gr) {
-                        const __half2 s = h2(sb[h][gr].x), bias = h2(sb[h][gr].y), bias16 = __hsub2(bias, off);
+                        const __half2 s = h2(sb[h][gr].x), bias = h2(sb[h][gr].y), bias16 = minus16_of(bias);
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
                             __half2 v[4];
