@@ -42,16 +42,19 @@ __device__ __forceinline__ Run make_run(const Attention &a, int b, int row0, int
     return r;
 }
 
-// Units of all sequences (times the kv heads), the same in every warp that asks.
-__device__ __forceinline__ int64_t all_units(const Attention &a, int row0, int rows) {
-    int64_t sum = 0;
-    for (int b = threadIdx.x & 31; b < a.batch; b += 32) sum += make_run(a, b, row0, rows).units;
-#pragma unroll
-    for (int k = 16; k; k /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, k);
-    return sum * a.kv_heads;
+// Units of all runs, and of those of the sequences in front of b: the same in every warp that asks.
+__device__ __forceinline__ uint32_t count_units(const Attention &a, int row0, int rows, int b, uint32_t &in_front) {
+    uint32_t sum = 0, front = 0;
+    for (int k = threadIdx.x & 31; k < a.batch; k += 32) {
+        const uint32_t units = make_run(a, k, row0, rows).units;
+        sum += units;
+        if (k < b) front += units;
+    }
+    in_front = __reduce_add_sync(0xffffffffu, front) * a.kv_heads;
+    return __reduce_add_sync(0xffffffffu, sum) * a.kv_heads;
 }
-__device__ __forceinline__ int64_t units_per_warp(const Attention &a, int64_t total, int64_t warps) {
-    return max((total + warps - 1) / warps, (int64_t)a.min_units);
+__device__ __forceinline__ uint32_t units_per_warp(const Attention &a, uint32_t total, uint32_t warps) {
+    return max((total + warps - 1) / warps, (uint32_t)a.min_units);
 }
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -101,6 +104,7 @@ template <int D, int NT, int WARPS, int STAGES>
 struct Shape {
     static constexpr int ROWS = 8 * NT, GROUPS = D / 64, WORDS = D / 32;   // words: a lane's, of a token's key
     static constexpr int SLAB = kv_slab_bytes(D);
+    static constexpr bool PAIRS = NT == 1;                 // two slabs at a time
     static constexpr int PIECE_BYTES = D == 64 ? 8 : 16, KEY_ROW = 4 * PIECE_BYTES;   // of a lane's codes (in a plane); of a token's
     static constexpr int PIECE = ROWS * (D + 2) * 4;       // maximum, sum and output of the rows
     static constexpr int RING = STAGES * SLAB;             // a warp's; holds its last piece in the end
@@ -131,57 +135,85 @@ struct State {
     }
 };
 
+// Four channels of a row of a piece (maxima, sums, outputs of its rows), brought to the maximum m of all pieces.
+__device__ __forceinline__ void add_piece(const float *piece, int rows, int row, int d, int c, float m, float &l, float4 &o) {
+    const float pm = piece[row], w = pm == -INFINITY ? 0.0f : exp2_fast(pm - m);
+    const float4 po = *reinterpret_cast<const float4 *>(piece + 2 * rows + row * d + c);
+    l = fmaf(piece[rows + row], w, l);
+    o.x = fmaf(po.x, w, o.x), o.y = fmaf(po.y, w, o.y), o.z = fmaf(po.z, w, o.z), o.w = fmaf(po.w, w, o.w);
+}
+template <bool BF16>
+__device__ __forceinline__ void store_row(char *dst, int c, float l, const float4 &o) {
+    const float inv = l > 0.0f || l != l ? __frcp_rn(l) : 0.0f;
+    if (dst) *reinterpret_cast<uint2 *>(dst + c * 2) = pack4<BF16>(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+}
+
 template <int D, int NT, int WARPS, int STAGES, bool BF16>
 __global__ void __launch_bounds__(WARPS * 32, 1) kv_attention_kernel(const Attention a) {
     using S = Shape<D, NT, WARPS, STAGES>;
     extern __shared__ __align__(128) uint8_t smem[];
     uint8_t *const ring_all = smem, *const heads_all = smem + WARPS * S::RING;
     uint64_t *const bars = reinterpret_cast<uint64_t *>(heads_all + WARPS * S::PIECE);
-    // run (sequence * kv_heads + head) of every warp's first and last piece, or -1, and whether the run begins or ends there
+    // of every warp's first and last piece: its run (sequence * kv_heads + head) or -1, 1 if the run ends there + 2 if it began
+    // before, first query and queries of the sequence
     int4 *const notes = reinterpret_cast<int4 *>(bars + WARPS * STAGES);
     uint64_t *const slabs = reinterpret_cast<uint64_t *>(notes + 2 * WARPS) + (threadIdx.x / 32) * 32;
 
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, g = lane / 4, t = lane % 4;
     const int row0 = blockIdx.y * S::ROWS;
     const uint32_t ring = smem_u32(ring_all + warp * S::RING);
     const uint8_t *const ring_ptr = ring_all + warp * S::RING;
     const uint32_t bar = smem_u32(bars + warp * STAGES);
-    if (lane == 0) {
-        for (int i = 0; i < STAGES; ++i) mbar_init(bar + 8 * i, 1);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        notes[2 * warp] = notes[2 * warp + 1] = make_int4(-1, 0, 0, 0);
-    }
+    if (lane < STAGES) mbar_init(bar + 8 * lane, 1);
+    if (lane == 0) notes[2 * warp].x = notes[2 * warp + 1].x = -1;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     __syncwarp();
+    wait_for_front();
 
-    const int64_t total = all_units(a, row0, S::ROWS);
-    const int64_t quota = units_per_warp(a, total, (int64_t)gridDim.x * WARPS);
-    const int64_t begin = ((int64_t)blockIdx.x * WARPS + warp) * quota, end = min(total, begin + quota);
+    // Runs of the first 32 sequences, one a lane, and where they end among all units; those of more sequences are found again.
+    auto ends_of = [&](const Run &r) {
+        uint32_t sum = (uint32_t)r.units * a.kv_heads;
+#pragma unroll
+        for (int k = 1; k < 32; k *= 2) {
+            const uint32_t other = __shfl_up_sync(0xffffffffu, sum, k);
+            if (lane >= k) sum += other;
+        }
+        return sum;
+    };
+    auto run_of = [&](int b) {
+        Run r = {};
+        if (b < a.batch) r = make_run(a, b, row0, S::ROWS);
+        return r;
+    };
+    Run mine = run_of(lane);
+    uint32_t ends = ends_of(mine);
+    uint32_t total = __shfl_sync(0xffffffffu, ends, 31);
+    for (int base = 32; base < a.batch; base += 32) total += __reduce_add_sync(0xffffffffu, (uint32_t)run_of(base + lane).units) * a.kv_heads;
+    const uint32_t quota = units_per_warp(a, total, gridDim.x * WARPS);
+    const uint32_t begin = (blockIdx.x * WARPS + warp) * quota, end = min(total, begin + quota);
 
     if (begin < end) {
         // the sequence, head and unit that the range begins with
-        int b = 0;
-        int64_t before = 0;      // units of the sequences in front
-        for (int base = 0; base < a.batch; base += 32) {
-            const int mine = base + lane < a.batch ? make_run(a, base + lane, row0, S::ROWS).units : 0;
-            int64_t sum = (int64_t)mine * a.kv_heads;
-#pragma unroll
-            for (int k = 1; k < 32; k *= 2) {
-                const int64_t other = __shfl_up_sync(0xffffffffu, sum, k);
-                if (lane >= k) sum += other;
-            }
-            const uint32_t past = __ballot_sync(0xffffffffu, before + sum > begin);
-            if (past) {
-                const int at = __ffs(past) - 1;
-                b = base + at;
-                before += __shfl_sync(0xffffffffu, sum - (int64_t)mine * a.kv_heads, at);
-                break;
-            }
-            before += __shfl_sync(0xffffffffu, sum, 31);
+        uint32_t before = 0, past;
+        int base = 0;
+        while (!(past = __ballot_sync(0xffffffffu, before + ends > begin))) {
+            before += __shfl_sync(0xffffffffu, ends, 31);
+            base += 32;
+            mine = run_of(base + lane);
+            ends = ends_of(mine);
         }
-        Run run = make_run(a, b, row0, S::ROWS);
-        int head = (int)((begin - before) / run.units);
-        int unit = (int)((begin - before) % run.units);
+        const int at_lane = __ffs(past) - 1;
+        int b = base + at_lane;
+        Run run;
+        run.first_query = __shfl_sync(0xffffffffu, mine.first_query, at_lane);
+        run.length = __shfl_sync(0xffffffffu, mine.length, at_lane);
+        run.queries = __shfl_sync(0xffffffffu, mine.queries, at_lane);
+        run.sink_units = __shfl_sync(0xffffffffu, mine.sink_units, at_lane);
+        run.window_unit = __shfl_sync(0xffffffffu, mine.window_unit, at_lane);
+        run.units = __shfl_sync(0xffffffffu, mine.units, at_lane);
+        const uint32_t in_sequence = begin - (before + __shfl_sync(0xffffffffu, ends, at_lane) - (uint32_t)run.units * a.kv_heads);
+        int head = (int)(in_sequence / (uint32_t)run.units);
+        int unit = (int)(in_sequence - (uint32_t)head * run.units);
 
         // The producer's own place, up to STAGES units ahead.  Every lane finds the slab of one of the next 32 units of its run
         // (0: not in the cache); lane 0 asks for them one by one.
@@ -240,7 +272,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_attention_kernel(const Atten
         int done = 0, stage = 0;
         uint32_t parity = 0;
 
-        auto leave = [&](bool whole_run, bool ends) {
+        auto leave = [&](bool whole_run, bool ends_here) {
             // to the output (a run that began and ended here), or to shared memory
             if (whole_run) {
 #pragma unroll
@@ -272,10 +304,143 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_attention_kernel(const Atten
                         *reinterpret_cast<float4 *>(piece + 2 * S::ROWS + row * D + 32 * j + 4 * g) =
                             make_float4(st.o[n][2 * j][e], st.o[n][2 * j][2 + e], st.o[n][2 * j + 1][e], st.o[n][2 * j + 1][2 + e]);
                 }
-            if (lane == 0) notes[2 * warp + (first_piece ? 0 : 1)] = make_int4(b * a.kv_heads + head, 1, ends, 0);
+            if (lane == 0) notes[2 * warp + (first_piece ? 0 : 1)] = make_int4(b * a.kv_heads + head, (ends_here ? 1 : 0) + (first_piece && begins_inside ? 2 : 0), run.first_query, run.queries);
         };
 
-        for (; done < todo; ++done) {
+        // One or two slabs of the run (two: their chains of products and exponentials overlap).
+        auto work = [&](auto count, const uint8_t *const (&slab)[2], const int (&at)[2]) {
+            constexpr int N = decltype(count)::value;
+            float s[N][NT][4];
+#pragma unroll
+            for (int u = 0; u < N; ++u) {
+                uint32_t low[S::WORDS], high[S::WORDS], kl[S::GROUPS], kh[S::GROUPS];
+                read_words<D>(slab[u] + g * S::KEY_ROW + t * S::PIECE_BYTES, low);
+                read_words<D>(slab[u] + (g + 8) * S::KEY_ROW + t * S::PIECE_BYTES, high);
+                read_params<S::GROUPS>(slab[u] + kv_key_params(D) + g * S::GROUPS * 4, kl);
+                read_params<S::GROUPS>(slab[u] + kv_key_params(D) + (g + 8) * S::GROUPS * 4, kh);
+#pragma unroll
+                for (int gr = 0; gr < S::GROUPS; ++gr) {
+                    const __half2 lo = h2(kl[gr]), hi = h2(kh[gr]);
+                    const __half2 bl = __high2half2(lo), bh = __high2half2(hi), bl16 = minus16_of(bl), bh16 = minus16_of(bh);
+                    float acc[NT][4];
+#pragma unroll
+                    for (int j = 2 * gr; j < 2 * gr + 2; ++j) {
+                        __half2 x[4], y[4];
+                        open_word(low[j], bl, bl16, x);
+                        open_word(high[j], bh, bh16, y);
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) {
+                                if (j == 2 * gr && i == 0)
+                                    mma_f16_new(acc[n], h2(x[2 * i]), h2(y[2 * i]), h2(x[2 * i + 1]), h2(y[2 * i + 1]), qf[n][j][2 * i], qf[n][j][2 * i + 1]);
+                                else
+                                    mma_f16(acc[n], h2(x[2 * i]), h2(y[2 * i]), h2(x[2 * i + 1]), h2(y[2 * i + 1]), qf[n][j][2 * i], qf[n][j][2 * i + 1]);
+                            }
+                    }
+                    const float sl = __low2float(lo), sh = __low2float(hi);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) s[u][n][k] = gr ? fmaf(acc[n][k], k < 2 ? sl : sh, s[u][n][k]) : acc[n][k] * (k < 2 ? sl : sh);
+                }
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) s[u][n][k] *= factor[n][k & 1];
+                if (!(at[u] < plain_sinks || (at[u] >= plain_from && at[u] < plain_to))) {
+                    const int token0 = at[u] * KV_SLAB;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const int token = token0 + g + (k / 2) * 8, p = place[n][k & 1];
+                            if (token > p || (a.window && token <= p - a.window && token >= a.sinks)) s[u][n][k] = -INFINITY;
+                        }
+                }
+            }
+            // the maximum moves only where a score passes it by more than 2^8
+            float tops[NT][2];
+            bool passes = false;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    tops[n][e] = fmaxf(s[0][n][e], s[0][n][2 + e]);
+                    if (N == 2) tops[n][e] = fmaxf(tops[n][e], fmaxf(s[N - 1][n][e], s[N - 1][n][2 + e]));
+                    passes |= tops[n][e] > st.m[n][e] + KV_HEADROOM;
+                }
+            if (__any_sync(0xffffffffu, passes)) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float top = fmaxf(tops[n][e], st.m[n][e]);
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                        const float shrink = st.m[n][e] == -INFINITY ? 0.0f : exp2_fast(st.m[n][e] - top);
+                        st.m[n][e] = top;
+                        st.ref[n][e] = top == -INFINITY ? 0.0f : top - KV_SHIFT;
+                        st.l[n][e] *= shrink, st.l[n][2 + e] *= shrink;
+#pragma unroll
+                        for (int i = 0; i < D / 16; ++i) st.o[n][i][e] *= shrink, st.o[n][i][2 + e] *= shrink;
+                    }
+            }
+            uint32_t pb[N][NT][2];
+#pragma unroll
+            for (int u = 0; u < N; ++u)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    float p[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) p[k] = exp2_fast(s[u][n][k] - st.ref[n][k & 1]);
+                    pb[u][n][0] = transpose8x8(h2(__floats2half2_rn(p[0], p[1])));
+                    pb[u][n][1] = transpose8x8(h2(__floats2half2_rn(p[2], p[3])));
+                }
+#pragma unroll
+            for (int u = 0; u < N; ++u) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+                    mma_f16(st.l[n], 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, pb[u][n][0], pb[u][n][1]);   // sums of what is used
+                // outputs
+                uint32_t v0[S::WORDS], v1[S::WORDS], q0[2 * S::GROUPS], q1[2 * S::GROUPS];
+                read_words<D>(slab[u] + kv_value_codes(D) + lane * S::PIECE_BYTES, v0);
+                read_words<D>(slab[u] + kv_value_codes(D) + 32 * S::PIECE_BYTES + lane * S::PIECE_BYTES, v1);
+                read_params<2 * S::GROUPS>(slab[u] + kv_value_params(D) + t * S::GROUPS * 8, q0);
+                read_params<2 * S::GROUPS>(slab[u] + kv_value_params(D) + (t + 4) * S::GROUPS * 8, q1);
+                const int left = run.length - at[u] * KV_SLAB;
+                if (left < KV_SLAB) {   // tokens that are not there may hold anything
+                    const uint32_t keep0 = (2 * t < left ? 0xffffu : 0u) | (2 * t + 1 < left ? 0xffff0000u : 0u);
+                    const uint32_t keep1 = (2 * t + 8 < left ? 0xffffu : 0u) | (2 * t + 9 < left ? 0xffff0000u : 0u);
+#pragma unroll
+                    for (int gr = 0; gr < S::GROUPS; ++gr) {
+                        q0[2 * gr] &= keep0, q0[2 * gr + 1] = (q0[2 * gr + 1] & keep0) | (0x64006400u & ~keep0);
+                        q1[2 * gr] &= keep1, q1[2 * gr + 1] = (q1[2 * gr + 1] & keep1) | (0x64006400u & ~keep1);
+                    }
+                }
+#pragma unroll
+                for (int gr = 0; gr < S::GROUPS; ++gr) {
+                    const __half2 s0 = h2(q0[2 * gr]), s1 = h2(q1[2 * gr]), b0 = h2(q0[2 * gr + 1]), b1 = h2(q1[2 * gr + 1]);
+                    const __half2 b016 = minus16_of(b0), b116 = minus16_of(b1);
+#pragma unroll
+                    for (int j = 2 * gr; j < 2 * gr + 2; ++j) {
+                        __half2 x[4], y[4];
+                        open_word(v0[j], b0, b016, x);
+                        open_word(v1[j], b1, b116, y);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) x[i] = __hmul2(x[i], s0), y[i] = __hmul2(y[i], s1);
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+#pragma unroll
+                            for (int n = 0; n < NT; ++n)
+                                mma_f16(st.o[n][2 * j + i], h2(x[2 * i]), h2(x[2 * i + 1]), h2(y[2 * i]), h2(y[2 * i + 1]), pb[u][n][0], pb[u][n][1]);
+                    }
+                }
+            }
+        };
+
+        while (done < todo) {
             if (fresh) {           // another run: its queries into registers
                 st.clear();
                 fresh = false;
@@ -286,7 +451,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_attention_kernel(const Atten
                 for (int n = 0; n < NT; ++n) {
                     const int row = row0 + 8 * n + g, query = row / a.group;
                     const bool there = query < run.queries;
-                    const char *src = a.q + (run.first_query + query) * a.q_token_stride + (head * a.group + row % a.group) * a.q_head_stride;
+                    const char *src = a.q + (int64_t)(run.first_query + query) * a.q_token_stride + (head * a.group + row % a.group) * a.q_head_stride;
                     float top = 0.0f;
                     uint4 raw[S::WORDS];
 #pragma unroll
@@ -328,146 +493,53 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_attention_kernel(const Atten
                 }
             }
 
-            if (!__all_sync(0xffffffffu, mbar_try_wait(bar + 8 * stage, parity)) && !__all_sync(0xffffffffu, mbar_wait(bar + 8 * stage, parity))) {
-                failed = true;
-                break;
+            const int two = S::PAIRS && todo - done >= 2 && run.units - unit >= 2 ? 2 : 1;
+            const uint8_t *slab[2];
+            int at[2];
+            bool there[2] = {true, true};
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                if (u == two) break;
+                if (!__all_sync(0xffffffffu, mbar_try_wait(bar + 8 * stage, parity)) && !__all_sync(0xffffffffu, mbar_wait(bar + 8 * stage, parity))) {
+                    failed = true;
+                    break;
+                }
+                slab[u] = ring_ptr + stage * S::SLAB;
+                at[u] = run.slab(unit + u);
+                there[u] = *reinterpret_cast<const uint16_t *>(slab[u] + kv_key_params(D)) != 0x7fffu;
+                if (++stage == STAGES) stage = 0, parity ^= 1;
             }
-            const uint8_t *const slab = ring_ptr + stage * S::SLAB;
-            const int at = run.slab(unit);
-            if (++stage == STAGES) stage = 0, parity ^= 1;
-            if (*reinterpret_cast<const uint16_t *>(slab + kv_key_params(D)) != 0x7fffu) {
-                // scores
-                float s[NT][4];
-                uint32_t low[S::WORDS], high[S::WORDS], kl[S::GROUPS], kh[S::GROUPS];
-                read_words<D>(slab + g * S::KEY_ROW + t * S::PIECE_BYTES, low);
-                read_words<D>(slab + (g + 8) * S::KEY_ROW + t * S::PIECE_BYTES, high);
-                read_params<S::GROUPS>(slab + kv_key_params(D) + g * S::GROUPS * 4, kl);
-                read_params<S::GROUPS>(slab + kv_key_params(D) + (g + 8) * S::GROUPS * 4, kh);
-#pragma unroll
-                for (int gr = 0; gr < S::GROUPS; ++gr) {
-                    const __half2 lo = h2(kl[gr]), hi = h2(kh[gr]);
-                    const __half2 bl = __high2half2(lo), bh = __high2half2(hi), bl16 = minus16_of(bl), bh16 = minus16_of(bh);
-                    float acc[NT][4];
-#pragma unroll
-                    for (int j = 2 * gr; j < 2 * gr + 2; ++j) {
-                        __half2 x[4], y[4];
-                        open_word(low[j], bl, bl16, x);
-                        open_word(high[j], bh, bh16, y);
-#pragma unroll
-                        for (int i = 0; i < 2; ++i)
-#pragma unroll
-                            for (int n = 0; n < NT; ++n) {
-                                if (j == 2 * gr && i == 0)
-                                    mma_f16_new(acc[n], h2(x[2 * i]), h2(y[2 * i]), h2(x[2 * i + 1]), h2(y[2 * i + 1]), qf[n][j][2 * i], qf[n][j][2 * i + 1]);
-                                else
-                                    mma_f16(acc[n], h2(x[2 * i]), h2(y[2 * i]), h2(x[2 * i + 1]), h2(y[2 * i + 1]), qf[n][j][2 * i], qf[n][j][2 * i + 1]);
-                            }
-                    }
-                    const float sl = __low2float(lo), sh = __low2float(hi);
-#pragma unroll
-                    for (int n = 0; n < NT; ++n)
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) s[n][k] = gr ? fmaf(acc[n][k], k < 2 ? sl : sh, s[n][k]) : acc[n][k] * (k < 2 ? sl : sh);
-                }
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) s[n][k] *= factor[n][k & 1];
-                if (!(at < plain_sinks || (at >= plain_from && at < plain_to))) {
-                    const int token0 = at * KV_SLAB;
-#pragma unroll
-                    for (int n = 0; n < NT; ++n)
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const int token = token0 + g + (k / 2) * 8, p = place[n][k & 1];
-                            if (token > p || (a.window && token <= p - a.window && token >= a.sinks)) s[n][k] = -INFINITY;
-                        }
-                }
-                // the maximum moves only where a score passes it by more than 2^8
-                bool passes = false;
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) passes |= fmaxf(s[n][e], s[n][2 + e]) > st.m[n][e] + KV_HEADROOM;
-                if (__any_sync(0xffffffffu, passes)) {
-#pragma unroll
-                    for (int n = 0; n < NT; ++n)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            float top = fmaxf(fmaxf(s[n][e], s[n][2 + e]), st.m[n][e]);
-                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                            const float shrink = st.m[n][e] == -INFINITY ? 0.0f : exp2_fast(st.m[n][e] - top);
-                            st.m[n][e] = top;
-                            st.ref[n][e] = top == -INFINITY ? 0.0f : top - KV_SHIFT;
-                            st.l[n][e] *= shrink, st.l[n][2 + e] *= shrink;
-#pragma unroll
-                            for (int i = 0; i < D / 16; ++i) st.o[n][i][e] *= shrink, st.o[n][i][2 + e] *= shrink;
-                        }
-                }
-                uint32_t pb[NT][2];
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    float p[4];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) p[k] = exp2_fast(s[n][k] - st.ref[n][k & 1]);
-                    pb[n][0] = transpose8x8(h2(__floats2half2_rn(p[0], p[1])));
-                    pb[n][1] = transpose8x8(h2(__floats2half2_rn(p[2], p[3])));
-                    mma_f16(st.l[n], 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, pb[n][0], pb[n][1]);   // sums of what is used
-                }
-                // outputs
-                uint32_t v0[S::WORDS], v1[S::WORDS], q0[2 * S::GROUPS], q1[2 * S::GROUPS];
-                read_words<D>(slab + kv_value_codes(D) + lane * S::PIECE_BYTES, v0);
-                read_words<D>(slab + kv_value_codes(D) + 32 * S::PIECE_BYTES + lane * S::PIECE_BYTES, v1);
-                read_params<2 * S::GROUPS>(slab + kv_value_params(D) + t * S::GROUPS * 8, q0);
-                read_params<2 * S::GROUPS>(slab + kv_value_params(D) + (t + 4) * S::GROUPS * 8, q1);
-                const int left = run.length - at * KV_SLAB;
-                if (left < KV_SLAB) {   // tokens that are not there may hold anything
-                    const uint32_t keep0 = (2 * t < left ? 0xffffu : 0u) | (2 * t + 1 < left ? 0xffff0000u : 0u);
-                    const uint32_t keep1 = (2 * t + 8 < left ? 0xffffu : 0u) | (2 * t + 9 < left ? 0xffff0000u : 0u);
-#pragma unroll
-                    for (int gr = 0; gr < S::GROUPS; ++gr) {
-                        q0[2 * gr] &= keep0, q0[2 * gr + 1] = (q0[2 * gr + 1] & keep0) | (0x64006400u & ~keep0);
-                        q1[2 * gr] &= keep1, q1[2 * gr + 1] = (q1[2 * gr + 1] & keep1) | (0x64006400u & ~keep1);
-                    }
-                }
-#pragma unroll
-                for (int gr = 0; gr < S::GROUPS; ++gr) {
-                    const __half2 s0 = h2(q0[2 * gr]), s1 = h2(q1[2 * gr]), b0 = h2(q0[2 * gr + 1]), b1 = h2(q1[2 * gr + 1]);
-                    const __half2 b016 = minus16_of(b0), b116 = minus16_of(b1);
-#pragma unroll
-                    for (int j = 2 * gr; j < 2 * gr + 2; ++j) {
-                        __half2 x[4], y[4];
-                        open_word(v0[j], b0, b016, x);
-                        open_word(v1[j], b1, b116, y);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) x[i] = __hmul2(x[i], s0), y[i] = __hmul2(y[i], s1);
-#pragma unroll
-                        for (int i = 0; i < 2; ++i)
-#pragma unroll
-                            for (int n = 0; n < NT; ++n)
-                                mma_f16(st.o[n][2 * j + i], h2(x[2 * i]), h2(x[2 * i + 1]), h2(y[2 * i]), h2(y[2 * i + 1]), pb[n][0], pb[n][1]);
-                    }
+            if (failed) break;
+            if (S::PAIRS && two == 2 && there[0] && there[1]) {
+                work(std::integral_constant<int, S::PAIRS ? 2 : 1>(), slab, at);
+            } else {
+#pragma unroll 1
+                for (int u = 0; u < two; ++u) {
+                    const uint8_t *const one_slab[2] = {u ? slab[1] : slab[0], nullptr};
+                    const int one_at[2] = {u ? at[1] : at[0], 0};
+                    if (u ? there[1] : there[0]) work(std::integral_constant<int, 1>(), one_slab, one_at);
                 }
             }
-            __syncwarp();          // everyone has read the stage
+            __syncwarp();          // everyone has read the stages
             produce();
+            if (two == 2) produce();
+            done += two;
+            unit += two;
 
-            if (++unit == run.units) {
+            if (unit == run.units) {
                 const bool whole = !(first_piece && begins_inside);
                 leave(whole, true);
                 first_piece = false;
                 fresh = true;
                 unit = 0;
-                if (done + 1 < todo && ++head == a.kv_heads) {
+                if (done < todo && ++head == a.kv_heads) {
                     head = 0;
                     do run = make_run(a, ++b, row0, S::ROWS); while (run.units == 0);
                 }
             }
         }
         if (failed) {              // a copy that never came: those in flight land (or not, within the limit) before the CTA goes
-            for (int i = done + 1; i < issued; ++i) mbar_wait(bar + 8 * (i % STAGES), (i / STAGES) & 1);
+            for (int i = done; i < issued; ++i) mbar_wait(bar + 8 * (i % STAGES), (i / STAGES) & 1);
             if (lane == 0 && a.status) *a.status = 1;
         } else if (unit) {
             __syncwarp();
@@ -476,7 +548,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_attention_kernel(const Atten
     }
     __syncthreads();
 
-    // pieces in order: runs that are whole within the CTA go to the output, the others to the workspace
+    // Pieces in order: runs that are whole within the CTA go to the output, the others to the workspace.
     for (int i = 0; i < 2 * WARPS;) {
         const int4 note = notes[i];
         if (note.x < 0) {
@@ -484,44 +556,29 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_attention_kernel(const Atten
             continue;
         }
         int last = i;
-        bool ends = note.z != 0;
-        for (int k = i + 1; k < 2 * WARPS && !ends; ++k)
-            if (notes[k].x == note.x) last = k, ends = notes[k].z != 0;
-        const int b = note.x / a.kv_heads, head = note.x % a.kv_heads;
-        const Run run = make_run(a, b, row0, S::ROWS);
-        // whether its first unit lies in front of this CTA
-        bool begins = true;
-        {
-            const int64_t cta_begin = (int64_t)blockIdx.x * WARPS * quota;
-            // (only the CTA's first piece can have begun before it)
-            if (i == 0 || notes[0].x == note.x) {
-                int64_t before = 0;
-                for (int k = lane; k < b; k += 32) before += make_run(a, k, row0, S::ROWS).units;
-#pragma unroll
-                for (int k = 16; k; k /= 2) before += __shfl_xor_sync(0xffffffffu, before, k);
-                begins = before * a.kv_heads + (int64_t)head * run.units >= cta_begin;
-            }
-        }
+        bool ends_here = note.y & 1;
+        for (int k = i + 1; k < 2 * WARPS && !ends_here; ++k)
+            if (notes[k].x == note.x) last = k, ends_here = notes[k].y & 1;
+        const bool begins_here = !(i == 0 && (note.y & 2));   // (only the CTA's first piece can have begun before it)
+        const int head = note.x % a.kv_heads;
+        Sequence seq;
+        seq.first_query = note.z, seq.queries = note.w;
         for (int x = threadIdx.x; x < S::ROWS * (D / 4); x += WARPS * 32) {
             const int row = x / (D / 4), c = x % (D / 4) * 4;
-            float m = -INFINITY, l = 0.0f;
+            auto piece_of = [&](int k) { return reinterpret_cast<const float *>(k & 1 ? ring_all + (k / 2) * S::RING : heads_all + (k / 2) * S::PIECE); };
+            float m = -INFINITY;
+#pragma unroll 4
+            for (int k = i; k <= last; ++k)
+                if (notes[k].x == note.x) m = fmaxf(m, piece_of(k)[row]);
+            float l = 0.0f;
             float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            for (int k = i; k <= last; ++k) {
-                if (notes[k].x != note.x) continue;
-                const float *piece = reinterpret_cast<const float *>(k & 1 ? ring_all + (k / 2) * S::RING : heads_all + (k / 2) * S::PIECE);
-                const float pm = piece[row], top = fmaxf(m, pm);
-                const float wa = m == -INFINITY ? 0.0f : exp2_fast(m - top), wb = pm == -INFINITY ? 0.0f : exp2_fast(pm - top);
-                const float4 po = *reinterpret_cast<const float4 *>(piece + 2 * S::ROWS + row * D + c);
-                l = l * wa + piece[S::ROWS + row] * wb;
-                o.x = o.x * wa + po.x * wb, o.y = o.y * wa + po.y * wb, o.z = o.z * wa + po.z * wb, o.w = o.w * wa + po.w * wb;
-                m = top;
-            }
-            if (begins && ends) {
-                char *dst = out_row(a, run, head, row0 + row, D);
-                const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-                if (dst) *reinterpret_cast<uint2 *>(dst + c * 2) = pack4<BF16>(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+#pragma unroll 4
+            for (int k = i; k <= last; ++k)
+                if (notes[k].x == note.x) add_piece(piece_of(k), S::ROWS, row, D, c, m, l, o);
+            if (begins_here && ends_here) {
+                store_row<BF16>(out_row(a, seq, head, row0 + row, D), c, l, o);
             } else {
-                float *piece = a.partial + (((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 2 + (begins ? 1 : 0)) * (S::PIECE / 4);
+                float *piece = a.partial + (((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 2 + (begins_here ? 1 : 0)) * (S::PIECE / 4);
                 if (c == 0) piece[row] = m, piece[S::ROWS + row] = l;
                 *reinterpret_cast<float4 *>(piece + 2 * S::ROWS + row * D + c) = o;
             }
@@ -531,39 +588,33 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_attention_kernel(const Atten
 }
 
 // One CTA a run: joins what several CTAs of kv_attention_kernel have left of it, in their order, and zeroes rows of runs
-// without units.  It finds the CTAs from the lengths, before the kernel in front has ended.
+// without units.  It finds the CTAs from the lengths, before the kernel in front has ended (which began when they were there).
 template <int D, int NT, int WARPS, bool BF16>
-__global__ void __launch_bounds__(128) kv_join_kernel(const Attention a, int ctas) {
+__global__ void __launch_bounds__(256) kv_join_kernel(const Attention a, int ctas) {
     constexpr int ROWS = 8 * NT, PIECE = ROWS * (D + 2);
-    const int b = blockIdx.x / a.kv_heads, head = blockIdx.x % a.kv_heads, lane = threadIdx.x & 31, row0 = blockIdx.y * ROWS;
+    const int b = blockIdx.x / a.kv_heads, head = blockIdx.x - b * a.kv_heads, row0 = blockIdx.y * ROWS;
     const Run run = make_run(a, b, row0, ROWS);
-    int64_t before = 0;
-    for (int k = lane; k < b; k += 32) before += make_run(a, k, row0, ROWS).units;
-#pragma unroll
-    for (int k = 16; k; k /= 2) before += __shfl_xor_sync(0xffffffffu, before, k);
-    const int64_t quota = units_per_warp(a, all_units(a, row0, ROWS), (int64_t)ctas * WARPS) * WARPS;
-    const int64_t first = before * a.kv_heads + (int64_t)head * run.units;
-    const int64_t c0 = first / quota, c1 = run.units ? (first + run.units - 1) / quota : c0;
-    if (run.units && c0 == c1) return;
+    uint32_t first;
+    const uint32_t quota = units_per_warp(a, count_units(a, row0, ROWS, b, first), (uint32_t)ctas * WARPS) * WARPS;
+    first += (uint32_t)head * run.units;
+    const int c0 = first / quota, c1 = run.units ? (first + run.units - 1) / quota : c0;
+    // (CTAs without work wait too: what follows this kernel takes its end for that of the kernel in front)
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    for (int x = threadIdx.x; x < ROWS * (D / 4); x += 128) {
+    if (run.units && c0 == c1) return;
+    for (int x = threadIdx.x; x < ROWS * (D / 4); x += 256) {
         const int row = x / (D / 4), c = x % (D / 4) * 4;
         char *dst = out_row(a, run, head, row0 + row, D);
         if (!dst) continue;
         float m = -INFINITY, l = 0.0f;
         float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (run.units)
-            for (int64_t k = c0; k <= c1; ++k) {
-                const float *piece = a.partial + (((int64_t)blockIdx.y * ctas + k) * 2 + (k == c0 ? 1 : 0)) * PIECE;
-                const float pm = piece[row], top = fmaxf(m, pm);
-                const float wa = m == -INFINITY ? 0.0f : exp2_fast(m - top), wb = pm == -INFINITY ? 0.0f : exp2_fast(pm - top);
-                const float4 po = *reinterpret_cast<const float4 *>(piece + 2 * ROWS + row * D + c);
-                l = l * wa + piece[ROWS + row] * wb;
-                o.x = o.x * wa + po.x * wb, o.y = o.y * wa + po.y * wb, o.z = o.z * wa + po.z * wb, o.w = o.w * wa + po.w * wb;
-                m = top;
-            }
-        const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-        *reinterpret_cast<uint2 *>(dst + c * 2) = pack4<BF16>(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+        if (run.units) {
+            auto piece_of = [&](int k) { return a.partial + (((int64_t)blockIdx.y * ctas + k) * 2 + (k == c0 ? 1 : 0)) * PIECE; };
+#pragma unroll 4
+            for (int k = c0; k <= c1; ++k) m = fmaxf(m, piece_of(k)[row]);
+#pragma unroll 4
+            for (int k = c0; k <= c1; ++k) add_piece(piece_of(k), ROWS, row, D, c, m, l, o);
+        }
+        store_row<BF16>(dst, c, l, o);
     }
 }
 
@@ -595,28 +646,18 @@ Plan plan_of(const AtlasKvAttention &p) {
 template <int D, int NT, int WARPS, int STAGES, bool BF16>
 int launch(const Attention &a, int64_t tiles, int ctas, cudaStream_t stream) {
     using S = Shape<D, NT, WARPS, STAGES>;
+    const char *what = "atlas_kv_attention";
     auto *kernel = kv_attention_kernel<D, NT, WARPS, STAGES, BF16>;
-    int e = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM), "atlas_kv_attention");
+    int e = allow_smem<kv_attention_kernel<D, NT, WARPS, STAGES, BF16>>(S::SMEM, what);
+    if (e == ATLAS_OK) e = launch_early(kernel, dim3((unsigned)ctas, (unsigned)tiles), WARPS * 32, S::SMEM, stream, what, a);
     if (e != ATLAS_OK) return e;
-    kernel<<<dim3((unsigned)ctas, (unsigned)tiles), WARPS * 32, S::SMEM, stream>>>(a);
-    e = check_cuda(cudaGetLastError(), "atlas_kv_attention");
-    if (e != ATLAS_OK) return e;
-    cudaLaunchConfig_t config = {};
-    config.gridDim = dim3((unsigned)(a.batch * a.kv_heads), (unsigned)tiles);
-    config.blockDim = dim3(128);
-    config.stream = stream;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    config.attrs = &attr;
-    config.numAttrs = 1;
-    return check_cuda(cudaLaunchKernelEx(&config, kv_join_kernel<D, NT, WARPS, BF16>, a, ctas), "atlas_kv_attention");
+    return launch_early(kv_join_kernel<D, NT, WARPS, BF16>, dim3((unsigned)(a.batch * a.kv_heads), (unsigned)tiles), 256, 0, stream, what, a, ctas);
 }
 
 template <int D, bool BF16>
 int launch_nt(const Attention &a, const Plan &plan, int ctas, cudaStream_t stream) {
-    if constexpr (D == 64) return plan.nt == 1 ? launch<64, 1, 16, 8, BF16>(a, plan.tiles, ctas, stream) : launch<64, 2, 16, 8, BF16>(a, plan.tiles, ctas, stream);
-    if constexpr (D == 128) return plan.nt == 1 ? launch<128, 1, 16, 4, BF16>(a, plan.tiles, ctas, stream) : launch<128, 2, 12, 4, BF16>(a, plan.tiles, ctas, stream);
+    if constexpr (D == 64) return plan.nt == 1 ? launch<64, 1, 12, 8, BF16>(a, plan.tiles, ctas, stream) : launch<64, 2, 16, 8, BF16>(a, plan.tiles, ctas, stream);
+    if constexpr (D == 128) return plan.nt == 1 ? launch<128, 1, 12, 4, BF16>(a, plan.tiles, ctas, stream) : launch<128, 2, 12, 4, BF16>(a, plan.tiles, ctas, stream);
     if constexpr (D == 256) return plan.nt == 1 ? launch<256, 1, 8, 4, BF16>(a, plan.tiles, ctas, stream) : launch<256, 2, 6, 4, BF16>(a, plan.tiles, ctas, stream);
     return ATLAS_ERR_UNSUPPORTED;
 }
@@ -633,7 +674,7 @@ int check_arguments(const AtlasKvAttention *p, const char *what) {
     ATLAS_RETURN_IF(p->total_queries < 0 || p->batch < 0 || p->max_queries < 0 || p->window < 0 || p->sinks < 0 || p->max_pages < 0,
                     ATLAS_ERR_BAD_ARGUMENT, "%s: negative size", what);
     ATLAS_RETURN_IF(p->total_queries > (1 << 24) || p->batch * (int64_t)p->kv_heads > 0x7fffffff || p->max_queries > (1 << 24) ||
-                        p->max_pages * (int64_t)p->page_size > (1 << 30),
+                        p->max_pages * (int64_t)p->page_size > (1 << 30) || p->batch * (int64_t)p->kv_heads * (p->max_pages * (int64_t)p->page_size / KV_SLAB + 1) > 0x7fffffff,
                     ATLAS_ERR_UNSUPPORTED, "%s: %lld queries of %lld sequences over up to %lld tokens", what, (long long)p->total_queries,
                     (long long)p->batch, (long long)p->max_pages * p->page_size);
     return ATLAS_OK;
@@ -649,7 +690,7 @@ size_t atlas_kv_attention_workspace_bytes(const AtlasKvAttention *p) {
     if (check_arguments(p, "atlas_kv_attention_workspace_bytes") != ATLAS_OK) return 0;
     if (kv_prompt_serves(*p)) return kv_prompt_workspace_bytes(*p);
     const Plan plan = plan_of(*p);
-    return (size_t)plan.tiles * sm_count() * 2 * plan.piece_bytes;
+    return (size_t)plan.tiles * std::max<int64_t>(1, sm_count() / plan.tiles) * 2 * plan.piece_bytes;
 }
 
 int atlas_kv_attention(const AtlasKvAttention *p, void *stream) {
@@ -671,7 +712,7 @@ int atlas_kv_attention(const AtlasKvAttention *p, void *stream) {
     const int dev = check_device();
     if (dev != ATLAS_OK) return dev;
     const Plan plan = plan_of(*p);
-    const int ctas = sm_count();
+    const int ctas = (int)std::max<int64_t>(1, sm_count() / plan.tiles);   // (all row tiles at a time)
     ATLAS_RETURN_IF(!kv_prompt_serves(*p) && plan.tiles > 65535, ATLAS_ERR_UNSUPPORTED, "%s: %lld queries in a sequence", what, (long long)p->max_queries);
     const size_t bytes = atlas_kv_attention_workspace_bytes(p);
     ATLAS_RETURN_IF(bytes && (!p->workspace || p->workspace_bytes < bytes), ATLAS_ERR_CAPACITY, "%s: workspace of %zu bytes, %zu needed", what,

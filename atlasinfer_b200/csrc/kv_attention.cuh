@@ -24,10 +24,42 @@ bool kv_prompt_serves(const AtlasKvAttention &p);
 size_t kv_prompt_workspace_bytes(const AtlasKvAttention &p);
 int kv_prompt(const Attention &a, const AtlasKvAttention &p, cudaStream_t stream);
 
+// Launches a kernel that waits for the one in front itself (griddepcontrol.wait), so that its start overlaps with that one's end.
+template <typename... Parameters, typename... Arguments>
+int launch_early(void (*kernel)(Parameters...), dim3 grid, int threads, int smem, cudaStream_t stream, const char *what, Arguments... arguments) {
+    cudaLaunchConfig_t config = {};
+    config.gridDim = grid;
+    config.blockDim = dim3(threads);
+    config.dynamicSmemBytes = smem;
+    config.stream = stream;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &attr;
+    config.numAttrs = 1;
+    return check_cuda(cudaLaunchKernelEx(&config, kernel, Parameters(arguments)...), what);
+}
+// Dynamic shared memory above the default, set once for each device.
+template <auto Kernel>
+int allow_smem(int bytes, const char *what) {
+    static thread_local int known = -1;
+    int dev = 0;
+    if (cudaGetDevice(&dev) == cudaSuccess && dev == known) return ATLAS_OK;
+    const int e = check_cuda(cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), what);
+    if (e == ATLAS_OK) known = dev;
+    return e;
+}
+
 namespace {
 
+// Nothing is read before the kernels in front have ended; what follows may start then, and wait in turn.
+__device__ __forceinline__ void wait_for_front() {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 struct Sequence {
-    int64_t first_query;         // in q
+    int first_query;             // in q
     int length, queries;
 };
 __device__ __forceinline__ Sequence sequence(const Attention &a, int b) {
@@ -39,7 +71,7 @@ __device__ __forceinline__ Sequence sequence(const Attention &a, int b) {
     } else {
         q0 = b * a.uniform, q1 = q0 + a.uniform;
     }
-    r.first_query = q0;
+    r.first_query = (int)q0;
     r.queries = (int)(q1 - q0);
     r.length = (int)min(max((int64_t)a.lengths[b], (int64_t)0), a.max_tokens);
     return r;
@@ -48,7 +80,7 @@ __device__ __forceinline__ Sequence sequence(const Attention &a, int b) {
 __device__ __forceinline__ char *out_row(const Attention &a, const Sequence &r, int h, int row, int d) {
     const int query = row / a.group;
     if (query >= r.queries) return nullptr;
-    return a.out + ((r.first_query + query) * a.q_heads + h * a.group + row % a.group) * (int64_t)d * 2;
+    return a.out + ((int64_t)(r.first_query + query) * a.q_heads + h * a.group + row - query * a.group) * d * 2;
 }
 
 constexpr float KV_HEADROOM = 8.0f;   // log2: how far a score may pass the running maximum before sums are rescaled

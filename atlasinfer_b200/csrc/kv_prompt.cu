@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_prompt_kernel(const Attentio
     constexpr int PR_REBUILD = P::REBUILD, PR_REBUILDERS = P::REBUILDERS;
     constexpr int TILES = P::TILES, KEYS = P::KEYS, SLABS = P::SLABS, STAGES = P::STAGES, RING = P::RING;
     extern __shared__ uint8_t smem_raw[];
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    wait_for_front();
     const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
     const int head = blockIdx.x % a.kv_heads, b = blockIdx.x / a.kv_heads / splits, split = blockIdx.x / a.kv_heads % splits;
     // later rows see more: those of all heads and sequences go first
@@ -384,7 +384,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_prompt_kernel(const Attentio
             const uint32_t at = bar(P::Q_RAW + warp);
             if (lane == 0) mbar_arrive_expect_tx(at, (uint32_t)min(max(rows - warp * 32, 0), 32) * (D * 2));
             __syncwarp();
-            if (live) bulk_load_1d(smem_u32(raw), a.q + (seq.first_query + query) * a.q_token_stride + (head * a.group + row - query * a.group) * a.q_head_stride, D * 2, at);
+            if (live) bulk_load_1d(smem_u32(raw), a.q + (int64_t)(seq.first_query + query) * a.q_token_stride + (head * a.group + row - query * a.group) * a.q_head_stride, D * 2, at);
             ok = wait_warp<20>(at, 0, s_abort);
             const uint32_t flip = a.scale_log2 < 0.0f ? 0x80008000u : 0u;   // a negative scale turns the queries round: maxima of scores are maxima of products
             float down = 1.0f;
@@ -560,7 +560,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_prompt_kernel(const Attentio
 #pragma unroll 2
                 for (int r = lane / PIECES; r < 32; r += 32 / PIECES) {
                     if (warp * 32 + r < rows)
-                        *reinterpret_cast<uint4 *>(a.out + (((seq.first_query + at.query) * a.q_heads + head * a.group + at.member) * (int64_t)D + piece * 8) * 2) =
+                        *reinterpret_cast<uint4 *>(a.out + (((int64_t)(seq.first_query + at.query) * a.q_heads + head * a.group + at.member) * (int64_t)D + piece * 8) * 2) =
                             tiles ? *reinterpret_cast<const uint4 *>(stage + r * (D * 2) + ((piece ^ (r % 8)) << 4)) : make_uint4(0, 0, 0, 0);
                     at.advance(a, 32 / PIECES);
                 }
@@ -626,22 +626,13 @@ PromptPlan plan_of(const AtlasKvAttention &p) {
 template <int D, bool BF16>
 int launch(const Attention &a, const PromptPlan &plan, cudaStream_t stream) {
     using P = Prompt<D>;
+    const char *what = "atlas_kv_attention";
     auto *kernel = kv_prompt_kernel<D, BF16>;
-    int e = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, P::TOTAL), "atlas_kv_attention");
-    if (e != ATLAS_OK) return e;
-    kernel<<<dim3((unsigned)(a.batch * plan.splits * a.kv_heads), (unsigned)plan.blocks), PR_THREADS, P::TOTAL, stream>>>(a, plan.splits);
-    e = check_cuda(cudaGetLastError(), "atlas_kv_attention");
+    int e = allow_smem<kv_prompt_kernel<D, BF16>>(P::TOTAL, what);
+    if (e == ATLAS_OK) e = launch_early(kernel, dim3((unsigned)(a.batch * plan.splits * a.kv_heads), (unsigned)plan.blocks), PR_THREADS, P::TOTAL, stream, what, a, plan.splits);
     if (e != ATLAS_OK || plan.splits == 1) return e;
-    cudaLaunchConfig_t config = {};
-    config.gridDim = dim3((unsigned)(plan.blocks * P::ROWS * (D / 4) / 256), (unsigned)a.kv_heads, (unsigned)a.batch);
-    config.blockDim = dim3(256);
-    config.stream = stream;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    config.attrs = &attr;
-    config.numAttrs = 1;
-    return check_cuda(cudaLaunchKernelEx(&config, kv_prompt_join_kernel<D, BF16>, a, plan.splits, (int)plan.blocks), "atlas_kv_attention");
+    return launch_early(kv_prompt_join_kernel<D, BF16>, dim3((unsigned)(plan.blocks * P::ROWS * (D / 4) / 256), (unsigned)a.kv_heads, (unsigned)a.batch), 256, 0, stream, what, a,
+                        plan.splits, (int)plan.blocks);
 }
 
 }  // namespace
