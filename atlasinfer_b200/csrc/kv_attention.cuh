@@ -24,21 +24,6 @@ bool kv_prompt_serves(const AtlasKvAttention &p);
 size_t kv_prompt_workspace_bytes(const AtlasKvAttention &p);
 int kv_prompt(const Attention &a, const AtlasKvAttention &p, cudaStream_t stream);
 
-// Launches a kernel that waits for the one in front itself (griddepcontrol.wait), so that its start overlaps with that one's end.
-template <typename... Parameters, typename... Arguments>
-int launch_early(void (*kernel)(Parameters...), dim3 grid, int threads, int smem, cudaStream_t stream, const char *what, Arguments... arguments) {
-    cudaLaunchConfig_t config = {};
-    config.gridDim = grid;
-    config.blockDim = dim3(threads);
-    config.dynamicSmemBytes = smem;
-    config.stream = stream;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    config.attrs = &attr;
-    config.numAttrs = 1;
-    return check_cuda(cudaLaunchKernelEx(&config, kernel, Parameters(arguments)...), what);
-}
 // Dynamic shared memory above the default, set once for each device.
 template <auto Kernel>
 int allow_smem(int bytes, const char *what) {
@@ -51,12 +36,6 @@ int allow_smem(int bytes, const char *what) {
 }
 
 namespace {
-
-// Nothing is read before the kernels in front have ended; what follows may start then, and wait in turn.
-__device__ __forceinline__ void wait_for_front() {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-}
 
 struct Sequence {
     int first_query;             // in q

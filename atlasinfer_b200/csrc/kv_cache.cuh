@@ -41,4 +41,25 @@ __host__ __device__ constexpr int kv_value_unit(int d, int token, int u) {
 
 int check_kv_shape(int64_t num_pages, int64_t kv_heads, int64_t head_dim, int64_t page_size, const char *what);
 
+// Launches a kernel that waits for the one in front itself (griddepcontrol.wait), so that its start overlaps with that one's end.
+template <typename... Parameters, typename... Arguments>
+int launch_early(void (*kernel)(Parameters...), dim3 grid, int threads, int smem, cudaStream_t stream, const char *what, Arguments... arguments) {
+    cudaLaunchConfig_t config = {};
+    config.gridDim = grid;
+    config.blockDim = dim3(threads);
+    config.dynamicSmemBytes = smem;
+    config.stream = stream;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &attr;
+    config.numAttrs = 1;
+    return check_cuda(cudaLaunchKernelEx(&config, kernel, Parameters(arguments)...), what);
+}
+// Nothing is read before the kernels in front have ended; what follows may start then, and wait in turn.
+inline __device__ void wait_for_front() {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 }  // namespace atlas

@@ -38,7 +38,7 @@ struct Tokens {
     int q_heads, kv_heads, rotary, page_size;
     float eps, offset;
     bool wide_positions, wide_slots, wide_weights, interleaved;
-    int heads_per_warp;          // steps of a warp: heads of one token, 256 / D at a time
+    int steps_per_warp, parts, parts_q, parts_k;   // steps of a warp: 256 / D heads each; warps of a token, those for its queries, for its keys
 };
 
 __device__ __forceinline__ float from_bits(uint32_t v, bool high, bool bf16) {
@@ -74,8 +74,16 @@ __device__ __forceinline__ void load_weight(const char *w, bool wide, int channe
     }
 }
 
+// x / s as fp32 rounds it, from the reciprocal as fp32 rounds it: a product, its exact remainder, a correction (Markstein 1990).
+__device__ __forceinline__ float quotient(float x, float s, float inverse) {
+    const float q = __fmul_rn(x, inverse);
+    return __fmaf_rn(__fmaf_rn(-q, s, x), inverse, q);
+}
+// The integer nearest to |x| < 2^21, ties to even: it stands in the low bits of x + 1.5 * 2^23.
+__device__ __forceinline__ int nearest(float x) { return __float_as_int(__fadd_rn(x, 12582912.0f)) - 0x4b400000; }
+
 // Codes, scale and zero point of this thread's 8 channels; the 8 threads of a group hold neighbouring lanes.
-__device__ __forceinline__ void quantise8(float (&x)[8], int (&code)[8], float &scale, float &zero) {
+__device__ __forceinline__ void quantise8(float (&x)[8], int (&code)[8], float &scale, int &zero) {
     float lo = 0.0f, hi = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -88,24 +96,25 @@ __device__ __forceinline__ void quantise8(float (&x)[8], int (&code)[8], float &
         lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, k));
         hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, k));
     }
-    const float s = __fdiv_rn(__fsub_rn(hi, lo), 15.0f);
+    const float s = quotient(__fsub_rn(hi, lo), 15.0f, 1.0f / 15.0f);
     scale = fminf(fmaxf(__int_as_float((__float_as_int(s) + 0x1ffff) & ~0x1ffff), KV_MIN_SCALE), KV_MAX_SCALE);
-    zero = fminf(rintf(__fdiv_rn(-lo, scale)), 15.0f);
+    const float inverse = __frcp_rn(scale);
+    zero = min(nearest(quotient(-lo, scale, inverse)), 15);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) code[i] = (int)fminf(fmaxf(rintf(__fdiv_rn(x[i], scale)) + zero, 0.0f), 15.0f);
+    for (int i = 0; i < 8; ++i) code[i] = min(max(nearest(quotient(x[i], scale, inverse)) + zero, 0), 15);
 }
 
 template <int D>
-__device__ __forceinline__ void store_key(uint8_t *slab, int token, int unit, const int (&c)[8], float scale, float zero) {
+__device__ __forceinline__ void store_key(uint8_t *slab, int token, int unit, const int (&c)[8], float scale, int zero) {
     uint32_t w = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) w |= (uint32_t)c[i] << (4 * ((i & 1) * 4 + i / 2));
     *reinterpret_cast<uint32_t *>(slab + kv_key_word(D, token, unit)) = w;
     if (unit % 8 == 0)
-        *reinterpret_cast<__half2 *>(slab + kv_key_params(D) + (token * (D / 64) + unit / 8) * 4) = __floats2half2_rn(scale, 1024.0f + zero);
+        *reinterpret_cast<__half2 *>(slab + kv_key_params(D) + (token * (D / 64) + unit / 8) * 4) = __floats2half2_rn(scale, (float)(1024 + zero));
 }
 template <int D>
-__device__ __forceinline__ void store_value(uint8_t *slab, int token, int unit, const int (&c)[8], float scale, float zero) {
+__device__ __forceinline__ void store_value(uint8_t *slab, int token, int unit, const int (&c)[8], float scale, int zero) {
     uint8_t *codes = slab + kv_value_codes(D);
 #pragma unroll
     for (int h = 0; h < 2; ++h)
@@ -114,7 +123,7 @@ __device__ __forceinline__ void store_value(uint8_t *slab, int token, int unit, 
     if (unit % 8 == 0) {
         __half *p = reinterpret_cast<__half *>(slab + kv_value_params(D) + (token / 2 * (D / 64) + unit / 8) * 8) + (token & 1);
         p[0] = __float2half_rn(scale);
-        p[2] = __float2half_rn(1024.0f + zero);
+        p[2] = __int2half_rn(1024 + zero);
     }
 }
 
@@ -122,110 +131,168 @@ __device__ __forceinline__ int64_t index_at(const void *p, bool wide, int64_t i)
     return wide ? reinterpret_cast<const int64_t *>(p)[i] : reinterpret_cast<const int32_t *>(p)[i];
 }
 
-// A warp takes `heads_per_warp` steps over the heads of one token (q, then k, then v), 256 / D heads in a step.
-template <int D, bool BF16>
-__global__ void __launch_bounds__(256) tokens_kernel(const Tokens a) {
+// A warp takes up to `steps_per_warp` steps over the heads of one kind (q, k or v) of one token, 256 / D heads in a step; what
+// the token's heads share (angles, weights) stays in registers.
+template <int D, bool BF16, bool STORE>
+__global__ void __launch_bounds__(256, 4) tokens_kernel(const Tokens a) {
     constexpr int UNITS = D / 8, HEADS = 32 / UNITS;   // threads of a head, heads of a warp
     const int lane = threadIdx.x & 31, unit = lane % UNITS, sub = lane / UNITS;
-    const int heads = a.q_heads + 2 * a.kv_heads;   // (without a cache the values are not looked at)
-    const int used = a.cache ? heads : a.q_heads + a.kv_heads;
-    const int steps = (used + HEADS - 1) / HEADS, parts = (steps + a.heads_per_warp - 1) / a.heads_per_warp;
-    const int64_t warp = (int64_t)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
-    const int64_t token = warp / parts;
+    const uint32_t warp = blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
+    const int token = warp / a.parts;
+    int part = warp - token * a.parts;
+    wait_for_front();
     if (token >= a.tokens) return;
-    const int part = (int)(warp - token * parts);
+    const int kind = part < a.parts_q ? 0 : !STORE || part < a.parts_q + a.parts_k ? 1 : 2;
+    part -= kind == 0 ? 0 : kind == 1 ? a.parts_q : a.parts_q + a.parts_k;
+    const int heads = kind == 0 ? a.q_heads : a.kv_heads;
+    const int first = part * a.steps_per_warp * HEADS + sub, past = min(heads, (part + 1) * a.steps_per_warp * HEADS);
 
-    int64_t slot = a.cache ? index_at(a.slots, a.wide_slots, token) : -1;
-    if (slot >= a.num_slots) slot = -1;   // (not in the cache: not stored)
-    const int64_t page = slot >= 0 ? slot / a.page_size : 0;
-    const int in_page = slot >= 0 ? (int)(slot - page * a.page_size) : 0;
-    const int slabs = a.page_size / KV_SLAB;
+    const char *src = a.x[kind] + token * a.token_stride[kind] + unit * 16;
+    const int64_t src_stride = a.head_stride[kind];
+    char *out = kind < 2 ? a.out[kind] : nullptr;
+    if (out) out += ((int64_t)token * heads * D + unit * 8) * 2;
 
-    const bool turned = a.table && unit * 8 < a.rotary;
+    auto load = [&](int head) { return head < past ? *reinterpret_cast<const uint4 *>(src + head * src_stride) : make_uint4(0, 0, 0, 0); };
+    constexpr int AHEAD = 2;     // loads in flight
+    uint4 raw[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) raw[i] = load(first + i * HEADS);
+
+    int64_t slot = -1;
+    uint8_t *slab0 = nullptr;    // of head 0
+    int in_slab = 0;
+    int64_t slab_stride = 0;
+    if (STORE && kind > 0) {
+        slot = index_at(a.slots, a.wide_slots, token);
+        if (slot >= a.num_slots) slot = -1;   // (not in the cache: not stored)
+        if (slot >= 0) {
+            const int64_t page = slot / a.page_size;
+            const int in_page = (int)(slot - page * a.page_size), slabs = a.page_size / KV_SLAB;
+            slab_stride = slabs * (int64_t)kv_slab_bytes(D);
+            slab0 = a.cache + page * a.kv_heads * slab_stride + in_page / KV_SLAB * (int64_t)kv_slab_bytes(D);
+            in_slab = in_page % KV_SLAB;
+        }
+    }
+
     const int half_units = a.rotary / 16;
-    const int partner = sub * UNITS + (a.interleaved || !turned ? unit : unit < half_units ? unit + half_units : unit - half_units);
-    float cs[8], sn[8];
+    const bool turned = kind < 2 && a.table && unit * 8 < a.rotary;
+    const bool halves = kind < 2 && a.table && !a.interleaved;
+    const int mate = !turned || a.interleaved ? unit : unit < half_units ? unit + half_units : unit - half_units;
+    float cs[8], sn[8];          // of the own channels; the sine with the sign that it has there
     if (turned) {
         const int64_t at = index_at(a.positions, a.wide_positions, token);
         const bool known = at >= 0 && at < a.table_rows;   // (elsewhere there is no angle: the token becomes NaN)
         const float *row = a.table + (known ? at : 0) * a.rotary;
-        const int first = a.interleaved ? unit * 4 : (unit % half_units) * 8;   // angle of the first pair
+        if (a.interleaved) {
+            const float4 c = *reinterpret_cast<const float4 *>(row + unit * 4), n = *reinterpret_cast<const float4 *>(row + a.rotary / 2 + unit * 4);
+            cs[0] = cs[1] = c.x, cs[2] = cs[3] = c.y, cs[4] = cs[5] = c.z, cs[6] = cs[7] = c.w;
+            sn[1] = n.x, sn[3] = n.y, sn[5] = n.z, sn[7] = n.w;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int n = a.interleaved ? first + i / 2 : first + i;
-            cs[i] = known ? row[n] : __int_as_float(0x7fc00000);
-            sn[i] = row[a.rotary / 2 + n];
-        }
-        if (!a.interleaved) {
+            for (int i = 0; i < 8; i += 2) sn[i] = -sn[i + 1];
+        } else {
+            const float *c = row + (unit % half_units) * 8, *n = c + a.rotary / 2;
+            const float4 c0 = *reinterpret_cast<const float4 *>(c), c1 = *reinterpret_cast<const float4 *>(c + 4);
+            const float4 n0 = *reinterpret_cast<const float4 *>(n), n1 = *reinterpret_cast<const float4 *>(n + 4);
+            cs[0] = c0.x, cs[1] = c0.y, cs[2] = c0.z, cs[3] = c0.w, cs[4] = c1.x, cs[5] = c1.y, cs[6] = c1.z, cs[7] = c1.w;
+            sn[0] = n0.x, sn[1] = n0.y, sn[2] = n0.z, sn[3] = n0.w, sn[4] = n1.x, sn[5] = n1.y, sn[6] = n1.z, sn[7] = n1.w;
             if (unit < half_units) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) sn[i] = -sn[i];
             }
-        } else {
+        }
+        if (!known) {
 #pragma unroll
-            for (int i = 0; i < 8; i += 2) sn[i] = -sn[i];
+            for (int i = 0; i < 8; ++i) cs[i] = __int_as_float(0x7fc00000);
+        }
+    }
+    const char *weight = kind < 2 ? a.weight[kind] : nullptr;
+    if (weight) {                // weights go with the angles: (x norm) (w cos) + (y norm) (w' sin)
+        float w[8], wm[8];       // of the own channels and of those that they turn with
+        load_weight<BF16>(weight, a.wide_weights, unit * 8, w);
+        load_weight<BF16>(weight, a.wide_weights, mate * 8, wm);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float own = __fadd_rn(w[i], a.offset), other = __fadd_rn(a.interleaved ? w[i ^ 1] : wm[i], a.offset);
+            cs[i] = turned ? cs[i] * own : own;
+            sn[i] = sn[i] * other;
         }
     }
 
-    for (int step = part * a.heads_per_warp; step < min(steps, (part + 1) * a.heads_per_warp); ++step) {
-        const int head = step * HEADS + sub;
-        const bool live = head < used;
-        const int kind = head < a.q_heads ? 0 : head < a.q_heads + a.kv_heads ? 1 : 2;
-        const int own = kind == 0 ? head : kind == 1 ? head - a.q_heads : head - a.q_heads - a.kv_heads;
-        uint4 raw = make_uint4(0, 0, 0, 0);
-        if (live) raw = *reinterpret_cast<const uint4 *>(a.x[kind] + token * a.token_stride[kind] + own * a.head_stride[kind] + unit * 16);
+    auto work = [&](int head, const uint4 &raw) {
+        const bool live = head < past;
         float x[8];
         unpack8<BF16>(raw, x);
-        const bool any_turn = __any_sync(0xffffffffu, live && kind < 2);
-        if (any_turn) {
-            const char *weight = kind < 2 ? a.weight[kind] : nullptr;
-            float norm = 1.0f;
-            if (a.weight[0] || a.weight[1]) {
-                float sum = 0.0f;
+        if (weight) {
+            float sum = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) sum += x[i] * x[i];
+            for (int i = 0; i < 8; ++i) sum += x[i] * x[i];
 #pragma unroll
-                for (int k = 1; k < UNITS; k *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, k);
-                norm = rsqrtf(sum * (1.0f / D) + a.eps);
-            }
+            for (int k = 1; k < UNITS; k *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+            const float norm = rsqrtf(sum * (1.0f / D) + a.eps);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] *= norm;
+        }
+        if (halves) {            // the numbers that these turn with, of the same head
+            float y[8];
+            const int from = sub * UNITS + mate;
             if (weight) {
-                float w[8];
-                load_weight<BF16>(weight, a.wide_weights, unit * 8, w);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(__fmul_rn(x[i], norm), __fadd_rn(w[i], a.offset));
+                for (int i = 0; i < 8; ++i) y[i] = __shfl_sync(0xffffffffu, x[i], from);
+            } else {
+                uint4 other;
+                other.x = __shfl_sync(0xffffffffu, raw.x, from), other.y = __shfl_sync(0xffffffffu, raw.y, from);
+                other.z = __shfl_sync(0xffffffffu, raw.z, from), other.w = __shfl_sync(0xffffffffu, raw.w, from);
+                unpack8<BF16>(other, y);
             }
-            if (a.table) {
-                float y[8];
+            if (turned) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) y[i] = a.interleaved ? x[i ^ 1] : __shfl_sync(0xffffffffu, x[i], partner);
-                if (turned && kind < 2) {
+                for (int i = 0; i < 8; ++i) x[i] = __fadd_rn(__fmul_rn(x[i], cs[i]), __fmul_rn(y[i], sn[i]));
+            } else if (weight) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) x[i] = __fadd_rn(__fmul_rn(x[i], cs[i]), __fmul_rn(y[i], sn[i]));
-                }
+                for (int i = 0; i < 8; ++i) x[i] *= cs[i];
             }
+        } else if (turned) {
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                const float e = x[i], o = x[i + 1];
+                x[i] = __fadd_rn(__fmul_rn(e, cs[i]), __fmul_rn(o, sn[i]));
+                x[i + 1] = __fadd_rn(__fmul_rn(o, cs[i + 1]), __fmul_rn(e, sn[i + 1]));
+            }
+        } else if (weight) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] *= cs[i];
         }
-        if (live && kind < 2 && a.out[kind]) {
-            const int64_t n = kind ? a.kv_heads : a.q_heads;
-            *reinterpret_cast<uint4 *>(a.out[kind] + ((token * n + own) * D + unit * 8) * 2) = pack8<BF16>(x);
-        }
-        if (a.cache && __any_sync(0xffffffffu, live && kind > 0)) {
-            int code[8];
-            float scale, zero;
+        if (out && live) *reinterpret_cast<uint4 *>(out + (int64_t)head * (D * 2)) = pack8<BF16>(x);
+        if (STORE && kind > 0) {
+            int code[8], zero;
+            float scale;
             quantise8(x, code, scale, zero);
-            if (live && kind > 0 && slot >= 0) {
-                uint8_t *slab = a.cache + ((page * a.kv_heads + own) * slabs + in_page / KV_SLAB) * (int64_t)kv_slab_bytes(D);
-                if (kind == 1) store_key<D>(slab, in_page % KV_SLAB, unit, code, scale, zero);
-                else store_value<D>(slab, in_page % KV_SLAB, unit, code, scale, zero);
+            if (live && slot >= 0) {
+                uint8_t *slab = slab0 + head * slab_stride;
+                if (kind == 1) store_key<D>(slab, in_slab, unit, code, scale, zero);
+                else store_value<D>(slab, in_slab, unit, code, scale, zero);
             }
+        }
+    };
+    for (int head = first; head - sub < past; head += AHEAD * HEADS) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            if (head - sub + i * HEADS >= past) break;
+            const uint4 now = raw[i];
+            raw[i] = load(head + (i + AHEAD) * HEADS);
+            work(head + i * HEADS, now);
         }
     }
 }
 
 // Stored keys and values as fp16 (exact) or bf16; zeros for slots that are not in the cache.  A thread makes 8 channels of both.
 template <int D, bool BF16>
-__global__ void __launch_bounds__(256) load_kernel(const uint8_t *cache, const void *slots, bool wide_slots, int64_t tokens, int64_t num_slots,
-                                                   int kv_heads, int page_size, char *k_out, char *v_out) {
+__global__ void __launch_bounds__(256) load_kernel(const void *cache_bytes, const void *slots, bool wide_slots, int64_t tokens, int64_t num_slots,
+                                                   int kv_heads, int page_size, void *k_to, void *v_to) {
     constexpr int UNITS = D / 8;
+    const uint8_t *cache = (const uint8_t *)cache_bytes;
+    char *k_out = (char *)k_to, *v_out = (char *)v_to;
+    wait_for_front();
     const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     const int64_t row = i / UNITS;
     const int unit = (int)(i % UNITS);
@@ -300,7 +367,7 @@ int atlas_norm_rotate(const AtlasTokens *p, void *stream) {
     const bool q_fits = !p->q_heads || (aligned16(p->q, 2 * p->q_token_stride, 2 * p->q_head_stride) && aligned16(p->q_out, 0, 0));
     const bool v_fits = !store || (aligned16(p->v, 2 * p->v_token_stride, 2 * p->v_head_stride) && aligned16(p->cache, 0, 0));
     ATLAS_RETURN_IF(!q_fits || !v_fits || !aligned16(p->k, 2 * p->k_token_stride, 2 * p->k_head_stride) || !aligned16(p->k_out, 0, 0) ||
-                        !aligned16(p->q_weight, 0, 0) || !aligned16(p->k_weight, 0, 0),
+                        !aligned16(p->q_weight, 0, 0) || !aligned16(p->k_weight, 0, 0) || !aligned16(p->table, 0, 0),
                     ATLAS_ERR_BAD_ARGUMENT, "%s: pointers and strides must be multiples of 16 bytes", what);
     const int dev = check_device();
     if (dev != ATLAS_OK) return dev;
@@ -318,14 +385,18 @@ int atlas_norm_rotate(const AtlasTokens *p, void *stream) {
     a.eps = p->eps, a.offset = p->weight_offset;
     a.wide_positions = p->position_bytes == 8, a.wide_slots = p->slot_bytes == 8, a.wide_weights = p->weights_f32 != 0;
     a.interleaved = p->interleaved != 0;
-    const int heads = p->q_heads + (store ? 2 : 1) * p->kv_heads;
-    const int steps = (int)ceil_div_i64(heads, 256 / p->head_dim);
-    a.heads_per_warp = 1;
-    const int64_t warps = p->tokens * ceil_div_i64(steps, a.heads_per_warp), blocks = ceil_div_i64(warps, 8);
-    ATLAS_RETURN_IF(blocks > 0x7fffffff, ATLAS_ERR_UNSUPPORTED, "%s: %lld tokens", what, (long long)p->tokens);
+    // Few tokens: a step a warp, so that all loads are under way at once.  Many: up to 8 steps, which share angles and weights,
+    // as long as there are 16 warps an SM (4001 tokens of 72 heads of 128: 1 step XXX us, 4 XXX, 8 XXX).
+    const int64_t at_a_time = 256 / p->head_dim, q_steps = ceil_div_i64(p->q_heads, at_a_time), kv_steps = ceil_div_i64(p->kv_heads, at_a_time);
+    a.steps_per_warp = (int)std::min<int64_t>(8, std::max<int64_t>(1, p->tokens * (q_steps + (store ? 2 : 1) * kv_steps) / (148 * 16)));
+    a.parts_q = (int)ceil_div_i64(q_steps, a.steps_per_warp), a.parts_k = (int)ceil_div_i64(kv_steps, a.steps_per_warp);
+    a.parts = a.parts_q + (store ? 2 : 1) * a.parts_k;
+    const int64_t blocks = ceil_div_i64(p->tokens * a.parts, 8);
+    ATLAS_RETURN_IF(blocks > (1 << 28), ATLAS_ERR_UNSUPPORTED, "%s: %lld tokens", what, (long long)p->tokens);
     return by_type(p->head_dim, p->dtype, [&](auto d, auto bf16) {
-        tokens_kernel<decltype(d)::value, decltype(bf16)::value><<<(unsigned)blocks, 256, 0, (cudaStream_t)stream>>>(a);
-        return check_cuda(cudaGetLastError(), what);
+        constexpr int D = decltype(d)::value;
+        constexpr bool B = decltype(bf16)::value;
+        return launch_early(store ? tokens_kernel<D, B, true> : tokens_kernel<D, B, false>, dim3((unsigned)blocks), 256, 0, (cudaStream_t)stream, what, a);
     });
 }
 
@@ -348,9 +419,8 @@ int atlas_kv_load(const void *cache, int64_t num_pages, int kv_heads, int head_d
     const int64_t blocks = ceil_div_i64(tokens * kv_heads * (head_dim / 8), 256);
     ATLAS_RETURN_IF(blocks > 0x7fffffff, ATLAS_ERR_UNSUPPORTED, "%s: %lld tokens", what, (long long)tokens);
     return by_type(head_dim, dtype, [&](auto d, auto bf16) {
-        load_kernel<decltype(d)::value, decltype(bf16)::value><<<(unsigned)blocks, 256, 0, (cudaStream_t)stream>>>(
-            (const uint8_t *)cache, slots, slot_bytes == 8, tokens, num_pages * page_size, kv_heads, page_size, (char *)k_out, (char *)v_out);
-        return check_cuda(cudaGetLastError(), what);
+        return launch_early(load_kernel<decltype(d)::value, decltype(bf16)::value>, dim3((unsigned)blocks), 256, 0, (cudaStream_t)stream, what, cache, slots, slot_bytes == 8,
+                            tokens, num_pages * page_size, kv_heads, page_size, k_out, v_out);
     });
 }
 

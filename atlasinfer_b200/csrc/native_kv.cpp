@@ -84,7 +84,7 @@ std::pair<Maybe, Maybe> norm_rotate(const Maybe &q_in, const Tensor &k_in, const
         if (table_in->scalar_type() != at::kFloat) throw py::type_error("table must be fp32");
         if (table_in->dim() != 2 || table_in->size(0) < 1) throw py::value_error("table must be [positions, rotary_dim], got " + shape_of(*table_in));
         if (table_in->device() != k.device()) throw py::value_error("table must be on the device of the other tensors");
-        table = table_in->contiguous();
+        table = reinterpret_cast<uintptr_t>(table_in->data_ptr()) & 15 ? table_in->clone(at::MemoryFormat::Contiguous) : table_in->contiguous();
         positions = index_tensor(*positions_in, "positions", tokens, k.device());
         a.table = table.const_data_ptr<float>(), a.table_rows = table.size(0);
         a.rotary_dim = (int32_t)std::min<int64_t>(table.size(1), INT32_MAX);
