@@ -104,7 +104,6 @@ template <int D, int NT, int WARPS, int STAGES>
 struct Shape {
     static constexpr int ROWS = 8 * NT, GROUPS = D / 64, WORDS = D / 32;   // words: a lane's, of a token's key
     static constexpr int SLAB = kv_slab_bytes(D);
-    static constexpr bool PAIRS = NT == 1;                 // two slabs at a time
     static constexpr int PIECE_BYTES = D == 64 ? 8 : 16, KEY_ROW = 4 * PIECE_BYTES;   // of a lane's codes (in a plane); of a token's
     static constexpr int PIECE = ROWS * (D + 2) * 4;       // maximum, sum and output of the rows
     static constexpr int RING = STAGES * SLAB;             // a warp's; holds its last piece in the end
@@ -493,7 +492,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_attention_kernel(const Atten
                 }
             }
 
-            const int two = S::PAIRS && todo - done >= 2 && run.units - unit >= 2 ? 2 : 1;
+            const int two = todo - done >= 2 && run.units - unit >= 2 ? 2 : 1;
             const uint8_t *slab[2];
             int at[2];
             bool there[2] = {true, true};
@@ -510,8 +509,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_attention_kernel(const Atten
                 if (++stage == STAGES) stage = 0, parity ^= 1;
             }
             if (failed) break;
-            if (S::PAIRS && two == 2 && there[0] && there[1]) {
-                work(std::integral_constant<int, S::PAIRS ? 2 : 1>(), slab, at);
+            if (two == 2 && there[0] && there[1]) {
+                work(std::integral_constant<int, 2>(), slab, at);
             } else {
 #pragma unroll 1
                 for (int u = 0; u < two; ++u) {
@@ -548,33 +547,34 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_attention_kernel(const Atten
     }
     __syncthreads();
 
-    // Pieces in order: runs that are whole within the CTA go to the output, the others to the workspace.
-    for (int i = 0; i < 2 * WARPS;) {
-        const int4 note = notes[i];
-        if (note.x < 0) {
-            ++i;
-            continue;
-        }
-        int last = i;
-        bool ends_here = note.y & 1;
-        for (int k = i + 1; k < 2 * WARPS && !ends_here; ++k)
-            if (notes[k].x == note.x) last = k, ends_here = notes[k].y & 1;
-        const bool begins_here = !(i == 0 && (note.y & 2));   // (only the CTA's first piece can have begun before it)
-        const int head = note.x % a.kv_heads;
+    // Pieces in order: runs that are whole within the CTA go to the output, the others to the workspace.  Lane k looks at note k.
+    static_assert(2 * WARPS <= 32, "a lane a note");
+    const int4 note = lane < 2 * WARPS ? notes[lane] : make_int4(-1, 0, 0, 0);
+    for (uint32_t left = __ballot_sync(0xffffffffu, note.x >= 0); left;) {
+        const int i = __ffs(left) - 1, id = __shfl_sync(0xffffffffu, note.x, i);
+        const uint32_t members = __ballot_sync(0xffffffffu, note.x == id);
+        left &= ~members;
+        const bool ends_here = __any_sync(0xffffffffu, note.x == id && (note.y & 1));
+        const bool begins_here = !(i == 0 && (__shfl_sync(0xffffffffu, note.y, 0) & 2));   // (only the CTA's first piece can have begun before it)
         Sequence seq;
-        seq.first_query = note.z, seq.queries = note.w;
+        seq.first_query = __shfl_sync(0xffffffffu, note.z, i), seq.queries = __shfl_sync(0xffffffffu, note.w, i);
+        const int head = id % a.kv_heads;
         for (int x = threadIdx.x; x < S::ROWS * (D / 4); x += WARPS * 32) {
             const int row = x / (D / 4), c = x % (D / 4) * 4;
-            auto piece_of = [&](int k) { return reinterpret_cast<const float *>(k & 1 ? ring_all + (k / 2) * S::RING : heads_all + (k / 2) * S::PIECE); };
+            // first pieces are a piece apart, last ones a ring
             float m = -INFINITY;
 #pragma unroll 4
-            for (int k = i; k <= last; ++k)
-                if (notes[k].x == note.x) m = fmaxf(m, piece_of(k)[row]);
+            for (int w = 0; w < WARPS; ++w) {
+                if (members >> (2 * w) & 1) m = fmaxf(m, reinterpret_cast<const float *>(heads_all + w * S::PIECE)[row]);
+                if (members >> (2 * w) & 2) m = fmaxf(m, reinterpret_cast<const float *>(ring_all + w * S::RING)[row]);
+            }
             float l = 0.0f;
             float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
-            for (int k = i; k <= last; ++k)
-                if (notes[k].x == note.x) add_piece(piece_of(k), S::ROWS, row, D, c, m, l, o);
+            for (int w = 0; w < WARPS; ++w) {
+                if (members >> (2 * w) & 1) add_piece(reinterpret_cast<const float *>(heads_all + w * S::PIECE), S::ROWS, row, D, c, m, l, o);
+                if (members >> (2 * w) & 2) add_piece(reinterpret_cast<const float *>(ring_all + w * S::RING), S::ROWS, row, D, c, m, l, o);
+            }
             if (begins_here && ends_here) {
                 store_row<BF16>(out_row(a, seq, head, row0 + row, D), c, l, o);
             } else {
@@ -583,7 +583,6 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_attention_kernel(const Atten
                 *reinterpret_cast<float4 *>(piece + 2 * S::ROWS + row * D + c) = o;
             }
         }
-        i = last + 1;
     }
 }
 
@@ -607,12 +606,28 @@ __global__ void __launch_bounds__(256) kv_join_kernel(const Attention a, int cta
         if (!dst) continue;
         float m = -INFINITY, l = 0.0f;
         float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (run.units) {
-            auto piece_of = [&](int k) { return a.partial + (((int64_t)blockIdx.y * ctas + k) * 2 + (k == c0 ? 1 : 0)) * PIECE; };
-#pragma unroll 4
-            for (int k = c0; k <= c1; ++k) m = fmaxf(m, piece_of(k)[row]);
-#pragma unroll 4
-            for (int k = c0; k <= c1; ++k) add_piece(piece_of(k), ROWS, row, D, c, m, l, o);
+        for (int k0 = run.units ? c0 : c1 + 1; k0 <= c1; k0 += 4) {   // four pieces' loads at a time
+            float pm[4], pl[4];
+            float4 po[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int k = min(k0 + u, c1);
+                const float *piece = a.partial + (((int64_t)blockIdx.y * ctas + k) * 2 + (k == c0 ? 1 : 0)) * PIECE;
+                pm[u] = k0 + u <= c1 ? piece[row] : -INFINITY;
+                pl[u] = piece[ROWS + row];
+                po[u] = *reinterpret_cast<const float4 *>(piece + 2 * ROWS + row * D + c);
+            }
+            const float top = fmaxf(m, fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3])));
+            const float keep = m == -INFINITY ? 0.0f : exp2_fast(m - top);
+            m = top;
+            l *= keep, o.x *= keep, o.y *= keep, o.z *= keep, o.w *= keep;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const float w = pm[u] == -INFINITY ? 0.0f : exp2_fast(pm[u] - top);
+                if (k0 + u > c1) break;
+                l = fmaf(pl[u], w, l);
+                o.x = fmaf(po[u].x, w, o.x), o.y = fmaf(po[u].y, w, o.y), o.z = fmaf(po[u].z, w, o.z), o.w = fmaf(po[u].w, w, o.w);
+            }
         }
         store_row<BF16>(dst, c, l, o);
     }
@@ -637,7 +652,11 @@ struct Plan {
 Plan plan_of(const AtlasKvAttention &p) {
     Plan plan;
     const int64_t rows = p.max_queries * (p.q_heads / p.kv_heads);
-    plan.nt = rows > 8 ? 2 : 1;
+    // Rows 8 at a time, or 16, which takes 1.7 times as long a slab and more to start and to join: for 9 to 16 and 25 to 32 rows
+    // of 128 channels and contexts that may be long (16 sequences of 8000 tokens, 16 rows: 49 us 8 at a time, 42 16 at a time;
+    // 4 of 4000 on 2 kv heads: 15 and 24; 8 of 4000, 24 rows: 40 and 41).
+    const int64_t slabs = p.batch * p.kv_heads * (p.max_pages * p.page_size / KV_SLAB);
+    plan.nt = p.head_dim == 128 && ceil_div_i64(rows, 8) % 2 == 0 && slabs >= 12000 ? 2 : 1;
     plan.tiles = ceil_div_i64(std::max<int64_t>(rows, 1), 8 * plan.nt);
     plan.piece_bytes = (size_t)8 * plan.nt * (p.head_dim + 2) * 4;
     return plan;
@@ -656,9 +675,10 @@ int launch(const Attention &a, int64_t tiles, int ctas, cudaStream_t stream) {
 
 template <int D, bool BF16>
 int launch_nt(const Attention &a, const Plan &plan, int ctas, cudaStream_t stream) {
-    if constexpr (D == 64) return plan.nt == 1 ? launch<64, 1, 12, 8, BF16>(a, plan.tiles, ctas, stream) : launch<64, 2, 16, 8, BF16>(a, plan.tiles, ctas, stream);
-    if constexpr (D == 128) return plan.nt == 1 ? launch<128, 1, 12, 4, BF16>(a, plan.tiles, ctas, stream) : launch<128, 2, 12, 4, BF16>(a, plan.tiles, ctas, stream);
-    if constexpr (D == 256) return plan.nt == 1 ? launch<256, 1, 8, 4, BF16>(a, plan.tiles, ctas, stream) : launch<256, 2, 6, 4, BF16>(a, plan.tiles, ctas, stream);
+    // Warps and slabs in flight: what registers (168, 255) and shared memory hold.
+    if constexpr (D == 64) return launch<64, 1, 12, 8, BF16>(a, plan.tiles, ctas, stream);
+    if constexpr (D == 128) return plan.nt == 1 ? launch<128, 1, 12, 4, BF16>(a, plan.tiles, ctas, stream) : launch<128, 2, 8, 5, BF16>(a, plan.tiles, ctas, stream);
+    if constexpr (D == 256) return launch<256, 1, 8, 4, BF16>(a, plan.tiles, ctas, stream);
     return ATLAS_ERR_UNSUPPORTED;
 }
 

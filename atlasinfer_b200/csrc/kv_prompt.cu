@@ -20,6 +20,7 @@ namespace atlas {
 
 namespace {
 
+constexpr int PR_SMS = 148;
 constexpr int PR_THREADS = 16 * 32, PR_MMA = 14, PR_LOAD = 15;   // warps of the roles: softmax, rebuilding, MMA, loads
 
 template <int D>
@@ -618,8 +619,10 @@ PromptPlan plan_of(const AtlasKvAttention &p) {
     PromptPlan plan;
     const int64_t rows = p.max_queries * (p.q_heads / p.kv_heads), block = p.head_dim == 256 ? 128 : 256;
     plan.blocks = ceil_div_i64(std::max<int64_t>(rows, 1), block);
-    plan.splits = 1;
-    plan.bytes = 0;
+    // CTAs for most SMs: the tokens are split where there are few row blocks, into parts of four tiles at least.
+    const int64_t ctas = plan.blocks * p.kv_heads * p.batch, tiles = p.max_pages * p.page_size / 128;
+    plan.splits = (int)std::max<int64_t>(1, std::min<int64_t>({PR_SMS / std::max<int64_t>(ctas, 1), tiles / 4, 16}));
+    plan.bytes = plan.splits > 1 ? (size_t)(p.batch * plan.splits * p.kv_heads * plan.blocks * block * (p.head_dim + 4) * 4) : 0;
     return plan;
 }
 
@@ -637,7 +640,11 @@ int launch(const Attention &a, const PromptPlan &plan, cudaStream_t stream) {
 
 }  // namespace
 
-bool kv_prompt_serves(const AtlasKvAttention &p) { return p.max_queries * (p.q_heads / p.kv_heads) > 64 && p.batch * p.kv_heads <= (1 << 20); }
+// From 33 rows of a kv head on (25 of 256 channels): 8 sequences of 4000 tokens on 8 kv heads, 48 rows of 128 channels 45 us and
+// 55 by kv_attention_kernel, 32 rows 44 and 41; 32 rows of 256 channels (4 of 8000 on 2) 32 and 48, 16 rows 29 and 34.
+bool kv_prompt_serves(const AtlasKvAttention &p) {
+    return p.max_queries * (p.q_heads / p.kv_heads) > (p.head_dim == 256 ? 24 : 32) && p.batch * p.kv_heads <= (1 << 20);
+}
 
 size_t kv_prompt_workspace_bytes(const AtlasKvAttention &p) { return plan_of(p).bytes; }
 

@@ -79,6 +79,24 @@ def test_many_queries(cuda_device, lengths, queries, hq, hkv, d, dtype):
     Work(cuda_device, lengths, queries, hq, hkv, d, dtype=dtype, page=48).check()
 
 
+@pytest.mark.parametrize("dtype", (F16, BF16))
+@pytest.mark.parametrize("lengths,queries,hq,hkv,d,window", [([3000, 2100], [20, 33], 8, 2, 128, None), ([5000], [60], 2, 1, 64, None), ([2500, 70, 0], [30, 40, 9], 16, 2, 256, None),
+                                                             ([4000, 3100], [100, 90], 4, 2, 128, 700)])
+def test_split_contexts(cuda_device, lengths, queries, hq, hkv, d, window, dtype):
+    """Some tens of rows over long contexts: the tokens are split among CTAs and joined."""
+    Work(cuda_device, lengths, queries, hq, hkv, d, dtype=dtype, page=64, lean=0.3).check(window=window, sinks=5 if window else 0)
+
+
+@pytest.mark.parametrize("rows", (8, 9, 16, 17, 25, 32, 33))
+@pytest.mark.parametrize("d", (64, 128, 256))
+def test_rows_of_a_group(cuda_device, rows, d):
+    """Every number of row tiles, few tokens and many (with room in the page table, which the choice of the kernel goes by)."""
+    w = Work(cuda_device, [2000, 33, 500], [1, 1, 1], rows, 1, d, page=16)
+    w.check()
+    w.table = torch.cat([w.table, torch.full((3, 5000), -1, dtype=torch.int32, device=cuda_device)], 1)
+    w.check()
+
+
 @pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (16, 0), (17, 4), (100, 16), (100, 33), (5000, 7), (64, 500), (2 ** 31 - 1, 2 ** 31 - 1)])
 @pytest.mark.parametrize("lengths,queries,hq,hkv,d", [([1, 18, 500, 77, 1200], [1] * 5, 8, 2, 128), ([300, 40, 801], [90, 3, 260], 4, 1, 64), ([400], [400], 2, 2, 256)])
 def test_window_and_sinks(cuda_device, lengths, queries, hq, hkv, d, window, sinks):
