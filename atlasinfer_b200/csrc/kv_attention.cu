@@ -558,20 +558,20 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_attention_kernel(const Atten
         const bool begins_here = !(i == 0 && (__shfl_sync(0xffffffffu, note.y, 0) & 2));   // (only the CTA's first piece can have begun before it)
         Sequence seq;
         seq.first_query = __shfl_sync(0xffffffffu, note.z, i), seq.queries = __shfl_sync(0xffffffffu, note.w, i);
-        const int head = id % a.kv_heads;
+        const int head = id % a.kv_heads, w0 = i / 2, w1 = (31 - __clz(members)) / 2;
         for (int x = threadIdx.x; x < S::ROWS * (D / 4); x += WARPS * 32) {
             const int row = x / (D / 4), c = x % (D / 4) * 4;
             // first pieces are a piece apart, last ones a ring
             float m = -INFINITY;
 #pragma unroll 4
-            for (int w = 0; w < WARPS; ++w) {
+            for (int w = w0; w <= w1; ++w) {
                 if (members >> (2 * w) & 1) m = fmaxf(m, reinterpret_cast<const float *>(heads_all + w * S::PIECE)[row]);
                 if (members >> (2 * w) & 2) m = fmaxf(m, reinterpret_cast<const float *>(ring_all + w * S::RING)[row]);
             }
             float l = 0.0f;
             float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
-            for (int w = 0; w < WARPS; ++w) {
+            for (int w = w0; w <= w1; ++w) {
                 if (members >> (2 * w) & 1) add_piece(reinterpret_cast<const float *>(heads_all + w * S::PIECE), S::ROWS, row, D, c, m, l, o);
                 if (members >> (2 * w) & 2) add_piece(reinterpret_cast<const float *>(ring_all + w * S::RING), S::ROWS, row, D, c, m, l, o);
             }
