@@ -53,8 +53,18 @@ __device__ __forceinline__ uint32_t count_units(const Attention &a, int row0, in
     in_front = __reduce_add_sync(0xffffffffu, front) * a.kv_heads;
     return __reduce_add_sync(0xffffffffu, sum) * a.kv_heads;
 }
-__device__ __forceinline__ uint32_t units_per_warp(const Attention &a, uint32_t total, uint32_t warps) {
-    return max((total + warps - 1) / warps, (uint32_t)a.min_units);
+__device__ __forceinline__ uint32_t units_per_warp(uint32_t total, uint32_t warps) { return max((total + warps - 1) / warps, 1u); }
+
+// Few short runs take a CTA each, and nothing is left to join: no more runs than CTAs, none longer than this.  (4 sequences of 900
+// tokens on 32 kv heads of 128 channels 12.1 us and 15.3 cut evenly, 1 of 1000 on 8 12.0 and 11.6; on 8 of 256 channels 17.0 and
+// 14.6, of 500 9.3 and 10.8.)
+constexpr int kv_whole_units(int d) { return d == 256 ? 32 : 64; }
+template <int D>
+__device__ __forceinline__ bool whole_runs(const Attention &a, int row0, int rows) {
+    if (!a.few_runs) return false;
+    bool all = true;
+    for (int k = threadIdx.x & 31; k < a.batch; k += 32) all = all && make_run(a, k, row0, rows).units <= kv_whole_units(D);
+    return __all_sync(0xffffffffu, all);
 }
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -184,42 +194,54 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_attention_kernel(const Atten
         if (b < a.batch) r = make_run(a, b, row0, S::ROWS);
         return r;
     };
-    Run mine = run_of(lane);
-    uint32_t ends = ends_of(mine);
-    uint32_t total = __shfl_sync(0xffffffffu, ends, 31);
-    for (int base = 32; base < a.batch; base += 32) total += __reduce_add_sync(0xffffffffu, (uint32_t)run_of(base + lane).units) * a.kv_heads;
-    const uint32_t quota = units_per_warp(a, total, gridDim.x * WARPS);
-    const uint32_t begin = (blockIdx.x * WARPS + warp) * quota, end = min(total, begin + quota);
-
-    if (begin < end) {
-        // the sequence, head and unit that the range begins with
-        uint32_t before = 0, past;
-        int base = 0;
-        while (!(past = __ballot_sync(0xffffffffu, before + ends > begin))) {
-            before += __shfl_sync(0xffffffffu, ends, 31);
-            base += 32;
-            mine = run_of(base + lane);
-            ends = ends_of(mine);
+    Run mine = run_of(lane), run = {};
+    int b = 0, head = 0, unit = 0, todo = 0;
+    if (whole_runs<D>(a, row0, S::ROWS)) {
+        b = blockIdx.x / a.kv_heads, head = blockIdx.x - b * a.kv_heads;
+        run = run_of(b);
+        const int share = (run.units + WARPS - 1) / WARPS;
+        unit = warp * share;
+        todo = min(run.units, unit + share) - unit;
+        if (run.units == 0 && b < a.batch)
+            for (int x = threadIdx.x; x < S::ROWS * (D / 4); x += WARPS * 32)
+                store_row<BF16>(out_row(a, run, head, row0 + x / (D / 4), D), x % (D / 4) * 4, 0.0f, make_float4(0.0f, 0.0f, 0.0f, 0.0f));
+    } else {
+        uint32_t ends = ends_of(mine);
+        uint32_t total = __shfl_sync(0xffffffffu, ends, 31);
+        for (int base = 32; base < a.batch; base += 32) total += __reduce_add_sync(0xffffffffu, (uint32_t)run_of(base + lane).units) * a.kv_heads;
+        const uint32_t quota = units_per_warp(total, gridDim.x * WARPS);
+        const uint32_t begin = (blockIdx.x * WARPS + warp) * quota, end = min(total, begin + quota);
+        if (begin < end) {
+            // the sequence, head and unit that the range begins with
+            uint32_t before = 0, past;
+            int base = 0;
+            while (!(past = __ballot_sync(0xffffffffu, before + ends > begin))) {
+                before += __shfl_sync(0xffffffffu, ends, 31);
+                base += 32;
+                mine = run_of(base + lane);
+                ends = ends_of(mine);
+            }
+            const int at_lane = __ffs(past) - 1;
+            b = base + at_lane;
+            run.first_query = __shfl_sync(0xffffffffu, mine.first_query, at_lane);
+            run.length = __shfl_sync(0xffffffffu, mine.length, at_lane);
+            run.queries = __shfl_sync(0xffffffffu, mine.queries, at_lane);
+            run.sink_units = __shfl_sync(0xffffffffu, mine.sink_units, at_lane);
+            run.window_unit = __shfl_sync(0xffffffffu, mine.window_unit, at_lane);
+            run.units = __shfl_sync(0xffffffffu, mine.units, at_lane);
+            const uint32_t in_sequence = begin - (before + __shfl_sync(0xffffffffu, ends, at_lane) - (uint32_t)run.units * a.kv_heads);
+            head = (int)(in_sequence / (uint32_t)run.units);
+            unit = (int)(in_sequence - (uint32_t)head * run.units);
+            todo = (int)(end - begin);
         }
-        const int at_lane = __ffs(past) - 1;
-        int b = base + at_lane;
-        Run run;
-        run.first_query = __shfl_sync(0xffffffffu, mine.first_query, at_lane);
-        run.length = __shfl_sync(0xffffffffu, mine.length, at_lane);
-        run.queries = __shfl_sync(0xffffffffu, mine.queries, at_lane);
-        run.sink_units = __shfl_sync(0xffffffffu, mine.sink_units, at_lane);
-        run.window_unit = __shfl_sync(0xffffffffu, mine.window_unit, at_lane);
-        run.units = __shfl_sync(0xffffffffu, mine.units, at_lane);
-        const uint32_t in_sequence = begin - (before + __shfl_sync(0xffffffffu, ends, at_lane) - (uint32_t)run.units * a.kv_heads);
-        int head = (int)(in_sequence / (uint32_t)run.units);
-        int unit = (int)(in_sequence - (uint32_t)head * run.units);
+    }
 
+    if (todo > 0) {
         // The producer's own place, up to STAGES units ahead.  Every lane finds the slab of one of the next 32 units of its run
         // (0: not in the cache); lane 0 asks for them one by one.
         Run p_run = run;
         int p_b = b, p_head = head, p_unit = unit, p_left = 0, issued = 0, p_stage = 0;
         const uint64_t *p_next = slabs;
-        const int todo = (int)(end - begin);
         auto produce = [&]() {
             if (issued >= todo) return;
             if (p_left == 0) {
@@ -594,12 +616,13 @@ __global__ void __launch_bounds__(256) kv_join_kernel(const Attention a, int cta
     const int b = blockIdx.x / a.kv_heads, head = blockIdx.x - b * a.kv_heads, row0 = blockIdx.y * ROWS;
     const Run run = make_run(a, b, row0, ROWS);
     uint32_t first;
-    const uint32_t quota = units_per_warp(a, count_units(a, row0, ROWS, b, first), (uint32_t)ctas * WARPS) * WARPS;
+    const uint32_t quota = units_per_warp(count_units(a, row0, ROWS, b, first), (uint32_t)ctas * WARPS) * WARPS;
+    const bool whole = whole_runs<D>(a, row0, ROWS);
     first += (uint32_t)head * run.units;
     const int c0 = first / quota, c1 = run.units ? (first + run.units - 1) / quota : c0;
     // (CTAs without work wait too: what follows this kernel takes its end for that of the kernel in front)
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (run.units && c0 == c1) return;
+    if (whole || (run.units && c0 == c1)) return;
     for (int x = threadIdx.x; x < ROWS * (D / 4); x += 256) {
         const int row = x / (D / 4), c = x % (D / 4) * 4;
         char *dst = out_row(a, run, head, row0 + row, D);
@@ -669,7 +692,7 @@ int launch(const Attention &a, int64_t tiles, int ctas, cudaStream_t stream) {
     auto *kernel = kv_attention_kernel<D, NT, WARPS, STAGES, BF16>;
     int e = allow_smem<kv_attention_kernel<D, NT, WARPS, STAGES, BF16>>(S::SMEM, what);
     if (e == ATLAS_OK) e = launch_early(kernel, dim3((unsigned)ctas, (unsigned)tiles), WARPS * 32, S::SMEM, stream, what, a);
-    if (e != ATLAS_OK) return e;
+    if (e != ATLAS_OK || (a.few_runs && a.max_tokens <= kv_whole_units(D) * KV_SLAB)) return e;
     return launch_early(kv_join_kernel<D, NT, WARPS, BF16>, dim3((unsigned)(a.batch * a.kv_heads), (unsigned)tiles), 256, 0, stream, what, a, ctas);
 }
 
@@ -748,7 +771,7 @@ int atlas_kv_attention(const AtlasKvAttention *p, void *stream) {
     a.batch = (int)p->batch, a.q_heads = p->q_heads, a.kv_heads = p->kv_heads, a.group = p->q_heads / p->kv_heads;
     a.page_size = p->page_size, a.window = p->window, a.sinks = p->sinks;
     a.scale_log2 = p->scale * 1.4426950408889634f;
-    a.min_units = 1;
+    a.few_runs = p->batch * p->kv_heads <= ctas;
     const bool bf16 = p->dtype == ATLAS_DTYPE_BF16;
     cudaStream_t s = (cudaStream_t)stream;
     if (kv_prompt_serves(*p)) return kv_prompt(a, *p, s);

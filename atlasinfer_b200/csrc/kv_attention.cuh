@@ -16,7 +16,7 @@ struct Attention {
     int64_t num_pages, table_stride, max_tokens, total_queries, uniform;
     int batch, q_heads, kv_heads, group, page_size, window, sinks;   // group: query heads of a kv head
     float scale_log2;
-    int min_units;               // per warp
+    bool few_runs;               // no more sequences times kv heads than CTAs
 };
 
 // Prompts: kv_prompt.cu.  Bytes of workspace, and the launch.
