@@ -1,17 +1,26 @@
-// Attention of many queries over the 4-bit cache (prompts, chunks of prompts) on the tensor cores.
+// Attention of many queries over the 4-bit cache (prompts, chunks of prompts, long drafts) on the tensor cores.
 //
-// A CTA takes one kv head and TILES tiles of 128 rows (queries x the query heads that share the kv head) and walks the
-// tiles of 64 tokens that any of them sees:
-//   S = Q K^T      tcgen05, M 128 rows, N 64 tokens; Q stays in tensor memory as fp16 (bf16 rows times a power of two)
+// A CTA takes one kv head and two tiles of 128 rows (queries x the query heads that share the kv head; one tile if D is 256)
+// and walks the tiles of 128 tokens (64) that any of them sees:
+//   S = Q K^T      tcgen05, 128 rows x 128 tokens, both operands in shared memory (Q as fp16, bf16 rows times a power of two)
 //   P = 2^(S' - m) a thread a row; P goes back to tensor memory as fp16, over S
-//   O += P V       tcgen05, A from tensor memory, N = D channels, fp32 accumulators in tensor memory
+//   O += P V       tcgen05, P from tensor memory, N = D channels, fp32 accumulators in tensor memory
 // K and V are rebuilt from their codes into 128-byte-swizzled K-major tiles in shared memory, as the exact fp16 numbers that
 // the cache stands for, so the only roundings are those of P and of the output.  The running maximum of a row follows its
 // scores only where they pass it by 2^8 (O is rescaled then, which is rare); P keeps 14 bits of headroom for that.
 //
-// Warps: 0-3 and 4-7 softmax of the two row tiles (of one tile if D is 256, where O takes the tensor memory of both; its S
-// then has two buffers), 8-11 rebuild, 12 issues the MMAs, 13 brings slabs in by bulk copies.  While the softmax warps of one
-// row tile work, the tensor core works on the other.
+// Warps: four of softmax for each row tile, three that rebuild keys and three that rebuild values, one that issues the MMAs,
+// one that brings halves of slabs (keys, values) in by bulk copies, each half as far ahead as its ring has room.  While the
+// softmax warps of one row tile work, the tensor core works on the other.
+//
+// What bounds it (4096 queries on 32 heads of 128 over 8 kv heads, 168 us, 816 TFLOP/s, half of the measured peak): a CTA needs
+// 2800 cycles for a tile of 128 tokens, of which the tensor core works 2048 at its peak rate, and 24000 for its start and end
+// (15000 until the first S: rows of Q by bulk copies, slabs, rebuilding; 7000 behind the last P), a fifth of the largest.  In
+// the loop the chain of a row tile (S, maximum, weights, P, two products) is the bound: exponentials replaced by copies gave 7 %,
+// a polynomial for a quarter of them 0 %.  Built and slower: S in two buffers of 64 tokens for each row tile (an MMA of 64
+// columns with both operands in shared memory takes 80 cycles, one of 128 91; 5300 cycles for 128 tokens), two threads a row
+// (178 us against 173 then), registers shared out unevenly (setmaxnreg: spills), one pass over S that keeps P in registers
+// until the maximum is known (code too long for the instruction cache; 5400 cycles).
 #include <algorithm>
 
 #include "kv_attention.cuh"
