@@ -124,7 +124,7 @@ struct Shape {
     static constexpr int SLAB = kv_slab_bytes(D);
     static constexpr int PIECE_BYTES = D == 64 ? 8 : 16, KEY_ROW = 4 * PIECE_BYTES;   // of a lane's codes (in a plane); of a token's
     static constexpr int PIECE = ROWS * (D + 2) * 4;       // maximum, sum and output of the rows
-    static constexpr int RING = STAGES * SLAB;             // a warp's; holds its last piece in the end
+    static constexpr int RING = STAGES * 2 * SLAB;         // a warp's pairs of slabs; holds its last piece in the end
     static constexpr int SMEM = WARPS * (RING + PIECE + STAGES * 8 + 2 * 16 + 32 * 8);
     static_assert(STAGES * WARPS % 2 == 0 && SMEM <= 227 * 1024, "shared memory");
     static_assert(PIECE <= RING, "a piece has to fit the ring");
@@ -245,10 +245,10 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_attention_kernel(const Atten
     }
 
     if (todo > 0) {
-        // The producer's own place, up to STAGES units ahead.  Every lane finds the slab of one of the next 32 units of its run
+        // The producer's own place, up to STAGES pairs of units ahead (a run's last may be one).  Every lane finds the slab of one of the next 32 units of its run
         // (0: not in the cache); lane 0 asks for them one by one.
         Run p_run = run;
-        int p_b = b, p_head = head, p_unit = unit, p_left = 0, issued = 0, p_stage = 0;
+        int p_b = b, p_head = head, p_unit = unit, p_left = 0, issued = 0, asked = 0, p_stage = 0;
         const uint64_t *p_next = slabs;
         auto produce = [&]() {
             if (issued >= todo) return;
@@ -272,21 +272,29 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_attention_kernel(const Atten
                 p_unit += p_left;
                 p_next = slabs;
             }
+            const int count = min(min(2, p_left), todo - issued);
             if (lane == 0) {
-                const uint8_t *src = reinterpret_cast<const uint8_t *>(*p_next);
-                const uint32_t at = bar + 8 * p_stage;
-                if (src) {
-                    mbar_arrive_expect_tx(at, S::SLAB);
-                    bulk_load_1d(ring + p_stage * S::SLAB, src, S::SLAB, at);
-                } else {   // a page that is not there: a NaN in the first scale of the keys says so, the slab is passed over
-                    *reinterpret_cast<volatile uint16_t *>(ring_all + warp * S::RING + p_stage * S::SLAB + kv_key_params(D)) = 0x7fff;
-                    fence_async_smem();   // (the stage's next slab comes by the other proxy)
-                    mbar_arrive(at);
+                const uint64_t src0 = p_next[0], src1 = count == 2 ? p_next[1] : 0;
+                const uint32_t at = bar + 8 * p_stage, dst = ring + p_stage * (2 * S::SLAB);
+                if (!src0 || (count == 2 && !src1)) {
+                    // a page that is not there: a NaN in the first scale of the keys says so, the slab is passed over
+                    volatile uint8_t *const place = ring_all + warp * S::RING + p_stage * (2 * S::SLAB) + kv_key_params(D);
+                    if (!src0) *reinterpret_cast<volatile uint16_t *>(place) = 0x7fff;
+                    if (count == 2 && !src1) *reinterpret_cast<volatile uint16_t *>(place + S::SLAB) = 0x7fff;
+                    fence_async_smem();   // (the place's next slabs come by the other proxy)
+                }
+                mbar_arrive_expect_tx(at, (src0 ? S::SLAB : 0) + (src1 ? S::SLAB : 0));
+                if (src0 && src1 == src0 + S::SLAB) {
+                    bulk_load_1d(dst, reinterpret_cast<const void *>(src0), 2 * S::SLAB, at);
+                } else {
+                    if (src0) bulk_load_1d(dst, reinterpret_cast<const void *>(src0), S::SLAB, at);
+                    if (src1) bulk_load_1d(dst + S::SLAB, reinterpret_cast<const void *>(src1), S::SLAB, at);
                 }
             }
-            ++p_next;
-            --p_left;
-            ++issued;
+            p_next += count;
+            p_left -= count;
+            issued += count;
+            ++asked;
             p_stage = p_stage + 1 == STAGES ? 0 : p_stage + 1;
         };
         for (int i = 0; i < STAGES; ++i) produce();
@@ -298,7 +306,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_attention_kernel(const Atten
         int plain_sinks = 0, plain_from = 0, plain_to = 0;   // slabs that all rows see whole: below the first, or from the second to the third
         bool fresh = true, first_piece = true, failed = false;
         const bool begins_inside = unit != 0;
-        int done = 0, stage = 0;
+        int done = 0, taken = 0, stage = 0;
         uint32_t parity = 0;
 
         auto leave = [&](bool whole_run, bool ends_here) {
@@ -522,23 +530,17 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_attention_kernel(const Atten
                 }
             }
 
-            const int two = todo - done >= 2 && run.units - unit >= 2 ? 2 : 1;
-            const uint8_t *slab[2];
-            int at[2];
-            bool there[2] = {true, true};
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                if (u == two) break;
-                if (!__all_sync(0xffffffffu, mbar_try_wait(bar + 8 * stage, parity)) && !__all_sync(0xffffffffu, mbar_wait(bar + 8 * stage, parity))) {
-                    failed = true;
-                    break;
-                }
-                slab[u] = ring_ptr + stage * S::SLAB;
-                at[u] = run.slab(unit + u);
-                there[u] = *reinterpret_cast<const uint16_t *>(slab[u] + kv_key_params(D)) != 0x7fffu;
-                if (++stage == STAGES) stage = 0, parity ^= 1;
+            if (!__all_sync(0xffffffffu, mbar_try_wait(bar + 8 * stage, parity)) && !__all_sync(0xffffffffu, mbar_wait(bar + 8 * stage, parity))) {
+                failed = true;
+                break;
             }
-            if (failed) break;
+            const int two = min(min(2, run.units - unit), todo - done);
+            const uint8_t *slab[2] = {ring_ptr + stage * (2 * S::SLAB), ring_ptr + stage * (2 * S::SLAB) + S::SLAB};
+            const int at[2] = {run.slab(unit), run.slab(unit + 1)};
+            const bool there[2] = {*reinterpret_cast<const uint16_t *>(slab[0] + kv_key_params(D)) != 0x7fffu,
+                                   *reinterpret_cast<const uint16_t *>(slab[1] + kv_key_params(D)) != 0x7fffu};   // (of the second: if there are two)
+            ++taken;
+            if (++stage == STAGES) stage = 0, parity ^= 1;
             if (two == 2 && there[0] && there[1]) {
                 work(std::integral_constant<int, 2>(), slab, at);
             } else {
@@ -551,7 +553,6 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_attention_kernel(const Atten
             }
             __syncwarp();          // everyone has read the stages
             produce();
-            if (two == 2) produce();
             done += two;
             unit += two;
 
@@ -568,7 +569,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_attention_kernel(const Atten
             }
         }
         if (failed) {              // a copy that never came: those in flight land (or not, within the limit) before the CTA goes
-            for (int i = done; i < issued; ++i) mbar_wait(bar + 8 * (i % STAGES), (i / STAGES) & 1);
+            for (int i = taken; i < asked; ++i) mbar_wait(bar + 8 * (i % STAGES), (i / STAGES) & 1);
             if (lane == 0 && a.status) *a.status = 1;
         } else if (unit) {
             __syncwarp();
@@ -707,9 +708,9 @@ int launch(const Attention &a, int64_t tiles, int ctas, cudaStream_t stream) {
 template <int D, bool BF16>
 int launch_nt(const Attention &a, const Plan &plan, int ctas, cudaStream_t stream) {
     // Warps and slabs in flight: what registers (168, 255) and shared memory hold.
-    if constexpr (D == 64) return launch<64, 1, 12, 8, BF16>(a, plan.tiles, ctas, stream);
-    if constexpr (D == 128) return plan.nt == 1 ? launch<128, 1, 12, 4, BF16>(a, plan.tiles, ctas, stream) : launch<128, 2, 8, 5, BF16>(a, plan.tiles, ctas, stream);
-    if constexpr (D == 256) return launch<256, 1, 8, 4, BF16>(a, plan.tiles, ctas, stream);
+    if constexpr (D == 64) return launch<64, 1, 12, 4, BF16>(a, plan.tiles, ctas, stream);
+    if constexpr (D == 128) return plan.nt == 1 ? launch<128, 1, 12, 2, BF16>(a, plan.tiles, ctas, stream) : launch<128, 2, 8, 3, BF16>(a, plan.tiles, ctas, stream);
+    if constexpr (D == 256) return launch<256, 1, 8, 2, BF16>(a, plan.tiles, ctas, stream);
     return ATLAS_ERR_UNSUPPORTED;
 }
 
