@@ -13,11 +13,11 @@
 // A run that lies within a warp goes straight to the output; pieces of the others are joined in shared memory, in order, and
 // what goes beyond a CTA is left in the workspace for kv_join_kernel.
 //
-// What bounds it: 2 x 131071 tokens of 8 kv heads, 302 MB, take 87 us (3.5 TB/s, 0.53 of the measured copy rate).  A slab of
-// 128 channels (2304 bytes) costs some 400 warp instructions, 250 of them its arithmetic (5 to extract, 4 to centre and, for
-// values, 4 to scale 8 codes), and issue slots are 60 % used, mma.sync holding the issue port for 16 % more; DRAM waits are
-// few.  Two slabs at a time on 12 warps of 168 registers and one at a time on 16 of 128 measured the same on long contexts,
-// the former is ahead on short ones (4001 tokens of 32 heads 20.6 and 22.5 us); two at a time on 128 registers spills (129 us).
+// What bounds it: 2 x 131071 tokens of 8 kv heads, 302 MB, take 80 us (3.8 TB/s, 0.58 of the measured copy rate).  A slab of
+// 128 channels (2304 bytes) costs 341 warp instructions, 250 of them its arithmetic (5 to extract, 4 to centre and, for
+// values, 4 to scale 8 codes); issue slots are 60 % used, mma.sync holds the issue port for 16 % more, and DRAM waits are few.
+// Two slabs at a time on 12 warps of 168 registers: brought in one by one they took 87 us, as one at a time on 16 warps of 128
+// did, which is behind on short contexts (4001 tokens of 32 heads 22.5 us and 20.6); two at a time on 128 registers spills (129).
 // Short calls are a chain of waits: 1 us to plan, 1 to find pages, 1 for the first slab, 1 to join.
 #include <algorithm>
 

@@ -13,9 +13,9 @@
 // one that brings halves of slabs (keys, values) in by bulk copies, each half as far ahead as its ring has room.  While the
 // softmax warps of one row tile work, the tensor core works on the other.
 //
-// What bounds it (4096 queries on 32 heads of 128 over 8 kv heads, 168 us, 816 TFLOP/s, half of the measured peak): a CTA needs
-// 2800 cycles for a tile of 128 tokens, of which the tensor core works 2048 at its peak rate, and 24000 for its start and end
-// (15000 until the first S: rows of Q by bulk copies, slabs, rebuilding; 7000 behind the last P), a fifth of the largest.  In
+// What bounds it (4096 queries on 32 heads of 128 over 8 kv heads, 165 us, 833 TFLOP/s, half of the measured peak): a CTA needs
+// 2800 cycles for a tile of 128 tokens, of which the tensor core works 2048 at its peak rate, and some 23000 for its start and end
+// (14000 until the first S: rows of Q by bulk copies, slabs, rebuilding; 7000 behind the last P), a fifth of the largest.  In
 // the loop the chain of a row tile (S, maximum, weights, P, two products) is the bound: exponentials replaced by copies gave 7 %,
 // a polynomial for a quarter of them 0 %.  Built and slower: S in two buffers of 64 tokens for each row tile (an MMA of 64
 // columns with both operands in shared memory takes 80 cycles, one of 128 91; 5300 cycles for 128 tokens), two threads a row
@@ -163,17 +163,11 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_prompt_kernel(const Attentio
     volatile int *const s_abort = reinterpret_cast<volatile int *>(sm + P::OFF_TMEM + 8);
     volatile uint8_t *const gone = sm + P::OFF_INFO;   // [tile % 16][slab]: whether the slab is not there
 
-    if (tid == 0) {
-        for (int i = 0; i < 2 * RING; ++i) mbar_init(bar(P::RAW_FULL + i), 1), mbar_init(bar(P::RAW_EMPTY + i), 1);
-        for (int i = 0; i < STAGES; ++i) mbar_init(bar(P::K_FULL + i), SLABS), mbar_init(bar(P::V_FULL + i), SLABS);
-        for (int i = 0; i < 8; ++i) mbar_init(bar(P::S_FULL + i), 1);
-        for (int i = 0; i < 2; ++i) mbar_init(bar(P::P_FULL + i), 4);
-        for (int i = 0; i < 4; ++i) mbar_init(bar(P::O_DONE + i), 1);
-        mbar_init(bar(P::Q_FULL), 4 * TILES);
-        mbar_init(bar(P::DRAIN), 1);
-        for (int i = 0; i < 4 * TILES; ++i) mbar_init(bar(P::Q_RAW + i), 1);
-        for (int i = 0; i < 16; ++i) reinterpret_cast<volatile uint64_t *>(gone)[i] = 0;
-        *s_abort = 0;
+    if (warp == 0) {
+        for (int i = lane; i < P::BARS; i += 32)
+            mbar_init(bar(i), i >= P::K_FULL && i < P::V_FULL + STAGES ? SLABS : i >= P::P_FULL && i < P::P_FULL + 2 ? 4 : i == P::Q_FULL ? 4 * TILES : 1);
+        if (lane < 16) reinterpret_cast<volatile uint64_t *>(gone)[lane] = 0;
+        if (lane == 0) *s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == PR_MMA) {
@@ -394,7 +388,11 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_prompt_kernel(const Attentio
             const uint32_t at = bar(P::Q_RAW + warp);
             if (lane == 0) mbar_arrive_expect_tx(at, (uint32_t)min(max(rows - warp * 32, 0), 32) * (D * 2));
             __syncwarp();
-            if (live) bulk_load_1d(smem_u32(raw), a.q + (int64_t)(seq.first_query + query) * a.q_token_stride + (head * a.group + row - query * a.group) * a.q_head_stride, D * 2, at);
+            // (rows that lie behind one another, the heads of a token, in one copy: one takes some 36 cycles however small)
+            const int member = row - query * a.group, run = a.q_head_stride == D * 2 ? a.group : 1;
+            if (live && (run == 1 || member == 0 || lane == 0))
+                bulk_load_1d(smem_u32(raw), a.q + (int64_t)(seq.first_query + query) * a.q_token_stride + (head * a.group + member) * a.q_head_stride,
+                             min(min(run == 1 ? 1 : run - member, 32 - lane), rows - in_block) * (D * 2), at);
             ok = wait_warp<20>(at, 0, s_abort);
             const uint32_t flip = a.scale_log2 < 0.0f ? 0x80008000u : 0u;   // a negative scale turns the queries round: maxima of scores are maxima of products
             float down = 1.0f;
