@@ -249,6 +249,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_attention_kernel(const Atten
         // (0: not in the cache); lane 0 asks for them one by one.
         Run p_run = run;
         int p_b = b, p_head = head, p_unit = unit, p_left = 0, issued = 0, asked = 0, p_stage = 0;
+        uint32_t absent = 0;   // of each stage two bits: slabs that are not in the cache (they are passed over)
         const uint64_t *p_next = slabs;
         auto produce = [&]() {
             if (issued >= todo) return;
@@ -273,16 +274,10 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_attention_kernel(const Atten
                 p_next = slabs;
             }
             const int count = min(min(2, p_left), todo - issued);
+            const uint64_t src0 = p_next[0], src1 = count == 2 ? p_next[1] : 0;
+            absent = (absent & ~(3u << (2 * p_stage))) | ((src0 ? 0u : 1u) | (src1 ? 0u : 2u)) << (2 * p_stage);
             if (lane == 0) {
-                const uint64_t src0 = p_next[0], src1 = count == 2 ? p_next[1] : 0;
                 const uint32_t at = bar + 8 * p_stage, dst = ring + p_stage * (2 * S::SLAB);
-                if (!src0 || (count == 2 && !src1)) {
-                    // a page that is not there: a NaN in the first scale of the keys says so, the slab is passed over
-                    volatile uint8_t *const place = ring_all + warp * S::RING + p_stage * (2 * S::SLAB) + kv_key_params(D);
-                    if (!src0) *reinterpret_cast<volatile uint16_t *>(place) = 0x7fff;
-                    if (count == 2 && !src1) *reinterpret_cast<volatile uint16_t *>(place + S::SLAB) = 0x7fff;
-                    fence_async_smem();   // (the place's next slabs come by the other proxy)
-                }
                 mbar_arrive_expect_tx(at, (src0 ? S::SLAB : 0) + (src1 ? S::SLAB : 0));
                 if (src0 && src1 == src0 + S::SLAB) {
                     bulk_load_1d(dst, reinterpret_cast<const void *>(src0), 2 * S::SLAB, at);
@@ -537,8 +532,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_attention_kernel(const Atten
             const int two = min(min(2, run.units - unit), todo - done);
             const uint8_t *slab[2] = {ring_ptr + stage * (2 * S::SLAB), ring_ptr + stage * (2 * S::SLAB) + S::SLAB};
             const int at[2] = {run.slab(unit), run.slab(unit + 1)};
-            const bool there[2] = {*reinterpret_cast<const uint16_t *>(slab[0] + kv_key_params(D)) != 0x7fffu,
-                                   *reinterpret_cast<const uint16_t *>(slab[1] + kv_key_params(D)) != 0x7fffu};   // (of the second: if there are two)
+            const bool there[2] = {!(absent >> (2 * stage) & 1), !(absent >> (2 * stage) & 2)};   // (of the second: if there are two)
             ++taken;
             if (++stage == STAGES) stage = 0, parity ^= 1;
             if (two == 2 && there[0] && there[1]) {

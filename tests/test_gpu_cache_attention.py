@@ -137,6 +137,23 @@ def spoil_after(cache, page, count):
         params[:, token // 2, :, :, token % 2] = 0xFF
 
 
+@pytest.mark.parametrize("word", (0x7FFF, 0x7E00, 0xFC00, 0xFFFF))
+@pytest.mark.parametrize("queries", (1, 40))
+def test_hidden_tokens_of_a_slab_may_hold_anything(cuda_device, queries, word):
+    """What the window has left behind within the first slab that it still sees: no pattern there hides the slab."""
+    w = Work(cuda_device, [1000, 905], [queries, queries], 4, 2, 128, page=16)
+    want = w.run(window=64)
+    w.check(want, window=64)
+    for b, n in enumerate(w.lengths):
+        first = n - queries - 63   # (the first query's first key)
+        assert first % 16
+        data = w.cache.data[int(w.table[b, first // 16])]          # [head, bytes]: keys of tokens in front of it
+        patch = data.view(torch.int16)
+        patch[:, 16 * 64:17 * 64].view(-1, 16, 4)[:, :first % 16] = word - (1 << 16 if word > 0x7FFF else 0)
+        w.cache.data[int(w.table[b, first // 16])] = data
+    assert torch.equal(w.run(window=64), want)
+
+
 @pytest.mark.parametrize("queries", (1, 50))
 def test_unknown_pages_count_as_hidden(cuda_device, queries):
     w = Work(cuda_device, [200, 64], [queries] * 2, 4, 2, 64, page=16)
