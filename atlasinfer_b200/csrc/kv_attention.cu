@@ -772,7 +772,9 @@ int atlas_kv_attention(const AtlasKvAttention *p, void *stream) {
     a.num_pages = p->num_pages, a.table_stride = p->table_stride, a.max_tokens = p->max_pages * p->page_size;
     a.total_queries = p->total_queries, a.uniform = p->query_starts ? 0 : p->total_queries / p->batch;
     a.batch = (int)p->batch, a.q_heads = p->q_heads, a.kv_heads = p->kv_heads, a.group = p->q_heads / p->kv_heads;
-    a.page_size = p->page_size, a.window = p->window, a.sinks = p->sinks;
+    // A window of all tokens hides none: as no window it needs no masks, and position - window stays within 32 bits below (a query
+    // may be at a negative position, and 2^31 - 1 is a usual "no window").
+    a.page_size = p->page_size, a.window = p->window < a.max_tokens ? p->window : 0, a.sinks = p->sinks;
     a.scale_log2 = p->scale * 1.4426950408889634f;
     a.few_runs = p->batch * p->kv_heads <= ctas;
     const bool bf16 = p->dtype == ATLAS_DTYPE_BF16;

@@ -153,7 +153,7 @@ Tensor kv_attention(const Tensor &q_in, const Tensor &data, int64_t head_dim, in
         if (batch ? total % batch : total) throw py::value_error(std::to_string(total) + " queries of " + std::to_string(batch) + " sequences need query_starts");
         max_queries = batch ? total / batch : 0;
     }
-    if (window < 0 || sinks < 0 || window > INT32_MAX) throw py::value_error("window and sinks must not be negative");
+    if (window < 0 || sinks < 0) throw py::value_error("window and sinks must not be negative");
     const c10::cuda::CUDAGuard guard(q.device());
     Tensor out = at::empty({total, q.size(1), q.size(2)}, q.options());
     if (out.numel() == 0) return out;
@@ -164,7 +164,7 @@ Tensor kv_attention(const Tensor &q_in, const Tensor &data, int64_t head_dim, in
     a.out = out.data_ptr();
     a.total_queries = total, a.batch = batch, a.max_queries = std::min(max_queries, total);
     a.cache = data.numel() ? data.data_ptr() : nullptr, a.num_pages = data.size(0);
-    a.page_size = (int32_t)page_size, a.window = (int32_t)window, a.sinks = (int32_t)std::min<int64_t>(sinks, INT32_MAX);
+    a.page_size = (int32_t)page_size, a.window = (int32_t)std::min<int64_t>(window, INT32_MAX), a.sinks = (int32_t)std::min<int64_t>(sinks, INT32_MAX);
     a.scale = (float)scale;
     a.page_table = table.numel() ? table.const_data_ptr<int32_t>() : nullptr, a.table_stride = table.stride(0), a.max_pages = table.size(1);
     a.lengths = lengths.const_data_ptr<int32_t>(), a.query_starts = starts.defined() ? starts.const_data_ptr<int32_t>() : nullptr;
