@@ -299,6 +299,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_attention_kernel(const Atten
         float factor[NT][2];       // log2 units of a row's scores
         int place[NT][2];          // positions of rows 2 t and 2 t + 1, -1: no such row
         int plain_sinks = 0, plain_from = 0, plain_to = 0;   // slabs that all rows see whole: below the first, or from the second to the third
+        int seen_from = 0;         // first token in the window of any row
+        auto plain = [&](int slab) { return slab < plain_sinks || (slab >= plain_from && slab < plain_to); };
         bool fresh = true, first_piece = true, failed = false;
         const bool begins_inside = unit != 0;
         int done = 0, taken = 0, stage = 0;
@@ -380,7 +382,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_attention_kernel(const Atten
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
                     for (int k = 0; k < 4; ++k) s[u][n][k] *= factor[n][k & 1];
-                if (!(at[u] < plain_sinks || (at[u] >= plain_from && at[u] < plain_to))) {
+                if (!plain(at[u])) {
                     const int token0 = at[u] * KV_SLAB;
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
@@ -441,10 +443,11 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_attention_kernel(const Atten
                 read_words<D>(slab[u] + kv_value_codes(D) + 32 * S::PIECE_BYTES + lane * S::PIECE_BYTES, v1);
                 read_params<2 * S::GROUPS>(slab[u] + kv_value_params(D) + t * S::GROUPS * 8, q0);
                 read_params<2 * S::GROUPS>(slab[u] + kv_value_params(D) + (t + 4) * S::GROUPS * 8, q1);
-                const int left = run.length - at[u] * KV_SLAB;
-                if (left < KV_SLAB) {   // tokens that are not there may hold anything
-                    const uint32_t keep0 = (2 * t < left ? 0xffffu : 0u) | (2 * t + 1 < left ? 0xffff0000u : 0u);
-                    const uint32_t keep1 = (2 * t + 8 < left ? 0xffffu : 0u) | (2 * t + 9 < left ? 0xffff0000u : 0u);
+                if (!plain(at[u])) {   // tokens that no row sees may hold anything: zeros (their weights are zero too, but not times NaN)
+                    const int token = at[u] * KV_SLAB + 2 * t;
+                    auto seen = [&](int k) { return k < run.length && (k >= seen_from || k < a.sinks); };
+                    const uint32_t keep0 = (seen(token) ? 0xffffu : 0u) | (seen(token + 1) ? 0xffff0000u : 0u);
+                    const uint32_t keep1 = (seen(token + 8) ? 0xffffu : 0u) | (seen(token + 9) ? 0xffff0000u : 0u);
 #pragma unroll
                     for (int gr = 0; gr < S::GROUPS; ++gr) {
                         q0[2 * gr] &= keep0, q0[2 * gr + 1] = (q0[2 * gr + 1] & keep0) | (0x64006400u & ~keep0);
@@ -476,7 +479,9 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_attention_kernel(const Atten
             if (fresh) {           // another run: its queries into registers
                 st.clear();
                 fresh = false;
-                plain_to = max(0, run.length - run.queries + row0 / a.group + 1) / KV_SLAB;
+                const int past = max(0, run.length - run.queries + row0 / a.group + 1);   // of the tokens that the first row may see
+                plain_to = past / KV_SLAB;
+                seen_from = a.window ? max(0, past - a.window) : 0;
                 plain_from = a.window ? max(0, run.length - 1 - a.window + KV_SLAB) / KV_SLAB : 0;
                 plain_sinks = min(a.sinks / KV_SLAB, plain_to);
 #pragma unroll

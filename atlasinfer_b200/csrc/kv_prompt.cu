@@ -278,12 +278,13 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_prompt_kernel(const Attentio
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(P::RAW_EMPTY + slot));
                 const int token0 = walk.tile(j0 + j) * KEYS + slab * KV_SLAB;
-                if (absent || token0 + KV_SLAB > seq.length) {
-                    // tokens that are not there may hold anything: zeros (their weights are zero too, but not times NaN)
+                if (absent || token0 + KV_SLAB > seq.length || (token0 < walk.window_start && token0 + KV_SLAB > walk.sinks)) {
+                    // tokens that no row sees may hold anything: zeros (their weights are zero too, but not times NaN)
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const int token = token0 + 8 * h + 2 * t;
-                        const uint32_t keep = absent ? 0u : (token < seq.length ? 0xffffu : 0u) | (token + 1 < seq.length ? 0xffff0000u : 0u);
+                        auto seen = [&](int k) { return !absent && k < seq.length && (k >= walk.window_start || k < walk.sinks); };
+                        const uint32_t keep = (seen(token) ? 0xffffu : 0u) | (seen(token + 1) ? 0xffff0000u : 0u);
 #pragma unroll
                         for (int gr = 0; gr < P::GROUPS; ++gr) sb[h][gr].x &= keep, sb[h][gr].y = (sb[h][gr].y & keep) | (0x64006400u & ~keep);
                     }

@@ -22,3 +22,47 @@ def test_wide_windows_of_fewer_tokens_than_queries(cuda_device, lengths, queries
     w.check(got, window=window, sinks=sinks)
     if window >= w.table.shape[1] * 32:
         assert torch.equal(got, w.run())
+
+
+def owners(d):
+    """The token (0 to 15) that every byte of a slab of 16 tokens belongs to, from the documented order."""
+    planes, j = max(1, d // 128), min(4, d // 32)
+    token = torch.arange(16)
+    keys = token.view(1, 16, 1).expand(planes, 16, 8 * d // planes // 16)
+    half, t, odd = torch.arange(2).view(2, 1, 1, 1, 1, 1), torch.arange(4).view(1, 1, 4, 1, 1, 1), torch.arange(2).view(1, 1, 1, 1, 2, 1)
+    values = (8 * half + 2 * t + odd).expand(2, 8, 4, j, 2, 2).expand(planes, 2, 8, 4, j, 2, 2)
+    key_params = token.view(16, 1).expand(16, d // 16)
+    value_params = (2 * torch.arange(8).view(8, 1, 1, 1, 1) + torch.arange(2).view(1, 1, 1, 2, 1)).expand(8, d // 64, 2, 2, 2)
+    return torch.cat([x.reshape(-1) for x in (keys, values, key_params, value_params)])
+
+
+def spoil(w, b, hidden, word):
+    """Every byte of the hidden tokens (a mask over the sequence's pages) becomes that of a 16-bit word."""
+    d, page = w.cache.head_dim, w.cache.page_size
+    own = owners(d)
+    pattern = torch.tensor([word & 255, word >> 8], dtype=torch.uint8).repeat(9 * d)
+    for i in range(hidden.shape[0] // page):
+        at = int(w.table[b, i])
+        data = w.cache.data[at].cpu().view(w.cache.kv_heads, page // 16, 18 * d)
+        gone = hidden[i * page:(i + 1) * page].view(page // 16, 16)[:, own]
+        w.cache.data[at] = torch.where(gone, pattern, data).view(w.cache.kv_heads, -1).to(w.device)
+
+
+@pytest.mark.parametrize("word", (0x7FFF, 0x7C00, 0xFC00))
+@pytest.mark.parametrize("queries", (1, 5, 40))
+@pytest.mark.parametrize("d,window,sinks", [(64, 64, 4), (128, 64, 0), (128, 50, 20), (256, 100, 17), (128, None, 0), (64, 33, 16)])
+def test_what_no_query_sees_may_hold_anything(cuda_device, d, window, sinks, queries, word):
+    """Keys and values, codes and scales, of tokens in front of the window, between the sinks and it, and behind the end: NaN
+    and infinities there change no bit of the result."""
+    w = Work(cuda_device, [1000, 905, 70], [queries] * 3, 4, 2, d, page=32, dtype=F16)
+    how = dict(window=window, sinks=sinks)
+    want = w.run(**how)
+    w.check(want, **how)
+    for b, n in enumerate(w.lengths):
+        key = torch.arange(-(-n // 32) * 32)
+        hidden = key >= n
+        if window:
+            hidden |= (key <= n - queries - window) & (key >= sinks)
+        assert hidden.any()
+        spoil(w, b, hidden, word)
+    assert torch.equal(w.run(**how), want)
