@@ -298,9 +298,9 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_attention_kernel(const Atten
         uint32_t qf[NT][S::WORDS][4];
         float factor[NT][2];       // log2 units of a row's scores
         int place[NT][2];          // positions of rows 2 t and 2 t + 1, -1: no such row
-        int plain_sinks = 0, plain_from = 0, plain_to = 0;   // slabs that all rows see whole: below the first, or from the second to the third
+        int plain_sinks = 0, plain_from = 0, plain_count = 0;   // slabs that all rows see whole: below the first, and so many from the second on
         int seen_from = 0;         // first token in the window of any row
-        auto plain = [&](int slab) { return slab < plain_sinks || (slab >= plain_from && slab < plain_to); };
+        auto plain = [&](int slab) { return slab < plain_sinks || (uint32_t)(slab - plain_from) < (uint32_t)plain_count; };
         bool fresh = true, first_piece = true, failed = false;
         const bool begins_inside = unit != 0;
         int done = 0, taken = 0, stage = 0;
@@ -341,7 +341,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_attention_kernel(const Atten
             if (lane == 0) notes[2 * warp + (first_piece ? 0 : 1)] = make_int4(b * a.kv_heads + head, (ends_here ? 1 : 0) + (first_piece && begins_inside ? 2 : 0), run.first_query, run.queries);
         };
 
-        // One or two slabs of the run (two: their chains of products and exponentials overlap).
+        // Two slabs of the run that all rows see whole (their chains of products and exponentials overlap), or any one.  (With masks
+        // in the pair's code 2 x 131071 tokens take 79 us instead of 76, with a third form of it 78.)
         auto work = [&](auto count, const uint8_t *const (&slab)[2], const int (&at)[2]) {
             constexpr int N = decltype(count)::value;
             float s[N][NT][4];
@@ -382,7 +383,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_attention_kernel(const Atten
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
                     for (int k = 0; k < 4; ++k) s[u][n][k] *= factor[n][k & 1];
-                if (!plain(at[u])) {
+                if (N == 1 && !plain(at[u])) {
                     const int token0 = at[u] * KV_SLAB;
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
@@ -443,7 +444,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_attention_kernel(const Atten
                 read_words<D>(slab[u] + kv_value_codes(D) + 32 * S::PIECE_BYTES + lane * S::PIECE_BYTES, v1);
                 read_params<2 * S::GROUPS>(slab[u] + kv_value_params(D) + t * S::GROUPS * 8, q0);
                 read_params<2 * S::GROUPS>(slab[u] + kv_value_params(D) + (t + 4) * S::GROUPS * 8, q1);
-                if (!plain(at[u])) {   // tokens that no row sees may hold anything: zeros (their weights are zero too, but not times NaN)
+                if (N == 1 && !plain(at[u])) {   // tokens that no row sees may hold anything: zeros (their weights are zero too, but not times NaN)
                     const int token = at[u] * KV_SLAB + 2 * t;
                     auto seen = [&](int k) { return k < run.length && (k >= seen_from || k < a.sinks); };
                     const uint32_t keep0 = (seen(token) ? 0xffffu : 0u) | (seen(token + 1) ? 0xffff0000u : 0u);
@@ -480,10 +481,10 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_attention_kernel(const Atten
                 st.clear();
                 fresh = false;
                 const int past = max(0, run.length - run.queries + row0 / a.group + 1);   // of the tokens that the first row may see
-                plain_to = past / KV_SLAB;
                 seen_from = a.window ? max(0, past - a.window) : 0;
                 plain_from = a.window ? max(0, run.length - 1 - a.window + KV_SLAB) / KV_SLAB : 0;
-                plain_sinks = min(a.sinks / KV_SLAB, plain_to);
+                plain_count = max(0, past / KV_SLAB - plain_from);
+                plain_sinks = min(a.sinks, past) / KV_SLAB;
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     const int row = row0 + 8 * n + g, query = row / a.group;
@@ -540,7 +541,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_attention_kernel(const Atten
             const bool there[2] = {!(absent >> (2 * stage) & 1), !(absent >> (2 * stage) & 2)};   // (of the second: if there are two)
             ++taken;
             if (++stage == STAGES) stage = 0, parity ^= 1;
-            if (two == 2 && there[0] && there[1]) {
+            if (two == 2 && there[0] && there[1] && plain(at[0]) && plain(at[1])) {
                 work(std::integral_constant<int, 2>(), slab, at);
             } else {
 #pragma unroll 1
