@@ -37,9 +37,9 @@ __device__ __forceinline__ Run make_run(const Attention &a, int b, int row0, int
     Run r;
     static_cast<Sequence &>(r) = sequence(a, b);
     r.sink_units = r.window_unit = r.units = 0;
-    const int64_t all = (int64_t)r.queries * a.group;
+    const int64_t all = (int64_t)r.served(a) * a.group;
     if (row0 >= all) return r;
-    const int p0 = r.length - r.queries + row0 / a.group, p1 = r.length - r.queries + (int)((min(all, (int64_t)row0 + rows) - 1) / a.group);
+    const int p0 = r.start() + row0 / a.group, p1 = r.start() + (int)((min(all, (int64_t)row0 + rows) - 1) / a.group);
     if (p1 < 0) return r;
     const int end = p1 / KV_SLAB + 1;
     if (a.window) {
@@ -480,7 +480,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_attention_kernel(const Atten
             if (fresh) {           // another run: its queries into registers
                 st.clear();
                 fresh = false;
-                const int past = max(0, run.length - run.queries + row0 / a.group + 1);   // of the tokens that the first row may see
+                const int past = max(0, run.start() + row0 / a.group + 1);   // of the tokens that the first row may see
                 seen_from = a.window ? max(0, past - a.window) : 0;
                 plain_from = a.window ? max(0, run.length - 1 - a.window + KV_SLAB) / KV_SLAB : 0;
                 plain_count = max(0, past / KV_SLAB - plain_from);
@@ -488,7 +488,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_attention_kernel(const Atten
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     const int row = row0 + 8 * n + g, query = row / a.group;
-                    const bool there = query < run.queries;
+                    const bool there = query < run.served(a);
                     const char *src = a.q + (int64_t)(run.first_query + query) * a.q_token_stride + (head * a.group + row % a.group) * a.q_head_stride;
                     float top = 0.0f;
                     uint4 raw[S::WORDS];
@@ -526,7 +526,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_attention_kernel(const Atten
                     for (int e = 0; e < 2; ++e) {
                         factor[n][e] = a.scale_log2 * __shfl_sync(0xffffffffu, unscale, (2 * t + e) * 4);
                         const int r = row0 + 8 * n + 2 * t + e;
-                        place[n][e] = r / a.group < run.queries ? run.length - run.queries + r / a.group : -1;
+                        place[n][e] = r / a.group < run.served(a) ? run.start() + r / a.group : -1;
                     }
                 }
             }
@@ -618,7 +618,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv_attention_kernel(const Atten
 }
 
 // One CTA a run: joins what several CTAs of kv_attention_kernel have left of it, in their order, and zeroes rows of runs
-// without units.  It finds the CTAs from the lengths, before the kernel in front has ended (which began when they were there).
+// without units and rows that are no sequence's.  It finds the CTAs from the lengths, before the kernel in front has ended (which began when they were there).
 template <int D, int NT, int WARPS, bool BF16>
 __global__ void __launch_bounds__(256) kv_join_kernel(const Attention a, int ctas) {
     constexpr int ROWS = 8 * NT, PIECE = ROWS * (D + 2);
@@ -629,6 +629,7 @@ __global__ void __launch_bounds__(256) kv_join_kernel(const Attention a, int cta
     const bool whole = whole_runs<D>(a, row0, ROWS);
     first += (uint32_t)head * run.units;
     const int c0 = first / quota, c1 = run.units ? (first + run.units - 1) / quota : c0;
+    if (blockIdx.y == 0) zero_rows_next_to(a, run, b, D, head * 256 + threadIdx.x, (int64_t)a.kv_heads * 256);
     // (CTAs without work wait too: what follows this kernel takes its end for that of the kernel in front)
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (whole || (run.units && c0 == c1)) return;
@@ -701,7 +702,7 @@ int launch(const Attention &a, int64_t tiles, int ctas, cudaStream_t stream) {
     auto *kernel = kv_attention_kernel<D, NT, WARPS, STAGES, BF16>;
     int e = allow_smem<kv_attention_kernel<D, NT, WARPS, STAGES, BF16>>(S::SMEM, what);
     if (e == ATLAS_OK) e = launch_early(kernel, dim3((unsigned)ctas, (unsigned)tiles), WARPS * 32, S::SMEM, stream, what, a);
-    if (e != ATLAS_OK || (a.few_runs && a.max_tokens <= kv_whole_units(D) * KV_SLAB)) return e;
+    if (e != ATLAS_OK || (a.few_runs && a.max_tokens <= kv_whole_units(D) * KV_SLAB && !a.query_starts)) return e;
     return launch_early(kv_join_kernel<D, NT, WARPS, BF16>, dim3((unsigned)(a.batch * a.kv_heads), (unsigned)tiles), 256, 0, stream, what, a, ctas);
 }
 
@@ -751,7 +752,9 @@ int atlas_kv_attention(const AtlasKvAttention *p, void *stream) {
     const char *what = "atlas_kv_attention";
     const int args = check_arguments(p, what);
     if (args != ATLAS_OK) return args;
-    if (p->total_queries == 0 || p->batch == 0) return ATLAS_OK;
+    if (p->total_queries == 0 || (p->batch == 0 && !p->out)) return ATLAS_OK;
+    if (p->batch == 0)   // (no sequence has them)
+        return check_cuda(cudaMemsetAsync(p->out, 0, (size_t)p->total_queries * p->q_heads * p->head_dim * 2, (cudaStream_t)stream), what);
     ATLAS_RETURN_IF(!p->query_starts && p->total_queries % p->batch, ATLAS_ERR_BAD_ARGUMENT, "%s: %lld queries of %lld sequences without query_starts", what,
                     (long long)p->total_queries, (long long)p->batch);
     ATLAS_RETURN_IF(p->max_queries < (p->query_starts ? 1 : p->total_queries / p->batch), ATLAS_ERR_BAD_ARGUMENT, "%s: max_queries %lld", what,
@@ -777,6 +780,7 @@ int atlas_kv_attention(const AtlasKvAttention *p, void *stream) {
     a.partial = (float *)p->workspace, a.status = p->status;
     a.num_pages = p->num_pages, a.table_stride = p->table_stride, a.max_tokens = p->max_pages * p->page_size;
     a.total_queries = p->total_queries, a.uniform = p->query_starts ? 0 : p->total_queries / p->batch;
+    a.max_queries = (int)p->max_queries;
     a.batch = (int)p->batch, a.q_heads = p->q_heads, a.kv_heads = p->kv_heads, a.group = p->q_heads / p->kv_heads;
     // A window of all tokens hides none: as no window it needs no masks, and position - window stays within 32 bits below (a query
     // may be at a negative position, and 2^31 - 1 is a usual "no window").

@@ -14,7 +14,7 @@ struct Attention {
     float *partial;
     int32_t *status;
     int64_t num_pages, table_stride, max_tokens, total_queries, uniform;
-    int batch, q_heads, kv_heads, group, page_size, window, sinks;   // group: query heads of a kv head
+    int batch, q_heads, kv_heads, group, page_size, window, sinks, max_queries;   // group: query heads of a kv head
     float scale_log2;
     bool few_runs;               // no more sequences times kv heads than CTAs
 };
@@ -40,6 +40,8 @@ namespace {
 struct Sequence {
     int first_query;             // in q
     int length, queries;
+    __device__ __forceinline__ int start() const { return length - queries; }   // position of the first query (negative if there are fewer tokens than queries)
+    __device__ __forceinline__ int served(const Attention &a) const { return min(queries, a.max_queries); }
 };
 __device__ __forceinline__ Sequence sequence(const Attention &a, int b) {
     Sequence r;
@@ -55,10 +57,25 @@ __device__ __forceinline__ Sequence sequence(const Attention &a, int b) {
     r.length = (int)min(max((int64_t)a.lengths[b], (int64_t)0), a.max_tokens);
     return r;
 }
+// Rows of q next to a sequence that are no sequence's, or beyond max_queries: in front of the first, and behind those served.
+__device__ __forceinline__ int rows_in_front(const Sequence &r, int b) { return b == 0 ? r.first_query : 0; }
+__device__ __forceinline__ int rows_behind(const Attention &a, const Sequence &r, int b) {
+    return (b + 1 == a.batch ? (int)a.total_queries - r.first_query : r.queries) - r.served(a);
+}
+// Their outputs are zeros, by `threads` threads of which this one is `thread`.
+__device__ __forceinline__ void zero_rows(const Attention &a, int first, int count, int d, int64_t thread, int64_t threads) {
+    const int64_t pieces = (int64_t)a.q_heads * d / 8;
+    uint4 *out = reinterpret_cast<uint4 *>(a.out) + first * pieces;
+    for (int64_t i = thread; i < count * pieces; i += threads) out[i] = make_uint4(0, 0, 0, 0);
+}
+__device__ __forceinline__ void zero_rows_next_to(const Attention &a, const Sequence &r, int b, int d, int64_t thread, int64_t threads) {
+    zero_rows(a, 0, rows_in_front(r, b), d, thread, threads);
+    zero_rows(a, r.first_query + r.served(a), rows_behind(a, r, b), d, thread, threads);
+}
 // Where a row's output is, or null.
 __device__ __forceinline__ char *out_row(const Attention &a, const Sequence &r, int h, int row, int d) {
     const int query = row / a.group;
-    if (query >= r.queries) return nullptr;
+    if (query >= r.served(a)) return nullptr;
     return a.out + ((int64_t)(r.first_query + query) * a.q_heads + h * a.group + row - query * a.group) * d * 2;
 }
 

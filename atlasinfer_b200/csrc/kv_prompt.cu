@@ -149,10 +149,17 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_prompt_kernel(const Attentio
     // later rows see more: those of all heads and sequences go first
     const int row0 = (int)(gridDim.y - 1 - blockIdx.y) * P::ROWS;
     const Sequence seq = sequence(a, b);
-    const int rows = (int)min((int64_t)P::ROWS, (int64_t)seq.queries * a.group - row0);
-    if (rows <= 0) return;
+    // (rows that are no sequence's: one warp of each CTA of the sequence next to them)
+    auto zero_rest = [&]() {
+        zero_rows_next_to(a, seq, b, D, ((int64_t)(split * a.kv_heads + head) * gridDim.y + blockIdx.y) * 32 + lane, (int64_t)splits * a.kv_heads * gridDim.y * 32);
+    };
+    const int rows = (int)min((int64_t)P::ROWS, (int64_t)seq.served(a) * a.group - row0);
+    if (rows <= 0) {
+        if (warp == PR_LOAD) zero_rest();
+        return;
+    }
     const int used = TILES == 2 && rows > 128 ? 2 : 1;   // row tiles with rows
-    const int p_first = seq.length - seq.queries + row0 / a.group, p_last = seq.length - seq.queries + (row0 + rows - 1) / a.group;
+    const int p_first = seq.start() + row0 / a.group, p_last = seq.start() + (row0 + rows - 1) / a.group;
     const Walk<KEYS> walk(a, p_first, p_last);
     const int j0 = (int)((int64_t)walk.tiles * split / splits), tiles = (int)((int64_t)walk.tiles * (split + 1) / splits) - j0;
 
@@ -221,6 +228,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_prompt_kernel(const Attentio
                 __nanosleep(100);
             }
         }
+        zero_rest();
     } else if (warp >= PR_REBUILD && warp < PR_REBUILD + PR_REBUILDERS) {
         // ------------------------------ codes to fp16: a warp a slab, half of the warps keys, half values ------------------------------
         const int g = lane / 4, t = lane % 4;
@@ -431,10 +439,10 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_prompt_kernel(const Attentio
 
         // ------------------------------ softmax: a thread a row ------------------------------
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-        const int place = live ? seq.length - seq.queries + query : -1;
+        const int place = live ? seq.start() + query : -1;
         // first and last position of this row tile, for tiles that need no mask
-        const int t_first = seq.length - seq.queries + (row0 + tile * 128) / a.group;
-        const int t_last = min(p_last, seq.length - seq.queries + (row0 + tile * 128 + 127) / a.group);
+        const int t_first = seq.start() + (row0 + tile * 128) / a.group;
+        const int t_last = min(p_last, seq.start() + (row0 + tile * 128 + 127) / a.group);
         const uint32_t t_out = tmem + lanes + tile * D;
         const f32x2 factor2 = pair(factor, factor);
         float m = -INFINITY, l = 0.0f;

@@ -121,8 +121,9 @@ def cache_attention(q: torch.Tensor, cache: QuantizedKVCache, page_table: torch.
 
     Sequence ``b`` has ``lengths[b]`` tokens (int32) in the pages ``page_table[b]`` (int32 ``[sequences, pages]``); the last
     of them are those of its own queries, which must have been stored.  Its queries are rows ``query_starts[b]`` to
-    ``query_starts[b + 1]`` of ``q`` (int32 ``[sequences + 1]``; default: equally many each), at most ``max_queries`` (an upper
-    bound for choosing the kernel; default: all).  A query sees the keys up to its own position, with a ``window`` only the
+    ``query_starts[b + 1]`` of ``q`` (int32 ``[sequences + 1]``; default: equally many each), at most ``max_queries`` (on the
+    host: it decides which kernel runs and how many rows; default: all).  Rows that belong to no sequence, or to one beyond its
+    first ``max_queries``, give zeros.  A query sees the keys up to its own position, with a ``window`` only the
     last ``window`` of those and the first ``sinks``; pages that no query sees are not read, and their entries in
     ``page_table`` may be anything.  A query that sees nothing gives zeros.  ``scale`` defaults to ``head_dim ** -0.5``.
 

@@ -453,7 +453,9 @@ ATLAS_API int atlas_kv_load(const void *cache, int64_t num_pages, int kv_heads, 
  *                    the cache counts as hidden
  *   query_starts     int32 [batch + 1] first query of every sequence, or NULL:
  *                    total_queries / batch each
- *   max_queries      at least the queries of any sequence
+ *   max_queries      at least the queries of any sequence.  Rows of q that are
+ *                    no sequence's, and a sequence's queries beyond max_queries,
+ *                    give zeros
  *   workspace        atlas_kv_attention_workspace_bytes(...) bytes, 256-byte
  *                    aligned; contents irrelevant before and after
  *   status           device int32 or NULL, set non-zero if a bounded wait ran out

@@ -66,3 +66,56 @@ def test_what_no_query_sees_may_hold_anything(cuda_device, d, window, sinks, que
         assert hidden.any()
         spoil(w, b, hidden, word)
     assert torch.equal(w.run(**how), want)
+
+
+def spoil_free_memory(like):
+    """Blocks of this size that the allocator hands out next hold NaN."""
+    for _ in range(2):
+        blocks = [torch.full_like(like, float("nan")) for _ in range(4)]
+        del blocks
+
+
+@pytest.mark.parametrize("starts,total,most", [([3, 5, 9, 9], 14, 4), ([0, 1, 2, 3], 3, 1), ([2, 2, 2, 2], 40, 1), ([3, 63, 110, 150], 170, 60), ([0, 6, 8, 9], 9, 2), ([0, 50, 95, 96], 96, 40),
+                                               ([1, 41, 42, 130], 130, 40), ([0, 0, 1, 2], 4096, 2), ([0, 300, 500, 700], 2000, 200)])
+@pytest.mark.parametrize("d,hq,hkv", [(128, 4, 2), (64, 6, 2), (256, 2, 2)])
+def test_rows_of_no_sequence(cuda_device, d, hq, hkv, starts, total, most):
+    """Rows in front of the first start, behind the last and beyond max_queries are zeros; the others are as without them."""
+    counts = [b - a for a, b in zip(starts, starts[1:])]
+    w = Work(cuda_device, [400, 120, 333], counts, hq, hkv, d, page=32)
+    out, mass = R.attention(w.q, w.ks, w.vs, counts)
+    want, slack = torch.zeros(2, total, hq, d, dtype=torch.float64)
+    rows = []
+    for a, b in zip(starts, starts[1:]):
+        rows += list(range(a, min(b, a + most)))
+    at = torch.tensor(rows, dtype=torch.int64)
+    want[at], slack[at] = out[at - starts[0]], mass[at - starts[0]] * (2.0 ** -10 + 2e-5) + 1e-6
+    q = torch.full((total, hq, d), float("nan"), dtype=BF16, device=cuda_device)
+    q[starts[0]:starts[-1]] = w.q
+    lengths = torch.tensor(w.lengths, dtype=torch.int32, device=cuda_device)
+    spoil_free_memory(q)
+    got = ab.cache_attention(q, w.cache, w.table, lengths, query_starts=torch.tensor(starts, dtype=torch.int32, device=cuda_device), max_queries=most)
+    R.assert_rounded(got, want, slack)
+    rest = torch.ones(total, dtype=torch.bool)
+    rest[at] = False
+    assert not got[rest.to(cuda_device)].any()
+
+
+def test_starts_without_a_bound_and_out_of_order(cuda_device):
+    """All queries is the bound where none is given; a start behind the next one is the end of an empty sequence."""
+    w = Work(cuda_device, [64, 64], [2, 0], 4, 2, 64, page=16)
+    lengths = torch.tensor(w.lengths, dtype=torch.int32, device=cuda_device)
+    for starts in ([0, 2, 2], [0, 2, 1], [-5, 2, 2 ** 31 - 1]):
+        spoil_free_memory(w.q)
+        w.check(ab.cache_attention(w.q, w.cache, w.table, lengths, query_starts=torch.tensor(starts, dtype=torch.int32, device=cuda_device)))
+    w = Work(cuda_device, [300, 70], [90, 40], 4, 2, 64, page=16)
+    lengths = torch.tensor(w.lengths, dtype=torch.int32, device=cuda_device)
+    w.check(ab.cache_attention(w.q, w.cache, w.table, lengths, query_starts=w.starts))
+
+
+def test_queries_without_sequences(cuda_device):
+    cache = ab.QuantizedKVCache(2, 2, 64, page_size=16, device=cuda_device)
+    q = torch.ones(5, 4, 64, dtype=F16, device=cuda_device)
+    none = torch.zeros(0, dtype=torch.int32, device=cuda_device)
+    spoil_free_memory(q)
+    got = ab.cache_attention(q, cache, none.view(0, 3), none, query_starts=torch.zeros(1, dtype=torch.int32, device=cuda_device))
+    assert got.shape == q.shape and not got.any()
