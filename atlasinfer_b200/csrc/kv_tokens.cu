@@ -368,6 +368,8 @@ int atlas_norm_rotate(const AtlasTokens *p, void *stream) {
     ATLAS_RETURN_IF(p->table && (!p->positions || p->table_rows < 1), ATLAS_ERR_BAD_ARGUMENT, "%s: a table needs rows and positions", what);
     ATLAS_RETURN_IF(p->table && (p->rotary_dim < 16 || p->rotary_dim % 16 || p->rotary_dim > p->head_dim), ATLAS_ERR_UNSUPPORTED,
                     "%s: rotary_dim %d is not a multiple of 16 up to head_dim", what, p->rotary_dim);
+    ATLAS_RETURN_IF(p->table && p->position_bytes != 4 && p->position_bytes != 8, ATLAS_ERR_BAD_ARGUMENT, "%s: positions of %d bytes", what, p->position_bytes);
+    ATLAS_RETURN_IF(store && p->slot_bytes != 4 && p->slot_bytes != 8, ATLAS_ERR_BAD_ARGUMENT, "%s: slots of %d bytes", what, p->slot_bytes);
     const bool q_fits = !p->q_heads || (aligned16(p->q, 2 * p->q_token_stride, 2 * p->q_head_stride) && aligned16(p->q_out, 0, 0));
     const bool v_fits = !store || (aligned16(p->v, 2 * p->v_token_stride, 2 * p->v_head_stride) && aligned16(p->cache, 0, 0));
     ATLAS_RETURN_IF(!q_fits || !v_fits || !aligned16(p->k, 2 * p->k_token_stride, 2 * p->k_head_stride) || !aligned16(p->k_out, 0, 0) ||

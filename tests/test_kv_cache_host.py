@@ -21,3 +21,12 @@ def test_report_of_a_wait_that_ran_out():
         atlas_wrappers.check_status(cpu)
     assert e.value.status == _capi.ERR_TIMEOUT
     atlas_wrappers.check_status(cpu)   # cleared
+
+
+def test_index_types_are_checked(lib):
+    """Positions and slots of neither 4 nor 8 bytes are refused, not read as 4.  (k is at no address that would be used.)"""
+    for size in (0, 2, 16):
+        t = _capi.Tokens(dtype=0, kv_heads=1, head_dim=64, tokens=1, k=17, k_out=16, table=16, positions=16, table_rows=4, rotary_dim=32, position_bytes=size)
+        assert lib.atlas_norm_rotate(t, None) == _capi.ERR_BAD_ARGUMENT and b"positions" in lib.atlas_last_error()
+        t = _capi.Tokens(dtype=0, kv_heads=1, head_dim=64, tokens=1, k=17, v=16, cache=16, num_pages=1, page_size=16, slots=16, slot_bytes=size)
+        assert lib.atlas_norm_rotate(t, None) == _capi.ERR_BAD_ARGUMENT and b"slots" in lib.atlas_last_error()
