@@ -761,14 +761,15 @@ int atlas_kv_attention(const AtlasKvAttention *p, void *stream) {
                     (long long)p->max_queries);
     ATLAS_RETURN_IF(!p->q || !p->out || !p->lengths || (p->num_pages && !p->cache) || (p->max_pages && !p->page_table), ATLAS_ERR_BAD_ARGUMENT,
                     "%s: null pointer", what);
+    const Plan plan = plan_of(*p);
+    ATLAS_RETURN_IF((kv_prompt_serves(*p) ? kv_prompt_blocks(*p) : plan.tiles) > 65535, ATLAS_ERR_UNSUPPORTED, "%s: %lld queries in a sequence", what,
+                    (long long)p->max_queries);
     ATLAS_RETURN_IF(!aligned16(p->q, 2 * p->q_token_stride, 2 * p->q_head_stride) || !aligned16(p->out, 0, 0) || !aligned16(p->cache, 0, 0) ||
                         (reinterpret_cast<uintptr_t>(p->workspace) & 255),
                     ATLAS_ERR_BAD_ARGUMENT, "%s: pointers and strides must be multiples of 16 bytes, the workspace of 256", what);
     const int dev = check_device();
     if (dev != ATLAS_OK) return dev;
-    const Plan plan = plan_of(*p);
     const int ctas = (int)std::max<int64_t>(1, sm_count() / plan.tiles);   // (all row tiles at a time)
-    ATLAS_RETURN_IF(!kv_prompt_serves(*p) && plan.tiles > 65535, ATLAS_ERR_UNSUPPORTED, "%s: %lld queries in a sequence", what, (long long)p->max_queries);
     const size_t bytes = atlas_kv_attention_workspace_bytes(p);
     ATLAS_RETURN_IF(bytes && (!p->workspace || p->workspace_bytes < bytes), ATLAS_ERR_CAPACITY, "%s: workspace of %zu bytes, %zu needed", what,
                     p->workspace_bytes, bytes);

@@ -21,6 +21,7 @@ struct Attention {
 
 // Prompts: kv_prompt.cu.  Bytes of workspace, and the launch.
 bool kv_prompt_serves(const AtlasKvAttention &p);
+int64_t kv_prompt_blocks(const AtlasKvAttention &p);   // row blocks of a sequence: the grid's second dimension
 size_t kv_prompt_workspace_bytes(const AtlasKvAttention &p);
 int kv_prompt(const Attention &a, const AtlasKvAttention &p, cudaStream_t stream);
 

@@ -662,6 +662,8 @@ bool kv_prompt_serves(const AtlasKvAttention &p) {
     return p.max_queries * (p.q_heads / p.kv_heads) > (p.head_dim == 256 ? 24 : 32) && p.batch * p.kv_heads <= (1 << 20);
 }
 
+int64_t kv_prompt_blocks(const AtlasKvAttention &p) { return plan_of(p).blocks; }
+
 size_t kv_prompt_workspace_bytes(const AtlasKvAttention &p) { return plan_of(p).bytes; }
 
 int kv_prompt(const Attention &a, const AtlasKvAttention &p, cudaStream_t stream) {

@@ -30,3 +30,13 @@ def test_index_types_are_checked(lib):
         assert lib.atlas_norm_rotate(t, None) == _capi.ERR_BAD_ARGUMENT and b"positions" in lib.atlas_last_error()
         t = _capi.Tokens(dtype=0, kv_heads=1, head_dim=64, tokens=1, k=17, v=16, cache=16, num_pages=1, page_size=16, slots=16, slot_bytes=size)
         assert lib.atlas_norm_rotate(t, None) == _capi.ERR_BAD_ARGUMENT and b"slots" in lib.atlas_last_error()
+
+
+@pytest.mark.parametrize("d,block", [(64, 256), (128, 256), (256, 128)])
+def test_prompts_beyond_the_grid_are_refused(lib, d, block):
+    """A sequence of more row blocks than a grid's second dimension holds: refused by name, not by a failed launch."""
+    a = _capi.KvAttention(dtype=0, q_heads=64, kv_heads=1, head_dim=d, page_size=16, num_pages=1, max_pages=1, batch=1, q=17, out=16, cache=16, page_table=16, lengths=16)
+    a.total_queries = a.max_queries = 65535 * block // 64 + 1
+    assert lib.atlas_kv_attention(a, None) == _capi.ERR_UNSUPPORTED and b"queries in a sequence" in lib.atlas_last_error()
+    a.total_queries = a.max_queries = 65535 * block // 64
+    assert lib.atlas_kv_attention(a, None) == _capi.ERR_BAD_ARGUMENT   # (for its addresses, which are looked at after that)
