@@ -590,6 +590,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) kv_prompt_kernel(const Attentio
     if (*s_abort) {
         // a wait ran out somewhere: no copy may land, and no MMA run, once this CTA has gone
         if (warp == PR_LOAD && issued > 0) mbar_wait<100>(bar(P::RAW_FULL + lane / 16 * RING + lane % 16), (uint32_t)((issued - 1) & 1));
+        if (warp < PR_REBUILD) mbar_wait<100>(bar(P::Q_RAW + warp), 0);
         if (warp == PR_MMA && lane == 0) {
             umma_commit(bar(P::DRAIN));
             mbar_wait<100>(bar(P::DRAIN), 0);
