@@ -185,7 +185,7 @@ __global__ void __launch_bounds__(256, 4) tokens_kernel(const Tokens a) {
     float cs[8], sn[8];          // of the own channels; the sine with the sign that it has there
     if (turned) {
         const int64_t at = index_at(a.positions, a.wide_positions, token);
-        const bool known = at >= 0 && at < a.table_rows;   // (elsewhere there is no angle: the token becomes NaN)
+        const bool known = at >= 0 && at < a.table_rows;   // (elsewhere there is no angle: what it would turn becomes NaN)
         const float *row = a.table + (known ? at : 0) * a.rotary;
         if (a.interleaved) {
             const float4 c = *reinterpret_cast<const float4 *>(row + unit * 4), n = *reinterpret_cast<const float4 *>(row + a.rotary / 2 + unit * 4);

@@ -100,7 +100,7 @@ def norm_rotate(q: torch.Tensor, k: torch.Tensor, table: Optional[torch.Tensor] 
     With a weight a head becomes ``x * rsqrt(mean(x^2) + eps) * (weight + weight_offset)`` (weights ``[head_dim]``, of the
     tensors' dtype or fp32).  With a ``table`` (``rotary_table``) and ``positions`` (``[tokens]``, int32 or int64) its first
     ``table.shape[1]`` channels are rotated, in pairs half of them apart or (``interleaved``) next to each other.  Computed in
-    fp32, rounded once.  A token whose position is not in the table becomes NaN."""
+    fp32, rounded once.  The rotated channels of a token whose position is not in the table become NaN."""
     return _capi.native().norm_rotate(q, k, None, table, positions, q_weight, k_weight, eps, weight_offset, interleaved, None, 0, 0, None)
 
 
@@ -109,7 +109,10 @@ def norm_rotate_store(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: 
                       q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
                       weight_offset: float = 0.0, interleaved: bool = False) -> torch.Tensor:
     """``norm_rotate`` whose keys, with ``v``, go to ``slots`` of ``cache`` (as by ``QuantizedKVCache.store``, but without a
-    rounding to 16 bits in between); returns the queries."""
+    rounding to 16 bits in between); returns the queries.
+
+    The cache holds no NaN: of a token whose position is not in the table, the key's rotated channels are stored as zeros, and
+    only its query shows it."""
     return _capi.native().norm_rotate(q, k, v, table, positions, q_weight, k_weight, eps, weight_offset, interleaved,
                                       cache.data, cache.head_dim, cache.page_size, slots)[0]
 

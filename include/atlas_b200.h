@@ -408,8 +408,9 @@ ATLAS_API size_t atlas_kv_page_bytes(int head_dim, int page_size);
  *                    position's rotary_dim / 2 angles, or NULL (no rotation);
  *                    rotary_dim is a multiple of 16.  Pairs are channels i and
  *                    i + rotary_dim / 2, or 2 i and 2 i + 1 (`interleaved`)
- *   positions        [tokens] int32 or int64 (position_bytes); a token whose
- *                    position is not a row of the table becomes NaN
+ *   positions        [tokens] int32 or int64 (position_bytes); of a token whose
+ *                    position is not a row of the table the first rotary_dim
+ *                    channels become NaN (stored as zeros in the cache)
  *   q_weight, k_weight   [head_dim] of `dtype`, or fp32 (weights_f32), or NULL:
  *                    x * rsqrt(mean(x^2) + eps) * (weight + weight_offset)
  *   cache, slots     [tokens] int32 or int64 (slot_bytes); tokens whose slot is
