@@ -20,7 +20,7 @@ namespace atlas {
 
 constexpr int KV_SLAB = 16;                  // tokens
 constexpr float KV_MIN_SCALE = 0x1p-18f;     // s (c - z) is a multiple of 2^-24, the spacing of the smallest fp16 numbers
-constexpr float KV_MAX_SCALE = 4352.0f;      // 15 s stays below the largest fp16 number
+constexpr float KV_MAX_SCALE = 4352.0f;      // 15 s stays below the largest fp16 number (groups that span more than 15 s lose their upper end)
 constexpr float KV_MAX_VALUE = 15.0f * KV_MAX_SCALE;
 
 __host__ __device__ constexpr int kv_slab_bytes(int d) { return 18 * d; }

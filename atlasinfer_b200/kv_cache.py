@@ -41,7 +41,10 @@ class QuantizedKVCache:
     ``page * page_size + offset``, and which pages are whose is the caller's business.  Every 64 channels of a token and
     head share an fp16 scale and a zero point: value ``s * (c - z)``, ``c`` and ``z`` in 0..15, exact in fp16, at most half a
     step from the number stored, where a step is a fifteenth of the range of the 64 (zero included), rounded up to 7 bits.
-    NaN is stored as 0 and what passes 65280 as that, so the cache holds finite numbers only.
+    That holds for ranges up to 65280, as far as fp16 reaches to one side.  A step is never more than 4352, so 64 numbers of
+    both signs that lie further apart keep their low end, and what is more than ``4352 * (15 - z)`` is stored as that, which may
+    be far off (60000 beside -60000 as 4352): scale such keys or values down.  NaN is stored as 0, and what passes 65280 to
+    either side counts as that, so the cache holds finite numbers only.
 
     ``data``: storage to use (uint8 ``[num_pages, kv_heads, page_bytes]``, contiguous); default: zero-filled."""
 

@@ -391,9 +391,12 @@ ATLAS_API int atlas_qlinear_gemm(const void *x, int dtype, int64_t m, int64_t ld
  * value = s (c - z), c and z in 0..15, s of 7 significant bits, which is exact
  * in fp16.  For a group with lo = min(x, 0), hi = max(x, 0): s = (hi - lo) / 15
  * rounded up to 7 bits, in [2^-18, 4352]; z = rint(-lo / s);
- * c = clamp(rint(x / s) + z, 0, 15).  NaN is stored as 0, values saturate at
- * +-65280, so the cache holds finite numbers only.  A token's place is its
- * slot, page * page_size + offset.  head_dim is 64, 128 or 256.
+ * c = clamp(rint(x / s) + z, 0, 15).  NaN counts as 0, and what passes +-65280
+ * as that, so the cache holds finite numbers only.  A number is at most s / 2
+ * from what is stored if hi - lo <= 65280.  Beyond that (numbers of both signs,
+ * s = 4352) the group keeps its low end, and what is more than 4352 (15 - z) is
+ * stored as that: 60000 beside -60000 as 4352.  A token's place is its slot,
+ * page * page_size + offset.  head_dim is 64, 128 or 256.
  */
 ATLAS_API size_t atlas_kv_page_bytes(int head_dim, int page_size);
 
