@@ -136,6 +136,8 @@ def cache_attention(q: torch.Tensor, cache: QuantizedKVCache, page_table: torch.
     Everything about lengths stays on the device: the call can be captured, and replayed for other lengths."""
     if window is not None and window < 1:
         raise ValueError(f"cache_attention: window {window}")
+    if max_queries is not None and max_queries < 0:
+        raise ValueError(f"cache_attention: max_queries {max_queries}")
     return _capi.native().kv_attention(q, cache.data, cache.head_dim, cache.page_size, page_table, lengths, query_starts,
                                        -1 if max_queries is None else max_queries, window or 0, sinks,
                                        cache.head_dim ** -0.5 if scale is None else scale, status_word(q.device))

@@ -40,3 +40,12 @@ def test_prompts_beyond_the_grid_are_refused(lib, d, block):
     assert lib.atlas_kv_attention(a, None) == _capi.ERR_UNSUPPORTED and b"queries in a sequence" in lib.atlas_last_error()
     a.total_queries = a.max_queries = 65535 * block // 64
     assert lib.atlas_kv_attention(a, None) == _capi.ERR_BAD_ARGUMENT   # (for its addresses, which are looked at after that)
+
+
+def test_negative_bounds_are_refused():
+    """max_queries below 0 is no way to say "all"."""
+    import atlasinfer_b200 as ab
+
+    for bad in (-1, -7):
+        with pytest.raises(ValueError, match="max_queries"):
+            ab.cache_attention(None, None, None, None, max_queries=bad)
