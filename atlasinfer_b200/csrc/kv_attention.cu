@@ -13,11 +13,15 @@
 // A run that lies within a warp goes straight to the output; pieces of the others are joined in shared memory, in order, and
 // what goes beyond a CTA is left in the workspace for kv_join_kernel.
 //
-// What bounds it: 2 x 131071 tokens of 8 kv heads, 302 MB, take 80 us (3.8 TB/s, 0.58 of the measured copy rate).  A slab of
-// 128 channels (2304 bytes) costs 341 warp instructions, 250 of them its arithmetic (5 to extract, 4 to centre and, for
-// values, 4 to scale 8 codes); issue slots are 60 % used, mma.sync holds the issue port for 16 % more, and DRAM waits are few.
+// Tokens that no row sees may hold anything: their scores are masked, and their values are zeros in the products.
+//
+// What bounds it: 2 x 131071 tokens of 8 kv heads, 302 MB, take 76 us (4.0 TB/s, 0.61 of the measured copy rate).  A slab of
+// 128 channels (2304 bytes) costs 334 warp instructions, 250 of them its arithmetic (5 to extract, 4 to centre and, for
+// values, 4 to scale 8 codes).  Issue slots are 60 % used and mma.sync holds the issue port for some 16 % more; in the
+// rest all three warps of a scheduler wait for results of their own (few of them for DRAM).
 // Two slabs at a time on 12 warps of 168 registers: brought in one by one they took 87 us, as one at a time on 16 warps of 128
 // did, which is behind on short contexts (4001 tokens of 32 heads 22.5 us and 20.6); two at a time on 128 registers spills (129).
+// (All four with masks in the pairs' code.)
 // Short calls are a chain of waits: 1 us to plan, 1 to find pages, 1 for the first slab, 1 to join.
 #include <algorithm>
 

@@ -91,7 +91,9 @@ __device__ __forceinline__ float exp2_fast(float x) {
 __device__ __forceinline__ uint32_t h2(__half2 v) { return *reinterpret_cast<uint32_t *>(&v); }
 __device__ __forceinline__ __half2 h2(uint32_t v) { return *reinterpret_cast<__half2 *>(&v); }
 
-// The four pairs of a word of codes, minus the zero point: `bias` is 1024 + z, `minus16` is -(64 + z) = 960 - bias.
+// The four pairs of a word of codes, minus the zero point: `bias` is 1024 + z, `minus16` is -(64 + z) = 960 - bias.  (Small integers
+// become fp16 by the bits of 1024 in front of them, where a unit in the last place is 1: Kim et al. 2022, "Who Says Elephants Can't
+// Run".)
 __device__ __forceinline__ uint32_t masked_or(uint32_t w, uint32_t mask, uint32_t bits) {
     uint32_t r;
     asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "r"(mask), "r"(bits));

@@ -6,14 +6,17 @@
 //   P = 2^(S' - m) a thread a row; P goes back to tensor memory as fp16, over S
 //   O += P V       tcgen05, P from tensor memory, N = D channels, fp32 accumulators in tensor memory
 // K and V are rebuilt from their codes into 128-byte-swizzled K-major tiles in shared memory, as the exact fp16 numbers that
-// the cache stands for, so the only roundings are those of P and of the output.  The running maximum of a row follows its
+// the cache stands for, so the only roundings are those of P and of the output.  (The sum of a row is that of its weights before
+// they are rounded: values that are all alike can come out 2^-11 off.  Sums of the rounded ones, by adds of fp16 to fp32, took
+// 176 us for 166.)  Tokens that no row sees may hold anything, as in kv_attention.cu.  The running maximum of a row follows its
 // scores only where they pass it by 2^8 (O is rescaled then, which is rare); P keeps 14 bits of headroom for that.
 //
 // Warps: four of softmax for each row tile, three that rebuild keys and three that rebuild values, one that issues the MMAs,
 // one that brings halves of slabs (keys, values) in by bulk copies, each half as far ahead as its ring has room.  While the
 // softmax warps of one row tile work, the tensor core works on the other.
 //
-// What bounds it (4096 queries on 32 heads of 128 over 8 kv heads, 165 us, 833 TFLOP/s, half of the measured peak): a CTA needs
+// What bounds it (4096 queries on 32 heads of 128 over 8 kv heads: 166 us by itself, 830 TFLOP/s, half of the measured peak; 170
+// to 175 us in passes through the entry point, by the power that is left): a CTA needs
 // 2800 cycles for a tile of 128 tokens, of which the tensor core works 2048 at its peak rate, and some 23000 for its start and end
 // (14000 until the first S: rows of Q by bulk copies, slabs, rebuilding; 7000 behind the last P), a fifth of the largest.  In
 // the loop the chain of a row tile (S, maximum, weights, P, two products) is the bound: exponentials replaced by copies gave 7 %,
