@@ -11,7 +11,8 @@ Public surface (same names as the reference project):
 Additions next to that surface: ``quantize_tensors`` (batched), ``fuse_linears`` /
 ``fuse_sibling_linears`` (q/k/v and gate/up as one launch), ``save_quantized*`` /
 ``load_quantized*`` (on-disk format); ``QuantizedKVCache``, ``norm_rotate``, ``norm_rotate_store``, ``rotary_table`` and
-``cache_attention`` (queries, keys, a 4-bit key/value cache and the attention over it).
+``cache_attention`` (queries, keys, a 4-bit key/value cache and the attention over it); ``residual_norm``,
+``linear_epilogue``, ``gated_linear`` and ``token_logprobs`` (a decoder step around its linears).
 
 All arithmetic runs in ``lib/libatlas_b200.so`` (build: ``python -m atlasinfer_b200.build``).
 """
@@ -21,6 +22,7 @@ from .quant.serialization import (load_quantized, load_quantized_model, load_qua
                                   save_quantized_model, save_quantized_state)
 from .integration.atlas_wrappers import FusedLinearGroup, QuantizedLinear, fuse_linears
 from .integration.model_modifier import apply_atlas_quantization_to_model, fuse_sibling_linears
+from .decoder_ops import TokenLogprobs, gated_linear, linear_epilogue, residual_norm, token_logprobs
 from .kv_cache import QuantizedKVCache, cache_attention, norm_rotate, norm_rotate_store, rotary_table
 
 __all__ = [
@@ -31,5 +33,6 @@ __all__ = [
     "save_quantized", "load_quantized", "save_quantized_state", "load_quantized_state",
     "save_quantized_model", "load_quantized_model",
     "QuantizedKVCache", "norm_rotate", "norm_rotate_store", "rotary_table", "cache_attention",
+    "residual_norm", "linear_epilogue", "gated_linear", "token_logprobs", "TokenLogprobs",
 ]
 __version__ = "0.1.0"

@@ -29,6 +29,7 @@ EXPORTS = (
     "atlas_peer_release",
     "atlas_qlinear_gemm_workspace_bytes", "atlas_qlinear_gemm", "atlas_qlinear_gemm_gather",
     "atlas_kv_page_bytes", "atlas_norm_rotate", "atlas_kv_load", "atlas_kv_attention_workspace_bytes", "atlas_kv_attention",
+    "atlas_fused_linear_workspace_bytes", "atlas_fused_linear", "atlas_residual_norm", "atlas_token_logprobs",
 )
 
 MAX_PEERS = 8
@@ -93,6 +94,41 @@ class KvAttention(ctypes.Structure):
                 ("sinks", ctypes.c_int32), ("scale", ctypes.c_float), ("page_table", ctypes.c_void_p), ("table_stride", ctypes.c_int64),
                 ("max_pages", ctypes.c_int64), ("lengths", ctypes.c_void_p), ("query_starts", ctypes.c_void_p),
                 ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t), ("status", ctypes.c_void_p)]
+
+
+class Weight(ctypes.Structure):
+    """``AtlasWeight`` of include/atlas_b200.h."""
+
+    _fields_ = [("tiles", ctypes.c_void_p), ("scales_tiled", ctypes.c_void_p), ("outlier_chunk_ptr", ctypes.c_void_p),
+                ("outlier_entries", ctypes.c_void_p), ("outlier_vals_sorted", ctypes.c_void_p), ("bias", ctypes.c_void_p)]
+
+
+class FusedLinear(ctypes.Structure):
+    """``AtlasFusedLinear`` of include/atlas_b200.h."""
+
+    _fields_ = [("dtype", ctypes.c_int32), ("activation", ctypes.c_int32), ("x", ctypes.c_void_p), ("m", ctypes.c_int64), ("ldx", ctypes.c_int64),
+                ("n_rows", ctypes.c_int64), ("n_cols", ctypes.c_int64), ("block_size", ctypes.c_int32), ("scale", ctypes.c_float), ("weight", Weight),
+                ("up", Weight), ("residual", ctypes.c_void_p), ("ldr", ctypes.c_int64), ("y", ctypes.c_void_p), ("ldy", ctypes.c_int64),
+                ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t), ("status", ctypes.c_void_p)]
+
+
+class ResidualNorm(ctypes.Structure):
+    """``AtlasResidualNorm`` of include/atlas_b200.h."""
+
+    _fields_ = [("dtype", ctypes.c_int32), ("wide", ctypes.c_int32), ("centered", ctypes.c_int32), ("scale", ctypes.c_float), ("eps", ctypes.c_float),
+                ("weight_offset", ctypes.c_float), ("tokens", ctypes.c_int64), ("hidden", ctypes.c_int64), ("x", ctypes.c_void_p),
+                ("residual", ctypes.c_void_p), ("gate", ctypes.c_void_p), ("x_stride", ctypes.c_int64), ("residual_stride", ctypes.c_int64),
+                ("gate_stride", ctypes.c_int64), ("weight", ctypes.c_void_p), ("bias", ctypes.c_void_p), ("post_weight", ctypes.c_void_p),
+                ("normed", ctypes.c_void_p), ("stream_out", ctypes.c_void_p)]
+
+
+class TokenLogprobs(ctypes.Structure):
+    """``AtlasTokenLogprobs`` of include/atlas_b200.h."""
+
+    _fields_ = [("dtype", ctypes.c_int32), ("top", ctypes.c_int32), ("token_bytes", ctypes.c_int32), ("temperature", ctypes.c_float),
+                ("rows", ctypes.c_int64), ("vocab", ctypes.c_int64), ("logits_stride", ctypes.c_int64), ("logits", ctypes.c_void_p),
+                ("tokens", ctypes.c_void_p), ("logprobs", ctypes.c_void_p), ("entropy", ctypes.c_void_p), ("top_tokens", ctypes.c_void_p),
+                ("top_logprobs", ctypes.c_void_p)]
 
 
 _lib: Optional[ctypes.CDLL] = None
@@ -184,6 +220,11 @@ def load() -> ctypes.CDLL:
     L.atlas_kv_attention_workspace_bytes.argtypes = [ctypes.POINTER(KvAttention)]
     L.atlas_kv_attention.restype = i32
     L.atlas_kv_attention.argtypes = [ctypes.POINTER(KvAttention), vp]
+    L.atlas_fused_linear_workspace_bytes.restype = sz
+    L.atlas_fused_linear_workspace_bytes.argtypes = [ctypes.POINTER(FusedLinear)]
+    for name, struct in (("atlas_fused_linear", FusedLinear), ("atlas_residual_norm", ResidualNorm), ("atlas_token_logprobs", TokenLogprobs)):
+        getattr(L, name).restype = i32
+        getattr(L, name).argtypes = [ctypes.POINTER(struct), vp]
     _lib = L
     return L
 

@@ -22,7 +22,7 @@ LIB_DIR = os.path.join(PKG, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libatlas_b200.so")
 
 SOURCES = ["capi.cu", "quantize.cu", "dequant_repack.cu", "gemv.cu", "stream.cu", "peer.cu", "gemm.cu", "gemm_tile.cu",
-           "kv_tokens.cu", "kv_attention.cu", "kv_prompt.cu"]
+           "kv_tokens.cu", "kv_attention.cu", "kv_prompt.cu", "fused_linear.cu", "residual_norm.cu", "token_logprobs.cu"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
@@ -46,7 +46,7 @@ def _inputs():
 
 
 NATIVE_NAME = "_atlas_native"
-NATIVE_SOURCES = [os.path.join(CSRC, "native.cpp"), os.path.join(CSRC, "native_kv.cpp")]
+NATIVE_SOURCES = [os.path.join(CSRC, "native.cpp"), os.path.join(CSRC, "native_kv.cpp"), os.path.join(CSRC, "native_ops.cpp")]
 
 
 def native_path() -> str:

@@ -1,0 +1,49 @@
+// Quantized linears with an epilogue (epilogue.cuh): argument checks, and which kernel.
+//
+// One weight: as the linears without an epilogue, the per-strip kernel (gemv.cu) up to 16 rows of x, above that the tcgen05
+// kernels (gemm_tile.cu, gemm.cu); the epilogue stands where they round their sums.
+#include "common.cuh"
+#include "linear.cuh"
+
+namespace atlas {
+namespace {
+
+int check(const AtlasFusedLinear *p) {
+    const char *what = "atlas_fused_linear";
+    ATLAS_RETURN_IF(!p, ATLAS_ERR_BAD_ARGUMENT, "%s: no arguments", what);
+    ATLAS_RETURN_IF(p->activation < ATLAS_ACT_NONE || p->activation > ATLAS_ACT_GELU_TANH, ATLAS_ERR_BAD_ARGUMENT, "%s: activation %d", what, p->activation);
+    ATLAS_RETURN_IF(p->m < 0 || p->n_rows <= 0 || p->n_cols <= 0, ATLAS_ERR_BAD_ARGUMENT, "%s: m=%lld n_rows=%lld n_cols=%lld", what, (long long)p->m,
+                    (long long)p->n_rows, (long long)p->n_cols);
+    ATLAS_RETURN_IF(p->residual && p->m > 1 && p->ldr < p->n_rows, ATLAS_ERR_BAD_ARGUMENT, "%s: residual rows %lld apart", what, (long long)p->ldr);
+    ATLAS_RETURN_IF(p->up.tiles && (!p->up.scales_tiled || !p->up.outlier_chunk_ptr || ((uintptr_t)p->up.tiles & 15)), ATLAS_ERR_BAD_ARGUMENT,
+                    "%s: the second weight lacks a buffer, or its tiles are not 16-byte aligned", what);
+    return ATLAS_OK;
+}
+
+}  // namespace
+}  // namespace atlas
+
+extern "C" size_t atlas_fused_linear_workspace_bytes(const AtlasFusedLinear *p) {
+    using namespace atlas;
+    if (check(p) != ATLAS_OK || (!p->up.tiles && p->m <= STRIP_MAX_ROWS)) return 0;
+    return qlinear_gemm_workspace_bytes(p->m, p->n_rows, p->n_cols, p->up.tiles != nullptr);
+}
+
+extern "C" int atlas_fused_linear(const AtlasFusedLinear *p, void *stream) {
+    using namespace atlas;
+    clear_error();
+    const int rc = check(p);
+    if (rc != ATLAS_OK) return rc;
+    if (p->m == 0) return ATLAS_OK;
+    Epilogue epi;
+    epi.residual = (const uint16_t *)p->residual;
+    epi.ldr = p->ldr;
+    epi.scale = p->scale;
+    epi.act = p->activation;
+    const AtlasWeight &w = p->weight;
+    if (!p->up.tiles && p->m <= STRIP_MAX_ROWS)
+        return qlinear_gemv(p->x, p->dtype, p->m, p->ldx, w.tiles, w.scales_tiled, w.outlier_chunk_ptr, w.outlier_entries, w.outlier_vals_sorted, p->n_rows,
+                            p->n_cols, p->block_size, w.bias, p->y, p->ldy, (cudaStream_t)stream, epi);
+    return qlinear_gemm(p->x, p->dtype, p->m, p->ldx, w.tiles, w.scales_tiled, w.outlier_chunk_ptr, w.outlier_entries, w.outlier_vals_sorted, p->n_rows, p->n_cols,
+                        p->block_size, w.bias, p->y, p->ldy, p->workspace, p->workspace_bytes, p->status, stream, nullptr, epi, p->up.tiles ? &p->up : nullptr);
+}

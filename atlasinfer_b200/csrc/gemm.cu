@@ -54,6 +54,7 @@
 
 #include "common.cuh"
 #include "gemm_tile.cuh"
+#include "linear.cuh"
 #include "tensor_core.cuh"
 
 namespace atlas {
@@ -130,6 +131,7 @@ struct GemmParams {
     int wait_world;
     long long poll_limit;
     int *error_flag;
+    Epilogue epi;
 };
 
 template <int BN>
@@ -535,15 +537,21 @@ gemm_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ C
                 uint32_t v[32];
                 tmem_ld_32x32b_x32(tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(c * 32), v);
                 tmem_ld_wait();
+                float f[32];
 #pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                    unsigned char *row = stage + (size_t)(c * 32 + j) * st_bytes;
-                    if (partial) {
-                        reinterpret_cast<uint32_t *>(row)[nl] = v[j];
-                    } else {
-                        const float f = __uint_as_float(v[j]) + bv;
-                        reinterpret_cast<uint16_t *>(row)[nl] = p.out_bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(f))
-                                                                          : __half_as_ushort(__float2half_rn(f));
+                for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(v[j]);
+                if (partial) {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) reinterpret_cast<float *>(stage + (size_t)(c * 32 + j) * st_bytes)[nl] = f[j];
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) f[j] += bv;
+                    activate(f, p.epi.act);
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        const int m = m0 + c * 32 + j;   // (a warp's 32 lanes read 64 contiguous bytes of the residual)
+                        f[j] = scaled(p.epi, f[j], n < p.n_rows && m < p.m ? residual_at(p.epi, m, n, p.out_bf16) : 0.f);
+                        reinterpret_cast<uint16_t *>(stage + (size_t)(c * 32 + j) * st_bytes)[nl] = narrow(f[j], p.out_bf16);
                     }
                 }
             }
@@ -609,12 +617,13 @@ struct FinishGather {
     unsigned int *state;
 };
 
-// Adds the K-slice partial tiles in slice order (deterministic), adds the bias and writes y.
+// Adds the K-slice partial tiles in slice order (deterministic), adds the bias and writes y.  With `up` the same for a second
+// weight's tiles: the product of the two (epilogue.cuh).
 // VEC: 8 features (16 bytes of output) per thread; needs n_rows % 8 == 0 and 16-byte aligned output rows.
 template <bool VEC>
 __global__ void __launch_bounds__(256)
-gemm_finish_kernel(const float *partials, int splits, int m, int n_rows, const uint16_t *bias, void *y, int64_t ldy,
-                   int out_bf16, FinishGather fg) {
+gemm_finish_kernel(const float *partials, const float *up, int splits, int m, int n_rows, const uint16_t *bias, const uint16_t *up_bias, void *y,
+                   int64_t ldy, int out_bf16, FinishGather fg, Epilogue epi) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     constexpr int W = VEC ? 8 : 1;
@@ -622,26 +631,35 @@ gemm_finish_kernel(const float *partials, int splits, int m, int n_rows, const u
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < pieces; i += (int64_t)gridDim.x * 256) {
         const int64_t e0 = i * W;
         const int row = (int)(e0 / n_rows), n = (int)(e0 - (int64_t)row * n_rows);
-        float acc[W];
+        auto sums = [&](const float *parts, const uint16_t *b, float (&acc)[W]) {
 #pragma unroll
-        for (int e = 0; e < W; ++e) acc[e] = 0.f;
-        for (int z = 0; z < splits; ++z) {
-            const float *src = partials + (size_t)z * total + e0;
-            if (VEC) {
-                const float4 a = __ldcg(reinterpret_cast<const float4 *>(src)), b = __ldcg(reinterpret_cast<const float4 *>(src) + 1);
-                acc[0] += a.x; acc[1 % W] += a.y; acc[2 % W] += a.z; acc[3 % W] += a.w;
-                acc[4 % W] += b.x; acc[5 % W] += b.y; acc[6 % W] += b.z; acc[7 % W] += b.w;
-            } else {
-                acc[0] += __ldcg(src);
+            for (int e = 0; e < W; ++e) acc[e] = 0.f;
+            for (int z = 0; z < splits; ++z) {
+                const float *src = parts + (size_t)z * total + e0;
+                if (VEC) {
+                    const float4 a = __ldcg(reinterpret_cast<const float4 *>(src)), b = __ldcg(reinterpret_cast<const float4 *>(src) + 1);
+                    acc[0] += a.x; acc[1 % W] += a.y; acc[2 % W] += a.z; acc[3 % W] += a.w;
+                    acc[4 % W] += b.x; acc[5 % W] += b.y; acc[6 % W] += b.z; acc[7 % W] += b.w;
+                } else {
+                    acc[0] += __ldcg(src);
+                }
             }
+#pragma unroll
+            for (int e = 0; e < W; ++e)
+                if (b) acc[e] += __half2float(__ushort_as_half(__ldg(b + n + e)));
+        };
+        float acc[W];
+        sums(partials, bias, acc);
+        activate(acc, epi.act);
+        if (up) {
+            float other[W];
+            sums(up, up_bias, other);
+#pragma unroll
+            for (int e = 0; e < W; ++e) acc[e] *= other[e];
         }
         uint16_t out[W];
 #pragma unroll
-        for (int e = 0; e < W; ++e) {
-            float v = acc[e];
-            if (bias) v += __half2float(__ushort_as_half(__ldg(bias + n + e)));
-            out[e] = out_bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v));
-        }
+        for (int e = 0; e < W; ++e) out[e] = narrow(scaled(epi, acc[e], residual_at(epi, row, n + e, out_bf16)), out_bf16);
         const int64_t off = (int64_t)row * ldy + n;
         const int dests = fg.world > 0 ? fg.world : 1;
         for (int d = 0; d < dests; ++d) {
@@ -943,25 +961,26 @@ extern "C" int atlas_qlinear_gemm_plan(int64_t m, int64_t n_rows, int64_t n_cols
     return ATLAS_OK;
 }
 
-extern "C" size_t atlas_qlinear_gemm_workspace_bytes(int64_t m, int64_t n_rows, int64_t n_cols) {
-    if (m <= 0 || n_cols <= 0 || n_rows <= 0) return atlas::GM_WS_HEADER;
+size_t atlas::qlinear_gemm_workspace_bytes(int64_t m, int64_t n_rows, int64_t n_cols, bool two) {
+    if (m <= 0 || n_cols <= 0 || n_rows <= 0) return GM_WS_HEADER;
     // fp16 copy of x (bf16 or strided input), then room for the fp32 partial outputs of the K slices
     const size_t xcopy = ((size_t)m * (size_t)n_cols * 2 + 255) & ~(size_t)255;
-    // (one fp32 slice of the output per K slice; one even without slicing, for the gathered form)
-    const int splits = atlas::gemm_splits_for(m, n_rows, n_cols, atlas::gemm_sm_count());
-    const size_t part = m > atlas::TILE_MAX_TOKENS ? (splits > 1 ? (size_t)splits * (size_t)m * (size_t)n_rows * 4 : 0)
-                        : (m <= 64 ? (size_t)splits * (size_t)m * (size_t)n_rows * 4 : 0);
-    return atlas::GM_WS_HEADER + xcopy + part;
+    // (one fp32 slice of the output per K slice; one even without slicing, for the gathered form and for two weights)
+    const int splits = gemm_splits_for(m, n_rows, n_cols, gemm_sm_count());
+    const size_t slices = (size_t)splits * (size_t)m * (size_t)n_rows * 4;
+    const size_t part = two ? 2 * ((slices + 255) & ~(size_t)255) : (m > TILE_MAX_TOKENS ? (splits > 1 ? slices : 0) : (m <= 64 ? slices : 0));
+    return GM_WS_HEADER + xcopy + part;
+}
+extern "C" size_t atlas_qlinear_gemm_workspace_bytes(int64_t m, int64_t n_rows, int64_t n_cols) {
+    return atlas::qlinear_gemm_workspace_bytes(m, n_rows, n_cols, false);
 }
 
 namespace atlas {
-namespace {
 
-int gemm_entry(const void *x, int dtype, int64_t m, int64_t ldx, const uint8_t *tiles, const void *scales_tiled,
+int qlinear_gemm(const void *x, int dtype, int64_t m, int64_t ldx, const uint8_t *tiles, const void *scales_tiled,
                const int32_t *outlier_chunk_ptr, const uint32_t *outlier_entries, const void *outlier_vals_sorted,
                int64_t n_rows, int64_t n_cols, int block_size, const void *bias, void *y, int64_t ldy, void *workspace,
-               size_t workspace_bytes, int32_t *status, void *stream, const AtlasPeerGather *gather) {
-    clear_error();
+               size_t workspace_bytes, int32_t *status, void *stream, const AtlasPeerGather *gather, const Epilogue &epi, const AtlasWeight *up) {
     FinishGather fg;
     memset(&fg, 0, sizeof(fg));
     if (gather) {
@@ -995,7 +1014,7 @@ int gemm_entry(const void *x, int dtype, int64_t m, int64_t ldx, const uint8_t *
                     "atlas_qlinear_gemm: too large");
     ATLAS_RETURN_IF(((uintptr_t)tiles & 15) != 0 || ((uintptr_t)workspace & 255) != 0, ATLAS_ERR_BAD_ARGUMENT,
                     "atlas_qlinear_gemm: tiles must be 16-byte and workspace 256-byte aligned");
-    const size_t need = atlas_qlinear_gemm_workspace_bytes(m, n_rows, n_cols);
+    const size_t need = qlinear_gemm_workspace_bytes(m, n_rows, n_cols, up != nullptr);
     ATLAS_RETURN_IF(workspace_bytes < need, ATLAS_ERR_CAPACITY,
                     "atlas_qlinear_gemm: workspace holds %zu bytes, %zu needed", workspace_bytes, need);
     int rc = check_device();
@@ -1008,7 +1027,7 @@ int gemm_entry(const void *x, int dtype, int64_t m, int64_t ldx, const uint8_t *
     const bool bf16 = dtype == ATLAS_DTYPE_BF16;
     // (the gathered form's arrival protocol lives in the kernels of this file)
     Route route = {};
-    if (!gather && m <= TILE_MAX_TOKENS) {
+    if (!gather && !up && m <= TILE_MAX_TOKENS) {
         const bool aligned = n_rows % 8 == 0 && ldy % 8 == 0 && ((uintptr_t)y & 15) == 0;
         route = route_for(Shape{m, n_rows, n_cols, gemm_sm_count(), (bf16 ? 1 : 0) | (tma_ok ? 2 : 0) | (aligned ? 4 : 0)});
     }
@@ -1052,16 +1071,19 @@ int gemm_entry(const void *x, int dtype, int64_t m, int64_t ldx, const uint8_t *
                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     ATLAS_RETURN_IF(cr != CUDA_SUCCESS, ATLAS_ERR_LAUNCH, "cuTensorMapEncodeTiled failed with %d", (int)cr);
     // the code tiles as one matrix of 64-byte rows: tile (row tile rt, k-tile kt) = rows (rt * k_tiles + kt) * 128 .. + 127
-    CUtensorMap c_map;
-    {
+    auto code_map = [&](const uint8_t *codes, CUtensorMap &map) {
         const cuuint64_t cdim[2] = {(cuuint64_t)GM_BK, (cuuint64_t)(ceil_div_i64(n_rows, GM_BM) * (n_cols / GM_BK) * GM_BM)};
         const cuuint64_t cstride[1] = {(cuuint64_t)GM_BK};
         const cuuint32_t cbox[2] = {(cuuint32_t)GM_BK, (cuuint32_t)GM_BM};
-        cr = encode(&c_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t *>(tiles), cdim, cstride, cbox, estride,
-                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-        ATLAS_RETURN_IF(cr != CUDA_SUCCESS, ATLAS_ERR_LAUNCH, "cuTensorMapEncodeTiled (codes) failed with %d", (int)cr);
-    }
+        const CUresult r = encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t *>(codes), cdim, cstride, cbox, estride,
+                                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        ATLAS_RETURN_IF(r != CUDA_SUCCESS, ATLAS_ERR_LAUNCH, "cuTensorMapEncodeTiled (codes) failed with %d", (int)r);
+        return ATLAS_OK;
+    };
+    CUtensorMap c_map;
+    rc = code_map(tiles, c_map);
+    if (rc) return rc;
 
     if (tile) {
         TileParams t;
@@ -1082,6 +1104,7 @@ int gemm_entry(const void *x, int dtype, int64_t m, int64_t ldx, const uint8_t *
         t.x_bf16 = in_kernel_bf16;
         t.splits = route.plan.splits;
         t.error_flag = status;
+        t.epi = epi;
         return launch_tile(x_map, c_map, t, st);
     }
     GemmParams p;
@@ -1103,25 +1126,44 @@ int gemm_entry(const void *x, int dtype, int64_t m, int64_t ldx, const uint8_t *
     p.out_bf16 = dtype == ATLAS_DTYPE_BF16;
     p.splits = plan.splits;
     p.partials = (float *)((char *)workspace + GM_WS_HEADER + xcopy);
-    p.to_partials = gather != nullptr;   // the gather is the second kernel's job
+    p.to_partials = gather != nullptr || up != nullptr;   // the gather, and the product of two weights, are the second kernel's job
     p.x_bf16 = in_kernel_bf16;
     p.wait_flags = wait_in_copy ? nullptr : wait_flags;
     p.gather_state = gather ? (const unsigned int *)gather->state : nullptr;
     p.wait_world = gather ? gather->world : 0;
     p.poll_limit = gather ? (long long)gather->poll_limit : 0;
     p.error_flag = status;
-    switch (bn) {
-        case 32: rc = launch_gemm<32>(x_map, c_map, p, st); break;
-        case 64: rc = launch_gemm<64>(x_map, c_map, p, st); break;
-        case 128: rc = launch_gemm<128>(x_map, c_map, p, st); break;
-        case 160: rc = launch_gemm<160>(x_map, c_map, p, st); break;
-        case 192: rc = launch_gemm<192>(x_map, c_map, p, st); break;
-        case 224: rc = launch_gemm<224>(x_map, c_map, p, st); break;
-        case 256: rc = launch_gemm<256>(x_map, c_map, p, st); break;
-        case 320: rc = launch_gemm<320>(x_map, c_map, p, st); break;
-        default: rc = launch_gemm<384>(x_map, c_map, p, st); break;
-    }
+    p.epi = epi;
+    auto launch = [&](const CUtensorMap &codes, const GemmParams &q) {
+        switch (bn) {
+            case 32: return launch_gemm<32>(x_map, codes, q, st);
+            case 64: return launch_gemm<64>(x_map, codes, q, st);
+            case 128: return launch_gemm<128>(x_map, codes, q, st);
+            case 160: return launch_gemm<160>(x_map, codes, q, st);
+            case 192: return launch_gemm<192>(x_map, codes, q, st);
+            case 224: return launch_gemm<224>(x_map, codes, q, st);
+            case 256: return launch_gemm<256>(x_map, codes, q, st);
+            case 320: return launch_gemm<320>(x_map, codes, q, st);
+            default: return launch_gemm<384>(x_map, codes, q, st);
+        }
+    };
+    rc = launch(c_map, p);
     if (rc) return rc;
+    const float *up_partials = nullptr;
+    if (up) {
+        GemmParams q = p;
+        q.tiles = up->tiles;
+        q.scales_t = (const uint16_t *)up->scales_tiled;
+        q.chunk_ptr = up->outlier_chunk_ptr;
+        q.entries = up->outlier_entries;
+        q.ovals = (const uint16_t *)up->outlier_vals_sorted;
+        q.partials = p.partials + (((size_t)p.splits * (size_t)m * (size_t)n_rows * 4 + 255) & ~(size_t)255) / 4;
+        up_partials = q.partials;
+        CUtensorMap up_map;
+        rc = code_map(up->tiles, up_map);
+        if (!rc) rc = launch(up_map, q);
+        if (rc) return rc;
+    }
     if (p.splits > 1 || p.to_partials) {
         const bool vec = n_rows % 8 == 0 && ldy % 8 == 0 && (((uintptr_t)y & 15) == 0) &&
                          (((uintptr_t)p.partials & 15) == 0);
@@ -1131,13 +1173,12 @@ int gemm_entry(const void *x, int dtype, int64_t m, int64_t ldx, const uint8_t *
         const int64_t blocks = ceil_div_i64(pieces, 256);
         cudaLaunchConfig_t cfg = pdl_config(dim3((unsigned)(blocks < 2048 ? blocks : 2048)), dim3(256), 0, st);
         auto kern = vec_all ? gemm_finish_kernel<true> : gemm_finish_kernel<false>;
-        rc = check_cuda(cudaLaunchKernelEx(&cfg, kern, (const float *)p.partials, p.splits, (int)m, (int)n_rows,
-                                           (const uint16_t *)bias, y, ldy, p.out_bf16, fg), "gemm_finish_kernel launch");
+        rc = check_cuda(cudaLaunchKernelEx(&cfg, kern, (const float *)p.partials, up_partials, p.splits, (int)m, (int)n_rows, (const uint16_t *)bias,
+                                           up ? (const uint16_t *)up->bias : (const uint16_t *)nullptr, y, ldy, p.out_bf16, fg, epi), "gemm_finish_kernel launch");
     }
     return rc;
 }
 
-}  // namespace
 }  // namespace atlas
 
 extern "C" int atlas_qlinear_gemm(const void *x, int dtype, int64_t m, int64_t ldx, const uint8_t *tiles,
@@ -1146,9 +1187,10 @@ extern "C" int atlas_qlinear_gemm(const void *x, int dtype, int64_t m, int64_t l
                                   int64_t n_rows, int64_t n_cols, int block_size, const void *bias, void *y,
                                   int64_t ldy, void *workspace, size_t workspace_bytes, int32_t *status,
                                   void *stream) {
+    atlas::clear_error();
     ATLAS_RETURN_IF(!y, ATLAS_ERR_BAD_ARGUMENT, "atlas_qlinear_gemm: null buffer");
-    return atlas::gemm_entry(x, dtype, m, ldx, tiles, scales_tiled, outlier_chunk_ptr, outlier_entries, outlier_vals_sorted,
-                             n_rows, n_cols, block_size, bias, y, ldy, workspace, workspace_bytes, status, stream, nullptr);
+    return atlas::qlinear_gemm(x, dtype, m, ldx, tiles, scales_tiled, outlier_chunk_ptr, outlier_entries, outlier_vals_sorted,
+                             n_rows, n_cols, block_size, bias, y, ldy, workspace, workspace_bytes, status, stream, nullptr, atlas::Epilogue(), nullptr);
 }
 
 extern "C" int atlas_qlinear_gemm_gather(const void *x, int dtype, int64_t m, int64_t ldx, const uint8_t *tiles,
@@ -1157,7 +1199,8 @@ extern "C" int atlas_qlinear_gemm_gather(const void *x, int dtype, int64_t m, in
                                          int64_t n_rows, int64_t n_cols, int block_size, const void *bias,
                                          int64_t ldy, void *workspace, size_t workspace_bytes, int32_t *status,
                                          void *stream, const AtlasPeerGather *gather) {
+    atlas::clear_error();
     ATLAS_RETURN_IF(!gather, ATLAS_ERR_BAD_ARGUMENT, "atlas_qlinear_gemm_gather: null gather descriptor");
-    return atlas::gemm_entry(x, dtype, m, ldx, tiles, scales_tiled, outlier_chunk_ptr, outlier_entries, outlier_vals_sorted,
-                             n_rows, n_cols, block_size, bias, nullptr, ldy, workspace, workspace_bytes, status, stream, gather);
+    return atlas::qlinear_gemm(x, dtype, m, ldx, tiles, scales_tiled, outlier_chunk_ptr, outlier_entries, outlier_vals_sorted,
+                             n_rows, n_cols, block_size, bias, nullptr, ldy, workspace, workspace_bytes, status, stream, gather, atlas::Epilogue(), nullptr);
 }

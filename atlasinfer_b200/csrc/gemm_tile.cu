@@ -349,10 +349,12 @@ tile_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ C
             float f[4] = {a.x, a.y, a.z, a.w};
             uint16_t o[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
+            for (int e = 0; e < 4; ++e)
                 if (p.bias && n + e < p.n_rows) f[e] += __half2float(__ushort_as_half(__ldg(p.bias + n + e)));
-                o[e] = p.out_bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(f[e])) : __half_as_ushort(__float2half_rn(f[e]));
-            }
+            activate(f, p.epi.act);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                o[e] = narrow(scaled(p.epi, f[e], n + e < p.n_rows ? residual_at(p.epi, t, n + e, p.out_bf16) : 0.f), p.out_bf16);
             uint16_t *dst = reinterpret_cast<uint16_t *>(p.y) + (int64_t)t * p.ldy + n;
             if (vec && n + 4 <= p.n_rows) {
                 *reinterpret_cast<uint2 *>(dst) = make_uint2(o[0] | (uint32_t)o[1] << 16, o[2] | (uint32_t)o[3] << 16);

@@ -5,6 +5,8 @@
 
 #include <cstdint>
 
+#include "epilogue.cuh"
+
 namespace atlas {
 
 struct TileParams {
@@ -25,6 +27,7 @@ struct TileParams {
     int x_bf16;      // the tensor map delivers bf16 rows: converted in the kernel
     int splits;      // K slices = CTAs of a cluster
     int *error_flag;
+    Epilogue epi;
 };
 
 // Rows of x the kernel takes, and tokens per tile for m of them.

@@ -26,6 +26,7 @@
 #include <cuda_bf16.h>
 
 #include "common.cuh"
+#include "linear.cuh"
 
 namespace atlas {
 namespace {
@@ -50,6 +51,7 @@ struct GemvParams {
     int n_chunks;       // ceil(n_cols / 256)
     int blocks_per_row; // n_cols / bs
     int bs_shift;       // log2(block size) when it is a power of two, else -1
+    Epilogue epi;
 };
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -345,11 +347,15 @@ __global__ void __launch_bounds__((MT == 1 ? GS_MAX_WARPS : GS_WARPS2) * 32, 2) 
 
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) part[nt][warp][lane] = make_float4(acc[nt][0], acc[nt][1], acc[nt][2], acc[nt][3]);
+    const bool mine = tid < 128 * NT && out_m < p.m && out_n < p.n_rows;
+    const float residual = mine ? residual_at(p.epi, out_m, out_n, BF16) : 0.f;   // (travels while the other warps arrive)
     __syncthreads();
     if (tid < 128 * NT) {
-        float s = bias_v;
-        for (int w = 0; w < nwarps; ++w) s += reinterpret_cast<const float *>(&part[rT][w][rL])[rj];
-        if (out_m < p.m && out_n < p.n_rows) {
+        float sum[1] = {bias_v};
+        for (int w = 0; w < nwarps; ++w) sum[0] += reinterpret_cast<const float *>(&part[rT][w][rL])[rj];
+        if (mine) {
+            activate(sum, p.epi.act);
+            const float s = scaled(p.epi, sum[0], residual);
             if (BF16) reinterpret_cast<__nv_bfloat16 *>(p.y)[(size_t)out_m * p.ldy + out_n] = __float2bfloat16_rn(s);
             else reinterpret_cast<__half *>(p.y)[(size_t)out_m * p.ldy + out_n] = __float2half_rn(s);
         }
@@ -430,15 +436,10 @@ int launch_gemv_strip(const GemvParams &p, bool vec, cudaStream_t st) {
 }
 
 }  // namespace
-}  // namespace atlas
 
-extern "C" int atlas_qlinear_gemv(const void *x, int dtype, int64_t m, int64_t ldx, const uint8_t *tiles,
-                                  const void *scales_tiled, const int32_t *outlier_chunk_ptr,
-                                  const uint32_t *outlier_entries, const void *outlier_vals_sorted,
-                                  int64_t n_rows, int64_t n_cols, int block_size, const void *bias, void *y,
-                                  int64_t ldy, int32_t *status, void *stream) {
-    using namespace atlas;
-    clear_error();
+int qlinear_gemv(const void *x, int dtype, int64_t m, int64_t ldx, const uint8_t *tiles, const void *scales_tiled,
+                 const int32_t *outlier_chunk_ptr, const uint32_t *outlier_entries, const void *outlier_vals_sorted,
+                 int64_t n_rows, int64_t n_cols, int block_size, const void *bias, void *y, int64_t ldy, cudaStream_t st, const Epilogue &epi) {
     ATLAS_RETURN_IF(!x || !tiles || !scales_tiled || !outlier_chunk_ptr || !y, ATLAS_ERR_BAD_ARGUMENT,
                     "atlas_qlinear_gemv: null buffer");
     ATLAS_RETURN_IF(m < 0 || n_rows <= 0 || n_cols <= 0 || ldx < n_cols || ldy < n_rows, ATLAS_ERR_BAD_ARGUMENT,
@@ -454,10 +455,10 @@ extern "C" int atlas_qlinear_gemv(const void *x, int dtype, int64_t m, int64_t l
     int rc = check_device();
     if (rc) return rc;
     if (m == 0) return ATLAS_OK;
-    cudaStream_t st = (cudaStream_t)stream;
 
     GemvParams p;
     p.dtype = dtype;
+    p.epi = epi;
     p.ldx = ldx;
     p.tiles = tiles;
     p.scales_t = (const uint16_t *)scales_tiled;
@@ -474,13 +475,26 @@ extern "C" int atlas_qlinear_gemv(const void *x, int dtype, int64_t m, int64_t l
     p.blocks_per_row = (int)(n_cols / block_size);
     p.bs_shift = (block_size & (block_size - 1)) == 0 ? __builtin_ctz((unsigned)block_size) : -1;
     const bool vec = (((uintptr_t)x & 15) == 0) && (ldx % 8 == 0);   // x rows allow 16-byte loads
-    (void)status;   // no bounded wait in this kernel: nothing to report
     for (int64_t m0 = 0; m0 < m; m0 += 16) {   // one launch per 16 rows: the later passes find most of the weight in L2
         p.m = (int)(m - m0 < 16 ? m - m0 : 16);
         p.x = (const char *)x + (size_t)m0 * ldx * 2;
         p.y = (char *)y + (size_t)m0 * ldy * 2;
+        if (epi.residual) p.epi.residual = epi.residual + m0 * epi.ldr;
         rc = p.m <= 8 ? launch_gemv_strip<1>(p, vec, st) : launch_gemv_strip<2>(p, vec, st);
         if (rc) return rc;
     }
     return ATLAS_OK;
+}
+
+}  // namespace atlas
+
+extern "C" int atlas_qlinear_gemv(const void *x, int dtype, int64_t m, int64_t ldx, const uint8_t *tiles,
+                                  const void *scales_tiled, const int32_t *outlier_chunk_ptr,
+                                  const uint32_t *outlier_entries, const void *outlier_vals_sorted,
+                                  int64_t n_rows, int64_t n_cols, int block_size, const void *bias, void *y,
+                                  int64_t ldy, int32_t *status, void *stream) {
+    (void)status;   // no bounded wait in this kernel: nothing to report
+    atlas::clear_error();
+    return atlas::qlinear_gemv(x, dtype, m, ldx, tiles, scales_tiled, outlier_chunk_ptr, outlier_entries, outlier_vals_sorted, n_rows, n_cols,
+                               block_size, bias, y, ldy, (cudaStream_t)stream, atlas::Epilogue());
 }

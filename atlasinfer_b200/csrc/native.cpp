@@ -27,6 +27,7 @@ void check_status_code(int status, const char *what) {
 }
 
 void bind_kv(py::module_ &m);   // native_kv.cpp
+void bind_ops(py::module_ &m);  // native_ops.cpp
 
 namespace {
 
@@ -361,4 +362,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("quantize_many", &quantize_many, py::call_guard<py::gil_scoped_release>());
     m.def("linear", &linear, py::call_guard<py::gil_scoped_release>());
     bind_kv(m);
+    bind_ops(m);
 }

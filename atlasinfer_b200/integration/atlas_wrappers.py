@@ -422,6 +422,23 @@ class QuantizedLinear(nn.Module):
             self._kernel_layout = build_kernel_layout(q, wait=False)
         return self._kernel_layout
 
+    def kernel_form(self, device: torch.device):
+        """``(layout, bias)`` on a CUDA ``device``, laid out now if they are not there yet; ``bias`` is fp16 or None."""
+        q = self.quantized_weights
+        if not hasattr(q, "fp8_data"):
+            raise TypeError(f"Weight in QuantizedLinear ({id(self)}) is not a valid QuantizedTensor: {type(q)}")
+        if self._group is not None and (self._group.layout is None or self._group.layout.tiles.device != device):
+            self._group.build(device)
+            q = self.quantized_weights
+        layout = self._kernel_layout
+        if layout is None or layout.source is not q or layout.tiles.device != device:
+            if q.fp8_data.device != device:
+                self.quantized_weights = q = q.to(device)
+            layout = self._layout_for(q)
+        if self.bias is not None and self.bias.device != device:
+            self.bias = self.bias.to(device)
+        return layout, self._bias_for(self.bias)
+
     def offload_canonical(self, device="cpu") -> None:
         """Keep only the kernel layout on the GPU: the canonical streams move to ``device`` (host by default).
 

@@ -37,14 +37,13 @@ class Layer:
         self.cache = ab.QuantizedKVCache(pages, kv_heads, head_dim, page_size=page_size, device=device)
 
     def __call__(self, x, step):
-        h = torch.nn.functional.rms_norm(x, x.shape[-1:])
+        h, _ = ab.residual_norm(x)
         q, k, v = (m(h).unflatten(-1, (-1, self.head_dim)) for m in (self.q, self.k, self.v))
         q = ab.norm_rotate_store(q, k, v, self.cache, step["slots"], step["table"], step["positions"], q_weight=self.q_norm, k_weight=self.k_norm)
         a = ab.cache_attention(q, self.cache, step["pages"], step["lengths"], query_starts=step["starts"], max_queries=step["most"],
                                window=self.window, sinks=self.sinks)
-        x = x + self.o(a.flatten(1))
-        h = torch.nn.functional.rms_norm(x, x.shape[-1:])
-        return x + self.down(torch.nn.functional.silu(self.gate(h)) * self.up(h))
+        h, x = ab.residual_norm(self.o(a.flatten(1)), x)
+        return ab.linear_epilogue(self.down, ab.gated_linear(self.gate, self.up, h), residual=x)
 
 
 class Model:
@@ -67,7 +66,7 @@ class Model:
         x = self.embedding[tokens]
         for layer in self.layers:
             x = layer(x, step)
-        return torch.nn.functional.rms_norm(x, x.shape[-1:]) @ self.embedding.T
+        return ab.residual_norm(x)[0] @ self.embedding.T
 
     def prefill(self, prompts, chunk=256):
         """The logits behind every prompt's last token; the prompts go through in chunks, as ragged batches."""
@@ -112,18 +111,25 @@ class Model:
 
 
 @torch.no_grad()
-def generate(model, prompts, count):
-    """Greedy tokens behind every prompt, and the seconds that the steps took."""
+def generate(model, prompts, count, scores=None):
+    """Greedy tokens behind every prompt, and the seconds that the steps took; their log probabilities are appended to ``scores``."""
     logits = model.prefill(prompts)
     tokens, positions, out, replay = model.decoder()
     positions.copy_(torch.tensor([len(p) for p in prompts], device=model.device))
-    tokens.copy_(logits.argmax(-1))
+    scores = [] if scores is None else scores
+
+    def choose(logits):
+        found = ab.token_logprobs(logits, tokens, top=1)
+        tokens.copy_(found.top_tokens[:, 0])
+        scores.append(found.top_logprobs[:, 0])
+
+    choose(logits)
     made = [tokens.clone()]
     torch.cuda.synchronize(model.device)
     began = time.perf_counter()
     for _ in range(count - 1):
         replay()
-        tokens.copy_(out.argmax(-1))
+        choose(out)
         positions.add_(1)
         made.append(tokens.clone())
     torch.cuda.synchronize(model.device)
@@ -140,9 +146,11 @@ def main():
     model = Model(layers=args.layers, hidden=args.hidden, heads=heads, kv_heads=max(1, heads // 4), sequences=3, context=2048)
     gen = torch.Generator(device="cuda").manual_seed(1)
     prompts = [torch.randint(0, 1000, (n,), generator=gen, device="cuda") for n in (700, 33, 1500)]
-    made, seconds = generate(model, prompts, args.tokens)
+    scores = []
+    made, seconds = generate(model, prompts, args.tokens, scores)
     used = sum(layer.cache.data.numel() for layer in model.layers)
     print(made[:, :12].tolist())
+    print("log probabilities", [round(v, 2) for v in torch.stack(scores).sum(0).tolist()])
     print(f"{args.tokens - 1} steps of {len(prompts)} sequences in {seconds * 1e3:.1f} ms; caches {used / 1e6:.1f} MB")
 
 

@@ -486,6 +486,111 @@ typedef struct AtlasKvAttention {
 ATLAS_API size_t atlas_kv_attention_workspace_bytes(const AtlasKvAttention *attention);
 ATLAS_API int atlas_kv_attention(const AtlasKvAttention *attention, void *stream);
 
+/* ---- between a decoder step's linears and behind the last one ----------------------
+ * No counterpart in the reference (there the models' own modules compute these).
+ */
+
+/* Quantized linears with what follows them, in fp32 and rounded once:
+ *   y = residual + scale * act(x W^T + bias)                       (up.tiles NULL)
+ *   y = residual + scale * act(x W^T + bias) * (x V^T + up.bias)
+ * Weights as atlas_repack lays them out (x, m, ldx, n_rows, n_cols, block_size as
+ * for atlas_qlinear_gemm, `up` of the same shape and block size); bias fp16 or
+ * NULL; residual [m][n_rows] of `dtype`, row stride ldr, or NULL.  y overlaps
+ * neither residual nor x.  Weights and biases are read before the stream's
+ * earlier work has completed (see above), x and residual afterwards.
+ *   workspace   atlas_fused_linear_workspace_bytes(...) bytes, 256-byte aligned
+ *   status      device int32 or NULL, set non-zero if a bounded wait ran out
+ */
+#define ATLAS_ACT_NONE 0
+#define ATLAS_ACT_RELU 1
+#define ATLAS_ACT_SILU 2        /* v / (1 + exp(-v)) */
+#define ATLAS_ACT_GELU 3        /* v (1 + erf(v / sqrt 2)) / 2 */
+#define ATLAS_ACT_GELU_TANH 4   /* v (1 + tanh(sqrt(2 / pi) (v + 0.044715 v^3))) / 2 */
+typedef struct AtlasWeight {
+    const uint8_t *tiles;
+    const void *scales_tiled;
+    const int32_t *outlier_chunk_ptr;
+    const uint32_t *outlier_entries;
+    const void *outlier_vals_sorted;
+    const void *bias;
+} AtlasWeight;
+typedef struct AtlasFusedLinear {
+    int32_t dtype, activation;
+    const void *x;
+    int64_t m, ldx, n_rows, n_cols;
+    int32_t block_size;
+    float scale;
+    AtlasWeight weight, up;
+    const void *residual;
+    int64_t ldr;
+    void *y;
+    int64_t ldy;
+    void *workspace;
+    size_t workspace_bytes;
+    int32_t *status;
+} AtlasFusedLinear;
+ATLAS_API size_t atlas_fused_linear_workspace_bytes(const AtlasFusedLinear *linear);
+ATLAS_API int atlas_fused_linear(const AtlasFusedLinear *linear, void *stream);
+
+/* A block's output joins the stream, and the sum is normed for the next block:
+ *   b = x, or norm(x) * (post_weight + weight_offset)
+ *   stream = residual + scale * gate * b              (no residual: 0)
+ *   normed = norm(stream) * (weight + weight_offset) + bias
+ * norm(v) = v * rsqrt(mean(v^2) + eps), or of v - mean(v) if `centered`.  In fp32;
+ * `normed` is made of the stream before its rounding.
+ *   dtype        of x, normed; of the others too unless `wide` has their bit (fp32)
+ *   x, residual  [tokens][hidden], row strides in elements; residual may be NULL
+ *   gate         one row (gate_stride 0) or one for each token, or NULL
+ *   weight, bias, post_weight   [hidden] or NULL (no post_weight: x is taken as it is)
+ *   normed, stream_out   contiguous; stream_out of the residual's type (without one:
+ *                of dtype), or NULL if it is not wanted; it may be the residual
+ *                itself where that is contiguous
+ * hidden is at most 32768.
+ */
+#define ATLAS_WIDE_STREAM 1
+#define ATLAS_WIDE_GATE 2
+#define ATLAS_WIDE_WEIGHT 4
+#define ATLAS_WIDE_BIAS 8
+#define ATLAS_WIDE_POST_WEIGHT 16
+#define ATLAS_NORM_MAX_HIDDEN 32768
+typedef struct AtlasResidualNorm {
+    int32_t dtype, wide, centered;
+    float scale, eps, weight_offset;
+    int64_t tokens, hidden;
+    const void *x, *residual, *gate;
+    int64_t x_stride, residual_stride, gate_stride;
+    const void *weight, *bias, *post_weight;
+    void *normed, *stream_out;
+} AtlasResidualNorm;
+ATLAS_API int atlas_residual_norm(const AtlasResidualNorm *norm, void *stream);
+
+/* Log probabilities of one given token for each row of logits, the entropy of the
+ * rows, and their likeliest tokens, p = softmax(logits / temperature), in fp32:
+ *   logprobs[r]  log p(tokens[r]); 0 for a negative token (none), NaN for one
+ *                beyond the vocabulary
+ *   entropy[r]   -sum p log p
+ *   top_tokens, top_logprobs   [rows][top], the largest logits first, equal ones
+ *                by their index (NaN counts as the largest); NULL if top is 0
+ * Tokens of -inf have no probability (log -inf).  Of a row without any other, all log
+ * probabilities are -inf and the entropy is 0; one with +inf or NaN gives NaN.
+ *   logits       fp16, bf16 or (dtype ATLAS_DTYPE_F32) fp32, row stride in elements;
+ *                aligned to their type
+ *   tokens       [rows] int32 or int64 (token_bytes)
+ *   top          at most ATLAS_LOGPROBS_MAX_TOP and vocab
+ */
+#define ATLAS_DTYPE_F32 2      /* logits only */
+#define ATLAS_LOGPROBS_MAX_TOP 32
+typedef struct AtlasTokenLogprobs {
+    int32_t dtype, top, token_bytes;
+    float temperature;
+    int64_t rows, vocab, logits_stride;
+    const void *logits, *tokens;
+    float *logprobs, *entropy;
+    int64_t *top_tokens;
+    float *top_logprobs;
+} AtlasTokenLogprobs;
+ATLAS_API int atlas_token_logprobs(const AtlasTokenLogprobs *logprobs, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
