@@ -1,7 +1,7 @@
 // Quantized linears with an epilogue (epilogue.cuh): argument checks, and which kernel.
 //
-// One weight: as the linears without an epilogue, the per-strip kernel (gemv.cu) up to 16 rows of x, above that the tcgen05
-// kernels (gemm_tile.cu, gemm.cu); the epilogue stands where they round their sums.
+// As the linears without an epilogue: the per-strip kernel (gemv.cu) up to 16 rows of x, above that the tcgen05 kernels
+// (gemm_tile.cu, gemm.cu).  The epilogue stands where they round their sums.
 #include "common.cuh"
 #include "linear.cuh"
 
@@ -25,7 +25,7 @@ int check(const AtlasFusedLinear *p) {
 
 extern "C" size_t atlas_fused_linear_workspace_bytes(const AtlasFusedLinear *p) {
     using namespace atlas;
-    if (check(p) != ATLAS_OK || (!p->up.tiles && p->m <= STRIP_MAX_ROWS)) return 0;
+    if (check(p) != ATLAS_OK || p->m <= STRIP_MAX_ROWS) return 0;
     return qlinear_gemm_workspace_bytes(p->m, p->n_rows, p->n_cols, p->up.tiles != nullptr);
 }
 
@@ -35,15 +35,11 @@ extern "C" int atlas_fused_linear(const AtlasFusedLinear *p, void *stream) {
     const int rc = check(p);
     if (rc != ATLAS_OK) return rc;
     if (p->m == 0) return ATLAS_OK;
-    Epilogue epi;
-    epi.residual = (const uint16_t *)p->residual;
-    epi.ldr = p->ldr;
-    epi.scale = p->scale;
-    epi.act = p->activation;
-    const AtlasWeight &w = p->weight;
-    if (!p->up.tiles && p->m <= STRIP_MAX_ROWS)
+    const Epilogue epi = make_epilogue(p->residual, p->ldr, p->scale, p->activation);
+    const AtlasWeight &w = p->weight, *up = p->up.tiles ? &p->up : nullptr;
+    if (p->m <= STRIP_MAX_ROWS)
         return qlinear_gemv(p->x, p->dtype, p->m, p->ldx, w.tiles, w.scales_tiled, w.outlier_chunk_ptr, w.outlier_entries, w.outlier_vals_sorted, p->n_rows,
-                            p->n_cols, p->block_size, w.bias, p->y, p->ldy, (cudaStream_t)stream, epi);
+                            p->n_cols, p->block_size, w.bias, p->y, p->ldy, (cudaStream_t)stream, epi, up);
     return qlinear_gemm(p->x, p->dtype, p->m, p->ldx, w.tiles, w.scales_tiled, w.outlier_chunk_ptr, w.outlier_entries, w.outlier_vals_sorted, p->n_rows, p->n_cols,
-                        p->block_size, w.bias, p->y, p->ldy, p->workspace, p->workspace_bytes, p->status, stream, nullptr, epi, p->up.tiles ? &p->up : nullptr);
+                        p->block_size, w.bias, p->y, p->ldy, p->workspace, p->workspace_bytes, p->status, stream, nullptr, epi, up);
 }

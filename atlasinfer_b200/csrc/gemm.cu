@@ -55,6 +55,7 @@
 #include "common.cuh"
 #include "gemm_tile.cuh"
 #include "linear.cuh"
+#include "rows.cuh"
 #include "tensor_core.cuh"
 
 namespace atlas {
@@ -64,6 +65,9 @@ constexpr int GM_DQ_WARPS = 16;                      // dequantizer warps: 4 TME
 constexpr int GM_EPI_WARPS = 16;                     // all of them drain the accumulator: four per TMEM lane quarter
 constexpr int GM_CTRL_WARPS = 3;                     // activation producer (and converter), MMA issuer, code producer
 constexpr int GM_THREADS = (GM_CTRL_WARPS + GM_DQ_WARPS) * 32;
+// With two weights a fourth one fetches the second weight's codes: one thread that issues eight copies a stage holds the others up
+// (a k-tile of a 256-token tile takes 0.47 us then, 0.43 as with one weight).
+constexpr int GM_THREADS_TWO = GM_THREADS + 32;
 constexpr int GM_BM = 128;  // weight rows (output features) per CTA = UMMA M
 constexpr int GM_BK = 64;   // K per pipeline step (one 128-byte swizzle row of fp16)
 constexpr int GM_SK = 2;    // k-tiles per pipeline stage: one barrier round trip, poll and commit per 128 columns of K
@@ -132,11 +136,110 @@ struct GemmParams {
     long long poll_limit;
     int *error_flag;
     Epilogue epi;
+    int follows;          // something: an activation, a scale, a residual
+    AtlasWeight up;       // gate and up: the second weight,
+    float *up_partials;   // and its partial tiles
 };
 
-template <int BN>
-__global__ void __launch_bounds__(GM_THREADS, 1)
-gemm_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap c_map, GemmParams p) {
+// What follows the sums of a tile, fp32 [tokens][GM_BM + 4] in shared memory, 4 features a thread: its features stay the same from
+// row to row, and residual and outputs are read and written along the rows.
+struct WideEpilogue {
+    uint32_t stage;      // shared-memory address
+    int thread, rows;    // of GM_EPI_WARPS * 32; tokens
+    int64_t token, feature, n_rows;   // the tile's first ones; features in all
+    const uint16_t *bias, *up_bias;
+    uint16_t *y;
+    int64_t ldy;
+};
+constexpr int WIDE_ROW = (GM_BM + 4) * 4;   // bytes
+template <bool TWO, int ACT, bool BF16>
+__device__ __forceinline__ void wide_epilogue_of(const WideEpilogue &w, const Epilogue &epi) {
+    constexpr int PIECES = (TWO ? 64 : GM_BM) / 4, STEP = GM_EPI_WARPS * 32 / PIECES, AHEAD = 8;
+    const int piece = w.thread % PIECES, first = w.thread / PIECES;
+    const int64_t at = w.feature + piece * 4;
+    if (at >= w.n_rows) return;
+    const int left = (int)(w.n_rows - at < 4 ? w.n_rows - at : 4);
+    const bool vec_ok = left == 4 && w.ldy % 4 == 0 && ((uintptr_t)w.y & 7) == 0;
+    float b[4], c[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        b[e] = w.bias && e < left ? __half2float(__ushort_as_half(__ldg(w.bias + at + e))) : 0.f;
+        c[e] = TWO && w.up_bias && e < left ? __half2float(__ushort_as_half(__ldg(w.up_bias + at + e))) : 0.f;
+    }
+    auto sums = [&](int row, int shift) {
+        float4 v;
+        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                     : "r"(w.stage + (uint32_t)(row * WIDE_ROW + piece * 16 + shift)));
+        return v;
+    };
+    const uint16_t *res_at = epi.residual + (w.token + first) * epi.ldr + at;
+    uint16_t *dst = w.y + (w.token + first) * w.ldy + at;
+    const int64_t res_step = STEP * epi.ldr, dst_step = STEP * w.ldy;
+    for (int r0 = first; r0 < w.rows; r0 += AHEAD * STEP) {
+        uint2 res[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            res[i] = make_uint2(0, 0);
+            if (epi.residual && r0 + i * STEP < w.rows) {
+                const uint16_t *from = res_at + i * res_step;
+                if (epi.residual_by_4 && left == 4) {
+                    res[i] = __ldg(reinterpret_cast<const uint2 *>(from));
+                } else {
+                    res[i].x = __ldg(from);
+                    if (left > 1) res[i].x |= (uint32_t)__ldg(from + 1) << 16;
+                    if (left > 2) res[i].y = __ldg(from + 2);
+                    if (left > 3) res[i].y |= (uint32_t)__ldg(from + 3) << 16;
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            if (r0 + i * STEP < w.rows) {
+                const float4 g = sums(r0 + i * STEP, 0);
+                float f[4] = {g.x + b[0], g.y + b[1], g.z + b[2], g.w + b[3]};
+                activate_with<ACT>(f);
+                if (TWO) {
+                    const float4 u = sums(r0 + i * STEP, 256);
+                    f[0] *= u.x + c[0], f[1] *= u.y + c[1], f[2] *= u.z + c[2], f[3] *= u.w + c[3];
+                }
+                f[0] = fmaf(f[0], epi.scale, widen((uint16_t)res[i].x, BF16)), f[1] = fmaf(f[1], epi.scale, widen((uint16_t)(res[i].x >> 16), BF16));
+                f[2] = fmaf(f[2], epi.scale, widen((uint16_t)res[i].y, BF16)), f[3] = fmaf(f[3], epi.scale, widen((uint16_t)(res[i].y >> 16), BF16));
+                const uint32_t lo = close2<BF16>(f[0], f[1]), hi = close2<BF16>(f[2], f[3]);
+                uint16_t *to = dst + i * dst_step;
+                if (vec_ok) {
+                    *reinterpret_cast<uint2 *>(to) = make_uint2(lo, hi);
+                } else {
+                    to[0] = (uint16_t)lo;
+                    if (left > 1) to[1] = (uint16_t)(lo >> 16);
+                    if (left > 2) to[2] = (uint16_t)hi;
+                    if (left > 3) to[3] = (uint16_t)(hi >> 16);
+                }
+            }
+        }
+        res_at += AHEAD * res_step;
+        dst += AHEAD * dst_step;
+    }
+}
+// (not inlined: one copy for all token tiles.  Its arguments come by value: what is read through a pointer to the kernel's
+// parameters is read again behind every store.)
+template <bool TWO>
+__device__ __noinline__ void wide_epilogue(const WideEpilogue w, const Epilogue epi, int bf16) {
+#define ATLAS_EPILOGUE(ACT) \
+    case ACT: return bf16 ? wide_epilogue_of<TWO, ACT, true>(w, epi) : wide_epilogue_of<TWO, ACT, false>(w, epi);
+    switch (epi.act) {
+        ATLAS_EPILOGUE(ATLAS_ACT_RELU)
+        ATLAS_EPILOGUE(ATLAS_ACT_SILU)
+        ATLAS_EPILOGUE(ATLAS_ACT_GELU)
+        ATLAS_EPILOGUE(ATLAS_ACT_GELU_TANH)
+        default: ATLAS_EPILOGUE(ATLAS_ACT_NONE)
+    }
+#undef ATLAS_EPILOGUE
+}
+
+// TWO: a tile is 64 rows of either of two weights (gemm_tile.cuh).
+template <int BN, bool TWO>
+__global__ void __launch_bounds__(TWO ? GM_THREADS_TWO : GM_THREADS, 1)
+gemm_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap c_map, const __grid_constant__ CUtensorMap up_map, GemmParams p) {
     using SM = Smem<BN>;
     // the next kernel of the stream may start its own weight-only prologue right away
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -167,8 +270,10 @@ gemm_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ C
     volatile int *s_abort = reinterpret_cast<volatile int *>(base_ptr + OFF_BAR + 8 * N_BARS + 8);
     constexpr int AS = SM::A_STAGES;
 
+    constexpr int CTRL_WARPS = GM_CTRL_WARPS + (TWO ? 1 : 0);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int n0 = blockIdx.x * GM_BM;  // first weight row (output feature) of the tile
+    const int row_tile = TWO ? two_tile(blockIdx.x) : blockIdx.x, row0 = TWO ? two_row(blockIdx.x) : 0;   // of a weight: 128 rows, or 64 of them
+    const int n0 = blockIdx.x * (TWO ? 64 : GM_BM);  // first output feature of the tile
     const int m0 = blockIdx.y * BN;  // first token
     // this CTA's K steps (grid.z slices K)
     const int kt_begin = (int)((long long)p.k_tiles * blockIdx.z / p.splits);
@@ -188,7 +293,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ C
             mbar_init(mma_done(s), 1);
         }
         for (int s = 0; s < XS; ++s) mbar_init(x_landed(s), 1);
-        for (int s = 0; s < FB; ++s) mbar_init(full_c(s), 1);
+        for (int s = 0; s < FB; ++s) mbar_init(full_c(s), TWO ? 2 : 1);
         for (int s = 0; s < CS; ++s) mbar_init(empty_c(s), 4);
         mbar_init(accfull_bar, 1);
         *s_abort = 0;
@@ -286,25 +391,29 @@ gemm_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ C
                 if (!request(st)) { *s_abort = 1; break; }
             }
         }
-    } else if (warp == 2) {
-        // ------------------------------ code producer ------------------------------
+    } else if (warp == 2 || (TWO && warp == 3)) {
+        // ------------------------------ code producers, one for each weight ------------------------------
         if (lane == 0) {
-            const int64_t crow0 = (int64_t)blockIdx.x * p.k_tiles + kt_begin;   // code tiles are rows of 128 in the map
+            const int64_t crow0 = (int64_t)row_tile * p.k_tiles + kt_begin;   // code tiles are rows of 128 in the map
             const int bpr = p.n_cols / p.bs;
             for (int st = 0; st < NST; ++st) {
                 const int slot = st % CS, round = st / CS;
                 if (round > 0 && !mbar_wait<200>(empty_c(slot), (round - 1) & 1)) { *s_abort = 1; break; }
                 if (*s_abort) break;
                 const int nk = min(GM_SK, KT - st * GM_SK);
-                mbar_arrive_expect_tx(full_c(st % FB), (uint32_t)nk * (C_BYTES + (p.bs_tiles ? S_BYTES : 0)));
+                constexpr uint32_t HALF = TWO ? 2 : 1;
+                const bool other = TWO && warp == 3;
+                mbar_arrive_expect_tx(full_c(st % FB), (uint32_t)nk * (C_BYTES + (p.bs_tiles ? S_BYTES : 0)) / HALF);
                 for (int j = 0; j < nk; ++j) {
                     const int kt = st * GM_SK + j;
                     // an 8 KB code tile is a 128-row x 64-byte matrix; the 64-byte swizzle spreads a column of 16-byte
                     // chunks over all banks for the dequantizers (thread = row)
-                    tma_load_2d(base + OFF_C + (slot * GM_SK + j) * C_BYTES, &c_map, 0, (int)((crow0 + kt) * GM_BM), full_c(st % FB));
+                    tma_load_2d(base + OFF_C + (slot * GM_SK + j) * C_BYTES + (other ? C_BYTES / 2 : 0), other ? &up_map : &c_map, 0,
+                                (int)((crow0 + kt) * GM_BM) + row0, full_c(st % FB));
                     if (p.bs_tiles)
-                        bulk_load_1d(base + OFF_S + (slot * GM_SK + j) * S_BYTES,
-                                     p.scales_t + ((size_t)blockIdx.x * bpr + (kt_begin + kt) / p.bs_tiles) * 128, S_BYTES, full_c(st % FB));
+                        bulk_load_1d(base + OFF_S + (slot * GM_SK + j) * S_BYTES + (other ? S_BYTES / 2 : 0),
+                                     (other ? (const uint16_t *)p.up.scales_tiled : p.scales_t) + ((size_t)row_tile * bpr + (kt_begin + kt) / p.bs_tiles) * 128 + row0,
+                                     S_BYTES / HALF, full_c(st % FB));
                 }
             }
         }
@@ -352,17 +461,20 @@ gemm_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ C
         }
     } else {
         // ------------------------------ dequantizers, then epilogue ------------------------------
-        const int dwi = warp - GM_CTRL_WARPS;     // 0..15
+        const int dwi = warp - CTRL_WARPS;        // 0..15
         const int q = warp & 3;                   // TMEM lane quarter this warp may access: rows 32q .. 32q+31 of the tile
         const int ph = dwi >> 2;                  // this warp rebuilds the K steps it == ph (mod 4), always into A stage ph
         const int rl = q * 32 + lane;             // row of the tile (= TMEM lane) this thread rebuilds
         const int rs = lane & 15;                 // its row inside the 16-row strip
         const int swz = (lane >> 1) & 3;          // 64-byte swizzle of this row's 16-byte chunks
         const int bpr = p.n_cols / p.bs;
-        const uint16_t *sc_tile = p.scales_t + (int64_t)blockIdx.x * bpr * 128;
+        const bool up = TWO && q >= 2;            // its rows are the second weight's
+        const uint16_t *sc_row = (up ? (const uint16_t *)p.up.scales_tiled : p.scales_t) + (int64_t)row_tile * bpr * 128 + (TWO ? row0 + rl % 64 : rl);
+        const uint32_t *entries = up ? p.up.outlier_entries : p.entries;
+        const uint16_t *ovals = up ? (const uint16_t *)p.up.outlier_vals_sorted : p.ovals;
         // outlier lists (sorted by column) of the warp's two strips: lanes 0-15 serve strip 2q, lanes 16-31 strip 2q+1
-        const int64_t strip = (int64_t)blockIdx.x * 8 + 2 * q + (lane >> 4);
-        const int32_t *cp = p.chunk_ptr + strip * (p.n_chunks + 1) + kt_begin;
+        const int64_t strip = (int64_t)row_tile * 8 + (TWO ? row0 / 16 + (2 * q + (lane >> 4)) % 4 : 2 * q + (lane >> 4));
+        const int32_t *cp = (up ? p.up.outlier_chunk_ptr : p.chunk_ptr) + strip * (p.n_chunks + 1) + kt_begin;
         const int ej = lane & 15;                 // which entry of its strip's list this lane buffers
         const uint32_t code_off = (uint32_t)rl * 64u;   // the tile is a 128 x 64-byte row-major matrix
         const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)BN + (uint32_t)((ph % AS) * GM_A_COLS);
@@ -396,8 +508,8 @@ gemm_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ C
         uint32_t ent0 = 0, val0 = 0, ent1 = 0, val1 = 0;
         range_of(0, b0, e0);
         range_of(1, b1, e1);
-        if (b0 + ej < e0) { ent0 = __ldg(p.entries + b0 + ej); val0 = __ldg(p.ovals + b0 + ej); }
-        if (b1 + ej < e1) { ent1 = __ldg(p.entries + b1 + ej); val1 = __ldg(p.ovals + b1 + ej); }
+        if (b0 + ej < e0) { ent0 = __ldg(entries + b0 + ej); val0 = __ldg(ovals + b0 + ej); }
+        if (b1 + ej < e1) { ent1 = __ldg(entries + b1 + ej); val1 = __ldg(ovals + b1 + ej); }
         bool ok = true;
         for (int n = 0; n < nsteps && ok; ++n) {
             const int st = ph + 4 * n;
@@ -405,7 +517,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ C
             int b2, e2;
             range_of(n + 2, b2, e2);
             uint32_t ent2 = 0, val2 = 0;
-            if (b2 + ej < e2) { ent2 = __ldg(p.entries + b2 + ej); val2 = __ldg(p.ovals + b2 + ej); }
+            if (b2 + ej < e2) { ent2 = __ldg(entries + b2 + ej); val2 = __ldg(ovals + b2 + ej); }
             if (((n + 2) & 15) == 0) {
                 const int block = (n + 2) >> 4;
                 if (block & 1) load_ranges(block + 1, rbA, reA); else load_ranges(block + 1, rbB, reB);
@@ -447,7 +559,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ C
                     } else {
 #pragma unroll
                         for (int c = 0; c < 4; ++c)
-                            sh[c] = __ushort_as_half(__ldg(sc_tile + (int64_t)((k0 + j * GM_BK + c * 16) / p.bs) * 128 + rl));
+                            sh[c] = __ushort_as_half(__ldg(sc_row + (int64_t)((k0 + j * GM_BK + c * 16) / p.bs) * 128));
                     }
                     if (j == nk - 1) {   // the code slot is in registers: hand it back (one arrival per warp)
                         __syncwarp();
@@ -488,7 +600,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ C
                         if (cnt > 16) {
                             const int bb = __shfl_sync(0xffffffffu, b0, h * 16);
                             for (int i = 16; i < cnt; ++i) {
-                                const uint32_t pk = pack((uint32_t)(h * 16), __ldg(p.entries + bb + i), (uint32_t)__ldg(p.ovals + bb + i));
+                                const uint32_t pk = pack((uint32_t)(h * 16), __ldg(entries + bb + i), (uint32_t)__ldg(ovals + bb + i));
                                 put(pk, (pk >> 23) == (uint32_t)lane && (int)((pk >> 22) & 1u) == j);
                             }
                         }
@@ -523,57 +635,50 @@ gemm_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ C
             : "=r"(all_ok) : "r"((uint32_t)acc_ok), "n"(GM_EPI_WARPS * 32) : "memory");
         if (all_ok) {
             tcgen05_fence_after();
-            const int part = (warp - GM_CTRL_WARPS) >> 2;   // four warps share a TMEM lane quarter: 32-column chunks part, part + 4, ..
-            const int nl = q * 32 + lane;                   // feature inside the tile
-            const int n = n0 + nl;
-            const float bv = (p.bias && n < p.n_rows) ? __half2float(__ushort_as_half(__ldg(p.bias + n))) : 0.f;
-            // staging tile [BN tokens][128 features (+ pad)] in the idle rings: 16-bit outputs, or fp32
-            // partial sums when K is split between CTAs
-            const bool partial = p.splits > 1 || p.to_partials;
+            const int part = (warp - CTRL_WARPS) >> 2;   // four warps share a TMEM lane quarter: 32-column chunks part, part + 4, ..
+            const int nl = q * 32 + lane;                   // row of the tile
+            const int n = n0 + (TWO ? nl % 64 : nl);        // feature
+            const float bv = (!TWO && p.bias && n < p.n_rows) ? __half2float(__ushort_as_half(__ldg(p.bias + n))) : 0.f;
+            // staging tile [BN tokens][128 features (+ pad)] in the idle rings: 16-bit outputs, or fp32 sums when K is split
+            // between CTAs or something follows
+            const bool partial = p.splits > 1 || p.to_partials, wide = TWO || partial || p.follows;
             unsigned char *stage = base_ptr + OFF_B;
-            const int st_bytes = partial ? (GM_BM + 4) * 4 : (GM_BM + 8) * 2;   // row stride; pads keep banks apart
+            const int st_bytes = wide ? (GM_BM + 4) * 4 : (GM_BM + 8) * 2;   // row stride; pads keep banks apart
             for (int c = part; c < BN / 32; c += 4) {
                 if (m0 + c * 32 >= p.m) break;  // warp-uniform: no tokens left in this tile
                 uint32_t v[32];
                 tmem_ld_32x32b_x32(tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(c * 32), v);
                 tmem_ld_wait();
-                float f[32];
 #pragma unroll
-                for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(v[j]);
-                if (partial) {
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) reinterpret_cast<float *>(stage + (size_t)(c * 32 + j) * st_bytes)[nl] = f[j];
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) f[j] += bv;
-                    activate(f, p.epi.act);
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        const int m = m0 + c * 32 + j;   // (a warp's 32 lanes read 64 contiguous bytes of the residual)
-                        f[j] = scaled(p.epi, f[j], n < p.n_rows && m < p.m ? residual_at(p.epi, m, n, p.out_bf16) : 0.f);
-                        reinterpret_cast<uint16_t *>(stage + (size_t)(c * 32 + j) * st_bytes)[nl] = narrow(f[j], p.out_bf16);
-                    }
+                for (int j = 0; j < 32; ++j) {
+                    unsigned char *row = stage + (size_t)(c * 32 + j) * st_bytes;
+                    if (wide) reinterpret_cast<uint32_t *>(row)[nl] = v[j];
+                    else reinterpret_cast<uint16_t *>(row)[nl] = narrow(__uint_as_float(v[j]) + bv, p.out_bf16);
                 }
             }
-            // all eight epilogue warps have staged their part
+            // all epilogue warps have staged their part
             asm volatile("bar.sync 1, %0;" ::"n"(GM_EPI_WARPS * 32) : "memory");
-            const int et = tid - GM_CTRL_WARPS * 32;         // 0..511
+            const int et = tid - CTRL_WARPS * 32;            // 0..511
             const int rows_left = min(BN, p.m - m0);
             if (partial) {
                 // fp32 partial tile -> partials[z][m][n], 16 bytes (4 features) per thread and store
-                float *dst0 = p.partials + (size_t)blockIdx.z * p.m * p.n_rows;
-                const bool vec_ok = (n0 + GM_BM <= p.n_rows) && (p.n_rows % 4 == 0);
+                const size_t slice0 = (size_t)blockIdx.z * p.m * p.n_rows;
+                const bool vec_ok = (n0 + (TWO ? 64 : GM_BM) <= p.n_rows) && (p.n_rows % 4 == 0);
                 for (int idx = et; idx < rows_left * (GM_BM / 4); idx += GM_EPI_WARPS * 32) {
                     const int row = idx >> 5, piece = idx & 31;
+                    const int at = n0 + (TWO ? piece % 16 : piece) * 4;
                     const float *src = reinterpret_cast<const float *>(stage + (size_t)row * st_bytes) + piece * 4;
-                    float *dst = dst0 + (size_t)(m0 + row) * p.n_rows + n0 + piece * 4;
+                    float *dst = (TWO && piece >= 16 ? p.up_partials : p.partials) + slice0 + (size_t)(m0 + row) * p.n_rows + at;
                     if (vec_ok) {
                         *reinterpret_cast<float4 *>(dst) = *reinterpret_cast<const float4 *>(src);
                     } else {
                         for (int e = 0; e < 4; ++e)
-                            if (n0 + piece * 4 + e < p.n_rows) dst[e] = src[e];
+                            if (at + e < p.n_rows) dst[e] = src[e];
                     }
                 }
+            } else if (wide) {
+                const WideEpilogue w = {base + OFF_B, et, rows_left, m0, n0, p.n_rows, p.bias, (const uint16_t *)p.up.bias, (uint16_t *)p.y, p.ldy};
+                wide_epilogue<TWO>(w, p.epi, p.out_bf16);
             } else {
                 const bool vec_ok = (n0 + GM_BM <= p.n_rows) && (p.ldy % 8 == 0) && (((uintptr_t)p.y & 15) == 0);
                 for (int idx = et; idx < rows_left * (GM_BM / 8); idx += GM_EPI_WARPS * 32) {
@@ -658,8 +763,19 @@ gemm_finish_kernel(const float *partials, const float *up, int splits, int m, in
             for (int e = 0; e < W; ++e) acc[e] *= other[e];
         }
         uint16_t out[W];
+        if (VEC) {
 #pragma unroll
-        for (int e = 0; e < W; ++e) out[e] = narrow(scaled(epi, acc[e], residual_at(epi, row, n + e, out_bf16)), out_bf16);
+            for (int h = 0; h < W; h += 4) {
+                float r[4];
+                residual_at(epi, row, n + h, 4, out_bf16, r);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[(h + e) % W] = scaled(epi, acc[(h + e) % W], r[e]);
+            }
+        } else {
+            acc[0] = scaled(epi, acc[0], residual_at(epi, row, n, out_bf16));
+        }
+#pragma unroll
+        for (int e = 0; e < W; ++e) out[e] = narrow(acc[e], out_bf16);
         const int64_t off = (int64_t)row * ldy + n;
         const int dests = fg.world > 0 ? fg.world : 1;
         for (int d = 0; d < dests; ++d) {
@@ -908,7 +1024,7 @@ int gemm_sm_count() {
 // host work is 5 (60.3 -> 61.5 us for the six linears of a small layer's 128-token prompt).
 struct Shape {
     int64_t m, n_rows, n_cols;
-    int sms, flags;   // 1: bf16, 2: a tensor map can take the rows, 4: output rows on 16-byte boundaries
+    int sms, flags;   // 1: bf16, 2: a tensor map can take the rows, 4: output rows on 16-byte boundaries, 8: two weights
 };
 struct Route {
     bool tile;
@@ -925,26 +1041,27 @@ Route route_for(const Shape &shape) {
         e.shape.flags != shape.flags) {
         const bool bf16 = shape.flags & 1, tma_ok = shape.flags & 2, aligned = shape.flags & 4;
         e.route.plan = plan_tile(shape.m, shape.n_rows, (int)(shape.n_cols / GM_BK), bf16 && tma_ok, bf16, shape.sms);
-        e.route.tile = e.route.plan.us <= gemm_us(shape.m, shape.n_rows, shape.n_cols, bf16, bf16 && tma_ok, aligned, shape.sms);
+        // (two weights: always the kernel that adds its slices up itself)
+        e.route.tile = (shape.flags & 8) || e.route.plan.us <= gemm_us(shape.m, shape.n_rows, shape.n_cols, bf16, bf16 && tma_ok, aligned, shape.sms);
         e.shape = shape;
     }
     return e.route;
 }
 
-template <int BN>
-int launch_gemm(const CUtensorMap &x_map, const CUtensorMap &c_map, const GemmParams &p, cudaStream_t st) {
+template <int BN, bool TWO>
+int launch_gemm(const CUtensorMap &x_map, const CUtensorMap &c_map, const CUtensorMap &up_map, const GemmParams &p, cudaStream_t st) {
     static thread_local int configured_dev = -1;
     int dev = 0;
     cudaGetDevice(&dev);
     if (configured_dev != dev) {
-        int rc = check_cuda(cudaFuncSetAttribute(gemm_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        int rc = check_cuda(cudaFuncSetAttribute(gemm_kernel<BN, TWO>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                  (int)Smem<BN>::TOTAL), "cudaFuncSetAttribute(gemm smem)");
         if (rc) return rc;
         configured_dev = dev;
     }
-    cudaLaunchConfig_t cfg = pdl_config(dim3((unsigned)ceil_div_i64(p.n_rows, GM_BM), (unsigned)ceil_div_i64(p.m, BN), (unsigned)p.splits),
-                                        dim3(GM_THREADS), Smem<BN>::TOTAL, st);
-    return check_cuda(cudaLaunchKernelEx(&cfg, gemm_kernel<BN>, x_map, c_map, p), "gemm_kernel launch");
+    cudaLaunchConfig_t cfg = pdl_config(dim3((unsigned)ceil_div_i64(p.n_rows, TWO ? 64 : GM_BM), (unsigned)ceil_div_i64(p.m, BN), (unsigned)p.splits),
+                                        dim3(TWO ? GM_THREADS_TWO : GM_THREADS), Smem<BN>::TOTAL, st);
+    return check_cuda(cudaLaunchKernelEx(&cfg, gemm_kernel<BN, TWO>, x_map, c_map, up_map, p), "gemm_kernel launch");
 }
 
 }  // namespace
@@ -961,14 +1078,17 @@ extern "C" int atlas_qlinear_gemm_plan(int64_t m, int64_t n_rows, int64_t n_cols
     return ATLAS_OK;
 }
 
+// Two weights take the tiles of one with so many rows.
+static int64_t two_rows(int64_t n_rows) { return atlas::ceil_div_i64(n_rows, 64) * 128; }
+
 size_t atlas::qlinear_gemm_workspace_bytes(int64_t m, int64_t n_rows, int64_t n_cols, bool two) {
     if (m <= 0 || n_cols <= 0 || n_rows <= 0) return GM_WS_HEADER;
     // fp16 copy of x (bf16 or strided input), then room for the fp32 partial outputs of the K slices
     const size_t xcopy = ((size_t)m * (size_t)n_cols * 2 + 255) & ~(size_t)255;
-    // (one fp32 slice of the output per K slice; one even without slicing, for the gathered form and for two weights)
-    const int splits = gemm_splits_for(m, n_rows, n_cols, gemm_sm_count());
+    // (one fp32 slice of the output per K slice, of either weight; one even without slicing, for the gathered form)
+    const int splits = gemm_splits_for(m, two ? two_rows(n_rows) : n_rows, n_cols, gemm_sm_count());
     const size_t slices = (size_t)splits * (size_t)m * (size_t)n_rows * 4;
-    const size_t part = two ? 2 * ((slices + 255) & ~(size_t)255) : (m > TILE_MAX_TOKENS ? (splits > 1 ? slices : 0) : (m <= 64 ? slices : 0));
+    const size_t part = two ? (m > TILE_MAX_TOKENS && splits > 1 ? 2 * ((slices + 255) & ~(size_t)255) : 0) : (m > TILE_MAX_TOKENS ? (splits > 1 ? slices : 0) : (m <= 64 ? slices : 0));
     return GM_WS_HEADER + xcopy + part;
 }
 extern "C" size_t atlas_qlinear_gemm_workspace_bytes(int64_t m, int64_t n_rows, int64_t n_cols) {
@@ -1027,12 +1147,13 @@ int qlinear_gemm(const void *x, int dtype, int64_t m, int64_t ldx, const uint8_t
     const bool bf16 = dtype == ATLAS_DTYPE_BF16;
     // (the gathered form's arrival protocol lives in the kernels of this file)
     Route route = {};
-    if (!gather && !up && m <= TILE_MAX_TOKENS) {
+    const int64_t tiled_rows = up ? two_rows(n_rows) : n_rows;
+    if (!gather && m <= TILE_MAX_TOKENS) {
         const bool aligned = n_rows % 8 == 0 && ldy % 8 == 0 && ((uintptr_t)y & 15) == 0;
-        route = route_for(Shape{m, n_rows, n_cols, gemm_sm_count(), (bf16 ? 1 : 0) | (tma_ok ? 2 : 0) | (aligned ? 4 : 0)});
+        route = route_for(Shape{m, tiled_rows, n_cols, gemm_sm_count(), (bf16 ? 1 : 0) | (tma_ok ? 2 : 0) | (aligned ? 4 : 0) | (up ? 8 : 0)});
     }
     const bool tile = route.tile;
-    const GemmPlan plan = tile ? GemmPlan{tile_tokens_for(m), route.plan.splits} : gemm_plan(m, n_rows, n_cols, gemm_sm_count());
+    const GemmPlan plan = tile ? GemmPlan{tile_tokens_for(m), route.plan.splits} : gemm_plan(m, tiled_rows, n_cols, gemm_sm_count());
     const int bn = plan.bn;
 
     // operand B must be fp16 with rows on 16-byte boundaries for the tensor map
@@ -1074,16 +1195,21 @@ int qlinear_gemm(const void *x, int dtype, int64_t m, int64_t ldx, const uint8_t
     auto code_map = [&](const uint8_t *codes, CUtensorMap &map) {
         const cuuint64_t cdim[2] = {(cuuint64_t)GM_BK, (cuuint64_t)(ceil_div_i64(n_rows, GM_BM) * (n_cols / GM_BK) * GM_BM)};
         const cuuint64_t cstride[1] = {(cuuint64_t)GM_BK};
-        const cuuint32_t cbox[2] = {(cuuint32_t)GM_BK, (cuuint32_t)GM_BM};
+        const cuuint32_t cbox[2] = {(cuuint32_t)GM_BK, (cuuint32_t)(up ? 64 : GM_BM)};
         const CUresult r = encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t *>(codes), cdim, cstride, cbox, estride,
                                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
         ATLAS_RETURN_IF(r != CUDA_SUCCESS, ATLAS_ERR_LAUNCH, "cuTensorMapEncodeTiled (codes) failed with %d", (int)r);
         return ATLAS_OK;
     };
-    CUtensorMap c_map;
+    CUtensorMap c_map, up_map;
     rc = code_map(tiles, c_map);
     if (rc) return rc;
+    up_map = c_map;
+    if (up) {
+        rc = code_map(up->tiles, up_map);
+        if (rc) return rc;
+    }
 
     if (tile) {
         TileParams t;
@@ -1105,7 +1231,9 @@ int qlinear_gemm(const void *x, int dtype, int64_t m, int64_t ldx, const uint8_t
         t.splits = route.plan.splits;
         t.error_flag = status;
         t.epi = epi;
-        return launch_tile(x_map, c_map, t, st);
+        t.two = up != nullptr;
+        t.up = up ? *up : AtlasWeight{};
+        return launch_tile(x_map, c_map, up_map, t, st);
     }
     GemmParams p;
     p.tiles = tiles;
@@ -1126,7 +1254,7 @@ int qlinear_gemm(const void *x, int dtype, int64_t m, int64_t ldx, const uint8_t
     p.out_bf16 = dtype == ATLAS_DTYPE_BF16;
     p.splits = plan.splits;
     p.partials = (float *)((char *)workspace + GM_WS_HEADER + xcopy);
-    p.to_partials = gather != nullptr || up != nullptr;   // the gather, and the product of two weights, are the second kernel's job
+    p.to_partials = gather != nullptr;   // the gather is the second kernel's job
     p.x_bf16 = in_kernel_bf16;
     p.wait_flags = wait_in_copy ? nullptr : wait_flags;
     p.gather_state = gather ? (const unsigned int *)gather->state : nullptr;
@@ -1134,36 +1262,27 @@ int qlinear_gemm(const void *x, int dtype, int64_t m, int64_t ldx, const uint8_t
     p.poll_limit = gather ? (long long)gather->poll_limit : 0;
     p.error_flag = status;
     p.epi = epi;
-    auto launch = [&](const CUtensorMap &codes, const GemmParams &q) {
-        switch (bn) {
-            case 32: return launch_gemm<32>(x_map, codes, q, st);
-            case 64: return launch_gemm<64>(x_map, codes, q, st);
-            case 128: return launch_gemm<128>(x_map, codes, q, st);
-            case 160: return launch_gemm<160>(x_map, codes, q, st);
-            case 192: return launch_gemm<192>(x_map, codes, q, st);
-            case 224: return launch_gemm<224>(x_map, codes, q, st);
-            case 256: return launch_gemm<256>(x_map, codes, q, st);
-            case 320: return launch_gemm<320>(x_map, codes, q, st);
-            default: return launch_gemm<384>(x_map, codes, q, st);
-        }
-    };
-    rc = launch(c_map, p);
-    if (rc) return rc;
-    const float *up_partials = nullptr;
-    if (up) {
-        GemmParams q = p;
-        q.tiles = up->tiles;
-        q.scales_t = (const uint16_t *)up->scales_tiled;
-        q.chunk_ptr = up->outlier_chunk_ptr;
-        q.entries = up->outlier_entries;
-        q.ovals = (const uint16_t *)up->outlier_vals_sorted;
-        q.partials = p.partials + (((size_t)p.splits * (size_t)m * (size_t)n_rows * 4 + 255) & ~(size_t)255) / 4;
-        up_partials = q.partials;
-        CUtensorMap up_map;
-        rc = code_map(up->tiles, up_map);
-        if (!rc) rc = launch(up_map, q);
-        if (rc) return rc;
+    p.follows = !is_plain(epi);
+    p.up = up ? *up : AtlasWeight{};
+    p.up_partials = up ? p.partials + (((size_t)p.splits * (size_t)m * (size_t)n_rows * 4 + 255) & ~(size_t)255) / 4 : nullptr;
+    switch (up ? -bn : bn) {
+        case 32: rc = launch_gemm<32, false>(x_map, c_map, up_map, p, st); break;
+        case 64: rc = launch_gemm<64, false>(x_map, c_map, up_map, p, st); break;
+        case 128: rc = launch_gemm<128, false>(x_map, c_map, up_map, p, st); break;
+        case 160: rc = launch_gemm<160, false>(x_map, c_map, up_map, p, st); break;
+        case 192: rc = launch_gemm<192, false>(x_map, c_map, up_map, p, st); break;
+        case 224: rc = launch_gemm<224, false>(x_map, c_map, up_map, p, st); break;
+        case 256: rc = launch_gemm<256, false>(x_map, c_map, up_map, p, st); break;
+        case 320: rc = launch_gemm<320, false>(x_map, c_map, up_map, p, st); break;
+        case 384: rc = launch_gemm<384, false>(x_map, c_map, up_map, p, st); break;
+        case -160: rc = launch_gemm<160, true>(x_map, c_map, up_map, p, st); break;
+        case -192: rc = launch_gemm<192, true>(x_map, c_map, up_map, p, st); break;
+        case -224: rc = launch_gemm<224, true>(x_map, c_map, up_map, p, st); break;
+        case -256: rc = launch_gemm<256, true>(x_map, c_map, up_map, p, st); break;
+        case -320: rc = launch_gemm<320, true>(x_map, c_map, up_map, p, st); break;
+        default: rc = launch_gemm<384, true>(x_map, c_map, up_map, p, st); break;
     }
+    if (rc) return rc;
     if (p.splits > 1 || p.to_partials) {
         const bool vec = n_rows % 8 == 0 && ldy % 8 == 0 && (((uintptr_t)y & 15) == 0) &&
                          (((uintptr_t)p.partials & 15) == 0);
@@ -1173,7 +1292,7 @@ int qlinear_gemm(const void *x, int dtype, int64_t m, int64_t ldx, const uint8_t
         const int64_t blocks = ceil_div_i64(pieces, 256);
         cudaLaunchConfig_t cfg = pdl_config(dim3((unsigned)(blocks < 2048 ? blocks : 2048)), dim3(256), 0, st);
         auto kern = vec_all ? gemm_finish_kernel<true> : gemm_finish_kernel<false>;
-        rc = check_cuda(cudaLaunchKernelEx(&cfg, kern, (const float *)p.partials, up_partials, p.splits, (int)m, (int)n_rows, (const uint16_t *)bias,
+        rc = check_cuda(cudaLaunchKernelEx(&cfg, kern, (const float *)p.partials, (const float *)p.up_partials, p.splits, (int)m, (int)n_rows, (const uint16_t *)bias,
                                            up ? (const uint16_t *)up->bias : (const uint16_t *)nullptr, y, ldy, p.out_bf16, fg, epi), "gemm_finish_kernel launch");
     }
     return rc;

@@ -20,6 +20,8 @@
 // covered by the other's stream, and the first CTAs of the next launch (programmatic dependent launch) fetch their
 // codes while the last ones of this launch finish.
 //
+// With two weights (gate and up) a tile holds 64 rows of either, and the sums of both are multiplied where y is written.
+//
 // The K slices of a tile add up through distributed shared memory: every CTA leaves its fp32 tile in its own shared
 // memory, and after a cluster barrier each one adds its share of the elements over all slices, in slice order
 // (deterministic), adds the bias and writes y.  No partial sums in global memory, no second kernel.
@@ -92,9 +94,9 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr, uint32_t rank) {
     return v;
 }
 
-template <int BN>
+template <int BN, bool TWO>
 __global__ void __launch_bounds__(TL_THREADS, 2)
-tile_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap c_map, TileParams p) {
+tile_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap c_map, const __grid_constant__ CUtensorMap up_map, TileParams p) {
     using SM = TileSmem<BN>;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     constexpr int CS = SM::CS, XS = SM::XS;
@@ -116,12 +118,14 @@ tile_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ C
     volatile int *s_abort = reinterpret_cast<volatile int *>(base_ptr + SM::OFF_BAR + 8 * N_BARS + 8);
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int n0 = blockIdx.x * TL_BM;
+    const int row_tile = TWO ? two_tile(blockIdx.x) : blockIdx.x, row0 = TWO ? two_row(blockIdx.x) : 0;   // of a weight: 128 rows, or 64 of them
+    const int n0 = blockIdx.x * (TWO ? 64 : TL_BM);
     const int slice = blockIdx.y;
     const int rows = p.m;   // tokens, at most BN
     const int kt_begin = (int)((long long)p.k_tiles * slice / p.splits);
     const int KT = (int)((long long)p.k_tiles * (slice + 1) / p.splits) - kt_begin;
 
+    if (TWO && tid == 32 * 2 + 2) asm volatile("prefetch.tensormap [%0];" ::"l"((const void *)&up_map) : "memory");
     if (tid == 1 || tid == 32 * 2 + 1)
         asm volatile("prefetch.tensormap [%0];" ::"l"(tid < 32 ? (const void *)&x_map : (const void *)&c_map) : "memory");
     if (tid == 0) {
@@ -182,16 +186,21 @@ tile_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ C
     } else if (warp == 2) {
         // ------------------------------ codes and scales ------------------------------
         if (lane == 0) {
-            const int64_t crow0 = (int64_t)blockIdx.x * p.k_tiles + kt_begin;   // code tiles are runs of 128 rows of the map
+            const int64_t crow0 = (int64_t)row_tile * p.k_tiles + kt_begin;   // code tiles are runs of 128 rows of the map
             for (int kt = 0; kt < KT; ++kt) {
                 const int slot = kt % CS, round = kt / CS;
                 if (round > 0 && !mbar_wait<40>(empty_c(slot), (uint32_t)((round - 1) & 1))) { *s_abort = 1; break; }
                 if (*s_abort) break;
                 mbar_arrive_expect_tx(full_c(slot), TL_C_BYTES + (p.bs_tiles ? TL_S_BYTES : 0u));
-                tma_load_2d(base + SM::OFF_C + slot * TL_C_BYTES, &c_map, 0, (int)((crow0 + kt) * TL_BM), full_c(slot));
-                if (p.bs_tiles)
-                    bulk_load_1d(base + SM::OFF_S + slot * TL_S_BYTES,
-                                 p.scales_t + ((size_t)blockIdx.x * p.blocks_per_row + (kt_begin + kt) / p.bs_tiles) * 128, TL_S_BYTES, full_c(slot));
+                const uint32_t c_dst = base + SM::OFF_C + slot * TL_C_BYTES, s_dst = base + SM::OFF_S + slot * TL_S_BYTES;
+                const int c_row = (int)((crow0 + kt) * TL_BM) + row0;
+                tma_load_2d(c_dst, &c_map, 0, c_row, full_c(slot));
+                if (TWO) tma_load_2d(c_dst + TL_C_BYTES / 2, &up_map, 0, c_row, full_c(slot));
+                if (p.bs_tiles) {
+                    const size_t s_at = ((size_t)row_tile * p.blocks_per_row + (kt_begin + kt) / p.bs_tiles) * 128 + row0;
+                    bulk_load_1d(s_dst, p.scales_t + s_at, TWO ? TL_S_BYTES / 2 : TL_S_BYTES, full_c(slot));
+                    if (TWO) bulk_load_1d(s_dst + TL_S_BYTES / 2, (const uint16_t *)p.up.scales_tiled + s_at, TL_S_BYTES / 2, full_c(slot));
+                }
                 issued = kt + 1;
             }
         }
@@ -225,17 +234,20 @@ tile_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ C
         // ahead, its first 16 entries two ahead: they come from HBM like the codes.  (Four ahead through an unrolled
         // loop was slower, 43 against 39 us at 22016 x 4096 and 32 tokens: the loop then misses the instruction cache.)
         const int half = lane >> 4, ej = lane & 15;
-        const int64_t strip = (int64_t)blockIdx.x * 8 + 2 * q + half;
-        const int32_t *cp = p.chunk_ptr + strip * (p.k_tiles + 1) + kt_begin;
+        const bool up = TWO && q >= 2;   // this warp's rows are the second weight's
+        const int64_t strip = (int64_t)row_tile * 8 + (TWO ? row0 / 16 + (2 * q + half) % 4 : 2 * q + half);
+        const int32_t *cp = (up ? p.up.outlier_chunk_ptr : p.chunk_ptr) + strip * (p.k_tiles + 1) + kt_begin;
+        const uint32_t *entries = up ? p.up.outlier_entries : p.entries;
+        const uint16_t *ovals = up ? (const uint16_t *)p.up.outlier_vals_sorted : p.ovals;
         unsigned char *a_strip = base_ptr + SM::OFF_A + ph * TL_A_BYTES + (q * 32 + half * 16) * 128;
-        const uint16_t *sc_tile = p.scales_t + (size_t)blockIdx.x * p.blocks_per_row * 128;
+        const uint16_t *sc_row = (up ? (const uint16_t *)p.up.scales_tiled : p.scales_t) + (size_t)row_tile * p.blocks_per_row * 128 + (TWO ? row0 + rl % 64 : rl);
         auto range = [&](int kt, int &b, int &e) {
             b = e = 0;
             if (kt < KT) { b = __ldg(cp + kt); e = __ldg(cp + kt + 1); }
         };
         auto entry = [&](int b, int e, uint32_t &ent, uint32_t &val) {
             ent = val = 0u;
-            if (b + ej < e) { ent = __ldg(p.entries + b + ej); val = __ldg(p.ovals + b + ej); }
+            if (b + ej < e) { ent = __ldg(entries + b + ej); val = __ldg(ovals + b + ej); }
         };
         int b0, e0, b1, e1, b2, e2;
         uint32_t ent0, val0, ent1, val1;
@@ -263,7 +275,7 @@ tile_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ C
                 sh[0] = sh[1] = sh[2] = sh[3] = __ushort_as_half(reinterpret_cast<const uint16_t *>(base_ptr + SM::OFF_S + slot * TL_S_BYTES)[rl]);
             } else {
 #pragma unroll
-                for (int c = 0; c < 4; ++c) sh[c] = __ushort_as_half(__ldg(sc_tile + (int64_t)((col0 + c * 16) / p.bs) * 128 + rl));
+                for (int c = 0; c < 4; ++c) sh[c] = __ushort_as_half(__ldg(sc_row + (int64_t)((col0 + c * 16) / p.bs) * 128));
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(empty_c(slot));
@@ -286,7 +298,7 @@ tile_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ C
                 *reinterpret_cast<uint16_t *>(a_strip + row * 128 + (((col >> 3) ^ (row & 7)) << 4) + (col & 7) * 2) = (uint16_t)v;
             };
             if (b0 + ej < e0) put(ent0, val0);
-            for (int i = b0 + 16 + ej; i < e0; i += 16) put(__ldg(p.entries + i), __ldg(p.ovals + i));
+            for (int i = b0 + 16 + ej; i < e0; i += 16) put(__ldg(entries + i), __ldg(ovals + i));
             fence_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(ready_bar(kt));
@@ -333,28 +345,40 @@ tile_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ C
     {
         const uint32_t red = base;
         const bool vec = (p.ldy % 4 == 0) && (((uintptr_t)p.y & 7) == 0);
-        for (int idx = slice * TL_THREADS + tid; idx < rows * (TL_BM / 4); idx += p.splits * TL_THREADS) {
-            const int t = idx >> 5, n = n0 + (idx & 31) * 4;
+        constexpr int PIECES = TWO ? TL_BM / 8 : TL_BM / 4;   // of 4 outputs
+        for (int idx = slice * TL_THREADS + tid; idx < rows * PIECES; idx += p.splits * TL_THREADS) {
+            const int t = idx / PIECES, n = n0 + idx % PIECES * 4;
             if (n >= p.n_rows) continue;
-            const uint32_t at = red + (uint32_t)(t * TL_RED + (idx & 31) * 4) * 4u;
-            float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (p.splits == 1) {
-                a = *reinterpret_cast<const float4 *>(base_ptr + (at - base));
-            } else {
-                for (int s = 0; s < p.splits; ++s) {
-                    const float4 b = ld_cluster_f4(at, (uint32_t)s);
-                    a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
+            auto sums = [&](int feature, const uint16_t *bias, float (&f)[4]) {
+                const uint32_t at = red + (uint32_t)(t * TL_RED + feature) * 4u;
+                float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (p.splits == 1) {
+                    a = *reinterpret_cast<const float4 *>(base_ptr + (at - base));
+                } else {
+                    for (int s = 0; s < p.splits; ++s) {
+                        const float4 b = ld_cluster_f4(at, (uint32_t)s);
+                        a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
+                    }
                 }
+                f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (bias && n + e < p.n_rows) f[e] += __half2float(__ushort_as_half(__ldg(bias + n + e)));
+            };
+            float f[4], res[4];
+            residual_at(p.epi, t, n, p.n_rows - n, p.out_bf16, res);
+            sums(idx % PIECES * 4, p.bias, f);
+            activate(f, p.epi.act);
+            if (TWO) {
+                float u[4];
+                sums(64 + idx % PIECES * 4, (const uint16_t *)p.up.bias, u);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) f[e] *= u[e];
             }
-            float f[4] = {a.x, a.y, a.z, a.w};
+            scale_and_add(p.epi, f, res);
             uint16_t o[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (p.bias && n + e < p.n_rows) f[e] += __half2float(__ushort_as_half(__ldg(p.bias + n + e)));
-            activate(f, p.epi.act);
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                o[e] = narrow(scaled(p.epi, f[e], n + e < p.n_rows ? residual_at(p.epi, t, n + e, p.out_bf16) : 0.f), p.out_bf16);
+            for (int e = 0; e < 4; ++e) o[e] = narrow(f[e], p.out_bf16);
             uint16_t *dst = reinterpret_cast<uint16_t *>(p.y) + (int64_t)t * p.ldy + n;
             if (vec && n + 4 <= p.n_rows) {
                 *reinterpret_cast<uint2 *>(dst) = make_uint2(o[0] | (uint32_t)o[1] << 16, o[2] | (uint32_t)o[3] << 16);
@@ -368,13 +392,13 @@ tile_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ C
     if (p.splits > 1) cluster_sync();   // nobody leaves while its tile is still being read
 }
 
-template <int BN>
-int launch_tile_bn(const CUtensorMap &x_map, const CUtensorMap &c_map, const TileParams &p, cudaStream_t st) {
+template <int BN, bool TWO>
+int launch_tile_bn(const CUtensorMap &x_map, const CUtensorMap &c_map, const CUtensorMap &up_map, const TileParams &p, cudaStream_t st) {
     static thread_local int configured_dev = -1;
     int dev = 0;
     cudaGetDevice(&dev);
     if (configured_dev != dev) {
-        int rc = check_cuda(cudaFuncSetAttribute(tile_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)TileSmem<BN>::TOTAL),
+        int rc = check_cuda(cudaFuncSetAttribute(tile_kernel<BN, TWO>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)TileSmem<BN>::TOTAL),
                             "cudaFuncSetAttribute(tile smem)");
         if (rc) return rc;
         configured_dev = dev;
@@ -387,14 +411,14 @@ int launch_tile_bn(const CUtensorMap &x_map, const CUtensorMap &c_map, const Til
     attr[1].val.clusterDim.y = (unsigned)p.splits;
     attr[1].val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)ceil_div_i64(p.n_rows, TL_BM), (unsigned)p.splits, 1);
+    cfg.gridDim = dim3((unsigned)ceil_div_i64(p.n_rows, TWO ? 64 : TL_BM), (unsigned)p.splits, 1);
     cfg.blockDim = dim3(TL_THREADS);
     cfg.dynamicSmemBytes = TileSmem<BN>::TOTAL;
     cfg.stream = st;
     const bool early = early_start();
     cfg.attrs = attr + (early ? 0 : 1);
     cfg.numAttrs = (early ? 1 : 0) + (p.splits > 1 ? 1 : 0);
-    return check_cuda(cudaLaunchKernelEx(&cfg, tile_kernel<BN>, x_map, c_map, p), "tile_kernel launch");
+    return check_cuda(cudaLaunchKernelEx(&cfg, tile_kernel<BN, TWO>, x_map, c_map, up_map, p), "tile_kernel launch");
 }
 
 // Clusters of s CTAs that are resident at once, two CTAs per SM.  A cluster lies within one GPC, so the sizes that do not
@@ -412,7 +436,7 @@ const int *resident_clusters(int sms) {
     int dev = 0;
     if (cudaGetDevice(&dev) == cudaSuccess && dev == cache.dev) return cache.resident;
     int raw[9];
-    bool ok = cudaFuncSetAttribute(tile_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)TileSmem<128>::TOTAL) == cudaSuccess;
+    bool ok = cudaFuncSetAttribute(tile_kernel<128, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)TileSmem<128>::TOTAL) == cudaSuccess;
     for (int s = 1; s <= 8 && ok; ++s) {
         cudaLaunchAttribute attr;
         attr.id = cudaLaunchAttributeClusterDimension;
@@ -425,7 +449,7 @@ const int *resident_clusters(int sms) {
         cfg.dynamicSmemBytes = TileSmem<128>::TOTAL;
         cfg.attrs = &attr;
         cfg.numAttrs = 1;
-        ok = cudaOccupancyMaxActiveClusters(&raw[s], tile_kernel<128>, &cfg) == cudaSuccess && raw[s] > 0;
+        ok = cudaOccupancyMaxActiveClusters(&raw[s], tile_kernel<128, false>, &cfg) == cudaSuccess && raw[s] > 0;
     }
     if (!ok) cudaGetLastError();   // (the launch that follows reports what is wrong)
     int *n = cache.resident;
@@ -491,14 +515,18 @@ TilePlan plan_tile(int64_t m, int64_t n_rows, int k_tiles, bool can_convert, boo
     return best;
 }
 
-int launch_tile(const CUtensorMap &x_map, const CUtensorMap &c_map, const TileParams &p, cudaStream_t st) {
+template <bool TWO>
+static int launch_tile_for(const CUtensorMap &x_map, const CUtensorMap &c_map, const CUtensorMap &up_map, const TileParams &p, cudaStream_t st) {
     switch (tile_tokens_for(p.m)) {
-        case 16: return launch_tile_bn<16>(x_map, c_map, p, st);
-        case 32: return launch_tile_bn<32>(x_map, c_map, p, st);
-        case 64: return launch_tile_bn<64>(x_map, c_map, p, st);
-        case 96: return launch_tile_bn<96>(x_map, c_map, p, st);
-        default: return launch_tile_bn<128>(x_map, c_map, p, st);
+        case 16: return launch_tile_bn<16, TWO>(x_map, c_map, up_map, p, st);
+        case 32: return launch_tile_bn<32, TWO>(x_map, c_map, up_map, p, st);
+        case 64: return launch_tile_bn<64, TWO>(x_map, c_map, up_map, p, st);
+        case 96: return launch_tile_bn<96, TWO>(x_map, c_map, up_map, p, st);
+        default: return launch_tile_bn<128, TWO>(x_map, c_map, up_map, p, st);
     }
+}
+int launch_tile(const CUtensorMap &x_map, const CUtensorMap &c_map, const CUtensorMap &up_map, const TileParams &p, cudaStream_t st) {
+    return p.two ? launch_tile_for<true>(x_map, c_map, up_map, p, st) : launch_tile_for<false>(x_map, c_map, up_map, p, st);
 }
 
 }  // namespace atlas

@@ -9,6 +9,12 @@
 
 namespace atlas {
 
+// Gate and up: act(x W^T + b) * (x V^T + c).  A tile of 128 rows is then 64 of either weight, its TMEM lanes 0 .. 63 the first
+// one's sums and 64 .. 127 the second one's, so that both sums of an output end up in one CTA.  Where the 64 rows of tile `t`
+// are among the weights' own tiles of 128:
+__host__ __device__ __forceinline__ int two_tile(int t) { return t >> 1; }
+__host__ __device__ __forceinline__ int two_row(int t) { return (t & 1) * 64; }
+
 struct TileParams {
     const uint16_t *scales_t;   // [row/128][block][row%128]
     const int32_t *chunk_ptr;   // [strip][k_tiles + 1]
@@ -28,6 +34,8 @@ struct TileParams {
     int splits;      // K slices = CTAs of a cluster
     int *error_flag;
     Epilogue epi;
+    AtlasWeight up;  // gate and up (`two`): the second weight
+    bool two;
 };
 
 // Rows of x the kernel takes, and tokens per tile for m of them.
@@ -47,7 +55,7 @@ inline double copy_us(int64_t m, int64_t k_tiles) { return 1. + 5.1e-5 * (double
 TilePlan plan_tile(int64_t m, int64_t n_rows, int k_tiles, bool can_convert, bool needs_copy, int sms);
 
 // x_map: boxes of 64 columns x tile_tokens_for(m) rows, 128-byte swizzle; c_map: the code tiles as 64-byte rows, boxes
-// of 128 rows, 64-byte swizzle.
-int launch_tile(const CUtensorMap &x_map, const CUtensorMap &c_map, const TileParams &p, cudaStream_t st);
+// of 128 rows, 64-byte swizzle.  With two weights both have boxes of 64 rows (up_map is read with two weights only).
+int launch_tile(const CUtensorMap &x_map, const CUtensorMap &c_map, const CUtensorMap &up_map, const TileParams &p, cudaStream_t st);
 
 }  // namespace atlas

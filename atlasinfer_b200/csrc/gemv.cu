@@ -52,6 +52,7 @@ struct GemvParams {
     int blocks_per_row; // n_cols / bs
     int bs_shift;       // log2(block size) when it is a power of two, else -1
     Epilogue epi;
+    AtlasWeight up;     // of gate and up: the second weight
 };
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -121,25 +122,37 @@ __device__ __forceinline__ void load_x16(const uint16_t *src, uint32_t (&xv)[8])
 // RS (strips per CTA; 2 only with FAST and one MMA tile): a step is one k-tile of both strips instead of two k-tiles of
 // one, so the activations of a step are loaded (and converted) once for two strips and a warp's set-up serves twice the
 // codes.  The bytes in flight stay the same.
-template <bool BF16, bool VEC, int MT, bool STAGE, bool FAST, int RS = 1>
+//
+// GATED (gate and up: act(x W^T + b) * (x V^T + c)): with RS 2 the two strips are one of either weight, and the CTA has both
+// sums of an output.  With RS 1 they are those of the two CTAs of a cluster; the second one leaves its sums in the first
+// one's shared memory.  No sum goes through global memory, and nothing is rounded before the product.
+template <bool BF16, bool VEC, int MT, bool STAGE, bool FAST, int RS = 1, bool GATED = false>
 __global__ void __launch_bounds__((MT == 1 ? GS_MAX_WARPS : GS_WARPS2) * 32, 2) gemv_strip_kernel(GemvParams p) {
     constexpr int U = MT == 1 ? GS_UNROLL : 2 * GS_UNROLL;
     constexpr int NT = RS * MT;   // 16 x 8 accumulator tiles of a warp
     static_assert(RS == 1 || (MT == 1 && FAST), "two strips: one token tile, whole chunks");
     __shared__ float4 part[NT][MT == 1 ? GS_MAX_WARPS : GS_WARPS2][32];
     extern __shared__ __align__(16) unsigned char xs_raw[];   // STAGE: [m][n_cols fp16 + 16 bytes of padding]
+    constexpr bool PAIR = GATED && RS == 1;   // clusters of two CTAs
+    __shared__ float up_sums[PAIR ? 128 * NT : 1];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (PAIR) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");   // (that the other CTA runs, is waited for at the end)
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nwarps = blockDim.x >> 5;
     const int g = lane >> 2, tig = lane & 3;
-    const int strip = blockIdx.x * RS;   // (an even one with RS 2: both strips lie in one 128-row tile)
+    const bool second = PAIR && (blockIdx.x & 1);   // this CTA serves the second weight
+    const int strip = PAIR ? blockIdx.x >> 1 : GATED ? blockIdx.x : blockIdx.x * RS;   // (with two strips of one weight an even one: both lie in one 128-row tile)
     // (a CTA has 16 warps unless K is short: the split of the chunks over them then needs no division)
     const int c0 = nwarps == 16 ? (p.n_chunks * warp) >> 4 : (nwarps == 8 ? (p.n_chunks * warp) >> 3 : (p.n_chunks * warp) / nwarps);
     const int c1 = nwarps == 16 ? (p.n_chunks * (warp + 1)) >> 4 : (nwarps == 8 ? (p.n_chunks * (warp + 1)) >> 3 : (p.n_chunks * (warp + 1)) / nwarps);
     const int kt0 = c0 * 4, kt1 = min(c1 * 4, p.k_tiles);
 
-    const uint8_t *wbase = p.tiles + ((size_t)(strip >> 3) * p.k_tiles * 8 + (strip & 7)) * 1024 + lane * 16;
-    const uint16_t *sbase = p.scales_t + (size_t)(strip >> 3) * p.blocks_per_row * 128 + (strip & 7) * 16 + g;
+    const size_t w_at = ((size_t)(strip >> 3) * p.k_tiles * 8 + (strip & 7)) * 1024 + lane * 16;
+    const size_t s_at = (size_t)(strip >> 3) * p.blocks_per_row * 128 + (strip & 7) * 16 + g;
+    const uint8_t *wbase = (second ? p.up.tiles : p.tiles) + w_at;
+    const uint16_t *sbase = (second ? (const uint16_t *)p.up.scales_tiled : p.scales_t) + s_at;
+    const uint8_t *wbase2 = p.up.tiles + w_at;   // (the other strip of two, of gate and up)
+    const uint16_t *sbase2 = (const uint16_t *)p.up.scales_tiled + s_at;
     // lanes whose batch row does not exist read row 0: their MMA columns are never stored
     const uint16_t *xg[MT], *xrow[MT];
 #pragma unroll
@@ -155,10 +168,11 @@ __global__ void __launch_bounds__((MT == 1 ? GS_MAX_WARPS : GS_WARPS2) * 32, 2) 
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if (RS == 2) {
-                const uint8_t *tp = wbase + (size_t)((uint32_t)kt << 13) + u * 1024;
+                const uint8_t *tp = GATED ? (u ? wbase2 : wbase) + (size_t)((uint32_t)kt << 13) : wbase + (size_t)((uint32_t)kt << 13) + u * 1024;
                 wa[u] = ldg_stream(tp);
                 wb[u] = ldg_stream(tp + 512);
-                const uint16_t *sp = sbase + (size_t)((uint32_t)(kt >> (p.bs_shift - 6)) << 7) + u * 16;
+                const uint16_t *sp = GATED ? (u ? sbase2 : sbase) + (size_t)((uint32_t)(kt >> (p.bs_shift - 6)) << 7)
+                                           : sbase + (size_t)((uint32_t)(kt >> (p.bs_shift - 6)) << 7) + u * 16;
                 sa[u] = __ldg(sp);
                 sb[u] = __ldg(sp + 8);
             } else if (FAST || kt + u < kt1) {
@@ -174,7 +188,8 @@ __global__ void __launch_bounds__((MT == 1 ? GS_MAX_WARPS : GS_WARPS2) * 32, 2) 
     };
     load_batch(kt0);
     // first group of outlier entries of the strip inside this warp's columns, and the bias
-    const int32_t *cptr = p.chunk_ptr + (size_t)strip * (p.k_tiles + 1);
+    // (strip r's; a strip of the second weight has that one's lists)
+    auto chunks = [&](int r) { return (second || (GATED && r) ? p.up.outlier_chunk_ptr : p.chunk_ptr + (GATED ? 0 : r * (p.k_tiles + 1))) + (size_t)strip * (p.k_tiles + 1); };
     int e_begin[RS], e_end[RS];
     // an empty slot of an outlier group: row 255 matches no lane; its column is one of this warp's own (with the staged
     // row a warp reads only what it has written itself)
@@ -182,7 +197,7 @@ __global__ void __launch_bounds__((MT == 1 ? GS_MAX_WARPS : GS_WARPS2) * 32, 2) 
 #pragma unroll
     for (int r = 0; r < RS; ++r) {
         e_begin[r] = e_end[r] = 0;
-        if (kt0 < kt1) { e_begin[r] = __ldg(cptr + r * (p.k_tiles + 1) + kt0); e_end[r] = __ldg(cptr + r * (p.k_tiles + 1) + kt1); }
+        if (kt0 < kt1) { e_begin[r] = __ldg(chunks(r) + kt0); e_end[r] = __ldg(chunks(r) + kt1); }
     }
     uint32_t pre_ent[4], pre_val[4];
     auto load_group = [&](int r, int e0) {
@@ -191,16 +206,21 @@ __global__ void __launch_bounds__((MT == 1 ? GS_MAX_WARPS : GS_WARPS2) * 32, 2) 
             const int e = e0 + 2 * tig + (q & 1) + (q >> 1) * 8;
             pre_ent[q] = no_entry;
             pre_val[q] = 0;
-            if (e < e_end[r]) { pre_ent[q] = __ldg(p.entries + e); pre_val[q] = __ldg(p.ovals + e); }
+            if (e < e_end[r]) {
+                const bool up = second || (GATED && r);
+                pre_ent[q] = __ldg((up ? p.up.outlier_entries : p.entries) + e);
+                pre_val[q] = __ldg((up ? (const uint16_t *)p.up.outlier_vals_sorted : p.ovals) + e);
+            }
         }
     };
     load_group(0, e_begin[0]);
     // (MMA tile, lane, component) this thread reduces at the end: 128 outputs per tile
     const int rT = tid >> 7, rL = (tid >> 2) & 31, rj = tid & 3;
     const int out_row = (rL >> 2) + (rj >> 1) * 8, out_m = (RS == 1 ? rT * 8 : 0) + (rL & 3) * 2 + (rj & 1);
-    const int out_n = (strip + (RS == 1 ? 0 : rT)) * 16 + out_row;
+    const int out_n = (strip + (RS == 1 || GATED ? 0 : rT)) * 16 + out_row;
+    const uint16_t *bias = second || (GATED && RS == 2 && rT) ? (const uint16_t *)p.up.bias : p.bias;
     float bias_v = 0.f;
-    if (tid < 128 * NT && p.bias && out_n < p.n_rows) bias_v = __half2float(__ushort_as_half(__ldg(p.bias + out_n)));
+    if (tid < 128 * NT && bias && out_n < p.n_rows) bias_v = __half2float(__ushort_as_half(__ldg(bias + out_n)));
 
     // ---- activations: only after the earlier kernels of the stream have completed ------------------
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -347,18 +367,37 @@ __global__ void __launch_bounds__((MT == 1 ? GS_MAX_WARPS : GS_WARPS2) * 32, 2) 
 
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) part[nt][warp][lane] = make_float4(acc[nt][0], acc[nt][1], acc[nt][2], acc[nt][3]);
-    const bool mine = tid < 128 * NT && out_m < p.m && out_n < p.n_rows;
+    // (of gate and up the first weight's threads, or CTA, write)
+    const bool mine = tid < 128 * (GATED ? MT : NT) && !second && out_m < p.m && out_n < p.n_rows;
     const float residual = mine ? residual_at(p.epi, out_m, out_n, BF16) : 0.f;   // (travels while the other warps arrive)
     __syncthreads();
-    if (tid < 128 * NT) {
-        float sum[1] = {bias_v};
+    float sum[1] = {bias_v};
+    if (tid < 128 * NT)
         for (int w = 0; w < nwarps; ++w) sum[0] += reinterpret_cast<const float *>(&part[rT][w][rL])[rj];
-        if (mine) {
-            activate(sum, p.epi.act);
-            const float s = scaled(p.epi, sum[0], residual);
-            if (BF16) reinterpret_cast<__nv_bfloat16 *>(p.y)[(size_t)out_m * p.ldy + out_n] = __float2bfloat16_rn(s);
-            else reinterpret_cast<__half *>(p.y)[(size_t)out_m * p.ldy + out_n] = __float2half_rn(s);
+    float other = 1.f;
+    if (GATED && RS == 2) {
+        float *to = reinterpret_cast<float *>(&part[1][0][0]);   // (each of these threads has read this place of its own, if any has)
+        __syncthreads();
+        if (tid >= 128 && tid < 256) to[tid - 128] = sum[0];
+        __syncthreads();
+        if (tid < 128) other = to[tid];
+    }
+    if (PAIR) {
+        __syncwarp();
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        if (second && tid < 128 * NT) {
+            uint32_t at = (uint32_t)__cvta_generic_to_shared(&up_sums[tid]);
+            asm volatile("mapa.shared::cluster.u32 %0, %0, 0;\n\tst.shared::cluster.f32 [%0], %1;" : "+r"(at) : "f"(sum[0]) : "memory");
         }
+        __syncwarp();
+        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        if (mine) other = up_sums[tid];
+    }
+    if (mine) {
+        activate(sum, p.epi.act);
+        const float s = scaled(p.epi, GATED ? sum[0] * other : sum[0], residual);
+        if (BF16) reinterpret_cast<__nv_bfloat16 *>(p.y)[(size_t)out_m * p.ldy + out_n] = __float2bfloat16_rn(s);
+        else reinterpret_cast<__half *>(p.y)[(size_t)out_m * p.ldy + out_n] = __float2half_rn(s);
     }
 }
 
@@ -386,31 +425,41 @@ bool strip_pairs_pay(int64_t pairs, int n_chunks, bool bf16) {
     return n_chunks >= 12 && n_chunks <= (bf16 ? 32 : 24) && (percent >= 85 || (waves >= 3 && percent >= 75));
 }
 
-template <int MT>
+template <int MT, bool GATED>
 int launch_gemv_strip(const GemvParams &p, bool vec, cudaStream_t st) {
     const int max_warps = MT == 1 ? GS_MAX_WARPS : GS_WARPS2;
     int nwarps = p.n_chunks < max_warps ? p.n_chunks : max_warps;
     const bool fast = vec && (p.k_tiles & 3) == 0 && p.bs_shift >= 6;   // whole chunks, blocks of whole tiles
+    const bool bf16 = p.dtype == ATLAS_DTYPE_BF16;
     const int64_t strips = ceil_div_i64(p.n_rows, 16);
-    const bool two = MT == 1 && fast && strip_pairs_pay((strips + 1) / 2, p.n_chunks, p.dtype == ATLAS_DTYPE_BF16);
+    const bool two = MT == 1 && fast && strip_pairs_pay(GATED ? strips : (strips + 1) / 2, p.n_chunks, bf16);
     if (nwarps < 4 * MT * (two ? 2 : 1)) nwarps = 4 * MT * (two ? 2 : 1);  // the reduction needs 128 threads per MMA tile
     // one or two rows of bf16 activations are converted once per CTA into shared memory (measured at 1 / 2 / 4 / 8
     // rows: 3.7 / 3.5 / 3.1 / 2.6 TB/s staged against 3.4 / 3.3 / 3.3 / 3.1 converted per step)
     const size_t stage_bytes = (size_t)p.m * ((size_t)p.n_cols * 2 + 16);
-    const bool stage = MT == 1 && p.dtype == ATLAS_DTYPE_BF16 && vec && p.m <= 2 && stage_bytes <= (size_t)GS_STAGE_MAX_BYTES;
+    const bool stage = MT == 1 && bf16 && vec && p.m <= 2 && stage_bytes <= (size_t)GS_STAGE_MAX_BYTES;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(two ? (strips + 1) / 2 : strips), 1, 1);
+    cfg.gridDim = dim3((unsigned)(two ? (GATED ? strips : (strips + 1) / 2) : (GATED ? 2 * strips : strips)), 1, 1);
     cfg.blockDim = dim3((unsigned)(nwarps * 32), 1, 1);
     cfg.dynamicSmemBytes = stage ? stage_bytes : 0;
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchAttribute attr[2];
+    int attrs = 0;
+    if (early_start()) {
+        attr[attrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[attrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (GATED && !two) {
+        attr[attrs].id = cudaLaunchAttributeClusterDimension;
+        attr[attrs].val.clusterDim.x = 2, attr[attrs].val.clusterDim.y = 1, attr[attrs].val.clusterDim.z = 1;
+        ++attrs;
+    }
     cfg.attrs = attr;
-    cfg.numAttrs = early_start() ? 1 : 0;
+    cfg.numAttrs = attrs;
+    const char *what = "gemv_strip_kernel launch";
     if (stage) {
-        auto kern = two ? gemv_strip_kernel<true, true, 1, true, true, 2>
-                        : (fast ? gemv_strip_kernel<true, true, 1, true, true> : gemv_strip_kernel<true, true, 1, true, false>);
+        auto kern = two ? gemv_strip_kernel<true, true, 1, true, true, 2, GATED>
+                        : (fast ? gemv_strip_kernel<true, true, 1, true, true, 1, GATED> : gemv_strip_kernel<true, true, 1, true, false, 1, GATED>);
         static thread_local int configured_dev[3] = {-1, -1, -1};   // more than the default dynamic shared memory: opt in once
         int dev = 0;
         cudaGetDevice(&dev);
@@ -420,26 +469,26 @@ int launch_gemv_strip(const GemvParams &p, bool vec, cudaStream_t st) {
             if (rc) return rc;
             configured_dev[two ? 2 : (int)fast] = dev;
         }
-        return check_cuda(cudaLaunchKernelEx(&cfg, kern, p), "gemv_strip_kernel launch");
+        return check_cuda(cudaLaunchKernelEx(&cfg, kern, p), what);
     }
     if (two) {
-        auto kern = p.dtype == ATLAS_DTYPE_BF16 ? gemv_strip_kernel<true, true, 1, false, true, 2> : gemv_strip_kernel<false, true, 1, false, true, 2>;
-        return check_cuda(cudaLaunchKernelEx(&cfg, kern, p), "gemv_strip_kernel launch");
+        auto kern = bf16 ? gemv_strip_kernel<true, true, 1, false, true, 2, GATED> : gemv_strip_kernel<false, true, 1, false, true, 2, GATED>;
+        return check_cuda(cudaLaunchKernelEx(&cfg, kern, p), what);
     }
     if (fast) {
-        auto kern = p.dtype == ATLAS_DTYPE_BF16 ? gemv_strip_kernel<true, true, MT, false, true> : gemv_strip_kernel<false, true, MT, false, true>;
-        return check_cuda(cudaLaunchKernelEx(&cfg, kern, p), "gemv_strip_kernel launch");
+        auto kern = bf16 ? gemv_strip_kernel<true, true, MT, false, true, 1, GATED> : gemv_strip_kernel<false, true, MT, false, true, 1, GATED>;
+        return check_cuda(cudaLaunchKernelEx(&cfg, kern, p), what);
     }
-    auto kern = p.dtype == ATLAS_DTYPE_BF16 ? (vec ? gemv_strip_kernel<true, true, MT, false, false> : gemv_strip_kernel<true, false, MT, false, false>)
-                                            : (vec ? gemv_strip_kernel<false, true, MT, false, false> : gemv_strip_kernel<false, false, MT, false, false>);
-    return check_cuda(cudaLaunchKernelEx(&cfg, kern, p), "gemv_strip_kernel launch");
+    auto kern = bf16 ? (vec ? gemv_strip_kernel<true, true, MT, false, false, 1, GATED> : gemv_strip_kernel<true, false, MT, false, false, 1, GATED>)
+                     : (vec ? gemv_strip_kernel<false, true, MT, false, false, 1, GATED> : gemv_strip_kernel<false, false, MT, false, false, 1, GATED>);
+    return check_cuda(cudaLaunchKernelEx(&cfg, kern, p), what);
 }
 
 }  // namespace
 
 int qlinear_gemv(const void *x, int dtype, int64_t m, int64_t ldx, const uint8_t *tiles, const void *scales_tiled,
                  const int32_t *outlier_chunk_ptr, const uint32_t *outlier_entries, const void *outlier_vals_sorted,
-                 int64_t n_rows, int64_t n_cols, int block_size, const void *bias, void *y, int64_t ldy, cudaStream_t st, const Epilogue &epi) {
+                 int64_t n_rows, int64_t n_cols, int block_size, const void *bias, void *y, int64_t ldy, cudaStream_t st, const Epilogue &epi, const AtlasWeight *up) {
     ATLAS_RETURN_IF(!x || !tiles || !scales_tiled || !outlier_chunk_ptr || !y, ATLAS_ERR_BAD_ARGUMENT,
                     "atlas_qlinear_gemv: null buffer");
     ATLAS_RETURN_IF(m < 0 || n_rows <= 0 || n_cols <= 0 || ldx < n_cols || ldy < n_rows, ATLAS_ERR_BAD_ARGUMENT,
@@ -459,6 +508,7 @@ int qlinear_gemv(const void *x, int dtype, int64_t m, int64_t ldx, const uint8_t
     GemvParams p;
     p.dtype = dtype;
     p.epi = epi;
+    p.up = up ? *up : AtlasWeight{};
     p.ldx = ldx;
     p.tiles = tiles;
     p.scales_t = (const uint16_t *)scales_tiled;
@@ -480,7 +530,8 @@ int qlinear_gemv(const void *x, int dtype, int64_t m, int64_t ldx, const uint8_t
         p.x = (const char *)x + (size_t)m0 * ldx * 2;
         p.y = (char *)y + (size_t)m0 * ldy * 2;
         if (epi.residual) p.epi.residual = epi.residual + m0 * epi.ldr;
-        rc = p.m <= 8 ? launch_gemv_strip<1>(p, vec, st) : launch_gemv_strip<2>(p, vec, st);
+        rc = up ? (p.m <= 8 ? launch_gemv_strip<1, true>(p, vec, st) : launch_gemv_strip<2, true>(p, vec, st))
+                : (p.m <= 8 ? launch_gemv_strip<1, false>(p, vec, st) : launch_gemv_strip<2, false>(p, vec, st));
         if (rc) return rc;
     }
     return ATLAS_OK;
@@ -496,5 +547,5 @@ extern "C" int atlas_qlinear_gemv(const void *x, int dtype, int64_t m, int64_t l
     (void)status;   // no bounded wait in this kernel: nothing to report
     atlas::clear_error();
     return atlas::qlinear_gemv(x, dtype, m, ldx, tiles, scales_tiled, outlier_chunk_ptr, outlier_entries, outlier_vals_sorted, n_rows, n_cols,
-                               block_size, bias, y, ldy, (cudaStream_t)stream, atlas::Epilogue());
+                               block_size, bias, y, ldy, (cudaStream_t)stream, atlas::Epilogue(), nullptr);
 }
