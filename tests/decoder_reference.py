@@ -99,10 +99,7 @@ def token_logprobs(logits, tokens, top=0, temperature=1.0):
     given = logp.gather(1, tokens.clamp(0, l.shape[1] - 1)[:, None])[:, 0]
     given[tokens < 0] = 0.0
     given[tokens >= l.shape[1]] = math.nan
-    # largest first, NaN above all, equal ones by their index
-    order = torch.where(z.isnan(), torch.full_like(z, math.inf), z)
-    order = torch.stack([torch.tensor(sorted(range(l.shape[1]), key=lambda i: (not bool(z[r, i].isnan()), -float(order[r, i]), i))[:top], dtype=torch.long)
-                         for r in range(l.shape[0])]) if top else torch.empty(l.shape[0], 0, dtype=torch.long)
+    order = l.double().sort(dim=-1, descending=True, stable=True).indices[:, :top]   # (NaN above all, equal ones by their index)
     return given, entropy, order, logp.gather(1, order)
 
 

@@ -37,7 +37,7 @@ def check(logits, tokens, top=0, temperature=1.0):
 
 
 @pytest.mark.parametrize("dtype", (F16, BF16, F32))
-@pytest.mark.parametrize("rows,vocab", [(1, 1), (2, 5), (3, 31), (1, 1000), (5, 4097), (2, 50272), (1, 131073), (40, 777), (200, 64), (3, 8192), (2, 32001)])
+@pytest.mark.parametrize("rows,vocab", [(1, 1), (2, 5), (3, 31), (1, 1000), (5, 4097), (2, 50272), (1, 131073), (40, 777), (200, 64), (3, 8192), (2, 32001), (64, 33001), (1, 24), (9, 20007)])
 def test_shapes(cuda_device, rows, vocab, dtype):
     logits = logits_of(rows, vocab, dtype, rows, cuda_device)
     tokens = torch.randint(0, vocab, (rows,), generator=torch.Generator().manual_seed(1)).to(torch.int32 if rows % 2 else torch.int64).to(cuda_device)
@@ -52,14 +52,15 @@ def test_every_top(cuda_device):
 
 
 @pytest.mark.parametrize("dtype", (F16, BF16, F32))
-def test_ties_and_orders(cuda_device, dtype):
+@pytest.mark.parametrize("v", (300, 9001, 60001))
+def test_ties_and_orders(cuda_device, dtype, v):
     """Rows of one number, of few, ascending, descending, in the period of the threads' pieces: equal ones by their index."""
-    v = 9001
     ramp = torch.arange(v, dtype=torch.float32)
     rows = [torch.zeros(v), torch.full((v,), -7.0), ramp / v * 8, -ramp / v * 8, ramp % 3, (ramp / 8).floor() % 2, (ramp % 4096 < 32) * 5.0, (ramp % 2048 < 8) * 5.0 - (ramp > 6000) * 1.0,
-            torch.where(ramp % 2 == 0, 0.0, -0.0), (ramp % 1024 == 77) * 3.0, (ramp % 4096) / 512]
+            torch.where(ramp % 2 == 0, 0.0, -0.0), (ramp % 1024 == 77) * 3.0, (ramp % 4096) / 512, (ramp >= v - 40) * 2.0 + (ramp == 3) * 2.0, (ramp % 384 < 24) * (ramp % 8) * 1.0,
+            torch.where(ramp % 7 == 0, 1.0, -math.inf), torch.where(ramp > v - 30, 1.0, -math.inf)]
     logits = torch.stack(rows).to(dtype).to(cuda_device)
-    tokens = torch.arange(len(rows), device=cuda_device) * 100
+    tokens = torch.arange(len(rows), device=cuda_device) * 17
     for top in (1, 20, 32):
         check(logits, tokens, top)
 
