@@ -26,7 +26,8 @@ def check(got, stream, want, dtype):
     assert_rounded(got, y, slack_y, "normed: ")
 
 
-SHAPES = [(1, 1), (3, 7), (1, 4096), (5, 64), (2, 33), (17, 1000), (4, 8192), (2, 8200), (1, 16392), (2, 20001), (1, 32768), (700, 96), (3, 2049), (300, 2048)]
+SHAPES = [(1, 1), (3, 7), (1, 4096), (5, 64), (2, 33), (17, 1000), (4, 8192), (2, 8200), (1, 16392), (2, 20001), (1, 32768), (700, 96), (3, 2049), (300, 2048), (2, 32767), (3, 32761), (1200, 33),
+          (1300, 255), (1201, 257), (1190, 1013), (400, 4091), (300, 8181), (350, 10001), (310, 8200), (297, 1024)]
 
 
 @pytest.mark.parametrize("dtype", (F16, BF16))
@@ -45,7 +46,8 @@ def test_plain_norm(cuda_device, tokens, hidden, dtype):
 @pytest.mark.parametrize("stream_type", ("same", "fp32"))
 @pytest.mark.parametrize("tokens,hidden,gate,post,centered", [
     (1, 4096, None, False, False), (3, 515, "rows", True, True), (33, 1024, "channels", True, False), (2, 16384, "rows", False, True), (130, 264, "channels", False, False),
-    (1, 1, "rows", True, False), (2, 32768, "channels", True, True), (5, 5001, None, True, False)])
+    (1, 1, "rows", True, False), (2, 32768, "channels", True, True), (5, 5001, None, True, False),
+    (350, 1003, "rows", True, True), (301, 1003, "channels", True, False), (1300, 200, "rows", False, True), (1250, 999, "rows", True, False), (320, 9000, "rows", True, False)])
 def test_with_everything(cuda_device, tokens, hidden, gate, post, centered, stream_type, dtype):
     x = randn((tokens, hidden), dtype, 0, cuda_device)
     residual = randn((tokens, hidden), dtype if stream_type == "same" else F32, 1, cuda_device, 4)
@@ -69,7 +71,7 @@ def test_shapes_and_strides(cuda_device):
     """Leading dimensions, views of wider rows at odd addresses, transposed rows, rows in reverse order: the numbers count."""
     wide = randn((6, 4, 200), BF16, 0, cuda_device)
     w = randn((96,), BF16, 1, cuda_device)
-    for x in (wide[..., :96], wide[..., 1:97], wide[:, 1, 8:104], wide[::2, :, 100:196], wide.transpose(0, 1)[..., :96], wide[:, :, 0:192:2], wide[:1, :1, 3:99].expand(5, 2, 96)):
+    for x in (wide[..., :96], wide[..., 1:97], wide.reshape(-1)[1:1 + 24 * 96].view(6, 4, 96), wide[:, 1, 8:104], wide[::2, :, 100:196], wide.transpose(0, 1)[..., :96], wide[:, :, 0:192:2], wide[:1, :1, 3:99].expand(5, 2, 96)):
         res = torch.flip(x, [0]).float()
         y, s = ab.residual_norm(x, res, w)
         want = D.residual_norm(x.reshape(-1, 96), res.reshape(-1, 96), w)
