@@ -20,12 +20,20 @@ int check(const AtlasFusedLinear *p) {
     return ATLAS_OK;
 }
 
+// Gate and up with 9 to 16 rows: two token tiles of strips leave no room for both weights' strips in one CTA, so pairs of CTAs
+// are only better than the tcgen05 kernel while all of them run at once (2 x 1000 x 1024 4.3 us, 5.5; 2 x 2048 x 1024 4.7, 7.7;
+// 2 x 5504 x 2048 17.7, 12.0; 2 x 11008 x 4096 44.4, 36.4).  Up to 8 rows strips are ahead everywhere (2 x 11008 x 4096 22.7 to
+// 26.2, 34.8 to 35.6; 2 x 8192 x 2048 12.2 to 13.6, 13.7 to 14.0).
+bool by_strips(const AtlasFusedLinear *p) {
+    return p->m <= STRIP_MAX_ROWS && (!p->up.tiles || p->m <= 8 || 2 * ceil_div_i64(p->n_rows, 16) <= 2 * 148);
+}
+
 }  // namespace
 }  // namespace atlas
 
 extern "C" size_t atlas_fused_linear_workspace_bytes(const AtlasFusedLinear *p) {
     using namespace atlas;
-    if (check(p) != ATLAS_OK || p->m <= STRIP_MAX_ROWS) return 0;
+    if (check(p) != ATLAS_OK || by_strips(p)) return 0;
     return qlinear_gemm_workspace_bytes(p->m, p->n_rows, p->n_cols, p->up.tiles != nullptr);
 }
 
@@ -37,7 +45,7 @@ extern "C" int atlas_fused_linear(const AtlasFusedLinear *p, void *stream) {
     if (p->m == 0) return ATLAS_OK;
     const Epilogue epi = make_epilogue(p->residual, p->ldr, p->scale, p->activation);
     const AtlasWeight &w = p->weight, *up = p->up.tiles ? &p->up : nullptr;
-    if (p->m <= STRIP_MAX_ROWS)
+    if (by_strips(p))
         return qlinear_gemv(p->x, p->dtype, p->m, p->ldx, w.tiles, w.scales_tiled, w.outlier_chunk_ptr, w.outlier_entries, w.outlier_vals_sorted, p->n_rows,
                             p->n_cols, p->block_size, w.bias, p->y, p->ldy, (cudaStream_t)stream, epi, up);
     return qlinear_gemm(p->x, p->dtype, p->m, p->ldx, w.tiles, w.scales_tiled, w.outlier_chunk_ptr, w.outlier_entries, w.outlier_vals_sorted, p->n_rows, p->n_cols,

@@ -94,9 +94,12 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr, uint32_t rank) {
     return v;
 }
 
-template <int BN, bool TWO>
+// KIND: nothing but a linear, one with something behind it, or two weights.
+enum Kind { PLAIN, FOLLOWED, GATE_AND_UP };
+template <int BN, int KIND>
 __global__ void __launch_bounds__(TL_THREADS, 2)
 tile_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap c_map, const __grid_constant__ CUtensorMap up_map, TileParams p) {
+    constexpr bool TWO = KIND == GATE_AND_UP;
     using SM = TileSmem<BN>;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     constexpr int CS = SM::CS, XS = SM::XS;
@@ -366,16 +369,16 @@ tile_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ C
                     if (bias && n + e < p.n_rows) f[e] += __half2float(__ushort_as_half(__ldg(bias + n + e)));
             };
             float f[4], res[4];
-            residual_at(p.epi, t, n, p.n_rows - n, p.out_bf16, res);
+            if (KIND != PLAIN) residual_at(p.epi, t, n, p.n_rows - n, p.out_bf16, res);
             sums(idx % PIECES * 4, p.bias, f);
-            activate(f, p.epi.act);
+            if (KIND != PLAIN) activate(f, p.epi.act);
             if (TWO) {
                 float u[4];
                 sums(64 + idx % PIECES * 4, (const uint16_t *)p.up.bias, u);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) f[e] *= u[e];
             }
-            scale_and_add(p.epi, f, res);
+            if (KIND != PLAIN) scale_and_add(p.epi, f, res);
             uint16_t o[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[e] = narrow(f[e], p.out_bf16);
@@ -392,13 +395,13 @@ tile_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ C
     if (p.splits > 1) cluster_sync();   // nobody leaves while its tile is still being read
 }
 
-template <int BN, bool TWO>
+template <int BN, int KIND>
 int launch_tile_bn(const CUtensorMap &x_map, const CUtensorMap &c_map, const CUtensorMap &up_map, const TileParams &p, cudaStream_t st) {
     static thread_local int configured_dev = -1;
     int dev = 0;
     cudaGetDevice(&dev);
     if (configured_dev != dev) {
-        int rc = check_cuda(cudaFuncSetAttribute(tile_kernel<BN, TWO>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)TileSmem<BN>::TOTAL),
+        int rc = check_cuda(cudaFuncSetAttribute(tile_kernel<BN, KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)TileSmem<BN>::TOTAL),
                             "cudaFuncSetAttribute(tile smem)");
         if (rc) return rc;
         configured_dev = dev;
@@ -411,14 +414,14 @@ int launch_tile_bn(const CUtensorMap &x_map, const CUtensorMap &c_map, const CUt
     attr[1].val.clusterDim.y = (unsigned)p.splits;
     attr[1].val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)ceil_div_i64(p.n_rows, TWO ? 64 : TL_BM), (unsigned)p.splits, 1);
+    cfg.gridDim = dim3((unsigned)ceil_div_i64(p.n_rows, KIND == GATE_AND_UP ? 64 : TL_BM), (unsigned)p.splits, 1);
     cfg.blockDim = dim3(TL_THREADS);
     cfg.dynamicSmemBytes = TileSmem<BN>::TOTAL;
     cfg.stream = st;
     const bool early = early_start();
     cfg.attrs = attr + (early ? 0 : 1);
     cfg.numAttrs = (early ? 1 : 0) + (p.splits > 1 ? 1 : 0);
-    return check_cuda(cudaLaunchKernelEx(&cfg, tile_kernel<BN, TWO>, x_map, c_map, up_map, p), "tile_kernel launch");
+    return check_cuda(cudaLaunchKernelEx(&cfg, tile_kernel<BN, KIND>, x_map, c_map, up_map, p), "tile_kernel launch");
 }
 
 // Clusters of s CTAs that are resident at once, two CTAs per SM.  A cluster lies within one GPC, so the sizes that do not
@@ -436,7 +439,7 @@ const int *resident_clusters(int sms) {
     int dev = 0;
     if (cudaGetDevice(&dev) == cudaSuccess && dev == cache.dev) return cache.resident;
     int raw[9];
-    bool ok = cudaFuncSetAttribute(tile_kernel<128, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)TileSmem<128>::TOTAL) == cudaSuccess;
+    bool ok = cudaFuncSetAttribute(tile_kernel<128, PLAIN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)TileSmem<128>::TOTAL) == cudaSuccess;
     for (int s = 1; s <= 8 && ok; ++s) {
         cudaLaunchAttribute attr;
         attr.id = cudaLaunchAttributeClusterDimension;
@@ -449,7 +452,7 @@ const int *resident_clusters(int sms) {
         cfg.dynamicSmemBytes = TileSmem<128>::TOTAL;
         cfg.attrs = &attr;
         cfg.numAttrs = 1;
-        ok = cudaOccupancyMaxActiveClusters(&raw[s], tile_kernel<128, false>, &cfg) == cudaSuccess && raw[s] > 0;
+        ok = cudaOccupancyMaxActiveClusters(&raw[s], tile_kernel<128, PLAIN>, &cfg) == cudaSuccess && raw[s] > 0;
     }
     if (!ok) cudaGetLastError();   // (the launch that follows reports what is wrong)
     int *n = cache.resident;
@@ -515,18 +518,19 @@ TilePlan plan_tile(int64_t m, int64_t n_rows, int k_tiles, bool can_convert, boo
     return best;
 }
 
-template <bool TWO>
+template <int KIND>
 static int launch_tile_for(const CUtensorMap &x_map, const CUtensorMap &c_map, const CUtensorMap &up_map, const TileParams &p, cudaStream_t st) {
     switch (tile_tokens_for(p.m)) {
-        case 16: return launch_tile_bn<16, TWO>(x_map, c_map, up_map, p, st);
-        case 32: return launch_tile_bn<32, TWO>(x_map, c_map, up_map, p, st);
-        case 64: return launch_tile_bn<64, TWO>(x_map, c_map, up_map, p, st);
-        case 96: return launch_tile_bn<96, TWO>(x_map, c_map, up_map, p, st);
-        default: return launch_tile_bn<128, TWO>(x_map, c_map, up_map, p, st);
+        case 16: return launch_tile_bn<16, KIND>(x_map, c_map, up_map, p, st);
+        case 32: return launch_tile_bn<32, KIND>(x_map, c_map, up_map, p, st);
+        case 64: return launch_tile_bn<64, KIND>(x_map, c_map, up_map, p, st);
+        case 96: return launch_tile_bn<96, KIND>(x_map, c_map, up_map, p, st);
+        default: return launch_tile_bn<128, KIND>(x_map, c_map, up_map, p, st);
     }
 }
 int launch_tile(const CUtensorMap &x_map, const CUtensorMap &c_map, const CUtensorMap &up_map, const TileParams &p, cudaStream_t st) {
-    return p.two ? launch_tile_for<true>(x_map, c_map, up_map, p, st) : launch_tile_for<false>(x_map, c_map, up_map, p, st);
+    return p.two ? launch_tile_for<GATE_AND_UP>(x_map, c_map, up_map, p, st)
+           : is_plain(p.epi) ? launch_tile_for<PLAIN>(x_map, c_map, up_map, p, st) : launch_tile_for<FOLLOWED>(x_map, c_map, up_map, p, st);
 }
 
 }  // namespace atlas

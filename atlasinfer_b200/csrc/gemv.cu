@@ -25,6 +25,8 @@
 // find most of the weight in L2.
 #include <cuda_bf16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "linear.cuh"
 
@@ -51,9 +53,17 @@ struct GemvParams {
     int n_chunks;       // ceil(n_cols / 256)
     int blocks_per_row; // n_cols / bs
     int bs_shift;       // log2(block size) when it is a power of two, else -1
-    Epilogue epi;
-    AtlasWeight up;     // of gate and up: the second weight
 };
+
+// What a launch does behind the products.  A linear and nothing else keeps its own code and arguments: with the others' in it,
+// registers spill and it takes 3 to 5 % longer.
+enum Kind { PLAIN, FOLLOWED, GATE_AND_UP };
+struct After {
+    Epilogue epi;
+    AtlasWeight up;                      // of gate and up: the second weight,
+    int64_t tiles_apart, scales_apart;   // and how far its tiles and scales are from the first one's (elements)
+};
+struct Nothing {};
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                         uint32_t b0, uint32_t b1) {
@@ -126,14 +136,15 @@ __device__ __forceinline__ void load_x16(const uint16_t *src, uint32_t (&xv)[8])
 // GATED (gate and up: act(x W^T + b) * (x V^T + c)): with RS 2 the two strips are one of either weight, and the CTA has both
 // sums of an output.  With RS 1 they are those of the two CTAs of a cluster; the second one leaves its sums in the first
 // one's shared memory.  No sum goes through global memory, and nothing is rounded before the product.
-template <bool BF16, bool VEC, int MT, bool STAGE, bool FAST, int RS = 1, bool GATED = false>
-__global__ void __launch_bounds__((MT == 1 ? GS_MAX_WARPS : GS_WARPS2) * 32, 2) gemv_strip_kernel(GemvParams p) {
+template <bool BF16, bool VEC, int MT, bool STAGE, bool FAST, int RS = 1, int KIND = PLAIN>
+__global__ void __launch_bounds__((MT == 1 ? GS_MAX_WARPS : GS_WARPS2) * 32, 2) gemv_strip_kernel(GemvParams p, std::conditional_t<KIND == PLAIN, Nothing, After> after) {
+    constexpr bool GATED = KIND == GATE_AND_UP;
     constexpr int U = MT == 1 ? GS_UNROLL : 2 * GS_UNROLL;
     constexpr int NT = RS * MT;   // 16 x 8 accumulator tiles of a warp
     static_assert(RS == 1 || (MT == 1 && FAST), "two strips: one token tile, whole chunks");
     __shared__ float4 part[NT][MT == 1 ? GS_MAX_WARPS : GS_WARPS2][32];
     extern __shared__ __align__(16) unsigned char xs_raw[];   // STAGE: [m][n_cols fp16 + 16 bytes of padding]
-    constexpr bool PAIR = GATED && RS == 1;   // clusters of two CTAs
+    constexpr bool PAIR = GATED && RS == 1, BOTH = GATED && RS == 2;   // clusters of two CTAs; both strips in one
     __shared__ float up_sums[PAIR ? 128 * NT : 1];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (PAIR) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");   // (that the other CTA runs, is waited for at the end)
@@ -147,12 +158,14 @@ __global__ void __launch_bounds__((MT == 1 ? GS_MAX_WARPS : GS_WARPS2) * 32, 2) 
     const int c1 = nwarps == 16 ? (p.n_chunks * (warp + 1)) >> 4 : (nwarps == 8 ? (p.n_chunks * (warp + 1)) >> 3 : (p.n_chunks * (warp + 1)) / nwarps);
     const int kt0 = c0 * 4, kt1 = min(c1 * 4, p.k_tiles);
 
-    const size_t w_at = ((size_t)(strip >> 3) * p.k_tiles * 8 + (strip & 7)) * 1024 + lane * 16;
-    const size_t s_at = (size_t)(strip >> 3) * p.blocks_per_row * 128 + (strip & 7) * 16 + g;
-    const uint8_t *wbase = (second ? p.up.tiles : p.tiles) + w_at;
-    const uint16_t *sbase = (second ? (const uint16_t *)p.up.scales_tiled : p.scales_t) + s_at;
-    const uint8_t *wbase2 = p.up.tiles + w_at;   // (the other strip of two, of gate and up)
-    const uint16_t *sbase2 = (const uint16_t *)p.up.scales_tiled + s_at;
+    const uint8_t *tiles = p.tiles;
+    const uint16_t *scales = p.scales_t;
+    const int32_t *chunk_ptr = p.chunk_ptr;
+    if constexpr (PAIR) {
+        if (second) tiles = after.up.tiles, scales = (const uint16_t *)after.up.scales_tiled, chunk_ptr = after.up.outlier_chunk_ptr;
+    }
+    const uint8_t *wbase = tiles + ((size_t)(strip >> 3) * p.k_tiles * 8 + (strip & 7)) * 1024 + lane * 16;
+    const uint16_t *sbase = scales + (size_t)(strip >> 3) * p.blocks_per_row * 128 + (strip & 7) * 16 + g;
     // lanes whose batch row does not exist read row 0: their MMA columns are never stored
     const uint16_t *xg[MT], *xrow[MT];
 #pragma unroll
@@ -168,11 +181,13 @@ __global__ void __launch_bounds__((MT == 1 ? GS_MAX_WARPS : GS_WARPS2) * 32, 2) 
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if (RS == 2) {
-                const uint8_t *tp = GATED ? (u ? wbase2 : wbase) + (size_t)((uint32_t)kt << 13) : wbase + (size_t)((uint32_t)kt << 13) + u * 1024;
+                const uint8_t *tp = wbase + (size_t)((uint32_t)kt << 13) + u * 1024;
+                // (of gate and up the other strip is as far away as the weights are: one base, so that fewer registers spill)
+                if constexpr (BOTH) tp = wbase + (size_t)((uint32_t)kt << 13) + u * after.tiles_apart;
                 wa[u] = ldg_stream(tp);
                 wb[u] = ldg_stream(tp + 512);
-                const uint16_t *sp = GATED ? (u ? sbase2 : sbase) + (size_t)((uint32_t)(kt >> (p.bs_shift - 6)) << 7)
-                                           : sbase + (size_t)((uint32_t)(kt >> (p.bs_shift - 6)) << 7) + u * 16;
+                const uint16_t *sp = sbase + (size_t)((uint32_t)(kt >> (p.bs_shift - 6)) << 7) + u * 16;
+                if constexpr (BOTH) sp = sbase + (size_t)((uint32_t)(kt >> (p.bs_shift - 6)) << 7) + u * after.scales_apart;
                 sa[u] = __ldg(sp);
                 sb[u] = __ldg(sp + 8);
             } else if (FAST || kt + u < kt1) {
@@ -188,16 +203,20 @@ __global__ void __launch_bounds__((MT == 1 ? GS_MAX_WARPS : GS_WARPS2) * 32, 2) 
     };
     load_batch(kt0);
     // first group of outlier entries of the strip inside this warp's columns, and the bias
-    // (strip r's; a strip of the second weight has that one's lists)
-    auto chunks = [&](int r) { return (second || (GATED && r) ? p.up.outlier_chunk_ptr : p.chunk_ptr + (GATED ? 0 : r * (p.k_tiles + 1))) + (size_t)strip * (p.k_tiles + 1); };
+    const int32_t *cptr = chunk_ptr + (size_t)strip * (p.k_tiles + 1);
     int e_begin[RS], e_end[RS];
     // an empty slot of an outlier group: row 255 matches no lane; its column is one of this warp's own (with the staged
     // row a warp reads only what it has written itself)
     const uint32_t no_entry = 0xff000000u | (uint32_t)(kt0 * 64);
 #pragma unroll
-    for (int r = 0; r < RS; ++r) {
+    for (int r = 0; r < (BOTH ? 1 : RS); ++r) {
         e_begin[r] = e_end[r] = 0;
-        if (kt0 < kt1) { e_begin[r] = __ldg(chunks(r) + kt0); e_end[r] = __ldg(chunks(r) + kt1); }
+        if (kt0 < kt1) { e_begin[r] = __ldg(cptr + r * (p.k_tiles + 1) + kt0); e_end[r] = __ldg(cptr + r * (p.k_tiles + 1) + kt1); }
+    }
+    if constexpr (BOTH) {   // the second strip has the second weight's lists
+        e_begin[1] = e_end[1] = 0;
+        const int32_t *up = after.up.outlier_chunk_ptr + (size_t)strip * (p.k_tiles + 1);
+        if (kt0 < kt1) { e_begin[1] = __ldg(up + kt0); e_end[1] = __ldg(up + kt1); }
     }
     uint32_t pre_ent[4], pre_val[4];
     auto load_group = [&](int r, int e0) {
@@ -206,11 +225,12 @@ __global__ void __launch_bounds__((MT == 1 ? GS_MAX_WARPS : GS_WARPS2) * 32, 2) 
             const int e = e0 + 2 * tig + (q & 1) + (q >> 1) * 8;
             pre_ent[q] = no_entry;
             pre_val[q] = 0;
-            if (e < e_end[r]) {
-                const bool up = second || (GATED && r);
-                pre_ent[q] = __ldg((up ? p.up.outlier_entries : p.entries) + e);
-                pre_val[q] = __ldg((up ? (const uint16_t *)p.up.outlier_vals_sorted : p.ovals) + e);
+            const uint32_t *entries = p.entries;
+            const uint16_t *ovals = p.ovals;
+            if constexpr (GATED) {
+                if (second || (BOTH && r)) entries = after.up.outlier_entries, ovals = (const uint16_t *)after.up.outlier_vals_sorted;
             }
+            if (e < e_end[r]) { pre_ent[q] = __ldg(entries + e); pre_val[q] = __ldg(ovals + e); }
         }
     };
     load_group(0, e_begin[0]);
@@ -218,9 +238,15 @@ __global__ void __launch_bounds__((MT == 1 ? GS_MAX_WARPS : GS_WARPS2) * 32, 2) 
     const int rT = tid >> 7, rL = (tid >> 2) & 31, rj = tid & 3;
     const int out_row = (rL >> 2) + (rj >> 1) * 8, out_m = (RS == 1 ? rT * 8 : 0) + (rL & 3) * 2 + (rj & 1);
     const int out_n = (strip + (RS == 1 || GATED ? 0 : rT)) * 16 + out_row;
-    const uint16_t *bias = second || (GATED && RS == 2 && rT) ? (const uint16_t *)p.up.bias : p.bias;
-    float bias_v = 0.f;
-    if (tid < 128 * NT && bias && out_n < p.n_rows) bias_v = __half2float(__ushort_as_half(__ldg(bias + out_n)));
+    const uint16_t *bias = p.bias;
+    if constexpr (PAIR) {
+        if (second) bias = (const uint16_t *)after.up.bias;
+    }
+    float bias_v = 0.f, up_bias = 0.f;
+    if (tid < 128 * (BOTH ? 1 : NT) && bias && out_n < p.n_rows) bias_v = __half2float(__ushort_as_half(__ldg(bias + out_n)));
+    if constexpr (BOTH) {
+        if (tid < 128 && after.up.bias && out_n < p.n_rows) up_bias = __half2float(__ushort_as_half(__ldg((const uint16_t *)after.up.bias + out_n)));
+    }
 
     // ---- activations: only after the earlier kernels of the stream have completed ------------------
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -367,41 +393,64 @@ __global__ void __launch_bounds__((MT == 1 ? GS_MAX_WARPS : GS_WARPS2) * 32, 2) 
 
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) part[nt][warp][lane] = make_float4(acc[nt][0], acc[nt][1], acc[nt][2], acc[nt][3]);
-    // (of gate and up the first weight's threads, or CTA, write)
-    const bool mine = tid < 128 * (GATED ? MT : NT) && !second && out_m < p.m && out_n < p.n_rows;
-    const float residual = mine ? residual_at(p.epi, out_m, out_n, BF16) : 0.f;   // (travels while the other warps arrive)
-    __syncthreads();
-    float sum[1] = {bias_v};
-    if (tid < 128 * NT)
-        for (int w = 0; w < nwarps; ++w) sum[0] += reinterpret_cast<const float *>(&part[rT][w][rL])[rj];
-    float other = 1.f;
-    if (GATED && RS == 2) {
-        float *to = reinterpret_cast<float *>(&part[1][0][0]);   // (each of these threads has read this place of its own, if any has)
+    if constexpr (KIND == PLAIN) {
         __syncthreads();
-        if (tid >= 128 && tid < 256) to[tid - 128] = sum[0];
-        __syncthreads();
-        if (tid < 128) other = to[tid];
-    }
-    if (PAIR) {
-        __syncwarp();
-        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-        if (second && tid < 128 * NT) {
-            uint32_t at = (uint32_t)__cvta_generic_to_shared(&up_sums[tid]);
-            asm volatile("mapa.shared::cluster.u32 %0, %0, 0;\n\tst.shared::cluster.f32 [%0], %1;" : "+r"(at) : "f"(sum[0]) : "memory");
+        if (tid < 128 * NT) {
+            float s = bias_v;
+            for (int w = 0; w < nwarps; ++w) s += reinterpret_cast<const float *>(&part[rT][w][rL])[rj];
+            if (out_m < p.m && out_n < p.n_rows) {
+                if (BF16) reinterpret_cast<__nv_bfloat16 *>(p.y)[(size_t)out_m * p.ldy + out_n] = __float2bfloat16_rn(s);
+                else reinterpret_cast<__half *>(p.y)[(size_t)out_m * p.ldy + out_n] = __float2half_rn(s);
+            }
         }
-        __syncwarp();
-        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-        if (mine) other = up_sums[tid];
-    }
-    if (mine) {
-        activate(sum, p.epi.act);
-        const float s = scaled(p.epi, GATED ? sum[0] * other : sum[0], residual);
-        if (BF16) reinterpret_cast<__nv_bfloat16 *>(p.y)[(size_t)out_m * p.ldy + out_n] = __float2bfloat16_rn(s);
-        else reinterpret_cast<__half *>(p.y)[(size_t)out_m * p.ldy + out_n] = __float2half_rn(s);
+    } else {
+        // (of gate and up the first weight's threads, or CTA, write)
+        const bool mine = tid < 128 * (GATED ? MT : NT) && !second && out_m < p.m && out_n < p.n_rows;
+        const float residual = mine ? residual_at(after.epi, out_m, out_n, BF16) : 0.f;   // (travels while the other warps arrive)
+        __syncthreads();
+        float sum[1] = {bias_v}, other = up_bias;
+        if (tid < 128 * (BOTH ? 1 : NT))
+            for (int w = 0; w < nwarps; ++w) sum[0] += reinterpret_cast<const float *>(&part[BOTH ? 0 : rT][w][rL])[rj];
+        if (BOTH && tid < 128)   // (the same threads add up both weights' sums: no barrier between them)
+            for (int w = 0; w < nwarps; ++w) other += reinterpret_cast<const float *>(&part[NT - 1][w][rL])[rj];
+        if (PAIR) {
+            __syncwarp();
+            asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+            if (second && tid < 128 * NT) {
+                uint32_t at = (uint32_t)__cvta_generic_to_shared(&up_sums[tid]);
+                asm volatile("mapa.shared::cluster.u32 %0, %0, 0;\n\tst.shared::cluster.f32 [%0], %1;" : "+r"(at) : "f"(sum[0]) : "memory");
+            }
+            __syncwarp();
+            asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+            if (mine) other = up_sums[tid];
+        }
+        if (mine) {
+            activate(sum, after.epi.act);
+            const float s = scaled(after.epi, GATED ? sum[0] * other : sum[0], residual);
+            if (BF16) reinterpret_cast<__nv_bfloat16 *>(p.y)[(size_t)out_m * p.ldy + out_n] = __float2bfloat16_rn(s);
+            else reinterpret_cast<__half *>(p.y)[(size_t)out_m * p.ldy + out_n] = __float2half_rn(s);
+        }
     }
 }
 
 constexpr int GS_STAGE_MAX_BYTES = 48 * 1024;   // staged fp16 activations per CTA, at most (two CTAs per SM)
+
+int sm_count() {
+    static thread_local int dev_cached = -1, sms = 148;
+    int dev = 0;
+    if (cudaGetDevice(&dev) == cudaSuccess && dev != dev_cached) {
+        if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) sms = 148;
+        dev_cached = dev;
+    }
+    return sms;
+}
+
+// Whether a CTA serves a strip of gate and one of up, or a pair of CTAs does: a pair while all pairs run at once (32 warps an
+// SM), one CTA from there on.  Time of pairs over single CTAs, 1 and 8 rows (rows x K, warps of all pairs over places):
+//   2048 x 1024, 0.22: 0.88 0.86   4096 x 1024, 0.43: 0.95 0.96   4096 x 2048, 0.86: 0.75 0.74   2048 x 4096, 0.86: 0.71 0.71
+//   5504 x 2048, 1.16: 1.05 1.00   8192 x 2048, 1.73: 1.19 1.22   4096 x 4096, 1.73: 1.23 1.24   11008 x 4096, 4.6: 1.29 1.25
+//   28672 x 8192, 12: 1.19 1.19    4096 x 14336, 1.73: 1.11 1.13  18944 x 3584, 8.0: 1.36 1.33
+bool one_cta_pays(int64_t strips, int nwarps) { return 2 * strips * (nwarps < 4 ? 4 : nwarps) > 32 * (int64_t)sm_count(); }
 
 // Whether a CTA serves two strips.  Pairs halve the CTAs, so the last wave must not be much emptier than the others; they
 // save the set-up of a warp, which counts while a warp has at most one and a half chunks of K, and half of the conversion
@@ -414,25 +463,21 @@ constexpr int GS_STAGE_MAX_BYTES = 48 * 1024;   // staged fp16 activations per C
 // What the rule gives away: 12288 x 4096, 1.3: 1.04 1.03 1.05 1.11 (its 64 % of two waves is refused with its neighbours
 // 11008 x 4096, 1.2: 0.94 0.95 0.94 1.00, 12288 x 3072, 1.3: 0.88 0.90 0.95 0.96 and 12288 x 6144, 1.3: 0.95 0.90 0.97 0.97).
 bool strip_pairs_pay(int64_t pairs, int n_chunks, bool bf16) {
-    static thread_local int dev_cached = -1, sms = 148;
-    int dev = 0;
-    if (cudaGetDevice(&dev) == cudaSuccess && dev != dev_cached) {
-        if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) sms = 148;
-        dev_cached = dev;
-    }
+    const int sms = sm_count();
     const int64_t places = 2 * sms, waves = ceil_div_i64(pairs, places);
     const int64_t percent = 100 * pairs / (waves * places);   // of the places of all waves that have a CTA
     return n_chunks >= 12 && n_chunks <= (bf16 ? 32 : 24) && (percent >= 85 || (waves >= 3 && percent >= 75));
 }
 
-template <int MT, bool GATED>
-int launch_gemv_strip(const GemvParams &p, bool vec, cudaStream_t st) {
+template <int MT, int KIND>
+int launch_gemv_strip(const GemvParams &p, const After &all, bool vec, cudaStream_t st) {
+    constexpr bool GATED = KIND == GATE_AND_UP;
     const int max_warps = MT == 1 ? GS_MAX_WARPS : GS_WARPS2;
     int nwarps = p.n_chunks < max_warps ? p.n_chunks : max_warps;
     const bool fast = vec && (p.k_tiles & 3) == 0 && p.bs_shift >= 6;   // whole chunks, blocks of whole tiles
     const bool bf16 = p.dtype == ATLAS_DTYPE_BF16;
     const int64_t strips = ceil_div_i64(p.n_rows, 16);
-    const bool two = MT == 1 && fast && strip_pairs_pay(GATED ? strips : (strips + 1) / 2, p.n_chunks, bf16);
+    const bool two = MT == 1 && fast && (GATED ? one_cta_pays(strips, nwarps) : strip_pairs_pay((strips + 1) / 2, p.n_chunks, bf16));
     if (nwarps < 4 * MT * (two ? 2 : 1)) nwarps = 4 * MT * (two ? 2 : 1);  // the reduction needs 128 threads per MMA tile
     // one or two rows of bf16 activations are converted once per CTA into shared memory (measured at 1 / 2 / 4 / 8
     // rows: 3.7 / 3.5 / 3.1 / 2.6 TB/s staged against 3.4 / 3.3 / 3.3 / 3.1 converted per step)
@@ -457,9 +502,11 @@ int launch_gemv_strip(const GemvParams &p, bool vec, cudaStream_t st) {
     cfg.attrs = attr;
     cfg.numAttrs = attrs;
     const char *what = "gemv_strip_kernel launch";
+    std::conditional_t<KIND == PLAIN, Nothing, After> after;
+    if constexpr (KIND != PLAIN) after = all;
     if (stage) {
-        auto kern = two ? gemv_strip_kernel<true, true, 1, true, true, 2, GATED>
-                        : (fast ? gemv_strip_kernel<true, true, 1, true, true, 1, GATED> : gemv_strip_kernel<true, true, 1, true, false, 1, GATED>);
+        auto kern = two ? gemv_strip_kernel<true, true, 1, true, true, 2, KIND>
+                        : (fast ? gemv_strip_kernel<true, true, 1, true, true, 1, KIND> : gemv_strip_kernel<true, true, 1, true, false, 1, KIND>);
         static thread_local int configured_dev[3] = {-1, -1, -1};   // more than the default dynamic shared memory: opt in once
         int dev = 0;
         cudaGetDevice(&dev);
@@ -469,19 +516,19 @@ int launch_gemv_strip(const GemvParams &p, bool vec, cudaStream_t st) {
             if (rc) return rc;
             configured_dev[two ? 2 : (int)fast] = dev;
         }
-        return check_cuda(cudaLaunchKernelEx(&cfg, kern, p), what);
+        return check_cuda(cudaLaunchKernelEx(&cfg, kern, p, after), what);
     }
     if (two) {
-        auto kern = bf16 ? gemv_strip_kernel<true, true, 1, false, true, 2, GATED> : gemv_strip_kernel<false, true, 1, false, true, 2, GATED>;
-        return check_cuda(cudaLaunchKernelEx(&cfg, kern, p), what);
+        auto kern = bf16 ? gemv_strip_kernel<true, true, 1, false, true, 2, KIND> : gemv_strip_kernel<false, true, 1, false, true, 2, KIND>;
+        return check_cuda(cudaLaunchKernelEx(&cfg, kern, p, after), what);
     }
     if (fast) {
-        auto kern = bf16 ? gemv_strip_kernel<true, true, MT, false, true, 1, GATED> : gemv_strip_kernel<false, true, MT, false, true, 1, GATED>;
-        return check_cuda(cudaLaunchKernelEx(&cfg, kern, p), what);
+        auto kern = bf16 ? gemv_strip_kernel<true, true, MT, false, true, 1, KIND> : gemv_strip_kernel<false, true, MT, false, true, 1, KIND>;
+        return check_cuda(cudaLaunchKernelEx(&cfg, kern, p, after), what);
     }
-    auto kern = bf16 ? (vec ? gemv_strip_kernel<true, true, MT, false, false, 1, GATED> : gemv_strip_kernel<true, false, MT, false, false, 1, GATED>)
-                     : (vec ? gemv_strip_kernel<false, true, MT, false, false, 1, GATED> : gemv_strip_kernel<false, false, MT, false, false, 1, GATED>);
-    return check_cuda(cudaLaunchKernelEx(&cfg, kern, p), what);
+    auto kern = bf16 ? (vec ? gemv_strip_kernel<true, true, MT, false, false, 1, KIND> : gemv_strip_kernel<true, false, MT, false, false, 1, KIND>)
+                     : (vec ? gemv_strip_kernel<false, true, MT, false, false, 1, KIND> : gemv_strip_kernel<false, false, MT, false, false, 1, KIND>);
+    return check_cuda(cudaLaunchKernelEx(&cfg, kern, p, after), what);
 }
 
 }  // namespace
@@ -507,8 +554,11 @@ int qlinear_gemv(const void *x, int dtype, int64_t m, int64_t ldx, const uint8_t
 
     GemvParams p;
     p.dtype = dtype;
-    p.epi = epi;
-    p.up = up ? *up : AtlasWeight{};
+    After after;
+    after.epi = epi;
+    after.up = up ? *up : AtlasWeight{};
+    after.tiles_apart = up ? (int64_t)((intptr_t)up->tiles - (intptr_t)tiles) : 0;
+    after.scales_apart = up ? (int64_t)((intptr_t)up->scales_tiled - (intptr_t)scales_tiled) / 2 : 0;
     p.ldx = ldx;
     p.tiles = tiles;
     p.scales_t = (const uint16_t *)scales_tiled;
@@ -529,9 +579,11 @@ int qlinear_gemv(const void *x, int dtype, int64_t m, int64_t ldx, const uint8_t
         p.m = (int)(m - m0 < 16 ? m - m0 : 16);
         p.x = (const char *)x + (size_t)m0 * ldx * 2;
         p.y = (char *)y + (size_t)m0 * ldy * 2;
-        if (epi.residual) p.epi.residual = epi.residual + m0 * epi.ldr;
-        rc = up ? (p.m <= 8 ? launch_gemv_strip<1, true>(p, vec, st) : launch_gemv_strip<2, true>(p, vec, st))
-                : (p.m <= 8 ? launch_gemv_strip<1, false>(p, vec, st) : launch_gemv_strip<2, false>(p, vec, st));
+        if (epi.residual) after.epi.residual = epi.residual + m0 * epi.ldr;
+        const bool one = p.m <= 8;
+        rc = up ? (one ? launch_gemv_strip<1, GATE_AND_UP>(p, after, vec, st) : launch_gemv_strip<2, GATE_AND_UP>(p, after, vec, st))
+             : is_plain(epi) ? (one ? launch_gemv_strip<1, PLAIN>(p, after, vec, st) : launch_gemv_strip<2, PLAIN>(p, after, vec, st))
+                             : (one ? launch_gemv_strip<1, FOLLOWED>(p, after, vec, st) : launch_gemv_strip<2, FOLLOWED>(p, after, vec, st));
         if (rc) return rc;
     }
     return ATLAS_OK;
