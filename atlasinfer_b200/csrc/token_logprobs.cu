@@ -10,8 +10,8 @@
 // those is at most the k-th largest logit.  Only threads whose own maximum reaches it look again, at the batch that holds it (at
 // all of theirs if more than one batch reaches it); what reaches it
 // (k and a few more) is collected as 64-bit keys (logit, lowest index first), and the place of a key is the number of keys
-// above it.  Where far more reach it (rows of equal logits, of few that are not masked) the k-th largest key of some of them is a
-// higher floor for another look.  No two keys are equal, so the answer does not depend on the order in which they are found.
+// above it.  Where far more reach it (rows of equal logits) the k-th largest key of some of them is a higher floor for another
+// look.  No two keys are equal, so the answer does not depend on the order in which they are found.
 #include <algorithm>
 
 #include "rows.cuh"
@@ -72,6 +72,12 @@ __device__ __forceinline__ float exp2_of(float x) {
     return r;
 }
 
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
 // A piece is 16 aligned bytes of a row.
 template <int DTYPE>
 struct Logits {
@@ -97,6 +103,27 @@ struct Logits {
             }
         }
         return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    static constexpr float LOWEST = DTYPE == ATLAS_DTYPE_F16 ? -65504.f : BF16 ? -0x1.fep127f : -0x1.fffffep127f;
+    // -inf becomes the lowest finite number (NaN stays).
+    static __device__ __forceinline__ uint4 finite(const uint4 &v) {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        uint32_t r[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (WIDE) r[i] = __float_as_uint(max_or_nan(__uint_as_float(w[i]), LOWEST));
+            else if (BF16) asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r[i]) : "r"(w[i]), "r"(0xff7fff7fu));
+            else asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r[i]) : "r"(w[i]), "r"(0xfbfffbffu));
+        }
+        return make_uint4(r[0], r[1], r[2], r[3]);
+    }
+    // Whether all of some pieces is -inf.
+    template <int N>
+    static __device__ __forceinline__ bool masked(const uint4 (&v)[N]) {
+        uint32_t other = 0;
+#pragma unroll
+        for (int a = 0; a < N; ++a) other |= (v[a].x ^ NONE) | (v[a].y ^ NONE) | (v[a].z ^ NONE) | (v[a].w ^ NONE);
+        return other == 0;
     }
     // Its logits, two by two.
     static constexpr int PAIRS = PER / 2;
@@ -274,18 +301,18 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel
         }
         const float base = base_of(m);
         const pair_t minus = pair_of(-base, -base);
-        pair_t batch = 0;
+        if (m < 1e30f && (L::LOWEST - m) * p.exponent < -160.f) {
+            // what is as low as the type reaches has e = 0, and -inf may be taken as that: no product with d = -inf
 #pragma unroll
-        for (int a = 0; a < AHEAD; ++a)
+            for (int a = 0; a < AHEAD; ++a)
 #pragma unroll
-            for (int i = 0; i < L::PAIRS; ++i) {
-                const pair_t d = add2(L::pair(raw[a], i), minus), z = mul2(d, exponent);
-                const pair_t e = pair_of(exp2_of(low(z)), exp2_of(high(z)));
-                sum = add2(sum, e);
-                batch = fma2(e, d, batch);
-            }
-        if (!(low(batch) + high(batch) > -INFINITY)) {   // (0 times -inf among them, or NaN: again, with the products of 0 left 0)
-            batch = 0;
+                for (int i = 0; i < L::PAIRS; ++i) {
+                    const pair_t d = add2(L::pair(L::finite(raw[a]), i), minus), z = mul2(d, exponent);
+                    const pair_t e = pair_of(exp2_of(low(z)), exp2_of(high(z)));
+                    sum = add2(sum, e);
+                    weighted = fma2(e, d, weighted);
+                }
+        } else if (!L::masked(raw)) {   // nothing but masked logits before this batch, or logits near the ends of their type
 #pragma unroll 1
             for (int a = 0; a < AHEAD; ++a) {
                 uint4 v = raw[0];
@@ -295,11 +322,12 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel
 #pragma unroll
                 for (int i = 0; i < L::PAIRS; ++i) {
                     const pair_t d = add2(L::pair(v, i), minus), z = mul2(d, exponent);
-                    batch = fma2(pair_of(exp2_of(low(z)), exp2_of(high(z))), pair_of(fmaxf(low(d), LP_FLOOR), fmaxf(high(d), LP_FLOOR)), batch);
+                    const pair_t e = pair_of(exp2_of(low(z)), exp2_of(high(z)));
+                    sum = add2(sum, e);
+                    weighted = fma2(e, pair_of(fmaxf(low(d), LP_FLOOR), fmaxf(high(d), LP_FLOOR)), weighted);
                 }
             }
         }
-        weighted = add2(weighted, batch);
         ++batches;
     };
     const uint4 none = make_uint4(L::NONE, L::NONE, L::NONE, L::NONE);
@@ -351,8 +379,11 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel
 
     // ---- the likeliest -----------------------------------------------------------------------------------
     if (p.top) {
-        // (no key with this logit is smaller)
-        unsigned long long floor = key_of(kth_largest(group_max[lane], group_max[lane + 32], p.top, lane), 0) & 0xffffffff00000000ull;
+        const float bound = kth_largest(group_max[lane], group_max[lane + 32], p.top, lane);
+        const int begins = max(0, at0), ends = min(p.vocab, at0 + pieces * PER);   // this CTA's logits
+        // no key with this logit is smaller; where it is -inf, as many as are wanted reach that of the last one of the first so many
+        unsigned long long floor = key_of(bound, 0) & 0xffffffff00000000ull;
+        if (bound == -INFINITY && ends - begins >= p.top) floor = key_of(-INFINITY, begins + p.top - 1);
         const unsigned long long mine_at_most = odd ? ~0ull : key_of(own, max(0, at0 + (tid ? front + tid : 0) * PER));
         const int steps = (whole + THREADS - 1) / THREADS + 2;   // (the last two: what thread 0 took care of)
         while (true) {
@@ -408,7 +439,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel
                 __syncthreads();
                 break;
             }
-            // Rows of equal logits, of few that are not masked, ascending ones: some of them give a higher floor.
+            // Rows of equal logits, ascending ones: some of the candidates give a higher floor.
             for (int c = tid; c < CANDIDATES / 2; c += THREADS)
                 if (above(candidates, CANDIDATES / 2, candidates[c]) == p.top - 1) raised = candidates[c];
             __syncthreads();
@@ -485,7 +516,8 @@ int launch_with(const LogprobParams &p, int64_t rows, cudaStream_t st, const cha
 //   2048 x 50272 bf16    42.9 45.7 55.2                         53.2  58.7 77.3
 //   2048 x 50272 fp32    64.4 68.8 73.2                         76.4  80.4 91.7
 //   2048 x 5000 bf16      9.9 12.9 27.2                         17.3  25.0 48.2
-// (The many rows of 16 bits are bound by the instructions of a logit, some 7, and their chain: 4.8 TB/s; those of 32 by HBM: 6.4.)
+// What bounds it: many rows of 16 bits the instructions of a logit and their chain (2048 x 50272 43 us, 4.8 TB/s: 7 instructions
+// and an exponential each), of 32 bits HBM (64 us, 6.45 TB/s); few rows a chain of waits (1 x 50272 3.8 us, with tokens 8).
 struct Shape {
     int threads, parts;
 };
