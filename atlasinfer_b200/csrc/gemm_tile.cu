@@ -349,6 +349,7 @@ tile_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ C
         const uint32_t red = base;
         const bool vec = (p.ldy % 4 == 0) && (((uintptr_t)p.y & 7) == 0);
         constexpr int PIECES = TWO ? TL_BM / 8 : TL_BM / 4;   // of 4 outputs
+        if (KIND != PLAIN) asm volatile("griddepcontrol.wait;" ::: "memory");   // (long since over; the residual is from a kernel in front)
         for (int idx = slice * TL_THREADS + tid; idx < rows * PIECES; idx += p.splits * TL_THREADS) {
             const int t = idx / PIECES, n = n0 + idx % PIECES * 4;
             if (n >= p.n_rows) continue;

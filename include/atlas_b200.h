@@ -544,7 +544,8 @@ ATLAS_API int atlas_fused_linear(const AtlasFusedLinear *linear, void *stream);
  *   weight, bias, post_weight   [hidden] or NULL (no post_weight: x is taken as it is)
  *   normed, stream_out   contiguous; stream_out of the residual's type (without one:
  *                of dtype), or NULL if it is not wanted; it may be the residual
- *                itself where that is contiguous
+ *                itself where that is contiguous.  Else neither overlaps anything
+ *                that is read
  * hidden is at most 32768.
  */
 #define ATLAS_WIDE_STREAM 1

@@ -169,6 +169,31 @@ def test_streams_graphs_and_first_use(cuda_device):
         assert torch.equal(first, mlp(x))
 
 
+@pytest.mark.parametrize("m", (1, 5, 12, 40, 140))
+def test_shared_tensors(cuda_device, m):
+    """One module as gate and as up, the input as the residual, members of a group of three, calls on two streams at once."""
+    (a, w), (b, v), (c, u) = (module(256, 256, s, cuda_device) for s in (12, 13, 14))
+    x = randn((m, 256), F16, m, cuda_device)
+    want, slack = D.fused(x, [w, w], [a.bias, a.bias], "gelu", x, 0.5)
+    assert_rounded(ab.gated_linear(a, a, x, "gelu", residual=x, scale=0.5), want, slack)
+    ab.fuse_linears([a, b, c])
+    want, slack = D.fused(x, [u, v], [c.bias, b.bias], "silu")
+    assert_rounded(ab.gated_linear(c, b, x), want, slack)
+    assert_rounded(c(x), *D.fused(x, [u], [c.bias], None))
+    torch.cuda.synchronize(cuda_device)
+    streams, outs = [torch.cuda.Stream(cuda_device) for _ in range(2)], []
+    inputs = [x, randn((m, 256), F16, m + 1, cuda_device)]
+    torch.cuda.synchronize(cuda_device)
+    for _ in range(5):
+        for s, t in zip(streams, inputs):
+            with torch.cuda.stream(s):
+                outs.append(ab.linear_epilogue(a, ab.gated_linear(b, c, t), "relu", residual=t))
+    torch.cuda.synchronize(cuda_device)
+    for i, t in enumerate(inputs):
+        want = ab.linear_epilogue(a, ab.gated_linear(b, c, t), "relu", residual=t)
+        assert all(torch.equal(o, want) for o in outs[i::2])
+
+
 def test_modules_and_refusals(cuda_device):
     (gate, w), (up, v), (small, _) = (module(n, 256, s, cuda_device) for n, s in ((64, 1), (64, 2), (32, 3)))
     x = torch.zeros(3, 256, dtype=F16, device=cuda_device)

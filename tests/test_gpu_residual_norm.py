@@ -79,6 +79,10 @@ def test_shapes_and_strides(cuda_device):
         check(y.reshape(-1, 96), s.reshape(-1, 96), want, BF16)
         y2, s2 = ab.residual_norm(x, x, w[:], gate=x)
         check(y2.reshape(-1, 96), s2.reshape(-1, 96), D.residual_norm(x.reshape(-1, 96), x.reshape(-1, 96), w, gate=x.reshape(-1, 96)), BF16)
+    for rows in (wide[:, 0, :96], wide[:, 0, 1:96]):   # one row as the residual or the input of all
+        res = rows[:1].expand(6, rows.shape[1])
+        check(*ab.residual_norm(rows, res, w[:rows.shape[1]]), D.residual_norm(rows, res, w[:rows.shape[1]]), BF16)
+        check(*ab.residual_norm(res, rows, w[:rows.shape[1]]), D.residual_norm(res, rows, w[:rows.shape[1]]), BF16)
     one = wide[0, 0, :96]
     assert ab.residual_norm(one, one, w)[0].shape == (96,)
     none = wide[:0, :, :96]
@@ -86,6 +90,24 @@ def test_shapes_and_strides(cuda_device):
     assert y.shape == s.shape == (0, 4, 96)
     odd = randn((97,), BF16, 2, cuda_device)[1:]   # weights at an odd address
     check(*ab.residual_norm(wide[:, 0, :96], None, odd), D.residual_norm(wide[:, 0, :96], None, odd), BF16)
+
+
+@pytest.mark.parametrize("hidden", (64, 1001, 2051))
+@pytest.mark.parametrize("wide", (False, True))
+def test_stream_in_place(cuda_device, hidden, wide):
+    """Through the C entry the stream may take the residual's place: rows that share 16 bytes with their neighbours too."""
+    from atlasinfer_b200 import _capi
+
+    tokens = 400
+    x, r = randn((tokens, hidden), F16, 0, cuda_device), randn((tokens, hidden), F32 if wide else F16, 1, cuda_device, 3)
+    w = randn((hidden,), F16, 2, cuda_device)
+    y, s = ab.residual_norm(x, r, w)
+    out = torch.empty_like(x)
+    a = _capi.ResidualNorm(dtype=0, wide=int(wide), scale=1.0, eps=1e-6, tokens=tokens, hidden=hidden, x=x.data_ptr(), residual=r.data_ptr(), x_stride=hidden, residual_stride=hidden,
+                           weight=w.data_ptr(), normed=out.data_ptr(), stream_out=r.data_ptr())
+    assert _capi.load().atlas_residual_norm(a, _capi.stream_ptr(cuda_device)) == 0
+    torch.cuda.synchronize(cuda_device)
+    assert torch.equal(out, y) and torch.equal(r, s)
 
 
 def test_special_numbers(cuda_device):
