@@ -272,15 +272,18 @@ int launch_as(const NormParams &p, int threads, cudaStream_t st, const char *wha
            : p.wide & ATLAS_WIDE_STREAM ? launch_early(residual_norm_kernel<V, BF16, ROWS, WIDE_STREAM, FULL, ONE, MAX, WIDE_MIN>, grid, threads, 0, st, what, p)
                                         : launch_early(residual_norm_kernel<V, BF16, ROWS, SAME_STREAM, FULL, ONE, MAX, MIN>, grid, threads, 0, st, what, p);
 }
+bool full(const NormParams &p) { return p.post_weight || p.gate || p.bias || p.centered; }
 template <int V, bool BF16, int ROWS, bool ONE, int MAX, int MIN>
 int launch(const NormParams &p, int threads, cudaStream_t st, const char *what) {
-    return p.post_weight || p.gate || p.bias || p.centered ? launch_as<V, BF16, ROWS, true, ONE, MAX, MIN>(p, threads, st, what)
+    return full(p) ? launch_as<V, BF16, ROWS, true, ONE, MAX, MIN>(p, threads, st, what)
                                                            : launch_as<V, BF16, ROWS, false, ONE, MAX, MIN>(p, threads, st, what);
 }
 // Pieces of 8 numbers a thread, and rows a CTA.  Few rows: one piece, so that a row has the most threads (1 x 4096 1.9 us, with two
 // pieces 2.1, with four 2.6).  Many: two, as soon as the CTAs no longer fit all at once (300 x 8192 4.6, 3.9, 4.7; 4096 x 8192 44.7,
 // 40.9, 41.5; with fp32 residuals 60.0, 60.1, 65.8), four for wide rows without a residual (37, 26.7, 24.8).  Many short rows: a
-// warp each (20000 x 128 5.1, a CTA each 21.3; 8192 x 1024 centered 7.2, 9.2).
+// warp each (20000 x 128 5.1, a CTA each 21.3; 8192 x 1024 centered 7.2, 9.2).  With gates, biases or norms in front, a few hundred
+// rows that just do not fit at once go to CTAs of few registers, at the price of spills (515 x 5001 with all there is 10.6, 13.2;
+// 600 x 4096 with a norm in front 4.7, 5.2; but 2048 x 4096 with all 27, 22.6).
 template <bool BF16, int ROWS>
 int by_pieces(const NormParams &p, cudaStream_t st, const char *what) {
     const int pieces = (p.hidden + (ROWS == SHIFTED ? 14 : 7)) / 8;
@@ -289,6 +292,7 @@ int by_pieces(const NormParams &p, cudaStream_t st, const char *what) {
         return pieces <= 32 ? launch<1, BF16, ROWS, true, 256, 4>(p, 256, st, what)
                : pieces <= 64 ? launch<2, BF16, ROWS, true, 256, 4>(p, 256, st, what) : launch<4, BF16, ROWS, true, 256, 4>(p, 256, st, what);
     if (p.tokens < 2 * 148 && pieces <= 1024) return launch<1, BF16, ROWS, false, 1024, 1>(p, threads(1), st, what);
+    if (full(p) && p.tokens <= 5 * 148 && pieces <= 640) return launch_as<2, BF16, ROWS, true, false, 320, 4>(p, threads(2), st, what);
     if (pieces <= 1024 && (p.residual || pieces <= 512)) return launch<2, BF16, ROWS, false, 512, 2>(p, threads(2), st, what);
     return pieces <= 2048 ? launch<4, BF16, ROWS, false, 512, 2>(p, threads(4), st, what) : launch<4, BF16, ROWS, false, 1024, 1>(p, threads(4), st, what);
 }

@@ -47,7 +47,8 @@ def test_plain_norm(cuda_device, tokens, hidden, dtype):
 @pytest.mark.parametrize("tokens,hidden,gate,post,centered", [
     (1, 4096, None, False, False), (3, 515, "rows", True, True), (33, 1024, "channels", True, False), (2, 16384, "rows", False, True), (130, 264, "channels", False, False),
     (1, 1, "rows", True, False), (2, 32768, "channels", True, True), (5, 5001, None, True, False),
-    (350, 1003, "rows", True, True), (301, 1003, "channels", True, False), (1300, 200, "rows", False, True), (1250, 999, "rows", True, False), (320, 9000, "rows", True, False)])
+    (350, 1003, "rows", True, True), (301, 1003, "channels", True, False), (1300, 200, "rows", False, True), (1250, 999, "rows", True, False), (320, 9000, "rows", True, False),
+    (600, 4096, None, True, False), (741, 2048, "rows", True, True)])
 def test_with_everything(cuda_device, tokens, hidden, gate, post, centered, stream_type, dtype):
     x = randn((tokens, hidden), dtype, 0, cuda_device)
     residual = randn((tokens, hidden), dtype if stream_type == "same" else F32, 1, cuda_device, 4)
