@@ -78,7 +78,8 @@ __device__ __forceinline__ float max_or_nan(float a, float b) {
     return r;
 }
 
-// A piece is 16 aligned bytes of a row.
+// A piece is 16 aligned bytes of a row; a batch is so many of a thread's.
+constexpr int batch_pieces(int dtype) { return dtype == ATLAS_DTYPE_F32 ? 4 : 3; }
 template <int DTYPE>
 struct Logits {
     static constexpr bool WIDE = DTYPE == ATLAS_DTYPE_F32, BF16 = DTYPE == ATLAS_DTYPE_BF16;
@@ -255,10 +256,11 @@ __device__ __forceinline__ Stats over_lanes(Stats all, int lanes, float exponent
 }
 
 // A row is a cluster's of p.parts CTAs, each of which has a run of its pieces.
-template <int DTYPE, int THREADS>
+// SLOTS: batches of a thread that travel through shared memory (one of them may be the one in use), or 0: two, through registers.
+template <int DTYPE, int THREADS, int SLOTS>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel(const LogprobParams p) {
     using L = Logits<DTYPE>;
-    constexpr int WARPS = THREADS / 32, PER = L::PER, AHEAD = L::WIDE ? 4 : 3, GROUP = THREADS / LP_GROUPS;
+    constexpr int WARPS = THREADS / 32, PER = L::PER, AHEAD = batch_pieces(DTYPE), GROUP = THREADS / LP_GROUPS;
     __shared__ Stats stats[WARPS], together;
     __shared__ float group_max[LP_GROUPS];
     constexpr int CANDIDATES = 512;
@@ -344,8 +346,45 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel
         next += AHEAD * THREADS;
         left -= AHEAD;
     };
-    uint4 even[AHEAD], odds[AHEAD];   // one batch travels while the other one is summed up
-    if (left > 0) {
+    uint4 even[AHEAD];
+    if constexpr (SLOTS > 0) {   // every thread's batches have places of their own: nothing but the thread waits for them
+        extern __shared__ uint4 ring[];   // [SLOTS][AHEAD][THREADS]
+        const uint32_t mine_at = (uint32_t)__cvta_generic_to_shared(ring + tid);
+        auto fetch = [&](int slot) {
+            auto one = [&](int a) {
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(mine_at + (slot * AHEAD + a) * THREADS * 16), "l"(next + a * THREADS) : "memory");
+            };
+            if (left >= AHEAD) {
+#pragma unroll
+                for (int a = 0; a < AHEAD; ++a) one(a);
+            } else {
+#pragma unroll
+                for (int a = 0; a < AHEAD; ++a)
+                    if (a < left) one(a);
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            next += AHEAD * THREADS;
+            left -= AHEAD;
+        };
+        int rest = left, from = 0, to = SLOTS - 1;
+#pragma unroll
+        for (int s = 0; s < SLOTS - 1; ++s) fetch(s);
+        for (; rest >= AHEAD; rest -= AHEAD) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(SLOTS - 2) : "memory");
+#pragma unroll
+            for (int a = 0; a < AHEAD; ++a) even[a] = ring[(from * AHEAD + a) * THREADS + tid];
+            fetch(to);   // (where the batch before this one was: it has been used)
+            add_up(even);
+            from = from + 1 == SLOTS ? 0 : from + 1, to = to + 1 == SLOTS ? 0 : to + 1;
+        }
+        if (rest > 0) {
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+#pragma unroll
+            for (int a = 0; a < AHEAD; ++a) even[a] = a < rest ? ring[(from * AHEAD + a) * THREADS + tid] : none;
+            add_up(even);
+        }
+    } else if (left > 0) {
+        uint4 odds[AHEAD];   // one batch travels while the other one is summed up
         load(even);
         while (true) {
             bool more = left > 0;
@@ -493,9 +532,11 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel
 
 template <int DTYPE, int THREADS>
 int launch_with(const LogprobParams &p, int64_t rows, cudaStream_t st, const char *what) {
+    constexpr int SLOTS = Logits<DTYPE>::WIDE || THREADS == 512 ? 0 : 3;
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3((unsigned)(rows * p.parts));
     config.blockDim = dim3(THREADS);
+    config.dynamicSmemBytes = SLOTS * batch_pieces(DTYPE) * THREADS * 16;
     config.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -504,20 +545,23 @@ int launch_with(const LogprobParams &p, int64_t rows, cudaStream_t st, const cha
     attr[1].val.clusterDim.x = (unsigned)p.parts, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
     config.attrs = attr;
     config.numAttrs = p.parts > 1 ? 2 : 1;
-    return check_cuda(cudaLaunchKernelEx(&config, token_logprobs_kernel<DTYPE, THREADS>, p), what);
+    return check_cuda(cudaLaunchKernelEx(&config, token_logprobs_kernel<DTYPE, THREADS, SLOTS>, p), what);
 }
 // Threads for a row: as many as fill the GPU (148 x 1024), but no more than leave each a batch; above 512, which are several CTAs,
 // as many as fill half of it, since clusters of CTAs are not placed as evenly.  us with 128 / 256 / 512 threads, and with 2 / 4 / 8
 // CTAs of 512, without likeliest tokens and with 20:
-//      1 x 50272 fp16    10.7  7.3  5.7   4.9  4.2  3.9         13.5  10.1  8.8    8.7  8.2  9.0
-//     64 x 128257 bf16   22.7 13.5 10.2   7.8  8.4 13.4         29.7  17.0 13.3   11.8 13.1 26.0
-//    200 x 50272 bf16    11.4  8.4  8.1                         15.9  11.5 11.7
-//    600 x 50272 bf16    22.3 16.4 17.7                         28.6  21.9 26.7
-//   2048 x 50272 bf16    42.9 45.7 55.2                         53.2  58.7 77.3
-//   2048 x 50272 fp32    64.4 68.8 73.2                         76.4  80.4 91.7
-//   2048 x 5000 bf16      9.9 12.9 27.2                         17.3  25.0 48.2
-// What bounds it: many rows of 16 bits the instructions of a logit and their chain (2048 x 50272 43 us, 4.8 TB/s: 7 instructions
-// and an exponential each), of 32 bits HBM (64 us, 6.45 TB/s); few rows a chain of waits (1 x 50272 3.8 us, with tokens 8).
+//      1 x 50272 bf16     6.7  5.1  5.3   4.5  3.9  3.6          9.6  8.0  8.4    8.4  7.9  8.4
+//     64 x 128257 bf16   14.1 10.3 10.0   7.5  7.6  9.8         21.4 13.8 13.1   11.6 12.2 22.9
+//    200 x 50272 bf16     8.0  8.0  7.9                         12.8 11.2 11.5
+//    600 x 50272 bf16    20.9 15.3 17.6                         27.1 20.6 26.4
+//   2048 x 50272 bf16    38.3 40.8 54.6                         50.0 52.9 76.7
+//   2048 x 50272 fp32    64.4 68.8 73.2                         76.4 80.4 91.7
+//   2048 x 5000 bf16      8.5 12.0 22.4                         16.5 24.7 44.4
+// 16-bit logits of CTAs of up to 256 threads travel through shared memory, where more of them fit than in registers (128 threads,
+// without and with: 300 x 128257 27.7, 22.1; 2048 x 50272 43.7, 38.3; 2048 x 24000 22.8, 20.1; 2048 x 5000 8.5, 8.6).  Of 32 bits
+// they gain nothing (2048 x 50272 63.7, 64.8), and with 512 threads there are seldom more than three batches.
+// What bounds it: many rows of 16 bits the exponentials and instructions of a logit and HBM about equally (2048 x 50272 38 us,
+// 5.4 TB/s), of 32 bits HBM (64 us, 6.45 TB/s); few rows a chain of waits (1 x 50272 3.6 us, with tokens 7.6).
 struct Shape {
     int threads, parts;
 };

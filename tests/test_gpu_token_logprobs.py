@@ -122,6 +122,20 @@ def test_many_rows_agree_with_few(cuda_device):
     assert all(torch.equal(a, b) for a, b in zip(many, again))
 
 
+@pytest.mark.parametrize("dtype", (F16, BF16, F32))
+@pytest.mark.parametrize("rows,vocab", [(1200, 5003), (800, 12289), (400, 20007)])
+def test_many_long_rows(cuda_device, rows, vocab, dtype):
+    """Rows of several batches a thread, with and without a rest, some of them masked in part or holding NaN."""
+    logits = logits_of(rows, vocab, dtype, 10, cuda_device)
+    logits[::7] = logits[::7].masked_fill(torch.rand(logits[::7].shape, generator=torch.Generator().manual_seed(4)).to(cuda_device) < 0.5, -math.inf)
+    logits[3] = -math.inf
+    logits[4, vocab - 2] = math.nan
+    logits[5, : vocab // 2] = torch.finfo(dtype).min
+    tokens = torch.randint(0, vocab, (rows,), generator=torch.Generator().manual_seed(5)).to(cuda_device)
+    for top, temperature in ((0, 1.0), (12, 0.7)):
+        check(logits, tokens, top, temperature)
+
+
 def test_streams_and_graphs(cuda_device):
     logits, tokens = logits_of(3, 40000, BF16, 7, cuda_device), torch.tensor([1, 2, 3], device=cuda_device)
     side = torch.cuda.Stream(cuda_device)
