@@ -29,8 +29,8 @@
 // Measured (us, launch chain, against gemm.cu's kernel that served these sizes before): 57344 x 8192 at 32 rows 201 -> 156,
 // 64 rows 207 -> 163; 8192 x 28672 at 32 rows 95 -> 76; 22016 x 4096 at 32 rows 52 -> 37, 128 rows 58 -> 48; 4096 x 11008
 // at 128 rows 66 -> 27 (where gemm.cu's kernel is the faster one, route_for in gemm.cu leaves it the call).  Issue slots are 45 % used (ncu, 22016 x 4096 at 32
-// rows); the rest is the chain of a k-tile through one A tile (rebuild, fence, MMA, commit), of which four are in flight
-// per SM.  Up to 16 rows (BN = 16) this is reached on request only: the per-strip kernel serves them.
+// rows), the shared-memory pipe half; a k-tile's chain (codes, rebuild, fence, MMA, commit) is not what is left: twice as many A tiles
+// give 1 to 3 %, half again as many dequantizer warps 2 %.  Up to 16 rows (BN = 16) this is reached on request only: the per-strip kernel serves them.
 //
 // Every mbarrier wait is bounded; when one runs out the CTA sets the caller's status word, the producers and the MMA
 // thread wait (bounded) for what they have issued, and the CTA takes part in the cluster barriers, frees its TMEM and
@@ -49,7 +49,6 @@ constexpr int TL_DQ_WARPS = 8;                        // 4 row quarters x 2 k-ti
 constexpr int TL_CTRL_WARPS = 4;
 constexpr int TL_THREADS = (TL_CTRL_WARPS + TL_DQ_WARPS) * 32;
 constexpr int TL_DONE = 8;                            // `done` barriers; a ring that waits on them has at most 8 slots
-constexpr int TL_AS = 2;                              // A tiles: one per phase
 constexpr uint32_t TL_A_BYTES = TL_BM * TL_BK * 2;    // 16 KB rebuilt weights
 constexpr uint32_t TL_C_BYTES = TL_BM * TL_BK;        // 8 KB codes
 constexpr uint32_t TL_S_BYTES = 256;                  // scales of 128 rows
@@ -58,16 +57,20 @@ constexpr int TL_RED = TL_BM + 4;                     // floats per token of the
 template <int BN>
 struct TileSmem {
     static constexpr uint32_t X_BYTES = BN * TL_BK * 2;
-    // Slots of the activation and of the code ring: what is left of half an SM's shared memory.  A load takes 2 to 3 us
-    // under this traffic whether it comes from HBM or, as the activations, from L2, so both rings must be deep.
-    static constexpr int XS = BN <= 16 ? 8 : (BN == 32 ? 7 : (BN == 64 ? 5 : (BN == 96 ? 3 : 2)));
-    static constexpr int CS = BN <= 16 ? 7 : (BN == 32 ? 6 : (BN == 64 ? 4 : 5));
+    // A tiles, at least one per phase, and slots of the activation and of the code ring, which share half an SM's shared memory.
+    // A load takes 2 to 3 us under this traffic whether it comes from HBM or, as the activations, from L2, so the rings must be
+    // deep; with more A tiles than phases a warp does not wait for the MMAs of its last k-tile.  AS, XS, CS = 4, 3, 4 against
+    // 2, 7, 6 (us, 24 fp16 rows): two of 28672 x 8192 153.8, 156.7; 22016 x 4096 33.9, 34.4; 12288 x 4096 21.1, 21.7; 8192 x 2048
+    // 9.6, 9.7; 57344 x 8192 147.1, 147.2; 8192 x 8192 23.4, 23.1.  For 64 rows 3, 3, 4 is no better than 2, 5, 4.
+    static constexpr int AS = BN == 32 ? 4 : 2;
+    static constexpr int XS = BN <= 16 ? 8 : (BN == 64 ? 5 : (BN <= 96 ? 3 : 2));
+    static constexpr int CS = BN <= 16 ? 7 : (BN <= 64 ? 4 : 5);
     // A dequantizer takes every second k-tile, so with an odd ring it comes back to a slot two rounds later, when a
     // parity can no longer tell the rounds apart.  It is never that far ahead: before k-tile kt - 2 it has waited for the
-    // MMAs of kt - 4, so k-tile kt - CS, the round in between, has landed.
-    static_assert(CS % 2 == 0 || CS >= 4, "code ring parity");
+    // MMAs of kt - 2 - AS, so k-tile kt - CS, the round in between, has landed.
+    static_assert(CS % 2 == 0 || CS >= AS + 2, "code ring parity");
     static constexpr uint32_t OFF_A = 0;
-    static constexpr uint32_t OFF_X = OFF_A + TL_AS * TL_A_BYTES;
+    static constexpr uint32_t OFF_X = OFF_A + AS * TL_A_BYTES;
     static constexpr uint32_t OFF_C = OFF_X + XS * X_BYTES;
     static constexpr uint32_t OFF_S = OFF_C + CS * TL_C_BYTES;
     static constexpr uint32_t OFF_BAR = OFF_S + CS * TL_S_BYTES;
@@ -102,7 +105,7 @@ tile_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ C
     constexpr bool TWO = KIND == GATE_AND_UP;
     using SM = TileSmem<BN>;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    constexpr int CS = SM::CS, XS = SM::XS;
+    constexpr int AS = SM::AS, CS = SM::CS, XS = SM::XS;
     extern __shared__ unsigned char smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t base = (raw + 1023u) & ~1023u;          // operand tiles need 1024-byte alignment
@@ -110,13 +113,13 @@ tile_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ C
     const uint32_t bars = base + SM::OFF_BAR;
     auto done_bar = [&](int kt) { return bars + 8u * (kt % TL_DONE); };               // MMAs of k-tile kt have finished
     auto done_par = [&](int kt) { return (uint32_t)((kt / TL_DONE) & 1); };
-    auto ready_bar = [&](int kt) { return bars + 8u * (TL_DONE + (kt & 1)); };        // A tile stored: 4 warps
-    auto x_full = [&](int s) { return bars + 8u * (TL_DONE + 2 + s); };               // fp16 activations in the slot
-    auto x_land = [&](int s) { return bars + 8u * (TL_DONE + 2 + XS + s); };          // bf16 activations in the slot
-    auto full_c = [&](int s) { return bars + 8u * (TL_DONE + 2 + 2 * XS + s); };
-    auto empty_c = [&](int s) { return bars + 8u * (TL_DONE + 2 + 2 * XS + CS + s); };
-    constexpr int N_BARS = TL_DONE + 2 + 2 * XS + 2 * CS;
-    static_assert(N_BARS * 8 + 16 <= 512 && XS <= TL_DONE, "barrier area");
+    auto ready_bar = [&](int kt) { return bars + 8u * (TL_DONE + kt % AS); };          // A tile stored: 4 warps
+    auto x_full = [&](int s) { return bars + 8u * (TL_DONE + AS + s); };               // fp16 activations in the slot
+    auto x_land = [&](int s) { return bars + 8u * (TL_DONE + AS + XS + s); };          // bf16 activations in the slot
+    auto full_c = [&](int s) { return bars + 8u * (TL_DONE + AS + 2 * XS + s); };
+    auto empty_c = [&](int s) { return bars + 8u * (TL_DONE + AS + 2 * XS + CS + s); };
+    constexpr int N_BARS = TL_DONE + AS + 2 * XS + 2 * CS;
+    static_assert(N_BARS * 8 + 16 <= 512 && XS <= TL_DONE && AS <= TL_DONE, "barrier area");
     volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(base_ptr + SM::OFF_BAR + 8 * N_BARS);
     volatile int *s_abort = reinterpret_cast<volatile int *>(base_ptr + SM::OFF_BAR + 8 * N_BARS + 8);
 
@@ -133,7 +136,7 @@ tile_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ C
         asm volatile("prefetch.tensormap [%0];" ::"l"(tid < 32 ? (const void *)&x_map : (const void *)&c_map) : "memory");
     if (tid == 0) {
         for (int s = 0; s < TL_DONE; ++s) mbar_init(done_bar(s), 1);
-        for (int s = 0; s < TL_AS; ++s) mbar_init(ready_bar(s), 4);
+        for (int s = 0; s < AS; ++s) mbar_init(ready_bar(s), 4);
         for (int s = 0; s < XS; ++s) { mbar_init(x_full(s), 1); mbar_init(x_land(s), 1); }
         for (int s = 0; s < CS; ++s) { mbar_init(full_c(s), 1); mbar_init(empty_c(s), 4); }
         *s_abort = 0;
@@ -213,10 +216,10 @@ tile_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ C
             const uint64_t da0 = make_smem_desc(base + SM::OFF_A), db0 = make_smem_desc(base + SM::OFF_X);
             bool ok = true;
             for (int kt = 0; kt < KT && ok; ++kt) {
-                ok = mbar_wait(x_full(kt % XS), (uint32_t)((kt / XS) & 1)) && mbar_wait(ready_bar(kt), (uint32_t)((kt >> 1) & 1));
+                ok = mbar_wait(x_full(kt % XS), (uint32_t)((kt / XS) & 1)) && mbar_wait(ready_bar(kt), (uint32_t)((kt / AS) & 1));
                 if (!ok || ((kt & 7) == 7 && *s_abort)) { ok = false; break; }
                 tcgen05_fence_after();
-                const uint64_t da = da0 + (uint64_t)(((kt & 1) * TL_A_BYTES) >> 4);   // the address field counts 16-byte units
+                const uint64_t da = da0 + (uint64_t)(((kt % AS) * TL_A_BYTES) >> 4);   // the address field counts 16-byte units
                 const uint64_t db = db0 + (uint64_t)(((kt % XS) * SM::X_BYTES) >> 4);
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
@@ -231,7 +234,6 @@ tile_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ C
         const int q = warp & 3, ph = (warp - TL_CTRL_WARPS) >> 2;   // TMEM lane quarter = row quarter, k-tile phase
         const int rl = q * 32 + lane;
         const uint32_t code_off = (uint32_t)rl * 64u, swz = (uint32_t)((rl >> 1) & 3);
-        unsigned char *a_row = base_ptr + SM::OFF_A + ph * TL_A_BYTES + rl * 128;
         const uint32_t a_swz = (uint32_t)(rl & 7);
         // Side-table: a half-warp serves its own strip.  The entry range of a k-tile is requested three of the warp's k-tiles
         // ahead, its first 16 entries two ahead: they come from HBM like the codes.  (Four ahead through an unrolled
@@ -242,7 +244,6 @@ tile_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ C
         const int32_t *cp = (up ? p.up.outlier_chunk_ptr : p.chunk_ptr) + strip * (p.k_tiles + 1) + kt_begin;
         const uint32_t *entries = up ? p.up.outlier_entries : p.entries;
         const uint16_t *ovals = up ? (const uint16_t *)p.up.outlier_vals_sorted : p.ovals;
-        unsigned char *a_strip = base_ptr + SM::OFF_A + ph * TL_A_BYTES + (q * 32 + half * 16) * 128;
         const uint16_t *sc_row = (up ? (const uint16_t *)p.up.scales_tiled : p.scales_t) + (size_t)row_tile * p.blocks_per_row * 128 + (TWO ? row0 + rl % 64 : rl);
         auto range = [&](int kt, int &b, int &e) {
             b = e = 0;
@@ -267,6 +268,7 @@ tile_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ C
             range(kt + 6, b3, e3);
             entry(b2, e2, ent2, val2);
             const int slot = kt % CS;
+            unsigned char *a_tile = base_ptr + SM::OFF_A + (kt % AS) * TL_A_BYTES, *a_row = a_tile + rl * 128, *a_strip = a_tile + (q * 32 + half * 16) * 128;
             if (!mbar_wait_warp<20>(full_c(slot), (uint32_t)((kt / CS) & 1), s_abort)) { ok = false; break; }
             const unsigned char *codes = base_ptr + SM::OFF_C + slot * TL_C_BYTES + code_off;
             uint4 L[4];   // chunk c sits at c ^ ((row >> 1) & 3) under the 64-byte swizzle
@@ -283,7 +285,7 @@ tile_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ C
             __syncwarp();
             if (lane == 0) mbar_arrive(empty_c(slot));
             // the A tile must have been read by the MMAs of its previous use
-            if (kt >= TL_AS && !mbar_wait_warp<20>(done_bar(kt - TL_AS), done_par(kt - TL_AS), s_abort)) { ok = false; break; }
+            if (kt >= AS && !mbar_wait_warp<20>(done_bar(kt - AS), done_par(kt - AS), s_abort)) { ok = false; break; }
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 const __half2 s2 = __half2half2(sh[c]);
