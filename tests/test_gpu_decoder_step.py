@@ -1,4 +1,9 @@
 """A decoder step from the stream to the answer: the operators together, each against its definition on what it was given."""
+import os
+import subprocess
+import sys
+import threading
+
 import pytest
 import torch
 
@@ -64,3 +69,97 @@ def test_step(cuda_device, tokens, dtype, stream_type):
         assert bool(((found.logprobs.cpu().double() - lp).abs() <= D.logprob_slack(vocab, lp, 1.0)).all())
         assert bool(((found.entropy.cpu().double() - ent).abs() <= 3 * (1 + ent) * D.logprob_slack(vocab, ent, 1.0)).all())
         assert bool(((found.top_logprobs.cpu().double() - tops).abs() <= D.logprob_slack(vocab, tops, 1.0)).all())
+
+
+def test_first_calls_may_be_captured(cuda_device):
+    """In a new process: nothing but the linears' layouts was there before the capture."""
+    program = """
+import torch
+import atlasinfer_b200 as ab
+gen = torch.Generator().manual_seed(3)
+rand = lambda *s: torch.randn(*s, generator=gen).half().cuda()
+up, down = (ab.QuantizedLinear(ab.quantize_tensor(rand(*s) * 0.05), None) for s in ((512, 256), (256, 512)))
+up(rand(1, 256)), down(rand(1, 512))
+for tokens in (1, 12, 30, 200):
+    x = rand(tokens, 256)
+    asked = torch.zeros(tokens, dtype=torch.long, device="cuda")
+
+    def step():
+        h, s = ab.residual_norm(x, x)
+        y = ab.linear_epilogue(down, ab.gated_linear(up, up, h), "gelu", residual=s)
+        return h, s, y, *ab.token_logprobs(y, asked, top=4)
+
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, step())), tokens
+print("all of it")
+"""
+    done = subprocess.run([sys.executable, "-c", program], capture_output=True, text=True, timeout=300, cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert done.returncode == 0 and "all of it" in done.stdout, done.stderr[-2000:]
+
+
+def test_calls_from_several_threads(cuda_device):
+    """The operators on a stream of each thread's own, all with the same weights, at once."""
+    (gate, _), (up, _), (down, _) = (module(n, k, s, cuda_device) for n, k, s in ((640, 256, 1), (640, 256, 2), (256, 640, 3)))
+    norm = randn((256,), F16, 4, cuda_device)
+
+    def step(x, asked):
+        h, s = ab.residual_norm(x, x, norm)
+        y = ab.linear_epilogue(down, ab.gated_linear(gate, up, h), residual=s)
+        return (h, s, y, *ab.token_logprobs(y, asked, top=5))
+
+    jobs = []
+    for tokens in (1, 11, 40, 300):
+        x, asked = randn((tokens, 256), F16, tokens, cuda_device), torch.arange(tokens, device=cuda_device) % 256
+        jobs.append((x, asked, step(x, asked)))
+    torch.cuda.synchronize(cuda_device)
+    errors = []
+
+    def work(x, asked, want):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream(cuda_device)):
+                got = [step(x, asked) for _ in range(20)]
+                torch.cuda.current_stream(cuda_device).synchronize()
+                assert all(torch.equal(a, b) for g in got for a, b in zip(g, want))
+        except BaseException as e:   # noqa: BLE001 - reported by the main thread
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=job) for job in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors[0]
+
+
+def test_more_than_32_bits_of_numbers(cuda_device):
+    """Tensors of more than 2^31 numbers: the last rows are as those of a small call's."""
+    rows, hidden = 300000, 8192
+    x = torch.empty(rows, hidden, dtype=BF16, device=cuda_device)
+    x[-3:] = randn((3, hidden), BF16, 1, cuda_device)
+    h, s = ab.residual_norm(x, x)
+    y, st, slack, slack_s = D.residual_norm(x[-3:], x[-3:])
+    assert_rounded(h[-3:], y, slack)
+    assert_rounded(s[-3:], st, slack_s)
+    del h, s
+    wide = x.view(-1)[: 75001 * 32003].view(75001, 32003)
+    wide[-2:] = randn((2, 32003), BF16, 2, cuda_device, 3)
+    asked = torch.zeros(75001, dtype=torch.long, device=cuda_device)
+    found = ab.token_logprobs(wide, asked, top=3)
+    lp, _, order, _ = D.token_logprobs(wide[-2:], asked[-2:], 3)
+    assert torch.equal(found.top_tokens[-2:].cpu(), order)
+    assert bool(((found.logprobs[-2:].cpu().double() - lp).abs() <= D.logprob_slack(32003, lp, 1.0)).all())
+    del wide, found
+    (gate, wg), (up, wu) = (module(hidden, 256, s, cuda_device) for s in (3, 4))
+    a = randn((rows, 256), BF16, 5, cuda_device)
+    x[-3:] = randn((3, hidden), BF16, 6, cuda_device)
+    got = ab.gated_linear(gate, up, a, residual=x)
+    want, slack = D.fused(a[-3:], [wg, wu], [gate.bias, up.bias], "silu", x[-3:])
+    assert_rounded(got[-3:], want, slack)
+    got = ab.linear_epilogue(gate, a, "gelu", residual=x)
+    want, slack = D.fused(a[-3:], [wg], [gate.bias], "gelu", x[-3:])
+    assert_rounded(got[-3:], want, slack)
