@@ -8,6 +8,12 @@
 namespace atlas {
 namespace {
 
+// What the kernels take for granted of a weight's buffers: codes are read, and scales copied, 16 bytes at a time.
+bool aligned(const AtlasWeight &w) {
+    return !(((uintptr_t)w.tiles | (uintptr_t)w.scales_tiled) & 15) && !(((uintptr_t)w.outlier_chunk_ptr | (uintptr_t)w.outlier_entries) & 3) &&
+           !(((uintptr_t)w.outlier_vals_sorted | (uintptr_t)w.bias) & 1);
+}
+
 int check(const AtlasFusedLinear *p) {
     const char *what = "atlas_fused_linear";
     ATLAS_RETURN_IF(!p, ATLAS_ERR_BAD_ARGUMENT, "%s: no arguments", what);
@@ -15,8 +21,11 @@ int check(const AtlasFusedLinear *p) {
     ATLAS_RETURN_IF(p->m < 0 || p->n_rows <= 0 || p->n_cols <= 0, ATLAS_ERR_BAD_ARGUMENT, "%s: m=%lld n_rows=%lld n_cols=%lld", what, (long long)p->m,
                     (long long)p->n_rows, (long long)p->n_cols);
     ATLAS_RETURN_IF(p->residual && p->m > 1 && p->ldr < p->n_rows, ATLAS_ERR_BAD_ARGUMENT, "%s: residual rows %lld apart", what, (long long)p->ldr);
-    ATLAS_RETURN_IF(p->up.tiles && (!p->up.scales_tiled || !p->up.outlier_chunk_ptr || ((uintptr_t)p->up.tiles & 15)), ATLAS_ERR_BAD_ARGUMENT,
-                    "%s: the second weight lacks a buffer, or its tiles are not 16-byte aligned", what);
+    ATLAS_RETURN_IF(p->up.tiles && (!p->up.scales_tiled || !p->up.outlier_chunk_ptr), ATLAS_ERR_BAD_ARGUMENT, "%s: the second weight lacks a buffer", what);
+    ATLAS_RETURN_IF(!aligned(p->weight) || (p->up.tiles && !aligned(p->up)), ATLAS_ERR_BAD_ARGUMENT,
+                    "%s: tiles and scales must be 16-byte aligned, a weight's other buffers to their types", what);
+    ATLAS_RETURN_IF(((uintptr_t)p->x | (uintptr_t)p->y | (uintptr_t)p->residual) & 1, ATLAS_ERR_BAD_ARGUMENT, "%s: x, y or residual is not aligned to its type", what);
+    ATLAS_RETURN_IF((uintptr_t)p->status & 3, ATLAS_ERR_BAD_ARGUMENT, "%s: status is not aligned to its type", what);
     return ATLAS_OK;
 }
 

@@ -497,7 +497,8 @@ ATLAS_API int atlas_kv_attention(const AtlasKvAttention *attention, void *stream
  * for atlas_qlinear_gemm, `up` of the same shape and block size); bias fp16 or
  * NULL; residual [m][n_rows] of `dtype`, row stride ldr, or NULL.  y overlaps
  * neither residual nor x.  Weights and biases are read before the stream's
- * earlier work has completed (see above), x and residual afterwards.
+ * earlier work has completed (see above), x and residual afterwards.  Buffers
+ * are aligned to their types, tiles and scales_tiled to 16 bytes.
  *   workspace   atlas_fused_linear_workspace_bytes(...) bytes, 256-byte aligned
  *   status      device int32 or NULL, set non-zero if a bounded wait ran out
  */
