@@ -597,7 +597,9 @@ extern "C" int atlas_token_logprobs(const AtlasTokenLogprobs *q, void *stream) {
     ATLAS_RETURN_IF(!q->logits || !q->tokens || !q->logprobs || !q->entropy || (q->top && (!q->top_tokens || !q->top_logprobs)), ATLAS_ERR_BAD_ARGUMENT,
                     "%s: null pointer", what);
     const int size = q->dtype == ATLAS_DTYPE_F32 ? 4 : 2;
-    ATLAS_RETURN_IF((uintptr_t)q->logits % size || (uintptr_t)q->tokens % q->token_bytes, ATLAS_ERR_BAD_ARGUMENT, "%s: a buffer is not aligned to its type", what);
+    ATLAS_RETURN_IF((uintptr_t)q->logits % size || (uintptr_t)q->tokens % q->token_bytes || (((uintptr_t)q->logprobs | (uintptr_t)q->entropy) & 3) ||
+                        (q->top && (((uintptr_t)q->top_logprobs & 3) || ((uintptr_t)q->top_tokens & 7))),
+                    ATLAS_ERR_BAD_ARGUMENT, "%s: a buffer is not aligned to its type", what);
     const int dev = check_device();
     if (dev != ATLAS_OK) return dev;
     LogprobParams p = {};

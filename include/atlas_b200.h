@@ -575,10 +575,10 @@ ATLAS_API int atlas_residual_norm(const AtlasResidualNorm *norm, void *stream);
  *                by their index (NaN counts as the largest); NULL if top is 0
  * Tokens of -inf have no probability (log -inf).  Of a row without any other, all log
  * probabilities are -inf and the entropy is 0; one with +inf or NaN gives NaN.
- *   logits       fp16, bf16 or (dtype ATLAS_DTYPE_F32) fp32, row stride in elements;
- *                aligned to their type
+ *   logits       fp16, bf16 or (dtype ATLAS_DTYPE_F32) fp32, row stride in elements
  *   tokens       [rows] int32 or int64 (token_bytes)
  *   top          at most ATLAS_LOGPROBS_MAX_TOP and vocab
+ * Every buffer is aligned to its type.
  */
 #define ATLAS_DTYPE_F32 2      /* logits only */
 #define ATLAS_LOGPROBS_MAX_TOP 32

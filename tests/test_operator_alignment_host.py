@@ -3,7 +3,7 @@ import pytest
 
 from atlasinfer_b200 import _capi
 
-from .test_decoder_ops_host import lib, linear  # noqa: F401
+from .test_decoder_ops_host import lib, linear, logprobs  # noqa: F401
 
 FINE = dict(tiles=16, scales_tiled=16, outlier_chunk_ptr=16)
 OFF = (dict(tiles=24), dict(scales_tiled=24), dict(scales_tiled=18), dict(outlier_chunk_ptr=18), dict(outlier_entries=18), dict(outlier_vals_sorted=17), dict(bias=17))
@@ -21,3 +21,8 @@ def test_weights(lib, m, off):  # noqa: F811
 @pytest.mark.parametrize("off", (dict(x=17), dict(y=17), dict(residual=17, ldr=64), dict(residual=16 + 1, ldr=65), dict(status=18)))
 def test_rows(lib, m, up, off):  # noqa: F811
     assert lib.atlas_fused_linear(linear(m, up, **off), None) == _capi.ERR_BAD_ARGUMENT and b"aligned" in lib.atlas_last_error()
+
+
+@pytest.mark.parametrize("off", (dict(logprobs=18), dict(entropy=18), dict(top_logprobs=18), dict(top_tokens=20), dict(logits=17), dict(tokens=18, token_bytes=4)))
+def test_log_probabilities(lib, off):  # noqa: F811
+    assert lib.atlas_token_logprobs(logprobs(**off), None) == _capi.ERR_BAD_ARGUMENT and b"aligned" in lib.atlas_last_error()
