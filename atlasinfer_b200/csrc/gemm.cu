@@ -1138,6 +1138,8 @@ int qlinear_gemm(const void *x, int dtype, int64_t m, int64_t ldx, const uint8_t
                     "atlas_qlinear_gemm: too large");
     ATLAS_RETURN_IF(((uintptr_t)tiles & 15) != 0 || ((uintptr_t)workspace & 255) != 0, ATLAS_ERR_BAD_ARGUMENT,
                     "atlas_qlinear_gemm: tiles must be 16-byte and workspace 256-byte aligned");
+    // (blocks of whole k-tiles: their scales come by bulk copies; of others they are read one by one)
+    ATLAS_RETURN_IF(block_size % GM_BK == 0 && ((uintptr_t)scales_tiled & 15) != 0, ATLAS_ERR_BAD_ARGUMENT, "atlas_qlinear_gemm: scales_tiled must be 16-byte aligned");
     const size_t need = qlinear_gemm_workspace_bytes(m, n_rows, n_cols, up != nullptr);
     ATLAS_RETURN_IF(workspace_bytes < need, ATLAS_ERR_CAPACITY,
                     "atlas_qlinear_gemm: workspace holds %zu bytes, %zu needed", workspace_bytes, need);

@@ -236,6 +236,7 @@ ATLAS_API int atlas_repack_many(int count, const AtlasRepackItem *items, void *s
  * of 160 to 384 and slices only where the tiles leave much of the chip idle
  * (atlas_qlinear_gemm_plan).
  * Deterministic either way.
+ * scales_tiled is 16-byte aligned where block_size is a multiple of 64.
  * `workspace` must hold atlas_qlinear_gemm_workspace_bytes(m, n_rows, n_cols)
  * bytes, 256-byte aligned.
  */

@@ -26,3 +26,11 @@ def test_rows(lib, m, up, off):  # noqa: F811
 @pytest.mark.parametrize("off", (dict(logprobs=18), dict(entropy=18), dict(top_logprobs=18), dict(top_tokens=20), dict(logits=17), dict(tokens=18, token_bytes=4)))
 def test_log_probabilities(lib, off):  # noqa: F811
     assert lib.atlas_token_logprobs(logprobs(**off), None) == _capi.ERR_BAD_ARGUMENT and b"aligned" in lib.atlas_last_error()
+
+
+def test_scales_of_plain_linears(lib):  # noqa: F811
+    def call(scales, block):
+        return lib.atlas_qlinear_gemm(16, 0, 40, 128, 16, scales, 16, None, None, 64, 128, block, None, 16, 64, 256, 1 << 40, None, None)
+
+    for block in (64, 128):   # copied in 16-byte units
+        assert call(18, block) == call(24, block) == _capi.ERR_BAD_ARGUMENT and b"scales_tiled" in lib.atlas_last_error()
