@@ -7,8 +7,13 @@ The reference leaves these to the model's own modules.
 * ``gated_linear``      two of them whose outputs are multiplied, one behind an activation: gate and up of an MLP
 * ``token_logprobs``    log probabilities of given tokens, the entropy of every row of logits, and its likeliest tokens
 
-Inference only: no gradients are recorded.  All of it is computed in fp32 and rounded once, on the current stream of the tensors'
-device, and decides nothing on the host that depends on their contents: it can be captured (linears that have run once before).
+Inference only: no gradients are recorded.  Outputs are computed in fp32 and rounded once, on the current stream of the tensors'
+device, and nothing is decided on the host that depends on their contents: it can be captured (linears that have run once before).
+
+The two linears multiply what ``QuantizedLinear`` multiplies, fp16 numbers: bf16 activations become fp16 first, so that those beyond
+65504, infinite ones among them, count as 65504 (of their sign; NaN stays NaN) and those below 2^-14 lose bits, down to 2^-25, which
+is 0.  The bf16 output of ``gated_linear`` may be larger; ``scale`` there, and its reciprocal in the next linear, keeps it in range.
+Residuals and outputs are of the full range.  Both take a module's weight and bias, and go around its forward hooks.
 """
 from __future__ import annotations
 
@@ -67,7 +72,7 @@ def _run(x, first, second, activation, residual, scale):
 
 def linear_epilogue(linear: QuantizedLinear, x: torch.Tensor, activation: Optional[str] = None, *, residual: Optional[torch.Tensor] = None,
                     scale: float = 1.0) -> torch.Tensor:
-    """``residual + scale * activation(linear(x))`` in one pass, rounded once.
+    """``residual + scale * activation(x W^T + bias)`` of ``linear`` in one pass, rounded once (bf16 activations: see above).
 
     ``activation``: None, "relu", "silu", "gelu" (by the error function) or "gelu_tanh".  ``residual`` has the result's shape
     and ``x``'s dtype.  ``linear`` may belong to a fused group; only its own rows are computed."""
@@ -76,8 +81,8 @@ def linear_epilogue(linear: QuantizedLinear, x: torch.Tensor, activation: Option
 
 def gated_linear(gate: QuantizedLinear, up: QuantizedLinear, x: torch.Tensor, activation: Optional[str] = "silu", *,
                  residual: Optional[torch.Tensor] = None, scale: float = 1.0) -> torch.Tensor:
-    """``residual + scale * activation(gate(x)) * up(x)`` in one pass, rounded once; ``gate`` and ``up`` have one shape and block
-    size and may, but need not, be in a fused group.  Arguments as for ``linear_epilogue``."""
+    """``residual + scale * activation(x G^T + b) * (x U^T + c)`` of ``gate`` and ``up`` in one pass, rounded once; they have one
+    shape and block size and may, but need not, be in a fused group.  Arguments as for ``linear_epilogue``."""
     return _run(x, gate, up, activation, residual, scale)
 
 

@@ -494,6 +494,8 @@ ATLAS_API int atlas_kv_attention(const AtlasKvAttention *attention, void *stream
 /* Quantized linears with what follows them, in fp32 and rounded once:
  *   y = residual + scale * act(x W^T + bias)                       (up.tiles NULL)
  *   y = residual + scale * act(x W^T + bias) * (x V^T + up.bias)
+ * bf16 x is used as fp16 inside, as above: |x| > 65504, infinities too, count as
+ * 65504 (NaN stays).  Residual and y have the full range of their type.
  * Weights as atlas_repack lays them out (x, m, ldx, n_rows, n_cols, block_size as
  * for atlas_qlinear_gemm, `up` of the same shape and block size); bias fp16 or
  * NULL; residual [m][n_rows] of `dtype`, row stride ldr, or NULL.  y overlaps
