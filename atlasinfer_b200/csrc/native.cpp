@@ -349,6 +349,13 @@ std::array<at::Tensor, 6> build_layout(const std::vector<std::tuple<at::Tensor, 
     return {tiles, scales, row_ptr, chunk_ptr, entries, vals};
 }
 
+// (device, how often it has been written to) of activations that a group of linears may compute once for all members; None of
+// others: those made in inference mode do not count their writes.
+py::object launch_key(const at::Tensor &x) {
+    if (!x.is_cuda() || (x.scalar_type() != at::kHalf && x.scalar_type() != at::kBFloat16) || x.numel() == 0 || x.is_inference()) return py::none();
+    return py::make_tuple((int)x.get_device(), (int64_t)x._version());
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -360,6 +367,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         .def("finish", &LayoutReady::finish, py::call_guard<py::gil_scoped_release>());
     m.def("build_layout", &build_layout, py::call_guard<py::gil_scoped_release>());
     m.def("quantize_many", &quantize_many, py::call_guard<py::gil_scoped_release>());
+    m.def("launch_key", &launch_key);
     m.def("linear", &linear, py::call_guard<py::gil_scoped_release>());
     bind_kv(m);
     bind_ops(m);

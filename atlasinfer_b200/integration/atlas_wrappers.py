@@ -306,7 +306,8 @@ class FusedLinearGroup:
     (``concat_layouts``); the first member that is called with an input computes the joined product and the
     other members, called with the very same tensor, return their slice of it (for prompt-sized inputs this
     also means one bf16 -> fp16 conversion of the activations instead of one per member).  A member called
-    with any other input computes the joined product anew.  A member's slice equals its stand-alone output up to the rounding of
+    with any other input computes the joined product anew; with one made in ``torch.inference_mode``, whose writes
+    torch does not count, it computes its own rows.  A member's slice equals its stand-alone output up to the rounding of
     the fp32 partial sums (the K range of a row tile is cut between CTAs at other places when the launch
     covers more rows), not bit for bit.
     """
@@ -314,9 +315,10 @@ class FusedLinearGroup:
     def __init__(self, members):
         self.members = list(members)
         self.layout: Optional[KernelLayout] = None
+        self._device = -1       # the GPU that has the layout
         self.bias: Optional[torch.Tensor] = None
         self.offsets = []
-        self._cache = None      # (x, x._version, y_all, members served)
+        self._cache = None      # (x, its launch_key, y_all, members served)
         self.launches = 0       # joined launches issued (for tests and launch counting)
         for i, mod in enumerate(self.members):
             mod._group = self
@@ -353,20 +355,22 @@ class FusedLinearGroup:
         for mod, q, n, o in zip(self.members, sources, rows, self.offsets):
             mod._kernel_layout = slice_layout(fused, o, n, q)
         self.layout = fused
+        self._device = fused.tiles.get_device()
         if fused.ready is None:
             torch.cuda.current_stream(dev).synchronize()
 
     def member_forward(self, index: int, x: torch.Tensor) -> Optional[torch.Tensor]:
         """Member ``index``'s output for ``x``, or None if the group does not apply (the member computes alone)."""
-        if not x.is_cuda or (x.dtype is not torch.float16 and x.dtype is not torch.bfloat16) or x.numel() == 0:
+        key = _capi.native().launch_key(x)
+        if key is None:
             return None
-        if self.layout is None or self.layout.tiles.device != x.device:
+        if key[0] != self._device:
             self.build(x.device)
         c = self._cache
-        if c is None or c[0] is not x or c[1] != x._version or index in c[3]:
+        if c is None or c[0] is not x or c[1] != key or index in c[3]:
             y_all = quantized_linear_forward(x, self.layout, self.bias)
             self.launches += 1
-            c = (x, x._version, y_all, set())
+            c = (x, key, y_all, set())
             self._cache = c
         c[3].add(index)
         off = self.offsets[index]
