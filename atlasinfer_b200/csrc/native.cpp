@@ -349,11 +349,15 @@ std::array<at::Tensor, 6> build_layout(const std::vector<std::tuple<at::Tensor, 
     return {tiles, scales, row_ptr, chunk_ptr, entries, vals};
 }
 
-// (device, how often it has been written to) of activations that a group of linears may compute once for all members; None of
-// others: those made in inference mode do not count their writes.
+// (device, how often it has been written to, current stream and the capture that this is in, 0 if none) of activations that a
+// group of linears may compute once for all members; None of others: those made in inference mode do not count their writes.
 py::object launch_key(const at::Tensor &x) {
     if (!x.is_cuda() || (x.scalar_type() != at::kHalf && x.scalar_type() != at::kBFloat16) || x.numel() == 0 || x.is_inference()) return py::none();
-    return py::make_tuple((int)x.get_device(), (int64_t)x._version());
+    const cudaStream_t stream = at::cuda::getCurrentCUDAStream(x.get_device()).stream();
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    C10_CUDA_CHECK(cudaStreamGetCaptureInfo(stream, &status, &id));
+    return py::make_tuple((int)x.get_device(), (int64_t)x._version(), (uintptr_t)stream, status == cudaStreamCaptureStatusNone ? 0 : id);
 }
 
 }  // namespace

@@ -304,7 +304,7 @@ class FusedLinearGroup:
     The reference issues q/k/v (and gate/up) as separate ``F.linear`` calls on the same input
     (integration/atlas_wrappers.py:67, once per module).  Here the members' kernel layouts are joined row-wise
     (``concat_layouts``); the first member that is called with an input computes the joined product and the
-    other members, called with the very same tensor, return their slice of it (for prompt-sized inputs this
+    other members, called with the very same tensor on the same stream, return their slice of it (for prompt-sized inputs this
     also means one bf16 -> fp16 conversion of the activations instead of one per member).  A member called
     with any other input computes the joined product anew; with one made in ``torch.inference_mode``, whose writes
     torch does not count, it computes its own rows.  A member's slice equals its stand-alone output up to the rounding of
@@ -318,7 +318,9 @@ class FusedLinearGroup:
         self._device = -1       # the GPU that has the layout
         self.bias: Optional[torch.Tensor] = None
         self.offsets = []
-        self._cache = None      # (x, its launch_key, y_all, members served)
+        self._sizes = []        # the joined rows cut into the members' and what pads them,
+        self._pieces = []       # and which of the pieces are the members'
+        self._cache = None      # (x, its launch_key, the pieces of y, members served)
         self.launches = 0       # joined launches issued (for tests and launch counting)
         for i, mod in enumerate(self.members):
             mod._group = self
@@ -355,6 +357,13 @@ class FusedLinearGroup:
         for mod, q, n, o in zip(self.members, sources, rows, self.offsets):
             mod._kernel_layout = slice_layout(fused, o, n, q)
         self.layout = fused
+        self._sizes, self._pieces, row = [], [], 0
+        for n, o in zip(rows, self.offsets):
+            if o > row:
+                self._sizes.append(o - row)
+            self._pieces.append(len(self._sizes))
+            self._sizes.append(n)
+            row = o + n
         self._device = fused.tiles.get_device()
         if fused.ready is None:
             torch.cuda.current_stream(dev).synchronize()
@@ -366,16 +375,15 @@ class FusedLinearGroup:
             return None
         if key[0] != self._device:
             self.build(x.device)
+        # (the key: another stream would not wait for the product, and a graph not hold its launch)
         c = self._cache
         if c is None or c[0] is not x or c[1] != key or index in c[3]:
             y_all = quantized_linear_forward(x, self.layout, self.bias)
             self.launches += 1
-            c = (x, key, y_all, set())
+            c = (x, key, y_all.unsafe_split_with_sizes(self._sizes, -1), set())
             self._cache = c
         c[3].add(index)
-        off = self.offsets[index]
-        n = self.members[index].original_shape[0]
-        out = c[2].narrow(-1, off, n)
+        out = c[2][self._pieces[index]]
         if len(c[3]) == len(self.members):
             self._cache = None   # everyone has been served: do not keep x and y alive
         return out

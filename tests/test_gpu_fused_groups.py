@@ -44,3 +44,59 @@ def test_inference_mode(cuda_device, m):
     for mod, w in zip(mods, weights):
         check(mod, w, x)
     assert mods[0]._group.launches == launches + 1
+
+
+@pytest.mark.parametrize("m", (1, 40))
+def test_members_on_streams_of_their_own(cuda_device, m):
+    """A member that is called on another stream than the one before it launches the product there."""
+    mods, weights = group(cuda_device)
+    x = randn((m, 256), F16, 0, cuda_device)
+    for mod in mods:
+        mod(x)
+    torch.cuda.synchronize(cuda_device)
+    launches = mods[0]._group.launches
+    streams, outs = [torch.cuda.Stream(cuda_device) for _ in mods], []
+    for mod, s in zip(mods, streams):
+        with torch.cuda.stream(s):
+            outs.append(mod(x))
+    assert mods[0]._group.launches == launches + len(mods)
+    torch.cuda.synchronize(cuda_device)
+    for mod, w, y in zip(mods, weights, outs):
+        check(mod, w, x, y)
+
+
+def test_outputs_may_be_written_to(cuda_device):
+    """In place, with gradients of what is added."""
+    mods, weights = group(cuda_device)
+    x = randn((3, 256), F16, 0, cuda_device)
+    outs = [mod(x) for mod in mods]
+    more = torch.ones(3, 160, dtype=F16, device=cuda_device, requires_grad=True)
+    outs[1] += 2 * more
+    outs[1].sum().backward()
+    assert bool((more.grad == 2).all())
+    check(mods[0], weights[0], x, outs[0])
+    check(mods[2], weights[2], x, outs[2])
+
+
+@pytest.mark.parametrize("m", (1, 40))
+def test_members_inside_and_outside_a_graph(cuda_device, m):
+    """A captured member is computed by the graph, and one outside it is not taken from the graph's memory."""
+    mods, weights = group(cuda_device)
+    x = randn((m, 256), F16, 0, cuda_device)
+    side = torch.cuda.Stream(cuda_device)
+    side.wait_stream(torch.cuda.current_stream(cuda_device))
+    with torch.cuda.stream(side):
+        for mod in mods:
+            mod(x)
+        mods[0](x)   # (only this one: the product of all of them is at hand)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            captured = mods[1](x)
+        outside = mods[2](x)
+    torch.cuda.synchronize(cuda_device)
+    check(mods[2], weights[2], x, outside)
+    for seed in (1, 2):
+        x.copy_(randn((m, 256), F16, seed, cuda_device))
+        graph.replay()
+        torch.cuda.synchronize(cuda_device)
+        check(mods[1], weights[1], x, captured)
