@@ -307,7 +307,7 @@ class FusedLinearGroup:
     other members, called with the very same tensor on the same stream, return their slice of it (for prompt-sized inputs this
     also means one bf16 -> fp16 conversion of the activations instead of one per member).  A member called
     with any other input computes the joined product anew; with one made in ``torch.inference_mode``, whose writes
-    torch does not count, it computes its own rows.  A member's slice equals its stand-alone output up to the rounding of
+    torch does not count, it computes its own rows, as a member whose weight or bias is given anew does from then on.  A member's slice equals its stand-alone output up to the rounding of
     the fp32 partial sums (the K range of a row tile is cut between CTAs at other places when the launch
     covers more rows), not bit for bit.
     """
@@ -320,6 +320,7 @@ class FusedLinearGroup:
         self.offsets = []
         self._sizes = []        # the joined rows cut into the members' and what pads them,
         self._pieces = []       # and which of the pieces are the members'
+        self._made_of = None    # the members' weights and biases that are in the joined buffers
         self._cache = None      # (x, its launch_key, the pieces of y, members served)
         self.launches = 0       # joined launches issued (for tests and launch counting)
         for i, mod in enumerate(self.members):
@@ -365,6 +366,7 @@ class FusedLinearGroup:
             self._sizes.append(n)
             row = o + n
         self._device = fused.tiles.get_device()
+        self._made_of = [(q, mod.bias) for mod, q in zip(self.members, sources)]
         if fused.ready is None:
             torch.cuda.current_stream(dev).synchronize()
 
@@ -375,6 +377,10 @@ class FusedLinearGroup:
             return None
         if key[0] != self._device:
             self.build(x.device)
+        if self._made_of:
+            member, (q, bias) = self.members[index], self._made_of[index]
+            if member.quantized_weights is not q or member.bias is not bias:
+                return None   # given anew since the buffers were joined
         # (the key: another stream would not wait for the product, and a graph not hold its launch)
         c = self._cache
         if c is None or c[0] is not x or c[1] != key or index in c[3]:
@@ -467,6 +473,8 @@ class QuantizedLinear(nn.Module):
         if self._group is not None and self._group.layout is not None:
             srcs = tuple(moved if s_ is q else s_ for s_ in self._group.layout.source)
             self._group.layout = self._group.layout._replace(source=srcs)
+            if self._group._made_of:
+                self._group._made_of = [(moved if s_ is q else s_, *rest) for s_, *rest in self._group._made_of]
         self._kernel_layout = lay._replace(source=moved)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:

@@ -1,4 +1,6 @@
 """Members of a fused group give what the module alone gives, whatever happens between their calls."""
+import copy
+
 import pytest
 import torch
 
@@ -100,3 +102,31 @@ def test_members_inside_and_outside_a_graph(cuda_device, m):
         graph.replay()
         torch.cuda.synchronize(cuda_device)
         check(mods[1], weights[1], x, captured)
+
+
+@pytest.mark.parametrize("m", (1, 40))
+def test_weights_and_biases_given_anew(cuda_device, m):
+    """A member computes with what it holds, the others as before; copies and modules without their streams stay joined."""
+    mods, weights = group(cuda_device)
+    x = randn((m, 256), F16, 0, cuda_device)
+    for mod, w in zip(mods, weights):
+        check(mod, w, x)
+    other, u = module(160, 256, 30, cuda_device)
+    mods[1].quantized_weights = other.quantized_weights
+    mods[2].bias = randn((224,), F16, 31, cuda_device)
+    for _ in range(2):
+        for mod, w in zip(mods, (weights[0], u, weights[2])):
+            check(mod, w, x)
+            check(mod, w, x, ab.linear_epilogue(mod, x))
+    mods[2].bias = None
+    assert_rounded(mods[2](x), *D.product(x, weights[2], None))
+    mods, weights = group(cuda_device)
+    for mod in mods:
+        mod(x)
+    for mod in mods:
+        mod.offload_canonical()
+    for those in (mods, copy.deepcopy(mods)):
+        launches = those[0]._group.launches
+        for mod, w in zip(those, weights):
+            check(mod, w, x)
+        assert those[0]._group.launches == launches + 1
