@@ -298,6 +298,14 @@ def slice_layout(fused: KernelLayout, row_offset: int, n_rows: int, source, entr
                         fused.entries, fused.vals_sorted, n_rows, k, bs, fused.ready)
 
 
+def _version(t: Optional[torch.Tensor]) -> Optional[int]:
+    """How often ``t`` has been written to in place; None for no tensor, and for one made in inference mode, which does not count."""
+    try:
+        return None if t is None else t._version
+    except RuntimeError:
+        return None
+
+
 class FusedLinearGroup:
     """Several ``QuantizedLinear`` layers that read the same activations, computed by one launch.
 
@@ -307,7 +315,7 @@ class FusedLinearGroup:
     other members, called with the very same tensor on the same stream, return their slice of it (for prompt-sized inputs this
     also means one bf16 -> fp16 conversion of the activations instead of one per member).  A member called
     with any other input computes the joined product anew; with one made in ``torch.inference_mode``, whose writes
-    torch does not count, it computes its own rows, as a member whose weight or bias is given anew does from then on.  A member's slice equals its stand-alone output up to the rounding of
+    torch does not count, it computes its own rows, as a member whose weight or bias is given anew or whose bias is written to does from then on.  A member's slice equals its stand-alone output up to the rounding of
     the fp32 partial sums (the K range of a row tile is cut between CTAs at other places when the launch
     covers more rows), not bit for bit.
     """
@@ -320,7 +328,7 @@ class FusedLinearGroup:
         self.offsets = []
         self._sizes = []        # the joined rows cut into the members' and what pads them,
         self._pieces = []       # and which of the pieces are the members'
-        self._made_of = None    # the members' weights and biases that are in the joined buffers
+        self._made_of = None    # the members' weights and biases that are in the joined buffers, and the biases' versions
         self._cache = None      # (x, its launch_key, the pieces of y, members served)
         self.launches = 0       # joined launches issued (for tests and launch counting)
         for i, mod in enumerate(self.members):
@@ -366,9 +374,20 @@ class FusedLinearGroup:
             self._sizes.append(n)
             row = o + n
         self._device = fused.tiles.get_device()
-        self._made_of = [(q, mod.bias) for mod, q in zip(self.members, sources)]
+        self._made_of = [(q, mod.bias, _version(mod.bias)) for mod, q in zip(self.members, sources)]
         if fused.ready is None:
             torch.cuda.current_stream(dev).synchronize()
+
+    def __getstate__(self):
+        state = {**self.__dict__, "_cache": None}
+        if self._made_of:   # (what has been written to since does not look new in a copy)
+            state["_made_of"] = [(q if _version(bias) == written else None, bias, written) for q, bias, written in self._made_of]
+        return state
+
+    def __setstate__(self, state):
+        self.__dict__.update(state)
+        if self._made_of:   # (a copy's tensors count their writes anew)
+            self._made_of = [(q, bias, _version(bias)) for q, bias, _ in self._made_of]
 
     def member_forward(self, index: int, x: torch.Tensor) -> Optional[torch.Tensor]:
         """Member ``index``'s output for ``x``, or None if the group does not apply (the member computes alone)."""
@@ -378,9 +397,9 @@ class FusedLinearGroup:
         if key[0] != self._device:
             self.build(x.device)
         if self._made_of:
-            member, (q, bias) = self.members[index], self._made_of[index]
-            if member.quantized_weights is not q or member.bias is not bias:
-                return None   # given anew since the buffers were joined
+            member, (q, bias, written) = self.members[index], self._made_of[index]
+            if member.quantized_weights is not q or member.bias is not bias or (bias is not None and _version(bias) != written):
+                return None   # given anew, or written to, since the buffers were joined
         # (the key: another stream would not wait for the product, and a graph not hold its launch)
         c = self._cache
         if c is None or c[0] is not x or c[1] != key or index in c[3]:
@@ -415,21 +434,21 @@ class QuantizedLinear(nn.Module):
         self._kernel_layout: Optional[KernelLayout] = None
         self._group: Optional[FusedLinearGroup] = None   # set by fuse_linears
         self._group_index = 0
-        self._bias_f16 = None   # (bias it was made from, its fp16 contiguous image)
+        self._bias_f16 = None   # (bias it was made from, its version, its fp16 contiguous image)
 
     def _bias_for(self, bias: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-        """The bias as the kernels want it (fp16, contiguous), converted once per bias tensor and made
-        final before any kernel that reads it is launched."""
+        """The bias as the kernels want it (fp16, contiguous), converted once per bias tensor, again when that has been
+        written to, and made final before any kernel that reads it is launched."""
         if bias is None or (bias.dtype == torch.float16 and bias.is_contiguous()):
             return bias
-        cached = self._bias_f16
-        if cached is None or cached[0] is not bias:
+        cached, version = self._bias_f16, _version(bias)
+        if cached is None or cached[0] is not bias or cached[1] != version:
             image = bias.to(torch.float16).contiguous()
             if image.device.type == "cuda":
                 torch.cuda.current_stream(image.device).synchronize()
-            cached = (bias, image)
+            cached = (bias, version, image)
             self._bias_f16 = cached
-        return cached[1]
+        return cached[2]
 
     def _has_layout_for(self, q: QuantizedTensor) -> bool:
         lay = self._kernel_layout

@@ -130,3 +130,34 @@ def test_weights_and_biases_given_anew(cuda_device, m):
         for mod, w in zip(those, weights):
             check(mod, w, x)
         assert those[0]._group.launches == launches + 1
+
+
+@pytest.mark.parametrize("dtype", (F16, torch.float32))
+@pytest.mark.parametrize("m", (1, 40))
+def test_biases_written_to(cuda_device, m, dtype):
+    """In place, alone and in a group: what the kernels read follows, once the write has ended."""
+    mods, weights = group(cuda_device)
+    x = randn((m, 256), F16, 0, cuda_device)
+    for mod in mods:
+        mod.bias = mod.bias.to(dtype)
+    alone = ab.QuantizedLinear(mods[0].quantized_weights, mods[0].bias)
+    for mod, w in zip((*mods, alone), (*weights, weights[0])):
+        check(mod, w, x)
+    for those in (mods, copy.deepcopy(mods)):
+        launches = those[0]._group.launches
+        for mod in those:
+            mod(x)
+        assert those[0]._group.launches == launches + 1
+        those[1].bias.add_(1.0)
+        those[2].bias.zero_()
+        torch.cuda.synchronize(cuda_device)
+        for mod, w in zip(those, weights):
+            check(mod, w, x)
+            check(mod, w, x, ab.linear_epilogue(mod, x))
+    late = copy.deepcopy(mods)   # (copied after the writes: what was joined is out of date there too)
+    for mod, w in zip(late, weights):
+        check(mod, w, x)
+    alone.bias.mul_(-2.0)
+    torch.cuda.synchronize(cuda_device)
+    check(alone, weights[0], x)
+    check(alone, weights[0], x, ab.linear_epilogue(alone, x))
