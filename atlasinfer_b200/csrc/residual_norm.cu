@@ -268,9 +268,11 @@ int launch_as(const NormParams &p, int threads, cudaStream_t st, const char *wha
     const dim3 grid((unsigned)(ONE ? ceil_div_i64(p.tokens, 8) : p.tokens));
     // (four pieces with fp32 residuals do not fit 64 registers: 4096 x 8192 65.8 us with spills, 61.6 with half as many CTAs)
     constexpr int WIDE_MIN = V == 4 && !ONE ? 1 : MIN;
+    constexpr bool WIDE = !(ONE && V == 4);   // (by_pieces has no fp32 residual in four pieces of a warp)
     return !p.residual ? launch_early(residual_norm_kernel<V, BF16, ROWS, NO_STREAM, FULL, ONE, MAX, MIN>, grid, threads, 0, st, what, p)
-           : p.wide & ATLAS_WIDE_STREAM ? launch_early(residual_norm_kernel<V, BF16, ROWS, WIDE_STREAM, FULL, ONE, MAX, WIDE_MIN>, grid, threads, 0, st, what, p)
-                                        : launch_early(residual_norm_kernel<V, BF16, ROWS, SAME_STREAM, FULL, ONE, MAX, MIN>, grid, threads, 0, st, what, p);
+           : WIDE && (p.wide & ATLAS_WIDE_STREAM)
+               ? launch_early(residual_norm_kernel<V, BF16, ROWS, WIDE ? WIDE_STREAM : SAME_STREAM, FULL, ONE, MAX, WIDE_MIN>, grid, threads, 0, st, what, p)
+               : launch_early(residual_norm_kernel<V, BF16, ROWS, SAME_STREAM, FULL, ONE, MAX, MIN>, grid, threads, 0, st, what, p);
 }
 bool full(const NormParams &p) { return p.post_weight || p.gate || p.bias || p.centered; }
 template <int V, bool BF16, int ROWS, bool ONE, int MAX, int MIN>
@@ -280,19 +282,27 @@ int launch(const NormParams &p, int threads, cudaStream_t st, const char *what) 
 }
 // Pieces of 8 numbers a thread, and rows a CTA.  Few rows: one piece, so that a row has the most threads (1 x 4096 1.9 us, with two
 // pieces 2.1, with four 2.6).  Many: two, as soon as the CTAs no longer fit all at once (300 x 8192 4.6, 3.9, 4.7; 4096 x 8192 44.7,
-// 40.9, 41.5; with fp32 residuals 60.0, 60.1, 65.8), four for wide rows without a residual (37, 26.7, 24.8).  Many short rows: a
-// warp each (20000 x 128 5.1, a CTA each 21.3; 8192 x 1024 centered 7.2, 9.2).  With gates, biases or norms in front, a few hundred
-// rows that just do not fit at once go to CTAs of few registers, at the price of spills (515 x 5001 with all there is 10.6, 13.2;
-// 600 x 4096 with a norm in front 4.7, 5.2; but 2048 x 4096 with all 27, 22.6).
+// 40.9, 41.5; with fp32 residuals 60.0, 60.1, 65.8), four for wide rows without a residual (37, 26.7, 24.8).
+// Many short rows: a warp each, up to 512 numbers, or up to 768 from 4096 rows on where the stream has 16 bits.  Time of a warp over
+// that of a CTA (140 to 350 MB a pass; fp16; without a residual / a residual / all there is / all there is, fp32 stream):
+//   20000 x 128 .27 .29 .48 .54    8192 x 256 .41 .48 .72 .86    2048 x 512 .94 .97 1.03 1.07   1184 x 512 .92 .93 1.00 1.07
+//   20000 x 768 .74 .92 1.07 1.22  4096 x 768 .91 .94 .95 1.12   2048 x 768 .99 .96 1.15 1.26   1184 x 768 1.00 1.04 1.37 1.38
+//   20000 x 1024 .95 1.02 1.23 1.35  4096 x 999 1.06 1.17 1.10 1.19   1184 x 999 1.25 1.26 1.59 1.64
+// With gates, biases, means or norms in front, rows that do not all fit at once in CTAs of 64 registers a thread, but do in CTAs of
+// 48, go there at the price of spills.  Time of the latter over that of the former (a norm in front / all, fp32 stream):
+//   515 x 5001 .72 .78   592 x 5104 .79 .88   620 x 4096 .82 .90   740 x 4096 .79 .88    fewer rows: 444 x 5001 1.07 1.11
+//   444 x 4096 1.07 1.23    more: 680 x 5104 1.00 1.18   900 x 4096 1.02 1.18
 template <bool BF16, int ROWS>
 int by_pieces(const NormParams &p, cudaStream_t st, const char *what) {
     const int pieces = (p.hidden + (ROWS == SHIFTED ? 14 : 7)) / 8;
     auto threads = [&](int v) { return (pieces + v * 32 - 1) / (v * 32) * 32; };
-    if (p.tokens >= 8 * 148 && pieces <= 128)
+    if (p.tokens >= 8 * 148 && (pieces <= 64 || (pieces <= 96 && p.tokens >= 4096 && !(p.wide & ATLAS_WIDE_STREAM))))
         return pieces <= 32 ? launch<1, BF16, ROWS, true, 256, 4>(p, 256, st, what)
                : pieces <= 64 ? launch<2, BF16, ROWS, true, 256, 4>(p, 256, st, what) : launch<4, BF16, ROWS, true, 256, 4>(p, 256, st, what);
     if (p.tokens < 2 * 148 && pieces <= 1024) return launch<1, BF16, ROWS, false, 1024, 1>(p, threads(1), st, what);
-    if (full(p) && p.tokens <= 5 * 148 && pieces <= 640) return launch_as<2, BF16, ROWS, true, false, 320, 4>(p, threads(2), st, what);
+    const int two = threads(2);
+    if (full(p) && pieces <= 640 && p.tokens <= 5 * 148 && p.tokens > 148 * (1024 / two) && p.tokens <= 148 * (1344 / two))
+        return launch_as<2, BF16, ROWS, true, false, 320, 4>(p, two, st, what);
     if (pieces <= 1024 && (p.residual || pieces <= 512)) return launch<2, BF16, ROWS, false, 512, 2>(p, threads(2), st, what);
     return pieces <= 2048 ? launch<4, BF16, ROWS, false, 512, 2>(p, threads(4), st, what) : launch<4, BF16, ROWS, false, 1024, 1>(p, threads(4), st, what);
 }
