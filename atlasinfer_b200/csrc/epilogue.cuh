@@ -3,8 +3,9 @@
 //   y = residual + scale * act(x W^T + bias)             one weight
 //   y = residual + scale * act(x W^T + bias) * (x V^T + c)     two of one shape (gate and up)
 //
-// in fp32.  Exponentials and reciprocals are the approximate instructions (some 2^-21 relative, where the result is not 0 or
-// x), which is nothing beside the rounding to 11 or 8 bits that follows.
+// in fp32.  Exponentials and reciprocals are the approximate instructions: 2^-21 relative for small arguments, and as the exponent's
+// argument is rounded, up to 2^-23 more for every unit that it is away from 0 (silu(-80) is off by 2^-18.5, gelu(-12), whose
+// argument is -72, by 2^-17).  That is nothing beside the rounding to 11 or 8 bits that follows.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

@@ -32,7 +32,9 @@ int check(const AtlasFusedLinear *p) {
 // Gate and up with 9 to 16 rows: two token tiles of strips leave no room for both weights' strips in one CTA, so pairs of CTAs
 // are only better than the tcgen05 kernel while all of them run at once (2 x 1000 x 1024 4.3 us, 5.5; 2 x 2048 x 1024 4.7, 7.7;
 // 2 x 5504 x 2048 17.7, 12.0; 2 x 11008 x 4096 44.4, 36.4).  Up to 8 rows strips are ahead everywhere (2 x 11008 x 4096 22.7 to
-// 26.2, 34.8 to 35.6; 2 x 8192 x 2048 12.2 to 13.6, 13.7 to 14.0).
+// 26.2, 34.8 to 35.6; 2 x 8192 x 2048 12.2 to 13.6, 13.7 to 14.0).  What a tile gives away to the joined linear alone, which strips
+// serve: 2 x 11008 x 4096 at 9 and 16 fp16 rows 35.4 and 35.7 us, 28.8 and 33.4; 2 x 8192 x 2048 14.3 and 14.5, 14.8 and 16.7.  The
+// joined linear with silu and the product behind it, as modules compute it, takes longer: 12 bf16 rows of the former 38.4, 35.7 here.
 bool by_strips(const AtlasFusedLinear *p) {
     return p->m <= STRIP_MAX_ROWS && (!p->up.tiles || p->m <= 8 || 2 * ceil_div_i64(p->n_rows, 16) <= 2 * 148);
 }

@@ -1045,7 +1045,10 @@ Route route_for(const Shape &shape) {
         e.shape.flags != shape.flags) {
         const bool bf16 = shape.flags & 1, tma_ok = shape.flags & 2, aligned = shape.flags & 4;
         e.route.plan = plan_tile(shape.m, shape.n_rows, (int)(shape.n_cols / GM_BK), bf16 && tma_ok, bf16, shape.sms);
-        // (two weights: always the kernel that adds its slices up itself)
+        // (two weights: always the kernel that adds its slices up itself; this file's has no token tiles below 160 for them.  Against
+        // the joined linear alone, which may go to either: 2 x 8192 x 2048 at 72, 96, 128 fp16 rows 17.3 17.5 19.6 us, 16.9 17.1 17.5;
+        // 2 x 9472 x 4096 28.4 28.7 31.8, 29.3 29.7 30.4; 2 x 11008 x 4096 40.8 42.4 47.0, 40.9 42.4 46.5.  With silu and the product
+        // behind it the former takes 25.4 at 100 rows, 18.4 here)
         e.route.tile = (shape.flags & 8) || e.route.plan.us <= gemm_us(shape.m, shape.n_rows, shape.n_cols, bf16, bf16 && tma_ok, aligned, shape.sms);
         e.shape = shape;
     }

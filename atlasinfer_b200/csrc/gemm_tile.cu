@@ -30,7 +30,8 @@
 // 64 rows 207 -> 163; 8192 x 28672 at 32 rows 95 -> 76; 22016 x 4096 at 32 rows 52 -> 37, 128 rows 58 -> 48; 4096 x 11008
 // at 128 rows 66 -> 27 (where gemm.cu's kernel is the faster one, route_for in gemm.cu leaves it the call).  Issue slots are 45 % used (ncu, 22016 x 4096 at 32
 // rows), the shared-memory pipe half; a k-tile's chain (codes, rebuild, fence, MMA, commit) is not what is left: twice as many A tiles
-// give 1 to 3 %, half again as many dequantizer warps 2 %.  Up to 16 rows (BN = 16) this is reached on request only: the per-strip kernel serves them.
+// give 1 to 3 %, half again as many dequantizer warps 2 %.  Up to 16 rows (BN = 16) the per-strip kernel serves one weight, and this one is
+// reached on request; gate and up of 9 to 16 rows come here where they have more strips than run at once (fused_linear.cu).
 //
 // Every mbarrier wait is bounded; when one runs out the CTA sets the caller's status word, the producers and the MMA
 // thread wait (bounded) for what they have issued, and the CTA takes part in the cluster barriers, frees its TMEM and
@@ -61,7 +62,9 @@ struct TileSmem {
     // A load takes 2 to 3 us under this traffic whether it comes from HBM or, as the activations, from L2, so the rings must be
     // deep; with more A tiles than phases a warp does not wait for the MMAs of its last k-tile.  AS, XS, CS = 4, 3, 4 against
     // 2, 7, 6 (us, 24 fp16 rows): two of 28672 x 8192 153.8, 156.7; 22016 x 4096 33.9, 34.4; 12288 x 4096 21.1, 21.7; 8192 x 2048
-    // 9.6, 9.7; 57344 x 8192 147.1, 147.2; 8192 x 8192 23.4, 23.1.  For 64 rows 3, 3, 4 is no better than 2, 5, 4.
+    // 9.6, 9.7; 57344 x 8192 147.1, 147.2; 8192 x 8192 23.4, 23.1.  For 64 rows 3, 3, 4 is no better than 2, 5, 4.  Linears with nothing
+    // behind them, whole launches of 16 shapes at 17, 24 and 32 rows in turn with the older rings: fp16 0.979 of the time, bf16, converted in
+    // the kernel or in front of it, 0.978 (22016 x 4096 at 24 bf16 rows 36.0, 37.5; 1024 x 8192 10.1, 10.8; 18944 x 3584 23.7, 23.6).
     static constexpr int AS = BN == 32 ? 4 : 2;
     static constexpr int XS = BN <= 16 ? 8 : (BN == 64 ? 5 : (BN <= 96 ? 3 : 2));
     static constexpr int CS = BN <= 16 ? 7 : (BN <= 64 ? 4 : 5);
@@ -471,7 +474,8 @@ const int *resident_clusters(int sms) {
 
 // us per k-tile and per CTA, for a CTA that has an SM to itself and for one of two that share it, by token tile.  Fitted
 // to 3760 shapes (1 to 448 row tiles, K 1024 to 28672, 17 to 128 rows, fp16 and bf16, each with 1 to 8 slices): what is
-// chosen by it takes 1.3 % longer than the best choice of kernel and slices, geometric mean.
+// chosen by it takes 1.3 % longer than the best choice of kernel and slices, geometric mean.  (The tile of 32 was fitted with
+// other rings and takes 2 % less since: nothing that decides between slices, which take less alike.)
 struct TileCost { int tokens; double alone_kt, alone, shared_kt, shared, convert_kt; };
 constexpr TileCost TILE_COST[] = {{16, .38, 3.1, .58, 4.4, .12}, {32, .405, 3.3, .60, 4.75, .16}, {64, .495, 3.2, .625, 5.7, .335},
                                   {96, .47, 5.3, .61, 6.55, 0.}, {128, .485, 5.95, .68, 7.4, 0.}};

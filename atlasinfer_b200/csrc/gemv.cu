@@ -458,11 +458,11 @@ bool one_cta_pays(int64_t strips, int nwarps) { return 2 * strips * (nwarps < 4 
 // of bf16 rows, which counts a little longer; with fewer than 12 chunks the small CTAs of single strips fill the SMs
 // better.  Time of single strips over pairs at 1 and 8 rows, fp16 and bf16 (rows x K, waves of pairs):
 //   22016 x 4096, 2.3: 1.06 1.05 1.08 1.14     18432 x 6144, 1.9: 1.08 1.08 1.11 1.14     9472 x 4096, 1.0: 1.08 1.13 1.14 1.21
-//   18432 x 3072, 1.9: 1.13 1.12 1.12 1.16     12288 x 5120, 1.3: 0.91 0.90 0.97 0.97    14336 x 7168, 1.5: 0.94 0.98 0.97 1.01
+//   12288 x 5120, 1.3: 0.91 0.90 0.97 0.97    14336 x 7168, 1.5: 0.94 0.98 0.97 1.01
 //   57344 x 8192, 6.1: 0.98 1.00 1.02 1.06     24576 x 7168, 2.6: 0.99 0.99 1.01 1.05    16384 x 11008, 1.7: 0.98 1.04 0.97 1.04
 //   12288 x 2048, 1.3: 0.90 0.93 0.92 0.97      9472 x 2048, 1.0: 0.88 0.90 0.91 0.97
 // What the rule gives away: 12288 x 4096, 1.3: 1.04 1.03 1.05 1.11 (its 64 % of two waves is refused with its neighbours
-// 11008 x 4096, 1.2: 0.94 0.95 0.94 1.00, 12288 x 3072, 1.3: 0.88 0.90 0.95 0.96 and 12288 x 6144, 1.3: 0.95 0.90 0.97 0.97).
+// 11008 x 4096, 1.2: 0.94 0.95 0.94 1.00, and 12288 x 6144, 1.3: 0.95 0.90 0.97 0.97).
 bool strip_pairs_pay(int64_t pairs, int n_chunks, bool bf16) {
     const int sms = sm_count();
     const int64_t places = 2 * sms, waves = ceil_div_i64(pairs, places);

@@ -1,4 +1,4 @@
-// Rows of numbers in 16 or 32 bits: loads and stores of 8 at a time, and sums over the threads of a row.
+// Numbers in 16 bits as fp32 and back, one, two and eight at a time.
 #pragma once
 #include "kv_cache.cuh"
 
