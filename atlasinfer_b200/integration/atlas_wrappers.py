@@ -354,6 +354,7 @@ class FusedLinearGroup:
         else:
             fused, self.offsets = build_joined_layout(sources, wait=False)
         rows = [int(q.original_shape[0]) for q in sources]
+        self.bias = None
         if any(mod.bias is not None for mod in self.members):
             b = torch.zeros(fused.n_rows, dtype=torch.float16, device=dev)
             for mod, n, o in zip(self.members, rows, self.offsets):

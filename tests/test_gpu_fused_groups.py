@@ -161,3 +161,15 @@ def test_biases_written_to(cuda_device, m, dtype):
     torch.cuda.synchronize(cuda_device)
     check(alone, weights[0], x)
     check(alone, weights[0], x, ab.linear_epilogue(alone, x))
+
+
+def test_biases_taken_away(cuda_device):
+    """Joined anew without them."""
+    mods, weights = group(cuda_device)
+    x = randn((2, 256), F16, 0, cuda_device)
+    for mod in mods:
+        mod(x)
+        mod.bias = None
+    mods[0]._group.build(x.device)
+    for mod, w in zip(mods, weights):
+        assert_rounded(mod(x), *D.product(x, w, None))
