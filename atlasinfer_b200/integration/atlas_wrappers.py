@@ -298,6 +298,9 @@ def slice_layout(fused: KernelLayout, row_offset: int, n_rows: int, source, entr
                         fused.entries, fused.vals_sorted, n_rows, k, bs, fused.ready)
 
 
+_building = threading.RLock()   # held while a group's buffers are joined
+
+
 def _version(t: Optional[torch.Tensor]) -> Optional[int]:
     """How often ``t`` has been written to in place; None for no tensor, and for one made in inference mode, which does not count."""
     try:
@@ -336,6 +339,18 @@ class FusedLinearGroup:
             mod._group_index = i
 
     def build(self, dev: torch.device) -> None:
+        """Join the members' layouts on ``dev``."""
+        with _building:
+            self._build(dev)
+
+    def ensure(self, dev: torch.device) -> None:
+        """Join the members' layouts on ``dev`` unless they are joined there."""
+        if self._device != dev.index:
+            with _building:
+                if self._device != dev.index:   # (another thread may just have done it)
+                    self._build(dev)
+
+    def _build(self, dev: torch.device) -> None:
         for mod in self.members:
             q = mod.quantized_weights
             if q.fp8_data.device != dev:
@@ -347,37 +362,39 @@ class FusedLinearGroup:
             # members that are laid out already are joined as they are
             layouts = [mod._layout_for(q) for mod, q in zip(self.members, sources)]
             fused = concat_layouts(layouts)
-            self.offsets, off = [], 0
+            offsets, off = [], 0
             for lay in layouts:
-                self.offsets.append(off)
+                offsets.append(off)
                 off += (lay.n_rows + 127) // 128 * 128
         else:
-            fused, self.offsets = build_joined_layout(sources, wait=False)
+            fused, offsets = build_joined_layout(sources, wait=False)
         rows = [int(q.original_shape[0]) for q in sources]
+        biases = [mod.bias for mod in self.members]
+        self._made_of = [(q, b, _version(b)) for q, b in zip(sources, biases)]
         self.bias = None
-        if any(mod.bias is not None for mod in self.members):
-            b = torch.zeros(fused.n_rows, dtype=torch.float16, device=dev)
-            for mod, n, o in zip(self.members, rows, self.offsets):
-                if mod.bias is not None:
-                    b[o:o + n] = mod.bias.to(torch.float16)
-            self.bias = b
+        if any(b is not None for b in biases):
+            joined = torch.zeros(fused.n_rows, dtype=torch.float16, device=dev)
+            for b, n, o in zip(biases, rows, offsets):
+                if b is not None:
+                    joined[o:o + n] = b.to(torch.float16)
+            self.bias = joined
             if fused.ready is not None:   # the bias is part of what a use waits for
                 fused = fused._replace(ready=_enqueued(dev))
         # the members now look at the joined buffers; their own copies are released
-        for mod, q, n, o in zip(self.members, sources, rows, self.offsets):
+        for mod, q, n, o in zip(self.members, sources, rows, offsets):
             mod._kernel_layout = slice_layout(fused, o, n, q)
-        self.layout = fused
-        self._sizes, self._pieces, row = [], [], 0
-        for n, o in zip(rows, self.offsets):
+        self.offsets, self.layout = offsets, fused
+        sizes, pieces, row = [], [], 0
+        for n, o in zip(rows, offsets):
             if o > row:
-                self._sizes.append(o - row)
-            self._pieces.append(len(self._sizes))
-            self._sizes.append(n)
+                sizes.append(o - row)
+            pieces.append(len(sizes))
+            sizes.append(n)
             row = o + n
-        self._device = fused.tiles.get_device()
-        self._made_of = [(q, mod.bias, _version(mod.bias)) for mod, q in zip(self.members, sources)]
+        self._sizes, self._pieces = sizes, pieces
         if fused.ready is None:
             torch.cuda.current_stream(dev).synchronize()
+        self._device = fused.tiles.get_device()   # (last: a call that finds it finds the rest)
 
     def __getstate__(self):
         state = {**self.__dict__, "_cache": None}
@@ -396,7 +413,7 @@ class FusedLinearGroup:
         if key is None:
             return None
         if key[0] != self._device:
-            self.build(x.device)
+            self.ensure(x.device)
         if self._made_of:
             member, (q, bias, written) = self.members[index], self._made_of[index]
             if member.quantized_weights is not q or member.bias is not bias or (bias is not None and _version(bias) != written):
@@ -465,8 +482,8 @@ class QuantizedLinear(nn.Module):
         q = self.quantized_weights
         if not hasattr(q, "fp8_data"):
             raise TypeError(f"Weight in QuantizedLinear ({id(self)}) is not a valid QuantizedTensor: {type(q)}")
-        if self._group is not None and (self._group.layout is None or self._group.layout.tiles.device != device):
-            self._group.build(device)
+        if self._group is not None:
+            self._group.ensure(device)
             q = self.quantized_weights
         layout = self._kernel_layout
         if layout is None or layout.source is not q or layout.tiles.device != device:

@@ -1,5 +1,6 @@
 """Members of a fused group give what the module alone gives, whatever happens between their calls."""
 import copy
+import threading
 
 import pytest
 import torch
@@ -161,6 +162,40 @@ def test_biases_written_to(cuda_device, m, dtype):
     torch.cuda.synchronize(cuda_device)
     check(alone, weights[0], x)
     check(alone, weights[0], x, ab.linear_epilogue(alone, x))
+
+
+@pytest.mark.parametrize("laid_out", (False, True))
+def test_first_calls_from_several_threads(cuda_device, laid_out):
+    """A group that several threads take into use at once, one of its members laid out before or none."""
+    for _ in range(6):
+        mods, weights = group(cuda_device)
+        if laid_out:
+            mods[1]._layout_for(mods[1].quantized_weights)
+        inputs = [randn((1 + i, 256), F16, i, cuda_device) for i in range(6)]
+        torch.cuda.synchronize(cuda_device)
+        outs, errors, start = [None] * len(inputs), [], threading.Barrier(len(inputs))
+
+        def work(i):
+            try:
+                with torch.cuda.stream(torch.cuda.Stream(cuda_device)):
+                    start.wait()
+                    if i % 2:
+                        outs[i] = [mod(inputs[i]) for mod in mods]
+                    else:
+                        outs[i] = [ab.linear_epilogue(mod, inputs[i]) for mod in mods]
+                    torch.cuda.current_stream(cuda_device).synchronize()
+            except BaseException as e:   # noqa: BLE001 - reported by the main thread
+                errors.append(e)
+
+        threads = [threading.Thread(target=work, args=(i,)) for i in range(len(inputs))]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        assert not errors, errors[0]
+        for x, ys in zip(inputs, outs):
+            for mod, w, y in zip(mods, weights, ys):
+                check(mod, w, x, y)
 
 
 def test_biases_taken_away(cuda_device):
