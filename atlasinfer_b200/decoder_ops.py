@@ -44,7 +44,7 @@ def residual_norm(x: torch.Tensor, residual: Optional[torch.Tensor] = None, weig
 
 
 def _laid_out(linear: QuantizedLinear, device: torch.device):
-    """``(layout, bias)`` of a module on ``device``, as its own forward uses them."""
+    """``(layout, bias, whether the bias may still be written)`` of a module on ``device``, as its own forward uses them."""
     if not isinstance(linear, QuantizedLinear):
         raise TypeError(f"expected a QuantizedLinear, got {type(linear)}")
     return linear.kernel_form(device)
@@ -55,16 +55,16 @@ def _run(x, first, second, activation, residual, scale):
         raise ValueError(f"activation {activation!r} is none of {tuple(ACTIVATIONS)}")
     if not x.is_cuda:
         raise ValueError("x must be on a CUDA device")
-    layout, bias = _laid_out(first, x.device)
-    pending = bool(layout.ready) and _pending(layout)
+    layout, bias, pending = _laid_out(first, x.device)
+    pending |= bool(layout.ready) and _pending(layout)
     buffers = lambda l: [l.tiles, l.scales_tiled, l.chunk_ptr, l.entries, l.vals_sorted]  # noqa: E731
     up, up_bias = [], None
     if second is not None:
-        other, up_bias = _laid_out(second, x.device)
+        other, up_bias, new = _laid_out(second, x.device)
         if (other.n_rows, other.n_cols, other.block_size) != (layout.n_rows, layout.n_cols, layout.block_size):
             raise ValueError(f"gate is [{layout.n_rows}, {layout.n_cols}] in blocks of {layout.block_size}, "
                              f"up [{other.n_rows}, {other.n_cols}] in blocks of {other.block_size}")
-        pending |= bool(other.ready) and _pending(other)
+        pending |= new | (bool(other.ready) and _pending(other))
         up = buffers(other)
     return _capi.native().fused_linear(x, buffers(layout), bias, up, up_bias, layout.n_rows, layout.n_cols, layout.block_size, residual,
                                        ACTIVATIONS[activation], scale, status_word(x.device), pending)

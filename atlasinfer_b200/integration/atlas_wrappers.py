@@ -205,11 +205,12 @@ def build_joined_layout(qs, wait: bool = True):
 
 
 def quantized_linear_forward(x: torch.Tensor, layout: KernelLayout, bias: Optional[torch.Tensor],
-                             force: Optional[str] = None) -> torch.Tensor:
+                             force: Optional[str] = None, new: bool = False) -> torch.Tensor:
     """``x @ W^T + bias`` on CUDA tensors through the C ABI.
 
     ``force``: "gemv" (per-strip streaming kernel), "gemm" (tcgen05 kernel) or "stream" (persistent streaming
-    kernel, one pass for up to 32 rows); default: "gemv" up to 16 rows of x, "gemm" above."""
+    kernel, one pass for up to 32 rows); default: "gemv" up to 16 rows of x, "gemm" above.  ``new``: the kernels in
+    front may still be writing the bias (a kernel reads it before they have ended, unless it is launched plainly)."""
     if x.dtype is not torch.float16 and x.dtype is not torch.bfloat16:
         raise RuntimeError(f"QuantizedLinear expects fp16 (or bf16) activations, got {x.dtype}")
     if force is None:
@@ -220,7 +221,7 @@ def quantized_linear_forward(x: torch.Tensor, layout: KernelLayout, bias: Option
         gemv_rows = _ANY_ROWS if force == "gemv" else 0
     else:
         raise ValueError(f"force={force!r}")
-    pending = bool(layout.ready) and _pending(layout)
+    pending = (bool(layout.ready) and _pending(layout)) or new
     return _capi.native().linear(x, layout.tiles, layout.scales_tiled, layout.chunk_ptr, layout.entries, layout.vals_sorted,
                                  layout.n_rows, layout.n_cols, layout.block_size, bias, status_word(x.device), gemv_rows, pending)
 
@@ -454,19 +455,25 @@ class QuantizedLinear(nn.Module):
         self._group_index = 0
         self._bias_f16 = None   # (bias it was made from, its version, its fp16 contiguous image)
 
-    def _bias_for(self, bias: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-        """The bias as the kernels want it (fp16, contiguous), converted once per bias tensor, again when that has been
-        written to, and made final before any kernel that reads it is launched."""
-        if bias is None or (bias.dtype == torch.float16 and bias.is_contiguous()):
-            return bias
-        cached, version = self._bias_f16, _version(bias)
-        if cached is None or cached[0] is not bias or cached[1] != version:
-            image = bias.to(torch.float16).contiguous()
+    def _bias_for(self, bias: Optional[torch.Tensor]):
+        """``(image, new)``: the bias as the kernels want it (fp16, contiguous), and whether the kernels in front may still be
+        writing it.
+
+        Converted once per bias tensor, again when that has been written to, and final on return then.  One that needs no
+        conversion is new when it is met first, or first after a write: a launch in stream order comes after that write,
+        and later ones after that launch."""
+        if bias is None:
+            return None, False
+        seen, version = self._bias_f16, _version(bias)
+        if seen is not None and seen[0] is bias and seen[1] == version:
+            return seen[2], False
+        image, new = bias, True
+        if bias.dtype != torch.float16 or not bias.is_contiguous():
+            image, new = bias.to(torch.float16).contiguous(), False
             if image.device.type == "cuda":
                 torch.cuda.current_stream(image.device).synchronize()
-            cached = (bias, version, image)
-            self._bias_f16 = cached
-        return cached[2]
+        self._bias_f16 = (bias, version, image)
+        return image, new
 
     def _has_layout_for(self, q: QuantizedTensor) -> bool:
         lay = self._kernel_layout
@@ -478,7 +485,8 @@ class QuantizedLinear(nn.Module):
         return self._kernel_layout
 
     def kernel_form(self, device: torch.device):
-        """``(layout, bias)`` on a CUDA ``device``, laid out now if they are not there yet; ``bias`` is fp16 or None."""
+        """``(layout, bias, new)`` on a CUDA ``device``, laid out now if they are not there yet; ``bias`` is fp16 or None, and
+        ``new`` if the kernels in front may still be writing it."""
         q = self.quantized_weights
         if not hasattr(q, "fp8_data"):
             raise TypeError(f"Weight in QuantizedLinear ({id(self)}) is not a valid QuantizedTensor: {type(q)}")
@@ -492,7 +500,7 @@ class QuantizedLinear(nn.Module):
             layout = self._layout_for(q)
         if self.bias is not None and self.bias.device != device:
             self.bias = self.bias.to(device)
-        return layout, self._bias_for(self.bias)
+        return (layout, *self._bias_for(self.bias))
 
     def offload_canonical(self, device="cpu") -> None:
         """Keep only the kernel layout on the GPU: the canonical streams move to ``device`` (host by default).
@@ -527,7 +535,8 @@ class QuantizedLinear(nn.Module):
         bias = self.bias
         if lay is not None and lay.source is q_tensor and x.is_cuda and lay.tiles.device == x.device and (
                 bias is None or bias.device == x.device):
-            return quantized_linear_forward(x, lay, self._bias_for(bias))
+            bias, new = self._bias_for(bias)
+            return quantized_linear_forward(x, lay, bias, None, new)
         # the kernels need a GPU; CPU activations are staged through it and the result returned
         compute_device = x.device if x.device.type == "cuda" else _capi.require_cuda()
         if lay is not None and lay.source is q_tensor and lay.tiles.device == compute_device:
@@ -538,7 +547,8 @@ class QuantizedLinear(nn.Module):
                 self.bias = bias.to(compute_device)
                 bias = self.bias
             xin = x if x.device == compute_device else x.to(compute_device)
-            y = quantized_linear_forward(xin, lay, self._bias_for(bias))
+            bias, new = self._bias_for(bias)
+            y = quantized_linear_forward(xin, lay, bias, None, new)
             return y if x.device == compute_device else y.to(x.device)
         if q_tensor.fp8_data.device != compute_device:
             if _VERBOSE:
@@ -551,7 +561,8 @@ class QuantizedLinear(nn.Module):
             bias = self.bias
         layout = self._layout_for(q_tensor)
         xin = x if x.device == compute_device else x.to(compute_device)
-        y = quantized_linear_forward(xin, layout, self._bias_for(bias))
+        bias, new = self._bias_for(bias)
+        y = quantized_linear_forward(xin, layout, bias, None, new)
         return y if x.device == compute_device else y.to(x.device)
 
     def extra_repr(self) -> str:

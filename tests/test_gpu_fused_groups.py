@@ -10,6 +10,7 @@ import atlasinfer_b200 as ab
 from . import decoder_reference as D
 from .kv_reference import assert_rounded
 from .test_gpu_fused_linear import module, randn
+from .test_gpu_plain_launch import _edges
 
 pytestmark = pytest.mark.gpu
 
@@ -208,3 +209,39 @@ def test_biases_taken_away(cuda_device):
     mods[0]._group.build(x.device)
     for mod, w in zip(mods, weights):
         assert_rounded(mod(x), *D.product(x, w, None))
+
+
+@pytest.mark.parametrize("m", (1, 12, 40, 200))
+def test_biases_that_kernels_in_front_write(cuda_device, m):
+    """A bias that another linear's launch is still writing when the module is called with it."""
+    long, w = module(1024, 16384, 40, cuda_device, bias=False)
+    (lin, v), (up, u) = (module(1024, 256, s, cuda_device) for s in (41, 42))
+    x = randn((m, 256), F16, 0, cuda_device)
+    for mod in (lin, up):
+        mod(x)
+    long(randn((1, 16384), F16, 0, cuda_device))
+    calls = (lambda: lin(x), lambda: ab.linear_epilogue(lin, x, "relu"), lambda: ab.gated_linear(up, lin, x, "relu"), lambda: ab.gated_linear(lin, up, x, "relu"))
+    for seed in range(4):
+        for call in calls:
+            z = randn((1, 16384), F16, seed, cuda_device)
+            torch.cuda.synchronize(cuda_device)
+            torch.cuda._sleep(200000)   # (both launches are there before the first one begins)
+            lin.bias = long(z)[0]   # (read by the next launch, which need not wait for this one but where it is told to)
+            got = call()
+            torch.cuda.synchronize(cuda_device)
+            assert torch.equal(got, call())
+            lin.bias = None
+    # in a captured graph: every launch of the call waits for the end of the one in front; later calls need not
+    for call in calls:
+        lin.bias = None
+        ordinary, early = _edges(cuda_device, call, call)
+        assert ordinary == 0
+        kernels = (early + 1) // 2
+        z = randn((1, 16384), F16, 9, cuda_device)
+
+        def front():
+            lin.bias = long(z)[0]
+
+        assert _edges(cuda_device, front, call) == (kernels, 0)
+        assert _edges(cuda_device, front, lambda: (call(), call())) == (kernels, kernels)
+    lin.bias = None
