@@ -404,7 +404,7 @@ class FusedLinearGroup:
         return state
 
     def __setstate__(self, state):
-        self.__dict__.update(state)
+        self.__dict__.update({"_device": -1, "_made_of": None, "_sizes": [], "_pieces": [], **state})   # (one pickled without them joins anew)
         if self._made_of:   # (a copy's tensors count their writes anew)
             self._made_of = [(q, bias, _version(bias)) for q, bias, _ in self._made_of]
 

@@ -245,3 +245,22 @@ def test_biases_that_kernels_in_front_write(cuda_device, m):
         assert _edges(cuda_device, front, call) == (kernels, 0)
         assert _edges(cuda_device, front, lambda: (call(), call())) == (kernels, kernels)
     lin.bias = None
+
+
+def test_a_group_pickled_without_what_it_joined(cuda_device):
+    """As an earlier version of the package wrote it: joined anew at its first call."""
+    mods, weights = group(cuda_device)
+    x = randn((2, 256), F16, 0, cuda_device)
+    for mod in mods:
+        mod(x)
+    old = mods[0]._group.__getstate__()
+    for name in ("_device", "_made_of", "_sizes", "_pieces"):
+        del old[name]
+    again = object.__new__(type(mods[0]._group))
+    again.__setstate__(old)
+    for mod in mods:
+        mod._group = again
+    launches = again.launches
+    for mod, w in zip(mods, weights):
+        check(mod, w, x)
+    assert again.launches == launches + 1
